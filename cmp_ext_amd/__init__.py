@@ -19,7 +19,7 @@ the `build` submodule stays usable.
 import torch  # noqa: F401  (loads PyTorch's HIP runtime before the extension binds to it)
 
 __all__ = ["fp16_matmul", "bf16_matmul", "fp32_matmul", "linear", "bmm", "conv2d", "plan", "last_plan",
-           "version"]
+           "qk_norm_rope", "kv_cache_write", "kv_cache_read", "attention", "paged_attention", "version"]
 
 try:
     from . import _cmpext3 as _ext
@@ -40,6 +40,11 @@ if _ext is not None:
     conv2d = _ext.conv2d
     plan = _ext.plan
     last_plan = _ext.last_plan
+    qk_norm_rope = _ext.qk_norm_rope
+    kv_cache_write = _ext.kv_cache_write
+    kv_cache_read = _ext.kv_cache_read
+    attention = _ext.attention
+    paged_attention = _ext.paged_attention
     version = _ext.version
     extension_path = _ext.__file__
 else:

@@ -1,7 +1,8 @@
-"""Build the gfx950 GEMM library and its Python binding, in-tree.
+"""Build the gfx950 library and its Python binding, in-tree.
 
 Outputs (git-ignored, shipped to the GPU box with the tree):
-  cmp_ext_amd/lib/libcmpext3_gemm.so   HIP kernels + C ABI (include/cmpext3_gemm.h)
+  cmp_ext_amd/lib/libcmpext3_gemm.so   HIP kernels + C ABI (include/cmpext3_gemm.h,
+                                       include/cmpext3_attention.h)
   cmp_ext_amd/_cmpext3<EXT_SUFFIX>      pybind11 module `cmpext3` (links the above)
 
 The kernels are compiled with hipcc for gfx950 only; the host-only sources
@@ -27,8 +28,12 @@ ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
 HIP_SOURCES = [f"tile_{t}_{lay}_{k}.hip" for t in ("f16", "bf16") for lay in ("kn", "nk") for k in ("whole", "ragged")] + \
-    ["skinny.hip", "tall.hip", "stream.hip", "stream_nk.hip", "f32.hip", "generic.hip", "pad.hip", "noalloc.hip", "sem.hip"]
-HOST_SOURCES = ["selector.cpp", "api.cpp"]
+    ["skinny.hip", "tall.hip", "stream.hip", "stream_nk.hip", "f32.hip", "generic.hip", "pad.hip", "noalloc.hip", "sem.hip"] + \
+    [f"attention_tile_{t}_{k}.hip" for t in ("f16", "bf16") for k in ("packed", "paged16", "paged8")] + \
+    [f"attention_few_{t}_{k}.hip" for t in ("f16", "bf16") for k in ("paged16", "paged8")] + \
+    ["attention_join.hip", "qk_norm_rope.hip", "kv_cache.hip"]
+HOST_SOURCES = ["selector.cpp", "api.cpp", "attention_api.cpp"]
+BINDING_SOURCES = ["main.cpp", "attention_ops.cpp"]
 
 HIP_FLAGS = [
     "--offload-arch=gfx950",
@@ -92,7 +97,7 @@ def build_binding() -> str:
            f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-DTORCH_API_INCLUDE_EXTENSION_H",
            "-DTORCH_EXTENSION_NAME=_cmpext3", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
            *("-I" + i for i in incs),
-           os.path.join(CSRC, "main.cpp"), "-o", out + ".tmp",
+           *(os.path.join(CSRC, f) for f in BINDING_SOURCES), "-o", out + ".tmp",
            "-L" + torch_lib, "-lc10", "-lc10_hip", "-ltorch", "-ltorch_cpu", "-ltorch_python",
            "-L" + LIBDIR, "-lcmpext3_gemm", "-Wl,-rpath,$ORIGIN/lib"]
     _run(cmd)

@@ -1,4 +1,5 @@
-"""ctypes view of the C ABI in include/cmpext3_gemm.h (libcmpext3_gemm.so).
+"""ctypes view of the C ABI in include/cmpext3_gemm.h and include/cmpext3_attention.h
+(libcmpext3_gemm.so).
 
 Used by the tests and the benchmark to drive the kernels through the same
 boundary a non-Python caller would bind.  PyTorch is imported first so that
@@ -14,7 +15,7 @@ import torch  # noqa: F401
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libcmpext3_gemm.so")
 
-F16, BF16, F32 = 0, 1, 2
+F16, BF16, F32, E4M3 = 0, 1, 2, 3
 B_KN, B_NK = 0, 1
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_TOO_LARGE, ERR_WORKSPACE, ERR_SCRATCH = 0, -1, -2, -3, -4, -5
 SCRATCH_BYTES = 64 << 20
@@ -45,6 +46,42 @@ SIGNATURES = {
     "cmpext3_version": (_cp, []),
 }
 
+
+
+def _fields(text: str, **types) -> list:
+    """ctypes fields from "type: name name ...; ..." in the order of the C structure."""
+    kinds = {"i32": ctypes.c_int32, "i64": ctypes.c_int64, "f32": ctypes.c_float, "ptr": ctypes.c_void_p, **types}
+    return [(name, kinds[part.split(":")[0].strip()]) for part in text.split(";") for name in part.split(":")[1].split()]
+
+
+# The structures of include/cmpext3_attention.h.
+class QkNormRopeArgs(ctypes.Structure):
+    _fields_ = _fields("""i32: dtype interleaved heads kv_heads dim rotary_dim; i64: tokens; ptr: q k q_out k_out;
+                          i64: q_token q_head k_token k_head q_out_token q_out_head k_out_token k_out_head;
+                          ptr: q_weight k_weight cos sin; i64: table_rows table_row; ptr: positions; f32: eps""")
+
+
+class KvCache(ctypes.Structure):
+    _fields_ = _fields("""i32: kv_dtype pages page_size kv_heads dim; ptr: k v; i64: k_page k_token k_head v_page v_token v_head;
+                          ptr: k_scale v_scale; i64: ks_page ks_token ks_head vs_page vs_token vs_head""")
+
+
+class AttentionArgs(ctypes.Structure):
+    _fields_ = _fields("""i32: dtype batch heads causal; f32: scale; i32: len_q len_k total_q total_k; ptr: q out;
+                          i64: q_batch q_token q_head out_batch out_token out_head; cache: cache;
+                          ptr: starts_q starts_k block_table; i64: table_row; i32: table_pages; ptr: seq_lens""", cache=KvCache)
+
+
+# Exported symbols of include/cmpext3_attention.h.
+ATTENTION_SIGNATURES = {
+    "cmpext3_qk_norm_rope": (_i, [_p, _p]),
+    "cmpext3_kv_cache_write": (_i, [_p, _i, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _p]),
+    "cmpext3_kv_cache_read": (_i, [_p, _p, _i64, ctypes.c_int32, _p, ctypes.c_int32, _i64, _i, _p, _p, _p]),
+    "cmpext3_attention_workspace_size": (_i64, [_p]),
+    "cmpext3_attention": (_i, [_p, _p, _i64, _p]),
+    "cmpext3_attention_describe": (_i, [_p, _cp, _i]),
+}
+
 _lib = None
 
 
@@ -54,7 +91,7 @@ def lib() -> ctypes.CDLL:
         if not os.path.exists(LIB_PATH):
             raise OSError(f"{LIB_PATH} not built; run `python -m cmp_ext_amd.build`")
         l = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in SIGNATURES.items():
+        for name, (res, args) in {**SIGNATURES, **ATTENTION_SIGNATURES}.items():
             f = getattr(l, name)
             f.restype = res
             f.argtypes = args

@@ -1,0 +1,157 @@
+// Device helpers of the attention operators: where a sequence's rows and keys are,
+// page lookups, and 8-bit floats.
+#pragma once
+
+#include "attention_params.h"
+#include "device_common.h"
+
+namespace cmpext3 {
+
+// One sequence of a call.
+struct Seq {
+  int b;           // -1: none
+  int q0, len_q;   // first row in the packed queries, number of queries
+  int k0, len_k;
+  int tile;        // row tile of the sequence
+};
+
+__device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
+
+// Row tile `slot` of the grid: which sequence, and which of its tiles of `rows` rows (a row
+// is one query of one head of the group).  With packed queries, sequence b owns the slots
+// from starts_q[b] * group / rows + b on: these grow by at least one per sequence and by
+// no less than its tiles, so the grid needs no lengths from the host; slots past a
+// sequence's last tile have nothing to do (b = -1).  64 starts are compared at once.
+__device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int rows) {
+  Seq s;
+  if (p.starts_q == nullptr) {
+    const int tiles = (p.len_q * p.group + rows - 1) / rows;
+    s.b = slot / tiles;
+    s.tile = slot - s.b * tiles;
+    s.q0 = 0;
+    s.len_q = p.len_q;
+  } else {
+    const int lane = threadIdx.x & 63;
+    int count = 0;
+    for (int b0 = 0; b0 < p.batch; b0 += 64) {
+      const int b = b0 + lane;
+      const bool below = b < p.batch && clampi(p.starts_q[b], 0, p.total_q) * p.group / rows + b <= slot;
+      const unsigned long long m = __builtin_amdgcn_ballot_w64(below);
+      count += __builtin_popcountll(m);
+      if (m != ~0ull) break;
+    }
+    s.b = count - 1;
+    if (s.b < 0) return s;
+    s.q0 = clampi(p.starts_q[s.b], 0, p.total_q);
+    s.len_q = clampi(p.starts_q[s.b + 1], s.q0, p.total_q) - s.q0;
+    s.tile = slot - (s.q0 * p.group / rows + s.b);
+  }
+  s.b = __builtin_amdgcn_readfirstlane(s.b);  // all of it is the workgroup's: scalar registers
+  s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
+  s.len_q = __builtin_amdgcn_readfirstlane(s.len_q);
+  s.tile = __builtin_amdgcn_readfirstlane(s.tile);
+  const int tiles = (s.len_q * p.group + rows - 1) / rows;
+  if (s.tile < 0 || s.tile >= tiles) {
+    s.b = -1;
+    return s;
+  }
+  s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
+  if (p.kv.table != nullptr) {
+    s.k0 = 0;
+    const int64_t most = (int64_t)p.kv.table_pages * p.kv.page_size;
+    s.len_k = (int)min((int64_t)max(p.seq_lens[s.b], 0), most);
+  } else if (p.starts_k != nullptr) {
+    s.k0 = clampi(p.starts_k[s.b], 0, p.total_k);
+    s.len_k = clampi(p.starts_k[s.b + 1], s.k0, p.total_k) - s.k0;
+  } else {
+    s.k0 = 0;
+    s.len_k = p.len_k;
+  }
+  s.k0 = __builtin_amdgcn_readfirstlane(s.k0);
+  s.len_k = __builtin_amdgcn_readfirstlane(s.len_k);
+  return s;
+}
+
+// The page of key `key` and its place in the page; -1 where the table names no page of the cache.
+__device__ __forceinline__ int page_of(const KvSource& kv, const int32_t* table, int key, int& place) {
+  const int n = kv.page_shift >= 0 ? key >> kv.page_shift : key / kv.page_size;
+  place = key - n * kv.page_size;
+  const int page = table[n];
+  return (unsigned)page < (unsigned)kv.pages ? page : -1;
+}
+
+// Four e4m3 codes (one dword) as four values of T: exact, both types hold every code.
+template <typename T>
+__device__ __forceinline__ u32x2 e4m3x4(uint32_t c) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
+  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
+  return u32x2{pack2<T>(lo[0], lo[1]), pack2<T>(hi[0], hi[1])};
+}
+
+// 2^x, the hardware's (relative error about 2^-23; 0 for -infinity).
+__device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
+
+typedef u32x4 u32x4_a8 __attribute__((aligned(8)));  // 16 bytes at an address aligned to 8
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+// Transposing LDS read: the 16 lanes of a group name four rows of 16 consecutive 16-bit
+// columns (lane r: row r / 4, columns 4 (r % 4) ..), lane r gets column r of the four rows.
+__device__ __forceinline__ u32x2 lds_read_tr(const unsigned char* q) {
+  return __builtin_bit_cast(
+      u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)q));
+}
+
+// ---- values of V that are not finite, at keys that only some rows see ----
+// A product adds 0 * v for a masked key, which is NaN where v is infinite or NaN: a row would
+// get a value it does not see.  Steps in which some row sees only part of the keys therefore
+// look V over first (any_not_finite), and in the rare step that holds such a value take the
+// products with those values as zeros and add them apart, to the rows whose weights for them
+// are not zero (kind_ones: 1 at +infinity, -infinity or NaN, whose products with the weights
+// are positive exactly there).
+template <typename T>
+constexpr uint32_t kExponents = std::is_same<T, _Float16>::value ? 0x7C007C00u : 0x7F807F80u;
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+// Whether the stretch of `bytes` of LDS (a multiple of 1024) holds one; the same for all lanes.
+template <typename T>
+__device__ __forceinline__ bool any_not_finite(const unsigned char* lds, int bytes) {
+  u16x2 most = u16x2{0, 0};
+  for (int i = 16 * (threadIdx.x & 63); i < bytes; i += 1024) {
+    const u32x4 x = *(const u32x4*)(lds + i);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) most = __builtin_elementwise_max(most, __builtin_bit_cast(u16x2, x[j] & kExponents<T>));
+  }
+  constexpr unsigned short e = (unsigned short)kExponents<T>;
+  return __builtin_amdgcn_ballot_w64(most.x == e || most.y == e) != 0;
+}
+// kind 0: +infinity, 1: -infinity, 2: NaN
+__device__ __forceinline__ float kind_value(int kind) {
+  return kind == 0 ? INFINITY : kind == 1 ? -INFINITY : __builtin_nanf("");
+}
+template <typename T>
+__device__ __forceinline__ u32x4 kind_ones(u32x4 v, int kind) {
+  constexpr uint32_t e = kExponents<T> & 0xFFFF, one = std::is_same<T, _Float16>::value ? 0x3C00u : 0x3F80u;
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    r[j] = 0;
+#pragma unroll
+    for (int h = 0; h < 32; h += 16) {
+      const uint32_t b = (v[j] >> h) & 0xFFFF;
+      const bool hit = kind == 0 ? b == e : kind == 1 ? b == (e | 0x8000) : (b & 0x7FFF) > e;
+      r[j] |= hit ? one << h : 0u;
+    }
+  }
+  return r;
+}
+template <typename T>
+__device__ __forceinline__ u32x4 finite_only(u32x4 v) {
+  constexpr uint32_t e = kExponents<T> & 0xFFFF;
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r[j] = ((v[j] & e) == e ? 0u : v[j] & 0xFFFFu) | ((v[j] >> 16 & e) == e ? 0u : v[j] & 0xFFFF0000u);
+  return r;
+}
+
+}  // namespace cmpext3

@@ -1,0 +1,315 @@
+// Attention of few query rows over a paged cache (gfx950): generation, bound by reading the
+// cache.
+//
+// Rows: a workgroup takes 16 MB rows of one sequence and one kv head (row r: query
+// r / group, head r % group), so that one pass over the cache serves the whole group of
+// heads, and one range of keys (split_keys of them); its four waves take steps of 32 keys in
+// turn, each with a running maximum and sum of its own, and are joined at the end in LDS.
+// The ranges are joined by a second launch, if there is more than one.
+//
+// Products (16x16x32, fp32 sums) run transposed as in the tile kernel: S^T = K Q^T with the
+// keys' fragments loaded straight from the cache into registers (a lane's 16 bytes are one
+// fragment; 8-bit codes are two, the head's elements then taken in another order by both
+// operands), O^T = V^T P^T with V through a stretch of LDS that only this wave uses, and
+// transposing reads.  Each step's loads start when the step before has used its registers.
+#pragma once
+
+#include "attention_common.h"
+
+namespace cmpext3 {
+
+template <int HD, int MB>
+struct FewShape {
+  static constexpr int BM = 16 * MB;
+  static constexpr int V_BYTES = kWaveKeys * HD * 2;
+  static constexpr int WAVE = V_BYTES + 2 * kWaveKeys * 4;  // V, then the scales of K and V
+  static constexpr int PITCH = HD + 4;                      // floats of a row of O in LDS
+  static constexpr int JOIN = kFewWaves * BM * PITCH * 4;
+  static constexpr int ML = kFewWaves * BM * 2 * 4;
+  static constexpr int LDS = (WAVE * kFewWaves > JOIN ? WAVE * kFewWaves : JOIN) + ML;
+};
+
+// Byte offset of byte column `bc` of V's row `row`: a transposing read by 32 lanes covers
+// eight rows of 32 bytes, which fall on all banks once.
+template <int HD>
+__device__ __forceinline__ int few_v_place(int row, int bc) {
+  if constexpr (HD == 64)
+    return row * 128 + (((bc >> 5) ^ ((row >> 1) & 3)) << 5) + (bc & 31);
+  else
+    return row * HD * 2 + (((bc >> 6) ^ (row & 3)) << 6) + ((bc & 63) ^ (((row >> 2) & 1) << 5));
+}
+
+template <typename T, int HD, int KIND, int MB>
+__global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_few_kernel(const AttnParams p) {
+  constexpr bool k8 = KIND == kKvPaged8;
+  using S = FewShape<HD, MB>;
+  constexpr int KK = HD / 32, DB = HD / 16;
+  constexpr int EPP = k8 ? 16 : 8, ES = k8 ? 1 : 2;
+  constexpr int KN = HD / (4 * EPP);              // 16-byte loads of a lane for a block of 16 keys
+  constexpr int PPR = HD / EPP, VN = kWaveKeys * PPR / 64;
+  __shared__ __attribute__((aligned(16))) unsigned char smem[S::LDS];
+
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, G = lane >> 4;
+  const int kvh = blockIdx.x % p.kv_heads;
+  const Seq sq = seq_of_slot(p, blockIdx.x / p.kv_heads, S::BM);
+  if (sq.b < 0) return;
+  const int split = blockIdx.y;
+  const int shift = sq.len_k - sq.len_q;
+  const int row0 = sq.tile * S::BM, rows = sq.len_q * p.group;
+  int end = sq.len_k;
+  if (p.causal) end = min(end, (min(row0 + S::BM, rows) - 1) / p.group + shift + 1);
+  const int begin = split * p.split_keys;
+  end = min(end, begin + p.split_keys);
+  if (begin >= sq.len_k && split > 0) return;  // this split has no keys: the join knows
+
+  // keys up to `all` are seen by every row of the tile
+  const int all = p.causal ? min(row0 / p.group + shift, sq.len_k - 1) : sq.len_k - 1;
+  int limit[MB];
+  u32x4 q[MB][KK];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    const int row = row0 + 16 * mb + r16;
+    const int tok = min(row, rows - 1) / p.group, head = kvh * p.group + min(row, rows - 1) - tok * p.group;
+    limit[mb] = p.causal ? min(tok + shift, sq.len_k - 1) : sq.len_k - 1;
+    const T* qp = (const T*)p.q + sq.b * p.q_batch + (int64_t)(sq.q0 + tok) * p.q_token + (int64_t)head * p.q_head;
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) {
+      const int d = k8 ? 64 * (kk / 2) + 16 * G + 8 * (kk & 1) : 32 * kk + 8 * G;
+      q[mb][kk] = row < rows && d < p.dim ? *(const u32x4*)(qp + d) : u32x4{0, 0, 0, 0};
+    }
+  }
+
+  unsigned char* vs = smem + wave * S::WAVE;
+  float* sc = (float*)(vs + S::V_BYTES);
+  const int32_t* table = p.kv.table + sq.b * p.kv.table_row;
+  const uint8_t* kc = (const uint8_t*)p.kv.k + (int64_t)kvh * p.kv.k_head * ES;
+  const uint8_t* vc = (const uint8_t*)p.kv.v + (int64_t)kvh * p.kv.v_head * ES;
+
+  u32x4 kr[2][KN], vr[VN];
+  float sr = 0.f;
+  // 16 bytes at element d of a row (8 where the head ends in the middle of 16 codes)
+  auto piece = [&](const uint8_t* at, int d) -> u32x4 {
+    if (k8 && d + 8 >= p.dim) {
+      const u32x2 h = *(const u32x2*)(at + d);
+      return u32x4{h.x, h.y, 0, 0};
+    }
+    return *(const u32x4_a8*)(at + d * ES);
+  };
+  auto load = [&](int key0) {
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      const int key = key0 + 16 * b + r16;
+      int place, page = -1;
+      if (key < sq.len_k) page = page_of(p.kv, table, key, place);
+#pragma unroll
+      for (int i = 0; i < KN; ++i) {
+        const int d = 4 * EPP * i + EPP * G;
+        kr[b][i] = u32x4{0, 0, 0, 0};
+        if (page >= 0 && d < p.dim) kr[b][i] = piece(kc + (page * p.kv.k_page + place * p.kv.k_token) * ES, d);
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int n = i * 64 + lane, key = key0 + n / PPR, d = (n % PPR) * EPP;
+      int place, page = -1;
+      if (key < sq.len_k) page = page_of(p.kv, table, key, place);
+      vr[i] = u32x4{0, 0, 0, 0};
+      if (page >= 0 && d < p.dim) vr[i] = piece(vc + (page * p.kv.v_page + place * p.kv.v_token) * ES, d);
+    }
+    if constexpr (k8) {
+      const int key = key0 + (lane & 31);
+      int place, page = -1;
+      if (key < sq.len_k) page = page_of(p.kv, table, key, place);
+      sr = 0.f;
+      if (page >= 0)
+        sr = lane < 32 ? p.kv.k_scale[page * p.kv.ks_page + place * p.kv.ks_token + kvh * p.kv.ks_head] * p.scale_log2
+                       : p.kv.v_scale[page * p.kv.vs_page + place * p.kv.vs_token + kvh * p.kv.vs_head];
+    }
+  };
+
+  f32x4 o[MB][DB];
+  float m_ref[MB], sum[MB];
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    m_ref[mb] = -INFINITY;
+    sum[mb] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) o[mb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const float unit = k8 ? 1.f : p.scale_log2;
+
+  int key0 = begin + wave * kWaveKeys;
+  if (key0 < end) load(key0);
+  for (; key0 < end; key0 += kFewWaves * kWaveKeys) {
+    // V into this wave's LDS
+#pragma unroll
+    for (int i = 0; i < VN; ++i) {
+      const int n = i * 64 + lane, r = n / PPR, c = (n % PPR) * EPP * 2;
+      if constexpr (k8) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const u32x2 a = e4m3x4<T>(vr[i][2 * h]), b = e4m3x4<T>(vr[i][2 * h + 1]);
+          *(u32x4*)(vs + few_v_place<HD>(r, c + 16 * h)) = u32x4{a.x, a.y, b.x, b.y};
+        }
+      } else {
+        *(u32x4*)(vs + few_v_place<HD>(r, c)) = vr[i];
+      }
+    }
+    if constexpr (k8) sc[lane] = sr;
+    f32x4 s[MB][2];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) s[mb][0] = s[mb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int kk = 0; kk < KK; ++kk) {
+        u32x4 k;
+        if constexpr (k8) {
+          const u32x2 lo = e4m3x4<T>(kr[b][kk / 2][2 * (kk & 1)]), hi = e4m3x4<T>(kr[b][kk / 2][2 * (kk & 1) + 1]);
+          k = u32x4{lo.x, lo.y, hi.x, hi.y};
+        } else {
+          k = kr[b][kk];
+        }
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) s[mb][b] = Mfma<T>::mma(k, q[mb][kk], s[mb][b]);
+      }
+    if (key0 + kFewWaves * kWaveKeys < end) load(key0 + kFewWaves * kWaveKeys);
+    f32x4 ksc[2], vsc[2];
+    if constexpr (k8) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        ksc[b] = *(const f32x4*)(sc + 16 * b + 4 * G);
+        vsc[b] = *(const f32x4*)(sc + 32 + 16 * b + 4 * G);
+      }
+    }
+    u32x4 pw[MB];
+#pragma unroll
+    for (int mb = 0; mb < MB; ++mb) {
+      float mx = -INFINITY;
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int key = key0 + 16 * b + 4 * G + i;
+          float x = s[mb][b][i];
+          if constexpr (k8) x *= ksc[b][i];
+          x = key <= limit[mb] && key < end ? x : -INFINITY;
+          s[mb][b][i] = x;
+          mx = fmaxf(mx, x);
+        }
+      mx = fmaxf(mx, __shfl_xor(mx, 16));
+      mx = fmaxf(mx, __shfl_xor(mx, 32));
+      const float m_new = fmaxf(m_ref[mb], mx);
+      if (__builtin_amdgcn_ballot_w64(m_new != m_ref[mb])) {
+        const float alpha = m_new == m_ref[mb] ? 1.f : exp2_hw((m_ref[mb] - m_new) * unit);
+        m_ref[mb] = m_new;
+        sum[mb] *= alpha;
+#pragma unroll
+        for (int d = 0; d < DB; ++d) o[mb][d] *= alpha;
+      }
+      const float base = m_ref[mb] == -INFINITY ? 0.f : m_ref[mb] * unit;
+      float w[8];
+#pragma unroll
+      for (int b = 0; b < 2; ++b)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float x = exp2_hw(k8 ? s[mb][b][i] - base : __builtin_fmaf(s[mb][b][i], unit, -base));
+          sum[mb] += x;
+          w[4 * b + i] = k8 ? x * vsc[b][i] : x;
+        }
+      pw[mb] = u32x4{pack2<T>(w[0], w[1]), pack2<T>(w[2], w[3]), pack2<T>(w[4], w[5]), pack2<T>(w[6], w[7])};
+    }
+    auto v_frag = [&](int d) {
+      const int row = 4 * G + (r16 >> 2), bc = 2 * (16 * d + 4 * (r16 & 3));
+      const u32x2 lo = lds_read_tr(vs + few_v_place<HD>(row, bc));
+      const u32x2 hi = lds_read_tr(vs + few_v_place<HD>(row + 16, bc));
+      return u32x4{lo.x, lo.y, hi.x, hi.y};
+    };
+    if (key0 + kWaveKeys - 1 > all && any_not_finite<T>(vs, S::V_BYTES)) {
+#pragma unroll 1
+      for (int kind = -1; kind < 3; ++kind)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          const u32x4 v = kind < 0 ? finite_only<T>(v_frag(d)) : kind_ones<T>(v_frag(d), kind);
+#pragma unroll
+          for (int mb = 0; mb < MB; ++mb) {
+            if (kind < 0) {
+              o[mb][d] = Mfma<T>::mma(v, pw[mb], o[mb][d]);
+            } else {
+              const f32x4 hit = Mfma<T>::mma(v, pw[mb], f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[mb][d][i] += hit[i] > 0.f ? kind_value(kind) : 0.f;
+            }
+          }
+        }
+    } else {
+#pragma unroll
+      for (int d = 0; d < DB; ++d) {
+        const u32x4 v = v_frag(d);
+#pragma unroll
+        for (int mb = 0; mb < MB; ++mb) o[mb][d] = Mfma<T>::mma(v, pw[mb], o[mb][d]);
+      }
+    }
+  }
+
+  // ---- join the waves ----
+  float* ml = (float*)(smem + S::LDS - S::ML);  // [wave][row][2]
+  __syncthreads();                              // every wave is done with its stretch of LDS
+#pragma unroll
+  for (int mb = 0; mb < MB; ++mb) {
+    sum[mb] += __shfl_xor(sum[mb], 16);
+    sum[mb] += __shfl_xor(sum[mb], 32);
+    const int r = 16 * mb + r16;
+    if (G == 0) {
+      ml[(wave * S::BM + r) * 2] = m_ref[mb] * unit;
+      ml[(wave * S::BM + r) * 2 + 1] = sum[mb];
+    }
+    float* po = (float*)smem + (wave * S::BM + r) * S::PITCH;
+#pragma unroll
+    for (int d = 0; d < DB; ++d) *(f32x4*)(po + 16 * d + 4 * G) = o[mb][d];
+  }
+  __syncthreads();
+  constexpr int QUADS = HD / 4;
+  for (int n = tid; n < S::BM * QUADS; n += 64 * kFewWaves) {
+    const int r = n / QUADS, e = (n % QUADS) * 4, row = row0 + r;
+    if (row >= rows || e >= p.dim) continue;
+    float m = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < kFewWaves; ++w) m = fmaxf(m, ml[(w * S::BM + r) * 2]);
+    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
+    float l = 0.f;
+    if (m != -INFINITY) {
+#pragma unroll
+      for (int w = 0; w < kFewWaves; ++w) {
+        const float f = exp2_hw(ml[(w * S::BM + r) * 2] - m);
+        l += f * ml[(w * S::BM + r) * 2 + 1];
+        acc += f * *(const f32x4*)((const float*)smem + (w * S::BM + r) * S::PITCH + e);
+      }
+    }
+    const int tok = row / p.group, head = kvh * p.group + row - tok * p.group;
+    if (p.splits > 1) {
+      const int64_t at = (int64_t)split * p.rows + ((int64_t)sq.b * (p.starts_q ? 0 : p.len_q) + sq.q0 + tok) * p.heads + head;
+      *(f32x4*)(p.part_o + at * p.dim + e) = acc;
+      if (e == 0) {
+        p.part_ml[2 * at] = m;
+        p.part_ml[2 * at + 1] = l;
+      }
+    } else {
+      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
+      *(u32x2*)(op + e) = u32x2{pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)};
+    }
+  }
+}
+
+template <typename T, int KIND, int MB>
+hipError_t launch_few_hd(int hd, const AttnParams& p, dim3 grid, hipStream_t s) {
+  const dim3 block(64 * kFewWaves);
+  if (hd == 64) return launch_kernel(attention_few_kernel<T, 64, KIND, MB>, grid, block, 0, s, p);
+  if (hd == 128) return launch_kernel(attention_few_kernel<T, 128, KIND, MB>, grid, block, 0, s, p);
+  return launch_kernel(attention_few_kernel<T, 256, KIND, MB>, grid, block, 0, s, p);
+}
+
+}  // namespace cmpext3

@@ -14,6 +14,7 @@
 #include <vector>
 
 #include "../../include/cmpext3_gemm.h"
+#include "attention_ops.h"
 
 namespace {
 
@@ -379,5 +380,6 @@ PYBIND11_MODULE(_cmpext3, m) {
   m.def("last_plan", &last_plan,
         "Describe the kernel(s) the last operator call on this thread ran (its actual pointers, pitches and "
         "workspace)");
+  register_attention_ops(m);
   m.def("version", []() { return std::string(cmpext3_version()); });
 }
