@@ -122,7 +122,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     return CMPEXT3_OK;
   }
   const int64_t mean_rows = queries * group / a->batch;  // of a sequence and kv head
-  r.blocks16 = paged && mean_rows <= 32 ? (mean_rows <= 16 ? 1 : 2) : 0;
+  r.blocks16 = paged && mean_rows <= 32 ? (mean_rows <= 16 || r.hd == 256 ? 1 : 2) : 0;
   const int bm = r.blocks16 ? 16 * r.blocks16 : 128;
   const int64_t slots = uniform_q ? (int64_t)a->batch * (((int64_t)a->len_q * group + bm - 1) / bm)
                                   : queries * group / bm + a->batch;
@@ -130,8 +130,8 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   p.slots = (int)slots;
   // Split the keys where the row tiles alone leave CUs idle.
   const int64_t groups = slots * c.kv_heads;
-  const int64_t want = r.blocks16 ? 2048 : 512;
-  const int least = r.blocks16 ? 256 : 512;
+  const int64_t want = r.blocks16 ? 1024 : 512;
+  const int least = 512;
   if (groups < want && keys > least && (paged || uniform_k || a->batch == 1)) {
     const int64_t n = std::min<int64_t>((want + groups - 1) / groups, 1024);
     const int64_t per = std::max<int64_t>(least, ((keys + n - 1) / n + 127) / 128 * 128);

@@ -83,10 +83,15 @@ __device__ __forceinline__ int page_of(const KvSource& kv, const int32_t* table,
 // Four e4m3 codes (one dword) as four values of T: exact, both types hold every code.
 template <typename T>
 __device__ __forceinline__ u32x2 e4m3x4(uint32_t c) {
-  typedef float f32x2 __attribute__((ext_vector_type(2)));
-  const f32x2 lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, false);
-  const f32x2 hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)c, true);
-  return u32x2{pack2<T>(lo[0], lo[1]), pack2<T>(hi[0], hi[1])};
+  u32x2 r;
+  if constexpr (std::is_same<T, _Float16>::value) {
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(c, 1.0f, true));
+  } else {
+    r.x = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, false));
+    r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, true));
+  }
+  return r;
 }
 
 // 2^x, the hardware's (relative error about 2^-23; 0 for -infinity).
@@ -104,10 +109,10 @@ __device__ __forceinline__ u32x2 lds_read_tr(const unsigned char* q) {
 // ---- values of V that are not finite, at keys that only some rows see ----
 // A product adds 0 * v for a masked key, which is NaN where v is infinite or NaN: a row would
 // get a value it does not see.  Steps in which some row sees only part of the keys therefore
-// look V over first (any_not_finite), and in the rare step that holds such a value take the
-// products with those values as zeros and add them apart, to the rows whose weights for them
-// are not zero (kind_ones: 1 at +infinity, -infinity or NaN, whose products with the weights
-// are positive exactly there).
+// look V over first (any_not_finite); in the rare step that holds such a value they are made
+// zeros, and when all keys are done a second pass over those steps adds them to the rows that
+// see them: kind_ones has 1 where V holds +infinity, -infinity or NaN, and its product with the
+// rows' seen keys is positive exactly there.
 template <typename T>
 constexpr uint32_t kExponents = std::is_same<T, _Float16>::value ? 0x7C007C00u : 0x7F807F80u;
 
@@ -152,6 +157,12 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
   for (int j = 0; j < 4; ++j)
     r[j] = ((v[j] & e) == e ? 0u : v[j] & 0xFFFFu) | ((v[j] >> 16 & e) == e ? 0u : v[j] & 0xFFFF0000u);
   return r;
+}
+// Two 16-bit ones, for keys `key` and `key` + 1 up to `limit`.
+template <typename T>
+__device__ __forceinline__ uint32_t ones_up_to(int key, int limit) {
+  constexpr uint32_t one = std::is_same<T, _Float16>::value ? 0x3C00u : 0x3F80u;
+  return (key <= limit ? one : 0u) | (key < limit ? one << 16 : 0u);
 }
 
 }  // namespace cmpext3

@@ -11,7 +11,10 @@
 // keys' fragments loaded straight from the cache into registers (a lane's 16 bytes are one
 // fragment; 8-bit codes are two, the head's elements then taken in another order by both
 // operands), O^T = V^T P^T with V through a stretch of LDS that only this wave uses, and
-// transposing reads.  Each step's loads start when the step before has used its registers.
+// transposing reads.  Each step's loads start when the step before has used its registers, and
+// its page numbers, one per lane, are fetched another step ahead.  A weight is taken as the sum
+// of two 16-bit numbers (the second product twice): there is time for it under the loads, and
+// the result is then off by its own rounding only.
 #pragma once
 
 #include "attention_common.h"
@@ -22,7 +25,8 @@ template <int HD, int MB>
 struct FewShape {
   static constexpr int BM = 16 * MB;
   static constexpr int V_BYTES = kWaveKeys * HD * 2;
-  static constexpr int WAVE = V_BYTES + 2 * kWaveKeys * 4;  // V, then the scales of K and V
+  // V, the scales of K and V, the byte offsets of the keys' and values' rows in the cache
+  static constexpr int WAVE = V_BYTES + 2 * kWaveKeys * 4 + 2 * kWaveKeys * 8;
   static constexpr int PITCH = HD + 4;                      // floats of a row of O in LDS
   static constexpr int JOIN = kFewWaves * BM * PITCH * 4;
   static constexpr int ML = kFewWaves * BM * 2 * 4;
@@ -84,9 +88,23 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   unsigned char* vs = smem + wave * S::WAVE;
   float* sc = (float*)(vs + S::V_BYTES);
   const int32_t* table = p.kv.table + sq.b * p.kv.table_row;
-  const uint8_t* kc = (const uint8_t*)p.kv.k + (int64_t)kvh * p.kv.k_head * ES;
-  const uint8_t* vc = (const uint8_t*)p.kv.v + (int64_t)kvh * p.kv.v_head * ES;
+  const uint8_t* kc = (const uint8_t*)p.kv.k;
+  const uint8_t* vc = (const uint8_t*)p.kv.v;
 
+  // ---- loads of a step: lane l < 32 looks after key l's row of K, lane 32 + l after V's ----
+  int64_t* row_at = (int64_t*)(sc + 2 * kWaveKeys);
+  const bool value = lane >= kWaveKeys;
+  const int64_t c_page = value ? p.kv.v_page : p.kv.k_page, c_token = value ? p.kv.v_token : p.kv.k_token;
+  const int64_t c_head = kvh * (value ? p.kv.v_head : p.kv.k_head);
+  const float* c_scale = k8 ? (value ? p.kv.v_scale + kvh * p.kv.vs_head : p.kv.k_scale + kvh * p.kv.ks_head) : nullptr;
+  const int64_t s_page = value ? p.kv.vs_page : p.kv.ks_page, s_token = value ? p.kv.vs_token : p.kv.ks_token;
+  const int my_key = lane & (kWaveKeys - 1);
+  // the page of this lane's key of a step, -1 past the sequence; fetched a step ahead
+  auto page_number = [&](int key0) -> int {
+    const int key = key0 + my_key;
+    if (key >= sq.len_k) return -1;
+    return table[p.kv.page_shift >= 0 ? key >> p.kv.page_shift : key / p.kv.page_size];
+  };
   u32x4 kr[2][KN], vr[VN];
   float sr = 0.f;
   // 16 bytes at element d of a row (8 where the head ends in the middle of 16 codes)
@@ -97,35 +115,45 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
     }
     return *(const u32x4_a8*)(at + d * ES);
   };
-  auto load = [&](int key0) {
-#pragma unroll
-    for (int b = 0; b < 2; ++b) {
-      const int key = key0 + 16 * b + r16;
-      int place, page = -1;
-      if (key < sq.len_k) page = page_of(p.kv, table, key, place);
-#pragma unroll
-      for (int i = 0; i < KN; ++i) {
-        const int d = 4 * EPP * i + EPP * G;
-        kr[b][i] = u32x4{0, 0, 0, 0};
-        if (page >= 0 && d < p.dim) kr[b][i] = piece(kc + (page * p.kv.k_page + place * p.kv.k_token) * ES, d);
-      }
-    }
-#pragma unroll
-    for (int i = 0; i < VN; ++i) {
-      const int n = i * 64 + lane, key = key0 + n / PPR, d = (n % PPR) * EPP;
-      int place, page = -1;
-      if (key < sq.len_k) page = page_of(p.kv, table, key, place);
-      vr[i] = u32x4{0, 0, 0, 0};
-      if (page >= 0 && d < p.dim) vr[i] = piece(vc + (page * p.kv.v_page + place * p.kv.v_token) * ES, d);
-    }
+  auto load = [&](int key0, int page) {
+    const int key = key0 + my_key;
+    const int place = p.kv.page_shift >= 0 ? key & (p.kv.page_size - 1) : key % p.kv.page_size;
+    const bool there = (unsigned)page < (unsigned)p.kv.pages;
+    row_at[lane] = there ? (page * c_page + place * c_token + c_head) * ES : -1;
     if constexpr (k8) {
-      const int key = key0 + (lane & 31);
-      int place, page = -1;
-      if (key < sq.len_k) page = page_of(p.kv, table, key, place);
       sr = 0.f;
-      if (page >= 0)
-        sr = lane < 32 ? p.kv.k_scale[page * p.kv.ks_page + place * p.kv.ks_token + kvh * p.kv.ks_head] * p.scale_log2
-                       : p.kv.v_scale[page * p.kv.vs_page + place * p.kv.vs_token + kvh * p.kv.vs_head];
+      if (there) sr = c_scale[page * s_page + place * s_token];
+    }
+    if (__builtin_amdgcn_ballot_w64(!there) == 0 && p.dim == HD) {
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const uint8_t* at = kc + row_at[16 * b + r16];
+#pragma unroll
+        for (int i = 0; i < KN; ++i) kr[b][i] = *(const u32x4_a8*)(at + (4 * EPP * i + EPP * G) * ES);
+      }
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        const int n = i * 64 + lane;
+        vr[i] = *(const u32x4_a8*)(vc + row_at[kWaveKeys + n / PPR] + (n % PPR) * EPP * ES);
+      }
+    } else {  // rows that are not there, and what lies past the head, are zeros
+#pragma unroll
+      for (int b = 0; b < 2; ++b) {
+        const int64_t at = row_at[16 * b + r16];
+#pragma unroll
+        for (int i = 0; i < KN; ++i) {
+          const int d = 4 * EPP * i + EPP * G;
+          kr[b][i] = u32x4{0, 0, 0, 0};
+          if (at >= 0 && d < p.dim) kr[b][i] = piece(kc + at, d);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < VN; ++i) {
+        const int n = i * 64 + lane, d = (n % PPR) * EPP;
+        const int64_t at = row_at[kWaveKeys + n / PPR];
+        vr[i] = u32x4{0, 0, 0, 0};
+        if (at >= 0 && d < p.dim) vr[i] = piece(vc + at, d);
+      }
     }
   };
 
@@ -140,10 +168,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   }
   const float unit = k8 ? 1.f : p.scale_log2;
 
-  int key0 = begin + wave * kWaveKeys;
-  if (key0 < end) load(key0);
-  for (; key0 < end; key0 += kFewWaves * kWaveKeys) {
-    // V into this wave's LDS
+  // V of a step into this wave's LDS, and its fragments from there: keys 4 G .. and 16 + 4 G ..
+  auto store_v = [&]() {
 #pragma unroll
     for (int i = 0; i < VN; ++i) {
       const int n = i * 64 + lane, r = n / PPR, c = (n % PPR) * EPP * 2;
@@ -157,7 +183,26 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
         *(u32x4*)(vs + few_v_place<HD>(r, c)) = vr[i];
       }
     }
+  };
+  auto v_frag = [&](int d) {
+    const int row = 4 * G + (r16 >> 2), bc = 2 * (16 * d + 4 * (r16 & 3));
+    const u32x2 lo = lds_read_tr(vs + few_v_place<HD>(row, bc));
+    const u32x2 hi = lds_read_tr(vs + few_v_place<HD>(row + 16, bc));
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
+
+  constexpr int STEP = kFewWaves * kWaveKeys;
+  bool spoilt = false;
+  int key0 = begin + wave * kWaveKeys;
+  int page = -1;
+  if (key0 < end) {
+    load(key0, page_number(key0));
+    page = page_number(key0 + STEP);
+  }
+  for (; key0 < end; key0 += STEP) {
+    store_v();
     if constexpr (k8) sc[lane] = sr;
+    __builtin_amdgcn_sched_barrier(0);  // V's registers are free
     f32x4 s[MB][2];
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) s[mb][0] = s[mb][1] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -175,7 +220,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) s[mb][b] = Mfma<T>::mma(k, q[mb][kk], s[mb][b]);
       }
-    if (key0 + kFewWaves * kWaveKeys < end) load(key0 + kFewWaves * kWaveKeys);
+    __builtin_amdgcn_sched_barrier(0);  // and K's
+    if (key0 + STEP < end) {
+      load(key0 + STEP, page);
+      page = page_number(key0 + 2 * STEP);
+    }
     f32x4 ksc[2], vsc[2];
     if constexpr (k8) {
 #pragma unroll
@@ -184,7 +233,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
         vsc[b] = *(const f32x4*)(sc + 32 + 16 * b + 4 * G);
       }
     }
-    u32x4 pw[MB];
+    u32x4 pw[MB], pl[MB];  // weights, and what their rounding left
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       float mx = -INFINITY;
@@ -194,7 +243,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
         for (int i = 0; i < 4; ++i) {
           const int key = key0 + 16 * b + 4 * G + i;
           float x = s[mb][b][i];
-          if constexpr (k8) x *= ksc[b][i];
+          if constexpr (k8) x *= ksc[b][i] * p.scale_log2;
           x = key <= limit[mb] && key < end ? x : -INFINITY;
           s[mb][b][i] = x;
           mx = fmaxf(mx, x);
@@ -219,38 +268,42 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
           sum[mb] += x;
           w[4 * b + i] = k8 ? x * vsc[b][i] : x;
         }
-      pw[mb] = u32x4{pack2<T>(w[0], w[1]), pack2<T>(w[2], w[3]), pack2<T>(w[4], w[5]), pack2<T>(w[6], w[7])};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        pw[mb][i] = pack2<T>(w[2 * i], w[2 * i + 1]);
+        pl[mb][i] = pack2<T>(w[2 * i] - from_bits<T>((uint16_t)pw[mb][i]), w[2 * i + 1] - from_bits<T>((uint16_t)(pw[mb][i] >> 16)));
+      }
     }
-    auto v_frag = [&](int d) {
-      const int row = 4 * G + (r16 >> 2), bc = 2 * (16 * d + 4 * (r16 & 3));
-      const u32x2 lo = lds_read_tr(vs + few_v_place<HD>(row, bc));
-      const u32x2 hi = lds_read_tr(vs + few_v_place<HD>(row + 16, bc));
-      return u32x4{lo.x, lo.y, hi.x, hi.y};
-    };
     if (key0 + kWaveKeys - 1 > all && any_not_finite<T>(vs, S::V_BYTES)) {
-#pragma unroll 1
-      for (int kind = -1; kind < 3; ++kind)
+      spoilt = true;
+      for (int i = 16 * lane; i < S::V_BYTES; i += 1024) *(u32x4*)(vs + i) = finite_only<T>(*(const u32x4*)(vs + i));
+    }
 #pragma unroll
-        for (int d = 0; d < DB; ++d) {
-          const u32x4 v = kind < 0 ? finite_only<T>(v_frag(d)) : kind_ones<T>(v_frag(d), kind);
+    for (int d = 0; d < DB; ++d) {
+      const u32x4 v = v_frag(d);
 #pragma unroll
-          for (int mb = 0; mb < MB; ++mb) {
-            if (kind < 0) {
-              o[mb][d] = Mfma<T>::mma(v, pw[mb], o[mb][d]);
-            } else {
-              const f32x4 hit = Mfma<T>::mma(v, pw[mb], f32x4{0.f, 0.f, 0.f, 0.f});
+      for (int mb = 0; mb < MB; ++mb) o[mb][d] = Mfma<T>::mma(v, pl[mb], Mfma<T>::mma(v, pw[mb], o[mb][d]));
+      if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+  }
+  if (spoilt) {  // add what was made zero (see any_not_finite)
+    for (key0 = begin + wave * kWaveKeys; key0 < end; key0 += STEP) {
+      if (key0 + kWaveKeys - 1 <= all) continue;
+      load(key0, page_number(key0));
+      store_v();
+      for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
-              for (int i = 0; i < 4; ++i) o[mb][d][i] += hit[i] > 0.f ? kind_value(kind) : 0.f;
-            }
+        for (int mb = 0; mb < MB; ++mb) {
+          const int key = key0 + 4 * G, most = min(limit[mb], end - 1);
+          const u32x4 seen = {ones_up_to<T>(key, most), ones_up_to<T>(key + 2, most), ones_up_to<T>(key + 16, most),
+                              ones_up_to<T>(key + 18, most)};
+#pragma unroll
+          for (int d = 0; d < DB; ++d) {
+            const f32x4 hit = Mfma<T>::mma(kind_ones<T>(v_frag(d), kind), seen, f32x4{0.f, 0.f, 0.f, 0.f});
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[mb][d][i] += hit[i] > 0.f ? kind_value(kind) : 0.f;
           }
         }
-    } else {
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-        const u32x4 v = v_frag(d);
-#pragma unroll
-        for (int mb = 0; mb < MB; ++mb) o[mb][d] = Mfma<T>::mma(v, pw[mb], o[mb][d]);
-      }
     }
   }
 
@@ -309,7 +362,8 @@ hipError_t launch_few_hd(int hd, const AttnParams& p, dim3 grid, hipStream_t s) 
   const dim3 block(64 * kFewWaves);
   if (hd == 64) return launch_kernel(attention_few_kernel<T, 64, KIND, MB>, grid, block, 0, s, p);
   if (hd == 128) return launch_kernel(attention_few_kernel<T, 128, KIND, MB>, grid, block, 0, s, p);
-  return launch_kernel(attention_few_kernel<T, 256, KIND, MB>, grid, block, 0, s, p);
+  if constexpr (MB == 1) return launch_kernel(attention_few_kernel<T, 256, KIND, MB>, grid, block, 0, s, p);
+  return hipErrorInvalidValue;  // heads over 128 take 16 rows: two blocks' sums do not fit the registers
 }
 
 }  // namespace cmpext3

@@ -243,6 +243,11 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
   for (int d = 0; d < DB; ++d)
     v_at[d] = S::BYTES + v_place<HD>(4 * half + ((lane & 15) >> 2), 2 * (32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)));
 
+  auto v_frag = [&](const unsigned char* slot, int g, int d) {
+    const u32x2 lo = lds_read_tr(slot + v_at[d] + 16 * g * S::ROW);
+    const u32x2 hi = lds_read_tr(slot + v_at[d] + (16 * g + 8) * S::ROW);
+    return u32x4{lo.x, lo.y, hi.x, hi.y};
+  };
   // masked: some row of the wave does not see all 64 keys
   auto compute = [&](int key0, int slot, bool masked) {
     const unsigned char* ks = smem + slot * S::SLOT;
@@ -306,35 +311,17 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
         }
         pw[2 * b + r / 8][(r % 8) / 2] = pack2<T>(w0, w1);
       }
-    auto v_frag = [&](int g, int d) {
-      const u32x2 lo = lds_read_tr(ks + v_at[d] + 16 * g * S::ROW);
-      const u32x2 hi = lds_read_tr(ks + v_at[d] + (16 * g + 8) * S::ROW);
-      return u32x4{lo.x, lo.y, hi.x, hi.y};
-    };
-    if (masked && any_not_finite<T>(ks + S::BYTES, S::BYTES)) {
-#pragma unroll
-      for (int d = 0; d < DB; ++d) {
-#pragma unroll
-        for (int g = 0; g < 4; ++g) o[d] = Mfma32<T>::mma(finite_only<T>(v_frag(g, d)), pw[g], o[d]);
-#pragma unroll 1
-        for (int kind = 0; kind < 3; ++kind) {
-          f32x16 hit = f32x16{0};
-#pragma unroll
-          for (int g = 0; g < 4; ++g) hit = Mfma32<T>::mma(kind_ones<T>(v_frag(g, d), kind), pw[g], hit);
-#pragma unroll
-          for (int r = 0; r < 16; ++r) o[d][r] += hit[r] > 0.f ? kind_value(kind) : 0.f;
-        }
-      }
-      return;
-    }
 #pragma unroll
     for (int g = 0; g < 4; ++g) {
 #pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = Mfma32<T>::mma(v_frag(g, d), pw[g], o[d]);
+      for (int d = 0; d < DB; ++d) o[d] = Mfma32<T>::mma(v_frag(ks, g, d), pw[g], o[d]);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
 
+  // keys that all rows of the workgroup see
+  const int tile_all = p.causal ? min(row0 / p.group + shift, last) : last;
+  bool spoilt = false;
   if (begin < end) {
     load(begin, 0);
     store(0);
@@ -342,9 +329,42 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
     for (int key0 = begin; key0 < end; key0 += kTileKeys) {
       ring_fence<0>();  // this step's keys and values are in LDS, and the other slot is read
       if (key0 + kTileKeys < end) load(key0 + kTileKeys, slot ^ 1);
+      if (key0 + kTileKeys - 1 > tile_all) {
+        unsigned char* vs = smem + slot * S::SLOT + S::BYTES;
+        if (any_not_finite<T>(vs, S::BYTES)) {  // all waves find the same
+          spoilt = true;
+          __syncthreads();
+          for (int i = 16 * tid; i < S::BYTES; i += 16 * 64 * NW) *(u32x4*)(vs + i) = finite_only<T>(*(const u32x4*)(vs + i));
+          __syncthreads();
+        }
+      }
       if (key0 <= wave_any) compute(key0, slot, key0 + kTileKeys - 1 > wave_all);
       if (key0 + kTileKeys < end) store(slot ^ 1);
       slot ^= 1;
+    }
+  }
+
+  if (spoilt) {  // add what was made zero (see any_not_finite)
+    for (int key0 = begin; key0 < end; key0 += kTileKeys) {
+      if (key0 + kTileKeys - 1 <= tile_all) continue;
+      ring_fence<0>();  // slot 0 is read
+      load(key0, 0);
+      store(0);
+      ring_fence<0>();
+      for (int kind = 0; kind < 3; ++kind)
+#pragma unroll
+        for (int d = 0; d < DB; ++d) {
+          f32x16 hit = f32x16{0};
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const int key = key0 + 16 * g + 4 * half;
+            const u32x4 seen = {ones_up_to<T>(key, limit), ones_up_to<T>(key + 2, limit), ones_up_to<T>(key + 8, limit),
+                                ones_up_to<T>(key + 10, limit)};
+            hit = Mfma32<T>::mma(kind_ones<T>(v_frag(smem, g, d), kind), seen, hit);
+          }
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] += hit[r] > 0.f ? kind_value(kind) : 0.f;
+        }
     }
   }
 
