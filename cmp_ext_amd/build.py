@@ -45,6 +45,16 @@ HIP_FLAGS = [
     "-I" + CSRC,
     "-I" + os.path.join(ROOT, "include"),
 ]
+# The attention tile kernels use all 512 registers of a lane (or 256 of two waves): scores, which
+# the vector unit reads, belong in its registers, and only what is left over goes to the other half.
+# Without the option every product's sums live there and each score is moved first.
+TILE_FLAGS = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
+
+
+def hip_flags(source: str) -> list[str]:
+    return HIP_FLAGS + (TILE_FLAGS if source.startswith("attention_tile_") else [])
+
+
 HOST_FLAGS = [
     "-O2", "-std=c++17", "-fPIC", "-Wall",
     "-D__HIP_PLATFORM_AMD__=1",
@@ -70,7 +80,7 @@ def build_library(jobs: int) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     cmds = []
     for s in HIP_SOURCES:
-        cmds.append([HIPCC, *HIP_FLAGS, "-c", os.path.join(CSRC, s), "-o", _obj(s)])
+        cmds.append([HIPCC, *hip_flags(s), "-c", os.path.join(CSRC, s), "-o", _obj(s)])
     for s in HOST_SOURCES:
         cmds.append(["g++", *HOST_FLAGS, "-c", os.path.join(CSRC, s), "-o", _obj(s)])
     with ThreadPoolExecutor(max_workers=jobs) as ex:

@@ -5,12 +5,13 @@
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <stdlib.h>
 
 #include <algorithm>
 
 #include "../../include/cmpext3_attention.h"
 #include "attention_params.h"
-#include "gemm_params.h"
+#include "kernels.h"
 
 using namespace cmpext3;
 
@@ -59,6 +60,7 @@ struct AttnPlan {
   KvKind kind;
   int hd;        // padded head
   int blocks16;  // few-rows kernel: its tiles of 16 rows; 0: tile kernel
+  int rows;      // of a workgroup
   bool empty;
   int64_t ws_bytes;
 };
@@ -112,7 +114,6 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   p.batch = a->batch, p.heads = a->heads, p.kv_heads = c.kv_heads, p.group = group, p.dim = c.dim;
   p.causal = a->causal != 0;
   p.scale_log2 = a->scale * 1.4426950408889634f;
-  p.rows = queries * a->heads;
   r.kind = !paged ? kKvPacked : c.kv_dtype == CMPEXT3_E4M3 ? kKvPaged8 : kKvPaged16;
   r.hd = c.dim <= 64 ? 64 : c.dim <= 128 ? 128 : 256;
   p.splits = 1;
@@ -123,23 +124,23 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   }
   const int64_t mean_rows = queries * group / a->batch;  // of a sequence and kv head
   r.blocks16 = paged && mean_rows <= 32 ? (mean_rows <= 16 || r.hd == 256 ? 1 : 2) : 0;
-  const int bm = r.blocks16 ? 16 * r.blocks16 : 128;
+  const int bm = r.rows = r.blocks16 ? 16 * r.blocks16 : 128;
   const int64_t slots = uniform_q ? (int64_t)a->batch * (((int64_t)a->len_q * group + bm - 1) / bm)
                                   : queries * group / bm + a->batch;
   if (slots * c.kv_heads > kMostGrid) return CMPEXT3_ERR_TOO_LARGE;
   p.slots = (int)slots;
   // Split the keys where the row tiles alone leave CUs idle.
   const int64_t groups = slots * c.kv_heads;
-  const int64_t want = r.blocks16 ? 1024 : 512;
-  const int least = 512;
+  const int64_t want = getenv("AW") ? atoi(getenv("AW")) : r.blocks16 ? 2048 : 512;
+  const int least = getenv("AL") ? atoi(getenv("AL")) : r.blocks16 ? 256 : 512;
   if (groups < want && keys > least && (paged || uniform_k || a->batch == 1)) {
-    const int64_t n = std::min<int64_t>((want + groups - 1) / groups, 1024);
+    const int64_t n = std::min<int64_t>((want + groups - 1) / groups, most_splits(bm));
     const int64_t per = std::max<int64_t>(least, ((keys + n - 1) / n + 127) / 128 * 128);
     const int64_t splits = (keys + per - 1) / per;
     if (splits > 1) {
       p.splits = (int)splits;
       p.split_keys = (int)per;
-      r.ws_bytes = splits * p.rows * (c.dim + 2) * 4;
+      r.ws_bytes = groups * splits * bm * (c.dim + 2) * 4;
     }
   }
   *out = r;
@@ -177,13 +178,14 @@ extern "C" int cmpext3_attention(const cmpext3_attention_args* args, void* works
   if (st != CMPEXT3_OK || r.empty) return st;
   if (r.ws_bytes > 0) {
     if (workspace == nullptr || workspace_bytes < r.ws_bytes || !aligned(workspace, 16)) return CMPEXT3_ERR_WORKSPACE;
-    r.p.part_o = (float*)workspace;
-    r.p.part_ml = r.p.part_o + (int64_t)r.p.splits * r.p.rows * r.p.dim;
+    r.p.part = (float*)workspace;
+    r.p.sem = split_counters((hipStream_t)stream, (int64_t)r.p.slots * r.p.kv_heads);
   }
   const dim3 grid((unsigned)((int64_t)r.p.slots * r.p.kv_heads), (unsigned)r.p.splits);
   hipError_t e = r.blocks16 ? launch_few_kernel(args->dtype, r, grid, (hipStream_t)stream)
                             : launch_tile_kernel(args->dtype, r, grid, (hipStream_t)stream);
-  if (e == hipSuccess && r.p.splits > 1) e = launch_attention_join(args->dtype, r.p, (hipStream_t)stream);
+  if (e == hipSuccess && r.p.splits > 1 && r.p.sem == nullptr)
+    e = launch_attention_join(args->dtype, r.rows, r.p, (hipStream_t)stream);
   return (int)e;
 }
 
@@ -197,7 +199,7 @@ extern "C" int cmpext3_attention_describe(const cmpext3_attention_args* args, ch
       snprintf(buf, (size_t)buflen, "kernel=none");
     else
       snprintf(buf, (size_t)buflen, "kernel=%s rows=%d keys=%s head=%d slots=%d splits=%d split_keys=%d",
-               r.blocks16 ? "attention_few" : "attention_tile", r.blocks16 ? 16 * r.blocks16 : 128, kinds[r.kind], r.hd,
+               r.blocks16 ? "attention_few" : "attention_tile", r.rows, kinds[r.kind], r.hd,
                r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0);
   }
   return CMPEXT3_OK;

@@ -12,57 +12,87 @@ struct Seq {
   int b;           // -1: none
   int q0, len_q;   // first row in the packed queries, number of queries
   int k0, len_k;
-  int tile;        // row tile of the sequence
+  int tile;        // row tile of the sequence (or query, seq_of_slot)
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
 
-// Row tile `slot` of the grid: which sequence, and which of its tiles of `rows` rows (a row
-// is one query of one head of the group).  With packed queries, sequence b owns the slots
-// from starts_q[b] * group / rows + b on: these grow by at least one per sequence and by
-// no less than its tiles, so the grid needs no lengths from the host; slots past a
-// sequence's last tile have nothing to do (b = -1).  64 starts are compared at once.
+// Keys of a paged sequence: its length, as far as the table goes.
+__device__ __forceinline__ int paged_keys(const AttnParams& p, int seq_len) {
+  return (int)min((int64_t)max(seq_len, 0), (int64_t)p.kv.table_pages * p.kv.page_size);
+}
+
+// The sequence that holds row tile `slot` of the grid (rows > 0), or, with rows = 0, the packed
+// query `slot`; and which of its tiles of `rows` rows it is (a row is one query of one head of
+// the group).  With packed queries, sequence b owns the slots from starts_q[b] * group / rows + b
+// on: these grow by at least one per sequence and by no less than its tiles, so the grid needs no
+// lengths from the host; slots past a sequence's last tile have nothing to do (b = -1).  Each lane
+// looks at one sequence, 64 at a time, and loads all that is known of it at once: what follows
+// waits for one memory access, not for three in a row.
 __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int rows) {
   Seq s;
+  int start_k = 0, end_k = p.len_k;  // or, paged, the length as end_k
   if (p.starts_q == nullptr) {
-    const int tiles = (p.len_q * p.group + rows - 1) / rows;
+    const int tiles = rows > 0 ? (p.len_q * p.group + rows - 1) / rows : p.len_q;
     s.b = slot / tiles;
     s.tile = slot - s.b * tiles;
     s.q0 = 0;
     s.len_q = p.len_q;
+    if (p.kv.table != nullptr) {
+      end_k = p.seq_lens[s.b];
+    } else if (p.starts_k != nullptr) {
+      start_k = p.starts_k[s.b];
+      end_k = p.starts_k[s.b + 1];
+    }
   } else {
     const int lane = threadIdx.x & 63;
-    int count = 0;
+    int at = -1, first = 0, q_from = 0, q_to = 0, k_from = 0, k_to = 0;
     for (int b0 = 0; b0 < p.batch; b0 += 64) {
-      const int b = b0 + lane;
-      const bool below = b < p.batch && clampi(p.starts_q[b], 0, p.total_q) * p.group / rows + b <= slot;
+      const int b = min(b0 + lane, p.batch - 1);
+      const int from = p.starts_q[b], to = p.starts_q[b + 1];
+      int kf = 0, kt = p.len_k;
+      if (p.kv.table != nullptr) {
+        kt = p.seq_lens[b];
+      } else if (p.starts_k != nullptr) {
+        kf = p.starts_k[b];
+        kt = p.starts_k[b + 1];
+      }
+      const int q = clampi(from, 0, p.total_q);
+      const bool below = b0 + lane < p.batch && (rows > 0 ? q * p.group / rows + b : q) <= slot;
       const unsigned long long m = __builtin_amdgcn_ballot_w64(below);
-      count += __builtin_popcountll(m);
-      if (m != ~0ull) break;
+      const int n = __builtin_popcountll(m);
+      if (n > 0) {
+        at = n - 1;
+        first = b0;
+        q_from = q, q_to = to, k_from = kf, k_to = kt;
+      }
+      if (n < 64) break;
     }
-    s.b = count - 1;
-    if (s.b < 0) return s;
-    s.q0 = clampi(p.starts_q[s.b], 0, p.total_q);
-    s.len_q = clampi(p.starts_q[s.b + 1], s.q0, p.total_q) - s.q0;
-    s.tile = slot - (s.q0 * p.group / rows + s.b);
+    s.b = -1;
+    if (at < 0) return s;
+    s.b = first + at;
+    s.q0 = __builtin_amdgcn_readlane(q_from, at);
+    s.len_q = clampi(__builtin_amdgcn_readlane(q_to, at), s.q0, p.total_q) - s.q0;
+    s.tile = rows > 0 ? slot - (s.q0 * p.group / rows + s.b) : slot - s.q0;
+    start_k = __builtin_amdgcn_readlane(k_from, at);
+    end_k = __builtin_amdgcn_readlane(k_to, at);
   }
   s.b = __builtin_amdgcn_readfirstlane(s.b);  // all of it is the workgroup's: scalar registers
   s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
   s.len_q = __builtin_amdgcn_readfirstlane(s.len_q);
   s.tile = __builtin_amdgcn_readfirstlane(s.tile);
-  const int tiles = (s.len_q * p.group + rows - 1) / rows;
+  const int tiles = rows > 0 ? (s.len_q * p.group + rows - 1) / rows : s.len_q;
   if (s.tile < 0 || s.tile >= tiles) {
     s.b = -1;
     return s;
   }
-  s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
+  if (rows > 0) s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
   if (p.kv.table != nullptr) {
     s.k0 = 0;
-    const int64_t most = (int64_t)p.kv.table_pages * p.kv.page_size;
-    s.len_k = (int)min((int64_t)max(p.seq_lens[s.b], 0), most);
+    s.len_k = paged_keys(p, end_k);
   } else if (p.starts_k != nullptr) {
-    s.k0 = clampi(p.starts_k[s.b], 0, p.total_k);
-    s.len_k = clampi(p.starts_k[s.b + 1], s.k0, p.total_k) - s.k0;
+    s.k0 = clampi(start_k, 0, p.total_k);
+    s.len_k = clampi(end_k, s.k0, p.total_k) - s.k0;
   } else {
     s.k0 = 0;
     s.len_k = p.len_k;
@@ -70,6 +100,11 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
   s.k0 = __builtin_amdgcn_readfirstlane(s.k0);
   s.len_k = __builtin_amdgcn_readfirstlane(s.len_k);
   return s;
+}
+
+// Keys that the sequence's row `row`, and all before it, may see end here.
+__device__ __forceinline__ int keys_end(const AttnParams& p, const Seq& s, int row) {
+  return p.causal ? min(s.len_k, row / p.group + s.len_k - s.len_q + 1) : s.len_k;
 }
 
 // The page of key `key` and its place in the page; -1 where the table names no page of the cache.
@@ -92,6 +127,24 @@ __device__ __forceinline__ u32x2 e4m3x4(uint32_t c) {
     r.y = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, true));
   }
   return r;
+}
+
+// Two floats rounded to nearest even, as one instruction.
+template <typename T>
+__device__ __forceinline__ uint32_t round2(float lo, float hi) {
+  typedef float f32x2 __attribute__((ext_vector_type(2)));
+  typedef T t2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), t2));
+}
+
+// The larger of two, NaN if one is: two of them are one instruction of three operands, while
+// fmaxf takes another to quiet each operand (the row is NaN in the end either way).
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+
+// The larger of x in this lane and in lane ^ 32.
+__device__ __forceinline__ float max_halves(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
 // 2^x, the hardware's (relative error about 2^-23; 0 for -infinity).

@@ -5,7 +5,7 @@
 // r / group, head r % group), so that one pass over the cache serves the whole group of
 // heads, and one range of keys (split_keys of them); its four waves take steps of 32 keys in
 // turn, each with a running maximum and sum of its own, and are joined at the end in LDS.
-// The ranges are joined by a second launch, if there is more than one.
+// The ranges are joined as attention_join.h says, if there is more than one.
 //
 // Products (16x16x32, fp32 sums) run transposed as in the tile kernel: S^T = K Q^T with the
 // keys' fragments loaded straight from the cache into registers (a lane's 16 bytes are one
@@ -17,7 +17,7 @@
 // the result is then off by its own rounding only.
 #pragma once
 
-#include "attention_common.h"
+#include "attention_join.h"
 
 namespace cmpext3 {
 
@@ -30,7 +30,9 @@ struct FewShape {
   static constexpr int PITCH = HD + 4;                      // floats of a row of O in LDS
   static constexpr int JOIN = kFewWaves * BM * PITCH * 4;
   static constexpr int ML = kFewWaves * BM * 2 * 4;
-  static constexpr int LDS = (WAVE * kFewWaves > JOIN ? WAVE * kFewWaves : JOIN) + ML;
+  static constexpr int SPLITS = 8 * BM * most_splits(BM);
+  static constexpr int BODY = WAVE * kFewWaves > JOIN ? WAVE * kFewWaves : JOIN;
+  static constexpr int LDS = BODY + ML > SPLITS ? BODY + ML : SPLITS;
 };
 
 // Byte offset of byte column `bc` of V's row `row`: a transposing read by 32 lanes covers
@@ -44,7 +46,7 @@ __device__ __forceinline__ int few_v_place(int row, int bc) {
 }
 
 template <typename T, int HD, int KIND, int MB>
-__global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_few_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : HD == 64 ? 4 : KIND == kKvPaged8 ? 3 : 2) attention_few_kernel(const AttnParams p) {
   constexpr bool k8 = KIND == kKvPaged8;
   using S = FewShape<HD, MB>;
   constexpr int KK = HD / 32, DB = HD / 16;
@@ -62,11 +64,11 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   const int split = blockIdx.y;
   const int shift = sq.len_k - sq.len_q;
   const int row0 = sq.tile * S::BM, rows = sq.len_q * p.group;
-  int end = sq.len_k;
-  if (p.causal) end = min(end, (min(row0 + S::BM, rows) - 1) / p.group + shift + 1);
+  int end = keys_end(p, sq, min(row0 + S::BM, rows) - 1);
+  const int splits = splits_of(p, end);
+  if (split >= splits) return;
   const int begin = split * p.split_keys;
   end = min(end, begin + p.split_keys);
-  if (begin >= sq.len_k && split > 0) return;  // this split has no keys: the join knows
 
   // keys up to `all` are seen by every row of the tile
   const int all = p.causal ? min(row0 / p.group + shift, sq.len_k - 1) : sq.len_k - 1;
@@ -99,11 +101,10 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   const float* c_scale = k8 ? (value ? p.kv.v_scale + kvh * p.kv.vs_head : p.kv.k_scale + kvh * p.kv.ks_head) : nullptr;
   const int64_t s_page = value ? p.kv.vs_page : p.kv.ks_page, s_token = value ? p.kv.vs_token : p.kv.ks_token;
   const int my_key = lane & (kWaveKeys - 1);
-  // the page of this lane's key of a step, -1 past the sequence; fetched a step ahead
+  // the page of this lane's key of a step, as far as the table goes; fetched a step ahead
   auto page_number = [&](int key0) -> int {
-    const int key = key0 + my_key;
-    if (key >= sq.len_k) return -1;
-    return table[p.kv.page_shift >= 0 ? key >> p.kv.page_shift : key / p.kv.page_size];
+    const int key = key0 + my_key, n = p.kv.page_shift >= 0 ? key >> p.kv.page_shift : key / p.kv.page_size;
+    return n < p.kv.table_pages ? table[n] : -1;
   };
   u32x4 kr[2][KN], vr[VN];
   float sr = 0.f;
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   auto load = [&](int key0, int page) {
     const int key = key0 + my_key;
     const int place = p.kv.page_shift >= 0 ? key & (p.kv.page_size - 1) : key % p.kv.page_size;
-    const bool there = (unsigned)page < (unsigned)p.kv.pages;
+    const bool there = key < sq.len_k && (unsigned)page < (unsigned)p.kv.pages;
     row_at[lane] = there ? (page * c_page + place * c_token + c_head) * ES : -1;
     if constexpr (k8) {
       sr = 0.f;
@@ -270,8 +271,8 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
         }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        pw[mb][i] = pack2<T>(w[2 * i], w[2 * i + 1]);
-        pl[mb][i] = pack2<T>(w[2 * i] - from_bits<T>((uint16_t)pw[mb][i]), w[2 * i + 1] - from_bits<T>((uint16_t)(pw[mb][i] >> 16)));
+        pw[mb][i] = round2<T>(w[2 * i], w[2 * i + 1]);
+        pl[mb][i] = round2<T>(w[2 * i] - from_bits<T>((uint16_t)pw[mb][i]), w[2 * i + 1] - from_bits<T>((uint16_t)(pw[mb][i] >> 16)));
       }
     }
     if (key0 + kWaveKeys - 1 > all && any_not_finite<T>(vs, S::V_BYTES)) {
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   }
 
   // ---- join the waves ----
-  float* ml = (float*)(smem + S::LDS - S::ML);  // [wave][row][2]
+  float* ml = (float*)(smem + S::BODY);         // [wave][row][2]
   __syncthreads();                              // every wave is done with its stretch of LDS
 #pragma unroll
   for (int mb = 0; mb < MB; ++mb) {
@@ -325,6 +326,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
   }
   __syncthreads();
   constexpr int QUADS = HD / 4;
+  float* part = part_of_tile(p, S::BM);
   for (int n = tid; n < S::BM * QUADS; n += 64 * kFewWaves) {
     const int r = n / QUADS, e = (n % QUADS) * 4, row = row0 + r;
     if (row >= rows || e >= p.dim) continue;
@@ -341,20 +343,17 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD <= 128 ? 2 : 1) attention_f
         acc += f * *(const f32x4*)((const float*)smem + (w * S::BM + r) * S::PITCH + e);
       }
     }
-    const int tok = row / p.group, head = kvh * p.group + row - tok * p.group;
-    if (p.splits > 1) {
-      const int64_t at = (int64_t)split * p.rows + ((int64_t)sq.b * (p.starts_q ? 0 : p.len_q) + sq.q0 + tok) * p.heads + head;
-      *(f32x4*)(p.part_o + at * p.dim + e) = acc;
-      if (e == 0) {
-        p.part_ml[2 * at] = m;
-        p.part_ml[2 * at + 1] = l;
-      }
+    if (splits > 1) {
+      store16_coherent(part, part_at(p, S::BM, split) + part_o(p, r) + 4 * e, acc);
+      if (e == 0) store8_coherent(part, part_at(p, S::BM, split) + part_ml(p, S::BM, r), m, l);
     } else {
+      const int tok = row / p.group, head = kvh * p.group + row - tok * p.group;
       const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
       T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
-      *(u32x2*)(op + e) = u32x2{pack2<T>(acc[0] * inv, acc[1] * inv), pack2<T>(acc[2] * inv, acc[3] * inv)};
+      *(u32x2*)(op + e) = u32x2{round2<T>(acc[0] * inv, acc[1] * inv), round2<T>(acc[2] * inv, acc[3] * inv)};
     }
   }
+  if (splits > 1) join_if_last<T>(p, sq, kvh, row0, min(S::BM, rows - row0), part, S::BM, splits, smem);
 }
 
 template <typename T, int KIND, int MB>

@@ -14,6 +14,11 @@ constexpr int kTileKeys = 64;
 constexpr int kWaveKeys = 32;
 constexpr int kFewWaves = 4;
 
+// LDS of the second phase of split keys, 8 bytes for each row and split of a tile: so many splits
+// at most.
+constexpr int kJoinBytes = 32 * 1024;
+constexpr int most_splits(int rows_of_tile) { return kJoinBytes / 8 / rows_of_tile; }
+
 // Keys and values: packed rows, or pages.
 struct KvSource {
   const void* k;
@@ -42,12 +47,10 @@ struct AttnParams {
   int causal;
   float scale_log2;  // scale * log2(e): the softmax runs on powers of two
   int slots;         // row tiles of the grid, for all sequences (see tile_of_slot)
-  // split keys: split s of a sequence covers its keys [s * split_keys, (s + 1) * split_keys);
-  // part_o[(s * rows + row) * dim], part_ml[(s * rows + row) * 2] with row = token * heads + head
+  // split keys: split s of a sequence covers its keys [s * split_keys, (s + 1) * split_keys)
   int splits, split_keys;
-  int64_t rows;
-  float* part_o;
-  float* part_ml;
+  float* part;        // sums of the splits (attention_join.h)
+  unsigned int* sem;  // counters of the row tiles, or nullptr: joined by a second launch
 };
 
 // hd: 64, 128 or 256, the head padded (dim <= hd).  grid: slots * kv_heads, splits.
@@ -62,7 +65,8 @@ hipError_t launch_attention_few_f16_paged16(int hd, int blocks16, const AttnPara
 hipError_t launch_attention_few_f16_paged8(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_attention_few_bf16_paged16(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_attention_few_bf16_paged8(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_join(int dtype, const AttnParams& p, hipStream_t s);
+// bm: rows of a row tile.
+hipError_t launch_attention_join(int dtype, int bm, const AttnParams& p, hipStream_t s);
 
 struct RopeParams {
   const void* x[2];  // queries, keys

@@ -1,10 +1,11 @@
 // Attention over many query rows (gfx950): O = softmax(scale Q K^T) V in one pass over the
 // keys with the running maximum and sum of the softmax.
 //
-// Rows: a workgroup takes NW x 32 rows of one sequence and one kv head, a row being one
-// query of one head of the group (row r: query r / group, head r % group), so that grouped
-// heads share each step's keys and values and short sequences fill their tiles.  A wave owns
-// 32 rows.
+// Rows: a workgroup of four waves takes 128 rows of one sequence and one kv head, a row being one
+// query of one head of the group (row r: query r / group, head r % group), so that grouped heads
+// share each step's keys and values and short sequences fill their tiles.  A wave owns 32 rows.
+// (8192 tokens, 32 heads of 128 on MI355X: 520 us; eight waves over 256 rows, whose barriers bind
+// all waves of a CU together, 550; four waves of 64 rows with a SIMD to themselves 643.)
 //
 // Products (32x32x16, fp32 sums) run transposed: S^T = K Q^T gives lane l the scores of row
 // l % 32 only (keys 8 (r / 4) + 4 (l / 32) + r % 4 of a block of 32), so the maximum, sum and
@@ -16,30 +17,41 @@
 // The maximum a row subtracts is only raised when a score exceeds it by more than 2^8
 // (kLazy): the sums stay far from overflow and the accumulators are rarely rescaled.
 //
-// Keys and values of a step (64 keys) lie in LDS as rows of HD 16-bit elements in one of two
-// slots, K with its 16-byte chunks and V with its 64-byte segments permuted by the row so
-// that the reads of both products hit all banks.  Packed ones come by LDS DMA, which zero
-// fills what lies past the sequence or the head; pages are read into registers (any page
-// size, 8-bit codes converted on the way) and stored.  One barrier a step: the next step's
-// loads start behind it, into the slot the step before has read.
+// Pipeline: step j (64 keys) has two phases, each a sequence of slots of one matrix product with
+// a share of the vector work, kept in that order: the scores of step j + 1 beside the first
+// weights of step j, then the weighted values of step j beside its other weights and the maximum
+// of step j + 1.  The vector work (per score: scale, exponential at half the rate, sum, half a
+// conversion, half a maximum) is over half as long as the products.
+//
+// Keys and values of a step lie in LDS as rows of HD 16-bit elements in rings of NS slots, K
+// with its 16-byte chunks and V with its 64-byte segments permuted by the row so that the reads
+// of both products hit all banks.  Packed ones come by LDS DMA, which zero fills what lies past
+// the sequence or the head; pages go through registers (any page size, 8-bit codes converted on
+// the way), their rows' addresses shared through LDS and their page numbers fetched steps ahead.
+// One barrier a step: K of step j + NS and V of step j + NS - 1 start to load behind it, into the
+// slots that the step before has read.
 #pragma once
 
-#include "attention_common.h"
+#include "attention_join.h"
 
 namespace cmpext3 {
 
 constexpr float kLazy = 8.0f;  // in powers of two
 
-template <int HD, int NW, bool PAGED>
+constexpr int kTileWaves = 4;
+
+template <int HD, bool PAGED, int NS>
 struct TileShape {
-  static constexpr int BM = 32 * NW;
-  static constexpr int ROW = HD * 2;              // bytes of a key's row in LDS
-  static constexpr int BYTES = kTileKeys * ROW;   // K or V of a step
-  static constexpr int SLOT = 2 * BYTES;
-  static constexpr int SCALES = 2 * kTileKeys * 4;  // 8-bit: the step's scales of K and V
-  static constexpr int LDS = 2 * SLOT + (PAGED ? 2 * SCALES : 0);
-  static constexpr int DMA = BYTES / 1024 / NW;  // 1 KB LDS-DMA loads per wave of K, and of V
-  static_assert(BYTES % (1024 * NW) == 0, "whole DMA loads per wave");
+  static constexpr int ROW = HD * 2;             // bytes of a key's row in LDS
+  static constexpr int BYTES = kTileKeys * ROW;  // K or V of a step
+  static constexpr int V0 = NS * BYTES;          // K's slots, then V's
+  static constexpr int ROWS_AT = 2 * NS * BYTES;    // paged: byte offsets of the rows of K and V, two steps'
+  static constexpr int SCALES = ROWS_AT + 2 * 2 * kTileKeys * 8;  // 8 bits: scales of K and V, four steps'
+  static constexpr int LDS = PAGED ? SCALES + 4 * 2 * kTileKeys * 4 : ROWS_AT;
+  static constexpr int DMA = BYTES / 1024 / kTileWaves;  // 1 KB LDS-DMA loads per wave of K, and of V
+  static_assert(BYTES % (1024 * kTileWaves) == 0, "whole DMA loads per wave");
+  static_assert(LDS <= 160 * 1024 && LDS >= 8 * 128 * most_splits(128), "LDS budget");
+  static_assert(!PAGED || NS == 2, "pages are loaded one step ahead");
 };
 
 // Byte offset in a K slot of the 16-byte chunk `chunk` of row `row`: 16 rows at one chunk
@@ -61,11 +73,12 @@ __device__ __forceinline__ int v_place(int row, int byte_col) {
   return row * HD * 2 + (((byte_col >> 6) ^ x) << 6) + (byte_col & 63);
 }
 
-template <typename T, int HD, int KIND, int NW>
-__global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_tile_kernel(const AttnParams p) {
+// Two waves share a SIMD's registers (packed heads up to 64: three; over 128: one has them all).
+template <typename T, int HD, int KIND, int NS>
+__global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && KIND == kKvPacked ? 3 : 2) attention_tile_kernel(const AttnParams p) {
   constexpr bool kPaged = KIND != kKvPacked, k8 = KIND == kKvPaged8;
-  using S = TileShape<HD, NW, kPaged>;
-  constexpr int KK = HD / 16, DB = HD / 32;
+  using S = TileShape<HD, kPaged, NS>;
+  constexpr int KK = HD / 16, DB = HD / 32, NW = kTileWaves, BM = 32 * NW;
   __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
 
   const int tid = threadIdx.x, lane = tid & 63;
@@ -74,263 +87,360 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
 
   // heads fastest: the workgroups of one kv head meet in the L2 of few XCDs
   const int kvh = blockIdx.x % p.kv_heads;
-  Seq sq = seq_of_slot(p, blockIdx.x / p.kv_heads, S::BM);
+  const Seq sq = seq_of_slot(p, blockIdx.x / p.kv_heads, BM);
   if (sq.b < 0) return;
   const int split = blockIdx.y;
   const int shift = sq.len_k - sq.len_q;  // causal: query i sees keys up to i + shift
-  const int row0 = sq.tile * S::BM, rows = sq.len_q * p.group;
-  // keys any row of the tile sees
-  const int last_q = min(row0 + S::BM, rows) - 1;
-  int end = sq.len_k;
-  if (p.causal) end = min(end, last_q / p.group + shift + 1);
+  const int row0 = sq.tile * BM, rows = sq.len_q * p.group;
+  int end = keys_end(p, sq, min(row0 + BM, rows) - 1);  // of the keys any row of the tile sees
+  const int splits = splits_of(p, end);
+  if (split >= splits) return;
   const int begin = split * p.split_keys;
   end = min(end, begin + p.split_keys);
-  if (p.splits > 1 && begin >= sq.len_k && split > 0) return;  // this split has no keys: the join knows
+  const int steps = end > begin ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
 
   // ---- this lane's row ----
-  const int row = row0 + wave * 32 + col;
-  const bool live = row < rows;
-  const int tok = min(row, rows - 1) / p.group;
-  const int head = kvh * p.group + (min(row, rows - 1) - tok * p.group);
   const int last = min(sq.len_k, end) - 1;  // keys past `end` are another split's
-  const int limit = p.causal ? min(tok + shift, last) : last;  // its last key
-  const int wtok0 = min(row0 + wave * 32, rows - 1) / p.group;
-  const int wtok1 = min(row0 + wave * 32 + 31, rows - 1) / p.group;
-  // keys that all rows of the wave see, and that any of them sees
-  const int wave_all = __builtin_amdgcn_readfirstlane(p.causal ? min(wtok0 + shift, last) : last);
-  const int wave_any = __builtin_amdgcn_readfirstlane(
-      row0 + wave * 32 < rows ? (p.causal ? min(wtok1 + shift, last) : last) : -1);
-
+  const int wrow0 = row0 + wave * 32, row = wrow0 + col;
+  const int tok = min(row, rows - 1) / p.group, head = kvh * p.group + min(row, rows - 1) - tok * p.group;
+  const int limit = p.causal ? min(tok + shift, last) : last;  // the last key it sees
   u32x4 q[KK];
   {
     const T* qp = (const T*)p.q + sq.b * p.q_batch + (int64_t)(sq.q0 + tok) * p.q_token + (int64_t)head * p.q_head;
 #pragma unroll
     for (int kk = 0; kk < KK; ++kk) {
       const int d = 16 * kk + 8 * half;
-      q[kk] = live && d < p.dim ? *(const u32x4*)(qp + d) : u32x4{0, 0, 0, 0};
+      q[kk] = row < rows && d < p.dim ? *(const u32x4*)(qp + d) : u32x4{0, 0, 0, 0};
     }
   }
+  // keys that all rows of the wave see, and that any of them sees; that all rows of the tile see
+  const int wave_all = __builtin_amdgcn_readfirstlane(p.causal ? min(min(wrow0, rows - 1) / p.group + shift, last) : last);
+  const int wave_any = __builtin_amdgcn_readfirstlane(
+      wrow0 < rows ? (p.causal ? min((min(wrow0 + 32, rows) - 1) / p.group + shift, last) : last) : -1);
+  const int tile_all = p.causal ? min(row0 / p.group + shift, last) : last;
 
-  // ---- loads of a step ----
-  const int32_t* table = kPaged ? p.kv.table + sq.b * p.kv.table_row : nullptr;
+  // ---- loads: K or V of a step into a slot ----
+  // packed: LDS-DMA loads i of this wave; where lane's 16 bytes of load i come from
   const T* kbase = nullptr;
   const T* vbase = nullptr;
   uint32_t k_off[kPaged ? 1 : S::DMA], v_off[kPaged ? 1 : S::DMA];
-  int k_row[kPaged ? 1 : S::DMA], v_row[kPaged ? 1 : S::DMA];
+  constexpr int ROWS1K = 1024 / S::ROW;  // rows of a DMA load
+  const int dma_row = wave * S::DMA * ROWS1K + 16 * lane / S::ROW;
   if constexpr (!kPaged) {
     kbase = (const T*)p.kv.k + sq.b * p.kv.k_page + (int64_t)sq.k0 * p.kv.k_token + (int64_t)kvh * p.kv.k_head;
     vbase = (const T*)p.kv.v + sq.b * p.kv.v_page + (int64_t)sq.k0 * p.kv.v_token + (int64_t)kvh * p.kv.v_head;
 #pragma unroll
     for (int i = 0; i < S::DMA; ++i) {
-      const int pos = (wave * S::DMA + i) * 1024 + 16 * lane;
+      const int row = dma_row + i * ROWS1K, at = 16 * lane % S::ROW;  // bytes into the row's place
       int c;
-      if constexpr (HD == 64) {
-        const int pr = pos >> 8, c16 = (pos & 255) >> 4;
-        k_row[i] = 2 * pr + (c16 >> 3);
-        c = (c16 ^ pr) & 7;
-      } else {
-        k_row[i] = pos / S::ROW;
-        const int c16 = (pos % S::ROW) >> 4;
-        c = (c16 & ~15) | ((c16 ^ k_row[i]) & 15);
-      }
-      k_off[i] = 8 * c < p.dim ? (uint32_t)(k_row[i] * (int)p.kv.k_token + 8 * c) * 2u : kBufOOB;
-      v_row[i] = pos / S::ROW;
-      const int x = HD == 64 ? (v_row[i] >> 1) & 1 : v_row[i] & 3;
-      const int bc = ((((pos % S::ROW) >> 6) ^ x) << 6) + (pos & 63);
-      v_off[i] = bc < 2 * p.dim ? (uint32_t)(v_row[i] * (int)p.kv.v_token * 2 + bc) : kBufOOB;
+      if constexpr (HD == 64)
+        c = ((at >> 4) ^ (row >> 1)) & 7;
+      else
+        c = ((at >> 4) & ~15) | (((at >> 4) ^ row) & 15);
+      k_off[i] = 8 * c < p.dim ? (uint32_t)(row * (int)p.kv.k_token + 8 * c) * 2u : kBufOOB;
+      const int x = HD == 64 ? (row >> 1) & 1 : row & 3;
+      const int bc = (((at >> 6) ^ x) << 6) + (at & 63);
+      v_off[i] = bc < 2 * p.dim ? (uint32_t)(row * (int)p.kv.v_token * 2 + bc) : kBufOOB;
     }
   }
-  // paged: 16-byte pieces of a step, in the order of the cache
-  constexpr int EPP = k8 ? 16 : 8;                                // elements of a piece
-  constexpr int PIECES = kTileKeys * HD / EPP / (64 * NW);        // per thread, of K and of V
-  constexpr int PPR = HD / EPP;                                   // pieces of a row
-  u32x4 kreg[kPaged ? PIECES : 1], vreg[kPaged ? PIECES : 1];
-  float sreg = 0.f;
-  auto load = [&](int key0, int slot) {
-    if constexpr (!kPaged) {
-      const int left = sq.len_k - key0;
-      const i32x4 kr = make_rsrc_sgpr(kbase + (int64_t)key0 * p.kv.k_token);
-      const i32x4 vr = make_rsrc_sgpr(vbase + (int64_t)key0 * p.kv.v_token);
-      const uint32_t dst = lds_addr(smem) + (uint32_t)(slot * S::SLOT + wave * S::DMA * 1024);
+  const uint32_t lds0 = lds_addr(smem) + (uint32_t)(wave * S::DMA * 1024);
+  // K or V of the step from key0 into a slot, zeros past the sequence and of steps past the last
+  auto dma = [&](bool value, int step, int slot) {
+    const int key0 = begin + step * kTileKeys;
+    const i32x4 r = make_rsrc_sgpr(value ? vbase + (int64_t)key0 * p.kv.v_token : kbase + (int64_t)key0 * p.kv.k_token);
+    const uint32_t dst = lds0 + (uint32_t)((value ? S::V0 : 0) + slot * S::BYTES);
+    const int left = step < steps ? sq.len_k - key0 : 0;
+    if (left >= kTileKeys) {
       static_for<S::DMA>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        dma_load16_m0(kr, k_row[i] < left ? k_off[i] : kBufOOB, 0, dst,
+        dma_load16_m0(r, value ? v_off[i] : k_off[i], 0, dst, std::integral_constant<uint32_t, i * 1024>{});
+      });
+    } else {
+      static_for<S::DMA>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        dma_load16_m0(r, dma_row + i * ROWS1K < left ? (value ? v_off[i] : k_off[i]) : kBufOOB, 0, dst,
                       std::integral_constant<uint32_t, i * 1024>{});
       });
-      static_for<S::DMA>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        dma_load16_m0(vr, v_row[i] < left ? v_off[i] : kBufOOB, 0, dst,
-                      std::integral_constant<uint32_t, S::BYTES + i * 1024>{});
-      });
+    }
+  };
+  // paged: thread t < 64 looks after row t of a step of K, thread 64 + t after one of V: finds its
+  // page, its byte offset in the cache (rows_at[step % 2][t], -1: zeros) and its scale
+  constexpr int EPP = k8 ? 16 : 8, ES = k8 ? 1 : 2;         // elements of a 16-byte piece, bytes of an element
+  constexpr int PIECES = kTileKeys * HD / EPP / (64 * NW);  // pieces a thread loads of K, and of V
+  constexpr int PPR = HD / EPP;                             // pieces of a row
+  int64_t* rows_at = (int64_t*)(smem + S::ROWS_AT);
+  float* scales = (float*)(smem + S::SCALES);  // [step % 4][K, V][64]
+  const int32_t* table = kPaged ? p.kv.table + sq.b * p.kv.table_row : nullptr;
+  const bool value_row = tid >= kTileKeys;
+  u32x4 reg[kPaged ? PIECES : 1];  // of K in a step's first phase, of V in its second
+  float sreg = 0.f;
+  auto page_number = [&](int key) -> int {  // of this thread's row
+    if (tid >= 2 * kTileKeys || key >= sq.len_k) return -1;
+    return table[p.kv.page_shift >= 0 ? key >> p.kv.page_shift : key / p.kv.page_size];
+  };
+  auto place_row = [&](int at, int key, int page) {
+    if (tid >= 2 * kTileKeys) return;
+    const int place = p.kv.page_shift >= 0 ? key & (p.kv.page_size - 1) : key % p.kv.page_size;
+    const bool there = (unsigned)page < (unsigned)p.kv.pages;
+    const int64_t o = value_row ? page * p.kv.v_page + place * p.kv.v_token + kvh * p.kv.v_head
+                                : page * p.kv.k_page + place * p.kv.k_token + kvh * p.kv.k_head;
+    rows_at[at * 2 * kTileKeys + tid] = there ? o * ES : -1;
+    if constexpr (k8) {
+      sreg = 0.f;
+      if (there)
+        sreg = value_row ? p.kv.v_scale[page * p.kv.vs_page + place * p.kv.vs_token + kvh * p.kv.vs_head]
+                         : p.kv.k_scale[page * p.kv.ks_page + place * p.kv.ks_token + kvh * p.kv.ks_head] * p.scale_log2;
+    }
+  };
+  auto store_scale = [&](int step_k, int step_v) {
+    if (k8 && tid < 2 * kTileKeys) scales[((value_row ? step_v : step_k) & 3) * 2 * kTileKeys + tid] = sreg;
+  };
+  auto load_pieces = [&](bool value, int at) {
+    const uint8_t* base = (const uint8_t*)(value ? p.kv.v : p.kv.k);
+    int64_t o[PIECES];
+    bool all = p.dim == HD;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      o[i] = rows_at[at * 2 * kTileKeys + (value ? kTileKeys : 0) + (i * 64 * NW + tid) / PPR];
+      all = all && o[i] >= 0;
+    }
+    const int d = tid % PPR * EPP;
+    if (__builtin_amdgcn_ballot_w64(!all) == 0) {
+#pragma unroll
+      for (int i = 0; i < PIECES; ++i) reg[i] = *(const u32x4_a8*)(base + o[i] + d * ES);
     } else {
 #pragma unroll
       for (int i = 0; i < PIECES; ++i) {
-        const int n = i * 64 * NW + tid, r = n / PPR, d = (n % PPR) * EPP;
-        const int key = key0 + r;
-        kreg[i] = vreg[i] = u32x4{0, 0, 0, 0};
-        if (key < sq.len_k && d < p.dim) {
-          int place;
-          const int page = page_of(p.kv, table, key, place);
-          if (page >= 0) {
-            const int64_t ko = page * p.kv.k_page + place * p.kv.k_token + kvh * p.kv.k_head + d;
-            const int64_t vo = page * p.kv.v_page + place * p.kv.v_token + kvh * p.kv.v_head + d;
-            if (k8 && d + 8 >= p.dim) {  // a row of an odd number of 8-byte pieces ends here
-              const u32x2 a = *(const u32x2*)((const uint8_t*)p.kv.k + ko), b = *(const u32x2*)((const uint8_t*)p.kv.v + vo);
-              kreg[i].x = a.x, kreg[i].y = a.y, vreg[i].x = b.x, vreg[i].y = b.y;
-            } else {
-              constexpr int es = k8 ? 1 : 2;
-              kreg[i] = *(const u32x4_a8*)((const uint8_t*)p.kv.k + ko * es);
-              vreg[i] = *(const u32x4_a8*)((const uint8_t*)p.kv.v + vo * es);
-            }
-          }
-        }
-      }
-      if constexpr (k8) {
-        if (tid < 2 * kTileKeys) {
-          const int key = key0 + (tid & (kTileKeys - 1));
-          sreg = 0.f;
-          if (key < sq.len_k) {
-            int place;
-            const int page = page_of(p.kv, table, key, place);
-            if (page >= 0)
-              sreg = tid < kTileKeys
-                         ? p.kv.k_scale[page * p.kv.ks_page + place * p.kv.ks_token + kvh * p.kv.ks_head] * p.scale_log2
-                         : p.kv.v_scale[page * p.kv.vs_page + place * p.kv.vs_token + kvh * p.kv.vs_head];
-          }
-        }
-      }
-    }
-  };
-  auto store = [&](int slot) {
-    if constexpr (kPaged) {
-      unsigned char* ks = smem + slot * S::SLOT;
-      unsigned char* vs = ks + S::BYTES;
-#pragma unroll
-      for (int i = 0; i < PIECES; ++i) {
-        const int n = i * 64 * NW + tid, r = n / PPR, c = (n % PPR) * (EPP / 8);
-        if constexpr (k8) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const u32x2 a = e4m3x4<T>(kreg[i][2 * h]), b = e4m3x4<T>(kreg[i][2 * h + 1]);
-            *(u32x4*)(ks + k_place<HD>(r, c + h)) = u32x4{a.x, a.y, b.x, b.y};
-            const u32x2 e = e4m3x4<T>(vreg[i][2 * h]), f = e4m3x4<T>(vreg[i][2 * h + 1]);
-            *(u32x4*)(vs + v_place<HD>(r, 16 * (c + h))) = u32x4{e.x, e.y, f.x, f.y};
-          }
+        reg[i] = u32x4{0, 0, 0, 0};
+        if (o[i] < 0 || d >= p.dim) continue;
+        if (k8 && d + 8 >= p.dim) {  // the head ends in the middle of 16 codes
+          const u32x2 h = *(const u32x2*)(base + o[i] + d);
+          reg[i].x = h.x, reg[i].y = h.y;
         } else {
-          *(u32x4*)(ks + k_place<HD>(r, c)) = kreg[i];
-          *(u32x4*)(vs + v_place<HD>(r, 16 * c)) = vreg[i];
+          reg[i] = *(const u32x4_a8*)(base + o[i] + d * ES);
         }
       }
-      if constexpr (k8)
-        if (tid < 2 * kTileKeys) *(float*)(smem + 2 * S::SLOT + slot * S::SCALES + 4 * tid) = sreg;
+    }
+  };
+  auto store_pieces = [&](bool value, int slot) {
+    unsigned char* to = smem + (value ? S::V0 : 0) + slot * S::BYTES;
+#pragma unroll
+    for (int i = 0; i < PIECES; ++i) {
+      const int n = i * 64 * NW + tid, r = n / PPR, c = (n % PPR) * (EPP / 8);
+#pragma unroll
+      for (int h = 0; h < EPP / 8; ++h) {
+        u32x4 x = reg[i];
+        if constexpr (k8) {
+          const u32x2 a = e4m3x4<T>(reg[i][2 * h]), b = e4m3x4<T>(reg[i][2 * h + 1]);
+          x = u32x4{a.x, a.y, b.x, b.y};
+        }
+        *(u32x4*)(to + (value ? v_place<HD>(r, 16 * (c + h)) : k_place<HD>(r, c + h))) = x;
+      }
     }
   };
 
-  f32x16 o[DB];
-#pragma unroll
-  for (int d = 0; d < DB; ++d) o[d] = f32x16{0};
-  float m_ref = -INFINITY;  // what the row's weights are relative to (in units of `unit`)
-  float sum = 0.f;          // of this lane's keys only
-  const float unit = k8 ? 1.f : p.scale_log2;  // scores times this are powers of two
-
-  // LDS offsets of this lane's fragments: K's row `col` at chunk 2 kk + half (the second block
-  // of 32 keys lies a fixed distance on), V's transposing reads: row 4 half + r16 / 4, columns
-  // 32 d + 16 (G % 2) + 4 (r16 % 4) (further rows, multiples of 8, keep the permutation)
+  // ---- fragments: K's row `col` at chunk 2 kk + half (the second block of 32 keys lies a fixed
+  // distance on), V's transposing reads: row 4 half + r16 / 4, columns 32 d + 16 (G % 2) +
+  // 4 (r16 % 4) (further rows, multiples of 8, keep the permutation) ----
   int k_at[KK], v_at[DB];
 #pragma unroll
   for (int kk = 0; kk < KK; ++kk) k_at[kk] = k_place<HD>(col, 2 * kk + half);
 #pragma unroll
   for (int d = 0; d < DB; ++d)
-    v_at[d] = S::BYTES + v_place<HD>(4 * half + ((lane & 15) >> 2), 2 * (32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)));
-
-  auto v_frag = [&](const unsigned char* slot, int g, int d) {
-    const u32x2 lo = lds_read_tr(slot + v_at[d] + 16 * g * S::ROW);
-    const u32x2 hi = lds_read_tr(slot + v_at[d] + (16 * g + 8) * S::ROW);
+    v_at[d] = S::V0 + v_place<HD>(4 * half + ((lane & 15) >> 2), 2 * (32 * d + 16 * ((lane >> 4) & 1) + 4 * (lane & 3)));
+  auto k_frag = [&](int slot, int n) {  // n: 2 kk + block
+    return *(const u32x4*)(smem + k_at[n / 2] + slot * S::BYTES + (n & 1) * 32 * S::ROW);
+  };
+  auto v_frag = [&](int slot, int n) {  // n: g DB + d
+    const unsigned char* at = smem + v_at[n % DB] + slot * S::BYTES + 16 * (n / DB) * S::ROW;
+    const u32x2 lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * S::ROW);
     return u32x4{lo.x, lo.y, hi.x, hi.y};
   };
-  // masked: some row of the wave does not see all 64 keys
-  auto compute = [&](int key0, int slot, bool masked) {
-    const unsigned char* ks = smem + slot * S::SLOT;
-    f32x16 s[2] = {f32x16{0}, f32x16{0}};
+
+  f32x16 o[DB];
 #pragma unroll
-    for (int kk = 0; kk < KK; ++kk) {
-#pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        const u32x4 k = *(const u32x4*)(ks + k_at[kk] + b * 32 * S::ROW);
-        s[b] = Mfma32<T>::mma(k, q[kk], s[b]);
-      }
-      if (kk % 2 == 1) __builtin_amdgcn_sched_barrier(0);  // no more fragments at once than four
-    }
-    const float* sc = (const float*)(smem + 2 * S::SLOT + slot * S::SCALES);
+  for (int d = 0; d < DB; ++d) o[d] = f32x16{0};
+  float m_ref = -INFINITY, sum = 0.f;
+  float base = 0.f;                             // what is subtracted, in powers of two (0 for no key yet)
+  const float unit = k8 ? 1.f : p.scale_log2;   // scores times this are powers of two
+  u32x4 pw[4];                                  // weights of 16 keys each
+
+  // scores of step j, before their maximum is taken: scales of 8-bit keys, keys that are not seen
+  auto finish_scores = [&](f32x16 (&s)[2], int j) {
+    const int key0 = begin + j * kTileKeys;
     if constexpr (k8) {
+      const float* sc = scales + (j & 3) * 2 * kTileKeys + 4 * half;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[b][r] *= sc[32 * b + 8 * (r / 4) + 4 * half + r % 4];
+        for (int r = 0; r < 16; r += 4) {
+          const f32x4 c = *(const f32x4*)(sc + 32 * b + 2 * r);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[b][r + i] *= c[i];
+        }
     }
-    if (masked) {
+    if (key0 + kTileKeys - 1 > wave_all) {
+      const int most = limit - key0 - 4 * half;
 #pragma unroll
       for (int b = 0; b < 2; ++b)
 #pragma unroll
-        for (int r = 0; r < 16; ++r)
-          s[b][r] = key0 + 32 * b + 8 * (r / 4) + 4 * half + r % 4 <= limit ? s[b][r] : -INFINITY;
+        for (int r = 0; r < 16; ++r) s[b][r] = 32 * b + 8 * (r / 4) + r % 4 <= most ? s[b][r] : -INFINITY;
     }
-    float mx = s[0][0];
-#pragma unroll
-    for (int r = 1; r < 32; ++r) mx = fmaxf(mx, s[r / 16][r % 16]);
-    mx = fmaxf(mx, __shfl_xor(mx, 32));
+  };
+  // with the maximum of a step's scores (of this lane's keys): the reference is raised
+  auto raise = [&](float mx) {
+    mx = max_halves(mx);
     if (__builtin_amdgcn_ballot_w64((mx - m_ref) * unit > kLazy)) {  // -inf - -inf is no reason
       const float m_new = fmaxf(m_ref, mx);
       const float alpha = m_new == m_ref ? 1.f : exp2_hw((m_ref - m_new) * unit);
       m_ref = m_new;
+      base = m_new == -INFINITY ? 0.f : m_new * unit;
       sum *= alpha;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
     }
-    const float base = m_ref == -INFINITY ? 0.f : m_ref * unit;
-    u32x4 pw[4];  // weights of 16 keys each
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; r += 2) {
-        float w0, w1;
-        if constexpr (k8) {
-          w0 = exp2_hw(s[b][r] - base);
-          w1 = exp2_hw(s[b][r + 1] - base);
-        } else {
-          w0 = exp2_hw(__builtin_fmaf(s[b][r], unit, -base));
-          w1 = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -base));
-        }
-        sum += w0 + w1;
-        if constexpr (k8) {
-          const int key = 32 * b + 8 * (r / 4) + 4 * half + r % 4;
-          w0 *= sc[kTileKeys + key];
-          w1 *= sc[kTileKeys + key + 1];
-        }
-        pw[2 * b + r / 8][(r % 8) / 2] = pack2<T>(w0, w1);
-      }
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-#pragma unroll
-      for (int d = 0; d < DB; ++d) o[d] = Mfma32<T>::mma(v_frag(ks, g, d), pw[g], o[d]);
-      __builtin_amdgcn_sched_barrier(0);
+  };
+  // pair t of a step's weights
+  auto weigh = [&](f32x16 (&s)[2], int j, auto tc) {
+    constexpr int t = decltype(tc)::value, b = t / 8, r = t % 8 * 2;
+    float w0, w1;
+    if constexpr (k8) {
+      w0 = exp2_hw(s[b][r] - base);
+      w1 = exp2_hw(s[b][r + 1] - base);
+    } else {
+      w0 = exp2_hw(__builtin_fmaf(s[b][r], unit, -base));
+      w1 = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -base));
     }
+    sum += w0 + w1;
+    if constexpr (k8) {
+      const float* sc = scales + (j & 3) * 2 * kTileKeys + kTileKeys + 4 * half + 32 * b + 8 * (r / 4) + r % 4;
+      w0 *= sc[0];
+      w1 *= sc[1];
+    }
+    uint32_t w = round2<T>(w0, w1);
+    asm volatile("" : "+v"(w), "+v"(sum));  // computed here: not moved to where it is used
+    pw[t / 4][t % 4] = w;
   };
 
-  // keys that all rows of the workgroup see
-  const int tile_all = p.causal ? min(row0 / p.group + shift, last) : last;
+  constexpr int AHEAD = kPaged ? 2 : 4;    // fragments on their way from LDS
+  constexpr int N1 = 2 * KK, N2 = 4 * DB;  // products of the two phases
+  constexpr int FIRST = 10;                // pairs of weights in the first phase (of 16), LEAD of them before
+  constexpr int LEAD = 2;                  //   its first product, while that one's fragment arrives
+  // step j: sc its scores, sn those of step j + 1 (past the last step whatever the slot holds, all
+  // of it masked); f: fragments on their way
+  auto first_phase = [&](int j, auto slotc, f32x16 (&sc)[2], f32x16 (&sn)[2], u32x4 (&f)[AHEAD]) {
+    constexpr int slot = decltype(slotc)::value, next = (slot + 1) % NS;
+#pragma unroll
+    for (int n = 0; n < AHEAD; ++n) f[n] = k_frag(next, n);
+    sn[0] = sn[1] = f32x16{0};
+    static_for<LEAD>([&](auto t) { weigh(sc, j, t); });
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<N1>([&](auto nc) {
+      constexpr int n = decltype(nc)::value;
+      sn[n & 1] = Mfma32<T>::mma(f[n % AHEAD], q[n / 2], sn[n & 1]);
+      if constexpr (n + AHEAD < N1) f[n % AHEAD] = k_frag(next, n + AHEAD);
+      else f[n % AHEAD] = v_frag(slot, n + AHEAD - N1);
+      static_for<FIRST - LEAD>([&](auto t) {
+        if constexpr (decltype(t)::value * N1 / (FIRST - LEAD) == n)
+          weigh(sc, j, std::integral_constant<int, LEAD + decltype(t)::value>{});
+      });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    finish_scores(sn, j + 1);
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  auto second_phase = [&](int j, auto slotc, f32x16 (&sc)[2], f32x16 (&sn)[2], u32x4 (&f)[AHEAD]) {
+    constexpr int slot = decltype(slotc)::value;
+    float mx = 0.f;
+    __builtin_amdgcn_sched_barrier(0);
+    // the other weights in the first half (groups 2 and 3 of 16 keys are used in the second), the
+    // maximum in the second
+    static_for<N2>([&](auto nc) {
+      constexpr int n = decltype(nc)::value, HALF = N2 / 2;
+      o[n % DB] = Mfma32<T>::mma(f[n % AHEAD], pw[n / DB], o[n % DB]);
+      if constexpr (n + AHEAD < N2) f[n % AHEAD] = v_frag(slot, n + AHEAD);
+      if constexpr (n < HALF) {
+        static_for<16 - FIRST>([&](auto t) {
+          if constexpr (decltype(t)::value * HALF / (16 - FIRST) == n)
+            weigh(sc, j, std::integral_constant<int, FIRST + decltype(t)::value>{});
+        });
+      } else {
+        static_for<16>([&](auto tc) {
+          constexpr int t = decltype(tc)::value;
+          if constexpr (t * HALF / 16 == n - HALF) {
+            const float a = sn[t / 8][t % 8 * 2], b = sn[t / 8][t % 8 * 2 + 1];
+            mx = t == 0 ? larger(a, b) : larger(mx, larger(a, b));
+          }
+        });
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    raise(mx);
+  };
+  static_assert(N1 % AHEAD == 0, "the fragments' places go on from one phase to the other");
+
   bool spoilt = false;
-  if (begin < end) {
-    load(begin, 0);
-    store(0);
-    int slot = 0;
-    for (int key0 = begin; key0 < end; key0 += kTileKeys) {
-      ring_fence<0>();  // this step's keys and values are in LDS, and the other slot is read
-      if (key0 + kTileKeys < end) load(key0 + kTileKeys, slot ^ 1);
+  if (steps > 0) {
+    int page = -1;  // paged: of this thread's row, for the loads of the step after next
+    if constexpr (!kPaged) {
+      dma(false, 0, 0);
+      static_for<NS - 1>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        dma(false, i + 1, i + 1);
+        dma(true, i, i);
+      });
+      ring_fence<(NS - 1) * 2 * S::DMA>();  // K of step 0
+    } else {
+      const int key = begin + (tid & (kTileKeys - 1));
+      place_row(0, key, page_number(key));  // K and V of step 0
+      store_scale(0, 0);
+      __syncthreads();
+      load_pieces(false, 0);
+      store_pieces(false, 0);
+      load_pieces(true, 0);
+      const int k1 = key + kTileKeys;
+      place_row(1, k1, page_number(k1));  // K of step 1 (and V's scales of it)
+      store_scale(1, 1);
+      store_pieces(true, 0);
+      __syncthreads();
+      load_pieces(false, 1);
+      const int k2 = value_row ? k1 : k1 + kTileKeys;
+      place_row(0, k2, page_number(k2));  // K of step 2, V of step 1: for step 0's loads
+      store_scale(2, 1);
+      page = page_number(k2 + kTileKeys);
+      store_pieces(false, 1);
+      ring_fence<0>();
+    }
+    f32x16 s0[2], s1[2];
+    if (begin <= wave_any) {
+      s0[0] = s0[1] = f32x16{0};
+#pragma unroll
+      for (int n = 0; n < N1; ++n) {
+        s0[n & 1] = Mfma32<T>::mma(k_frag(0, n), q[n / 2], s0[n & 1]);
+        if (n % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+      }
+      finish_scores(s0, 0);
+      float mx = s0[0][0];
+#pragma unroll
+      for (int r = 1; r < 32; ++r) mx = larger(mx, s0[r / 16][r % 16]);
+      raise(mx);
+    }
+    auto whole_step = [&](int j, auto slotc, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
+      constexpr int slot = decltype(slotc)::value;
+      const int key0 = begin + j * kTileKeys;
+      // K of step j + 1 and V of step j are in LDS; K of step j and V of step j - 1 are read
+      if constexpr (!kPaged) {
+        ring_fence<(NS - 2) * 2 * S::DMA>();
+        dma(false, j + NS, slot);
+        dma(true, j + NS - 1, (slot + NS - 1) % NS);
+      } else {
+        ring_fence<0>();
+        if (j + 1 < steps) load_pieces(false, slot);
+      }
       if (key0 + kTileKeys - 1 > tile_all) {
-        unsigned char* vs = smem + slot * S::SLOT + S::BYTES;
+        unsigned char* vs = smem + S::V0 + slot * S::BYTES;
         if (any_not_finite<T>(vs, S::BYTES)) {  // all waves find the same
           spoilt = true;
           __syncthreads();
@@ -338,18 +448,52 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
           __syncthreads();
         }
       }
-      if (key0 <= wave_any) compute(key0, slot, key0 + kTileKeys - 1 > wave_all);
-      if (key0 + kTileKeys < end) store(slot ^ 1);
-      slot ^= 1;
-    }
+      u32x4 f[AHEAD];
+      const bool active = key0 <= wave_any;
+      if (active) first_phase(j, slotc, sc, sn, f);
+      if constexpr (kPaged) {
+        if (j + 1 < steps) {
+          store_pieces(false, slot);
+          load_pieces(true, slot);
+          const int key = key0 + (value_row ? 2 : 3) * kTileKeys + (tid & (kTileKeys - 1));
+          place_row(slot ^ 1, key, page);
+          page = page_number(key + kTileKeys);
+        }
+      }
+      if (active) second_phase(j, slotc, sc, sn, f);
+      if constexpr (kPaged) {
+        if (j + 1 < steps) {
+          store_pieces(true, slot ^ 1);
+          store_scale(j + 3, j + 2);
+        }
+      }
+    };
+    for (int j = 0; j < steps; j += NS)
+      static_for<NS>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        if (i == 0 || j + i < steps) {
+          if constexpr (i % 2 == 0) whole_step(j + i, ic, s0, s1);
+          else whole_step(j + i, ic, s1, s0);
+        }
+      });
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no LDS DMA may outlive its slot's use, or the workgroup
   }
+  static_assert(NS % 2 == 0, "a step's scores change places with the next one's");
 
   if (spoilt) {  // add what was made zero (see any_not_finite)
-    for (int key0 = begin; key0 < end; key0 += kTileKeys) {
+    for (int j = 0; j < steps; ++j) {
+      const int key0 = begin + j * kTileKeys;
       if (key0 + kTileKeys - 1 <= tile_all) continue;
-      ring_fence<0>();  // slot 0 is read
-      load(key0, 0);
-      store(0);
+      ring_fence<0>();  // V's first slot is read
+      if constexpr (!kPaged) {
+        dma(true, j, 0);
+      } else {
+        const int key = key0 + (tid & (kTileKeys - 1));
+        place_row(0, key, page_number(key));
+        __syncthreads();
+        load_pieces(true, 0);
+        store_pieces(true, 0);
+      }
       ring_fence<0>();
       for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
@@ -360,7 +504,7 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
             const int key = key0 + 16 * g + 4 * half;
             const u32x4 seen = {ones_up_to<T>(key, limit), ones_up_to<T>(key + 2, limit), ones_up_to<T>(key + 8, limit),
                                 ones_up_to<T>(key + 10, limit)};
-            hit = Mfma32<T>::mma(kind_ones<T>(v_frag(smem, g, d), kind), seen, hit);
+            hit = Mfma32<T>::mma(kind_ones<T>(v_frag(0, g * DB + d), kind), seen, hit);
           }
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] += hit[r] > 0.f ? kind_value(kind) : 0.f;
@@ -370,23 +514,24 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
 
   // ---- out: lane has row `row`, elements 32 d + 8 (r / 4) + 4 half + r % 4 ----
   sum += __shfl_xor(sum, 32);
-  if (!live) return;
-  if (p.splits > 1) {
-    const int64_t at = (int64_t)split * p.rows + ((int64_t)sq.b * (p.starts_q ? 0 : p.len_q) + sq.q0 + tok) * p.heads + head;
-    float* po = p.part_o + at * p.dim;
+  if (splits > 1) {
+    float* part = part_of_tile(p, BM);
+    if (row < rows) {
+      const uint32_t at = part_at(p, BM, split);
 #pragma unroll
-    for (int d = 0; d < DB; ++d)
+      for (int d = 0; d < DB; ++d)
 #pragma unroll
-      for (int r = 0; r < 16; r += 4) {
-        const int e = 32 * d + 8 * (r / 4) + 4 * half;
-        if (e < p.dim) *(f32x4*)(po + e) = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
-      }
-    if (half == 0) {
-      p.part_ml[2 * at] = m_ref * unit;
-      p.part_ml[2 * at + 1] = sum;
+        for (int r = 0; r < 16; r += 4) {
+          const int e = 32 * d + 8 * (r / 4) + 4 * half;
+          if (e < p.dim)
+            store16_coherent(part, at + part_o(p, row - row0) + 4 * e, f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]});
+        }
+      if (half == 0) store8_coherent(part, at + part_ml(p, BM, row - row0), m_ref * unit, sum);
     }
+    join_if_last<T>(p, sq, kvh, row0, min(BM, rows - row0), part, BM, splits, smem);
     return;
   }
+  if (row >= rows) return;
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
 #pragma unroll
@@ -395,19 +540,17 @@ __global__ void __launch_bounds__(64 * NW, HD <= 128 ? 8 / NW : 1) attention_til
     for (int r = 0; r < 16; r += 4) {
       const int e = 32 * d + 8 * (r / 4) + 4 * half;
       if (e < p.dim)
-        *(u32x2*)(op + e) = u32x2{pack2<T>(o[d][r] * inv, o[d][r + 1] * inv), pack2<T>(o[d][r + 2] * inv, o[d][r + 3] * inv)};
+        *(u32x2*)(op + e) = u32x2{round2<T>(o[d][r] * inv, o[d][r + 1] * inv), round2<T>(o[d][r + 2] * inv, o[d][r + 3] * inv)};
     }
 }
 
-template <typename T, int HD, int KIND>
-hipError_t launch_tile_kind(const AttnParams& p, dim3 grid, hipStream_t s) {
-  return launch_kernel(attention_tile_kernel<T, HD, KIND, 4>, grid, dim3(256), 0, s, p);
-}
+// hd: the padded head.
 template <typename T, int KIND>
 hipError_t launch_tile_hd(int hd, const AttnParams& p, dim3 grid, hipStream_t s) {
-  if (hd == 64) return launch_tile_kind<T, 64, KIND>(p, grid, s);
-  if (hd == 128) return launch_tile_kind<T, 128, KIND>(p, grid, s);
-  return launch_tile_kind<T, 256, KIND>(p, grid, s);
+  const dim3 block(64 * kTileWaves);
+  if (hd == 64) return launch_kernel(attention_tile_kernel<T, 64, KIND, 2>, grid, block, 0, s, p);
+  if (hd == 128) return launch_kernel(attention_tile_kernel<T, 128, KIND, 2>, grid, block, 0, s, p);
+  return launch_kernel(attention_tile_kernel<T, 256, KIND, 2>, grid, block, 0, s, p);
 }
 
 }  // namespace cmpext3
