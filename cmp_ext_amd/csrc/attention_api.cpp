@@ -5,7 +5,6 @@
 #include <math.h>
 #include <stdint.h>
 #include <stdio.h>
-#include <stdlib.h>
 
 #include <algorithm>
 
@@ -131,10 +130,34 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   p.slots = (int)slots;
   // Split the keys where the row tiles alone leave CUs idle.
   const int64_t groups = slots * c.kv_heads;
-  const int64_t want = getenv("AW") ? atoi(getenv("AW")) : r.blocks16 ? 2048 : 512;
-  const int least = getenv("AL") ? atoi(getenv("AL")) : r.blocks16 ? 256 : 512;
-  if (groups < want && keys > least && (paged || uniform_k || a->batch == 1)) {
-    const int64_t n = std::min<int64_t>((want + groups - 1) / groups, most_splits(bm));
+  int64_t n = 1;  // splits of the longest sequence
+  int least = 0;  // keys of a split at least
+  if (r.blocks16) {
+    // MI355X, one token for each sequence, heads 32 / 8 of 128: two workgroups a CU keep it busy;
+    // sequences of one batch differ, so more of them want finer splits to even out (16 of up to
+    // 2000 keys: 512 workgroups 20.7 us, 1024 15.9; 64 of up to 8192 in 8 bits: splits of 8192 keys
+    // 154, 2048 130, 1024 123), but not below 256 keys, and none where the tiles fill the GPU (64 of
+    // up to 1000: 27.2 whole, 31.3 in splits of 512).  A few short ones are latency: 128 keys, one
+    // step of each wave (4 of 1000 keys: 10.3 us, in splits of 512 14.4).  Over 128 splits joining
+    // them costs more than they save (one of 65536, heads 8 / 2: 128 splits 22.3 us, 256 26.7).
+    const bool ragged = a->batch > 4;
+    least = ragged ? 256 : 128;
+    if (groups < 512) n = ((ragged ? 1024 : 512) + groups - 1) / groups;
+    n = std::min<int64_t>(std::max<int64_t>(n, keys / 1024), 128);
+  } else if (paged) {
+    // two workgroups a CU at once; more where sequences differ (8 bits, heads 32 / 8 of 128: one of
+    // 512 new tokens over 8192 keys, 136 tiles, 313 us whole, 134 in 3, 110 in 4, 142 in 6; 16 of up to
+    // 64 over up to 4096: 72 in 2, 60 in 4)
+    least = 256;
+    n = ((a->batch > 4 ? 1024 : 512) + groups - 1) / groups;
+  } else if ((uniform_k || a->batch == 1) && groups < 384 && keys >= 2048) {
+    // prompts see half their keys, the longest rows first: only long keys and few tiles gain (one of
+    // 4096 tokens, heads 8 / 2: 75 us whole, 57 in 3; one of 1000, 32 / 8, as many tiles: 25 and 33)
+    least = 512;
+    n = (768 + groups - 1) / groups;
+  }
+  n = std::min<int64_t>(n, most_splits(bm));
+  if (n > 1 && keys > least) {
     const int64_t per = std::max<int64_t>(least, ((keys + n - 1) / n + 127) / 128 * 128);
     const int64_t splits = (keys + per - 1) / per;
     if (splits > 1) {

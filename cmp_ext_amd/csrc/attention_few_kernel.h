@@ -30,9 +30,8 @@ struct FewShape {
   static constexpr int PITCH = HD + 4;                      // floats of a row of O in LDS
   static constexpr int JOIN = kFewWaves * BM * PITCH * 4;
   static constexpr int ML = kFewWaves * BM * 2 * 4;
-  static constexpr int SPLITS = 8 * BM * most_splits(BM);
   static constexpr int BODY = WAVE * kFewWaves > JOIN ? WAVE * kFewWaves : JOIN;
-  static constexpr int LDS = BODY + ML > SPLITS ? BODY + ML : SPLITS;
+  static constexpr int LDS = BODY + ML > kJoinBytes ? BODY + ML : kJoinBytes;
 };
 
 // Byte offset of byte column `bc` of V's row `row`: a transposing read by 32 lanes covers

@@ -31,66 +31,98 @@ __device__ __forceinline__ int splits_of(const AttnParams& p, int end) {
   return p.splits == 1 ? 1 : min(p.splits, max(1, (end + p.split_keys - 1) / p.split_keys));
 }
 
-// Joins n > 1 splits of a tile's `rows` rows (of room for bm) and writes them out.  256 threads,
-// all of them here, with 8 * bm * n bytes of LDS (at least 4 KB).
+// IT items (four elements of a row) of each thread, SP splits of each at a time: so many loads on
+// their way.  `share` threads take the splits of an item in turn (share > 1: all items at once).
+template <typename T, int IT, int SP>
+__device__ __forceinline__ void join_items(const AttnParams& p, const Seq& sq, int kvh, int row0, int rows, const float* part, int bm, int n,
+                                           int share, const float* weight, const float* inv, f32x4* sums) {
+  const int tid = threadIdx.x, quads = p.dim / 4, items = rows * quads;
+  const int mine = share > 1 ? tid / items : 0;
+  for (int i0 = 0; i0 < items; i0 += 256 * IT) {
+    f32x4 acc[IT];
+    int r[IT], e[IT];
+    bool busy[IT];
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      const int i = share > 1 ? tid - mine * items : i0 + t * 256 + tid;
+      busy[t] = i < items && mine < share;
+      r[t] = busy[t] ? i / quads : 0;
+      e[t] = busy[t] ? 4 * (i - r[t] * quads) : 0;
+      acc[t] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+    for (int s0 = mine; s0 < n; s0 += SP * share) {
+      f32x4 x[IT][SP];
+      float w[IT][SP];
+      // past the last split the last one again, with no weight: no load waits behind a branch
+#pragma unroll
+      for (int t = 0; t < IT; ++t)
+#pragma unroll
+        for (int j = 0; j < SP; ++j)
+          x[t][j] = load16_coherent(part, part_at(p, bm, min(s0 + j * share, n - 1)) + part_o(p, r[t]) + 4 * e[t]);
+#pragma unroll
+      for (int t = 0; t < IT; ++t)
+#pragma unroll
+        for (int j = 0; j < SP; ++j) {
+          const float y = weight[r[t] * n + min(s0 + j * share, n - 1)];
+          w[t][j] = s0 + j * share < n ? y : 0.f;
+        }
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int t = 0; t < IT; ++t)
+#pragma unroll
+        for (int j = 0; j < SP; ++j) acc[t] += w[t][j] * x[t][j];
+    }
+    if (share > 1) {  // uniform
+      sums[tid] = acc[0];
+      __syncthreads();
+      if (busy[0] && mine == 0)
+        for (int g = 1; g < share; ++g) acc[0] += sums[tid + g * items];
+    }
+#pragma unroll
+    for (int t = 0; t < IT; ++t) {
+      if (!busy[t] || mine != 0) continue;
+      const int row = row0 + r[t], tok = row / p.group, head = kvh * p.group + row - tok * p.group;
+      T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
+      const float f = inv[r[t]];
+      *(u32x2*)(op + e[t]) = u32x2{round2<T>(acc[t][0] * f, acc[t][1] * f), round2<T>(acc[t][2] * f, acc[t][3] * f)};
+    }
+  }
+}
+
+// Joins n > 1 splits of a tile's `rows` rows (of room for bm) and writes them out.  256 threads, all
+// of them here, with 4 KB + 4 bm (n + 1) bytes of LDS.
 template <typename T>
 __device__ __forceinline__ void join_rows(const AttnParams& p, const Seq& sq, int kvh, int row0, int rows, const float* part, int bm,
                                           int n, unsigned char* lds) {
   const int tid = threadIdx.x;
-  u32x2* ml = (u32x2*)lds;  // [row][split]
-  for (int i = tid; i < rows * n; i += 256) {
-    const int r = i / n, s = i - r * n;
-    ml[i] = load8_coherent(part, part_at(p, bm, s) + part_ml(p, bm, r));
-  }
+  f32x4* sums = (f32x4*)lds;
+  float* inv = (float*)(sums + 256);  // 1 / the rows' sums
+  float* weight = inv + bm;           // [row][split]: 2^(m_s - m)
+  // the lanes of a row, a power of two up to a wave
+  const int lanes = rows <= 4 ? 64 : rows <= 8 ? 32 : rows <= 16 ? 16 : rows <= 32 ? 8 : rows <= 64 ? 4 : 2;
+  const int r = tid / lanes;
+  float m = -INFINITY, l = 0.f;
+  if (r < rows)
+    for (int s = tid % lanes; s < n; s += lanes) {
+      const float x = __uint_as_float(load8_coherent(part, part_at(p, bm, s) + part_ml(p, bm, r)).x);
+      weight[r * n + s] = x;
+      m = fmaxf(m, x);
+    }
+  for (int x = 1; x < lanes; x <<= 1) m = fmaxf(m, __shfl_xor(m, x));
+  if (r < rows)
+    for (int s = tid % lanes; s < n; s += lanes) {
+      const float f = m == -INFINITY ? 0.f : exp2_hw(weight[r * n + s] - m);
+      weight[r * n + s] = f;
+      l += f * __uint_as_float(load8_coherent(part, part_at(p, bm, s) + part_ml(p, bm, r)).y);
+    }
+  for (int x = 1; x < lanes; x <<= 1) l += __shfl_xor(l, x);
+  if (r < rows && tid % lanes == 0) inv[r] = l > 0.f || l != l ? 1.f / l : 0.f;
   __syncthreads();
-  const int quads = p.dim / 4, items = rows * quads;  // an item: four elements of a row
-  // where the items are few, several threads take an item's splits in turn
-  const int share = max(1, 256 / items), mine = share > 1 ? tid / items : 0;
-  for (int i0 = 0; i0 < items; i0 += 256) {
-    const int i = share > 1 ? tid - mine * items : i0 + tid;
-    const bool busy = i < items && mine < share;
-    const int r = busy ? i / quads : 0, e = 4 * (i - r * quads);
-    f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
-    float l = 0.f;
-    if (busy) {
-      float m = -INFINITY;
-      for (int s = 0; s < n; ++s) m = fmaxf(m, __uint_as_float(ml[r * n + s].x));
-      if (m != -INFINITY) {
-        for (int s0 = mine; s0 < n; s0 += 8 * share) {
-          f32x4 x[8];
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (s0 + j * share < n) x[j] = load16_coherent(part, part_at(p, bm, s0 + j * share) + part_o(p, r) + 4 * e);
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (s0 + j * share < n) {
-              const u32x2 v = ml[r * n + s0 + j * share];
-              const float f = exp2_hw(__uint_as_float(v.x) - m);
-              l += f * __uint_as_float(v.y);
-              acc += f * x[j];
-            }
-        }
-      }
-    }
-    if (share > 1) {  // uniform; items <= 128 here, one turn
-      __syncthreads();
-      f32x4* sums = (f32x4*)lds;
-      float* ls = (float*)(sums + 256);
-      sums[tid] = acc;
-      ls[tid] = l;
-      __syncthreads();
-      if (!busy || mine != 0) continue;
-      for (int g = 1; g < share; ++g) {
-        acc += sums[tid + g * items];
-        l += ls[tid + g * items];
-      }
-    }
-    if (!busy) continue;
-    const int row = row0 + r, tok = row / p.group, head = kvh * p.group + row - tok * p.group;
-    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-    T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
-    *(u32x2*)(op + e) = u32x2{round2<T>(acc[0] * inv, acc[1] * inv), round2<T>(acc[2] * inv, acc[3] * inv)};
-  }
+  const int items = rows * (p.dim / 4);
+  if (items <= 128)
+    join_items<T, 1, 16>(p, sq, kvh, row0, rows, part, bm, n, 256 / items, weight, inv, sums);
+  else
+    join_items<T, 4, 4>(p, sq, kvh, row0, rows, part, bm, n, 1, weight, inv, sums);
 }
 
 // After a workgroup has stored its split: joins, if it is the last of its tile's n.

@@ -14,10 +14,10 @@ constexpr int kTileKeys = 64;
 constexpr int kWaveKeys = 32;
 constexpr int kFewWaves = 4;
 
-// LDS of the second phase of split keys, 8 bytes for each row and split of a tile: so many splits
-// at most.
-constexpr int kJoinBytes = 32 * 1024;
-constexpr int most_splits(int rows_of_tile) { return kJoinBytes / 8 / rows_of_tile; }
+// LDS to join split keys in: a sum for each of 256 threads, a number for each row of a tile and one
+// for each of its splits, of which there are so many at most.
+constexpr int kJoinBytes = 20 * 1024 + 512;
+constexpr int most_splits(int rows_of_tile) { return (kJoinBytes - 4096 - 4 * rows_of_tile) / (4 * rows_of_tile); }
 
 // Keys and values: packed rows, or pages.
 struct KvSource {

@@ -50,7 +50,7 @@ struct TileShape {
   static constexpr int LDS = PAGED ? SCALES + 4 * 2 * kTileKeys * 4 : ROWS_AT;
   static constexpr int DMA = BYTES / 1024 / kTileWaves;  // 1 KB LDS-DMA loads per wave of K, and of V
   static_assert(BYTES % (1024 * kTileWaves) == 0, "whole DMA loads per wave");
-  static_assert(LDS <= 160 * 1024 && LDS >= 8 * 128 * most_splits(128), "LDS budget");
+  static_assert(LDS <= 160 * 1024 && LDS >= kJoinBytes, "LDS budget");
   static_assert(!PAGED || NS == 2, "pages are loaded one step ahead");
 };
 

@@ -229,7 +229,7 @@ def test_plans():
     assert "attention_few rows=32" in plan(len_q=8)
     assert "attention_tile" in plan(len_q=64) and "splits=1 " in plan(len_q=64)
     assert "keys=paged8" in plan(cache=cache_args(kv_dtype=cabi.E4M3, k_scale=0x100, v_scale=0x200))
-    assert "splits=1 " in plan(batch=5000, table_pages=4096) and "splits=1 " not in plan(table_pages=4096)
+    assert "splits=1 " in plan(batch=5000, table_pages=60) and "splits=1 " not in plan(table_pages=4096)
     assert plan(batch=0) == "kernel=none"
 
 
