@@ -1,4 +1,4 @@
-"""cmpext3 dense GEMM operators for AMD Instinct MI355X (gfx950).
+"""cmpext3 operators for AMD Instinct MI355X (gfx950): dense GEMM, and the attention layer next to it.
 
 Python surface (same names and argument meaning as the reference extension's
 GEMM entry points, src/main.cpp:1594-1602, plus the dtype-specific matmuls):
@@ -9,7 +9,21 @@ GEMM entry points, src/main.cpp:1594-1602, plus the dtype-specific matmuls):
     conv2d(input, weight, bias=None, stride=1, padding=0, dilation=1, groups=1)
                                                                1x1 NCHW convolution as a GEMM
     plan(dtype, M, N, K, layout="KN", batch=1, has_bias=False) kernel the selector picks
-    last_plan()                                                kernel(s) this thread's last call ran
+    last_plan()                                                kernel(s) this thread's last product ran
+
+What stands between an attention layer's projections when it serves a model (forward only):
+
+    qk_norm_rope(q, k, cos, sin, positions, q_weight=None, k_weight=None, eps=1e-6, interleaved=False)
+                                                               norms of queries and keys, position rotation
+    rope_table(max_positions, rotary_dim, base=10000.0, ...)   its tables, also scaled for long contexts
+    kv_cache_write(k, v, k_cache, v_cache, slots, k_scale=None, v_scale=None)
+                                                               into a paged cache: 16 bits, or e4m3 with scales
+    kv_cache_read(k_cache, v_cache, block_table, cu_seqlens, total, dtype=None, k_scale=None, v_scale=None)
+                                                               sequences out of it, as packed rows
+    attention(q, k, v, cu_seqlens_q=None, cu_seqlens_k=None, causal=True, scale=None)
+                                                               whole prompts, packed or batched, grouped heads
+    paged_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q=None, k_scale=None,
+                    v_scale=None, causal=True, scale=None)     new tokens over a paged cache
 
 Every call runs the hand-written gfx950 kernels of lib/libcmpext3_gemm.so on
 PyTorch's current stream.  There is no fallback: if the compiled extension is
@@ -19,12 +33,14 @@ the `build` submodule stays usable.
 import torch  # noqa: F401  (loads PyTorch's HIP runtime before the extension binds to it)
 
 __all__ = ["fp16_matmul", "bf16_matmul", "fp32_matmul", "linear", "bmm", "conv2d", "plan", "last_plan",
-           "qk_norm_rope", "kv_cache_write", "kv_cache_read", "attention", "paged_attention", "version"]
+           "qk_norm_rope", "kv_cache_write", "kv_cache_read", "attention", "paged_attention", "rope_table", "version"]
+
+from .rope import rope_table  # noqa: E402
 
 try:
     from . import _cmpext3 as _ext
 
-    _missing = [n for n in __all__ if not hasattr(_ext, n)]
+    _missing = [n for n in __all__ if n not in globals() and not hasattr(_ext, n)]
     if _missing:  # built from older sources
         raise ImportError(f"{_ext.__file__} is stale (lacks {', '.join(_missing)}); rebuild it")
 except ImportError as _e:  # a tree that was not built: every operator access raises

@@ -150,7 +150,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     // 64 over up to 4096: 72 in 2, 60 in 4)
     least = 256;
     n = ((a->batch > 4 ? 1024 : 512) + groups - 1) / groups;
-  } else if ((uniform_k || a->batch == 1) && groups < 384 && keys >= 2048) {
+  } else if (groups < 384 && keys >= 2048) {
     // prompts see half their keys, the longest rows first: only long keys and few tiles gain (one of
     // 4096 tokens, heads 8 / 2: 75 us whole, 57 in 3; one of 1000, 32 / 8, as many tiles: 25 and 33)
     least = 512;

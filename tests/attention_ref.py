@@ -9,8 +9,8 @@ import math
 
 import torch
 
-UNIT = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24}  # half a spacing at 1
-TINY = {torch.float16: 2.0**-25, torch.bfloat16: 2.0**-134, torch.float32: 2.0**-150}  # half the least spacing
+UNIT = {torch.float16: 2.0**-11, torch.bfloat16: 2.0**-8, torch.float32: 2.0**-24, torch.float64: 0.0}  # half a spacing at 1
+TINY = {torch.float16: 2.0**-25, torch.bfloat16: 2.0**-134, torch.float32: 2.0**-150, torch.float64: 0.0}  # half the least spacing
 
 
 def rope(x, weight, cos, sin, positions, eps, interleaved):
