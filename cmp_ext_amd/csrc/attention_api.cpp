@@ -59,6 +59,7 @@ struct AttnPlan {
   KvKind kind;
   int hd;        // padded head
   int blocks16;  // few-rows kernel: its tiles of 16 rows; 0: tile kernel
+  int ks;        // tile kernel: groups of waves that share a tile's keys
   int rows;      // of a workgroup
   bool empty;
   int64_t ws_bytes;
@@ -122,6 +123,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     return CMPEXT3_OK;
   }
   const int64_t mean_rows = queries * group / a->batch;  // of a sequence and kv head
+  r.ks = 1;
   r.blocks16 = paged && mean_rows <= 32 ? (mean_rows <= 16 || r.hd == 256 ? 1 : 2) : 0;
   const int bm = r.rows = r.blocks16 ? 16 * r.blocks16 : 128;
   const int64_t slots = uniform_q ? (int64_t)a->batch * (((int64_t)a->len_q * group + bm - 1) / bm)
@@ -145,16 +147,33 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     if (groups < 512) n = ((ragged ? 1024 : 512) + groups - 1) / groups;
     n = std::min<int64_t>(std::max<int64_t>(n, keys / 1024), 128);
   } else if (paged) {
-    // two workgroups a CU at once; more where sequences differ (8 bits, heads 32 / 8 of 128: one of
-    // 512 new tokens over 8192 keys, 136 tiles, 313 us whole, 134 in 3, 110 in 4, 142 in 6; 16 of up to
-    // 64 over up to 4096: 72 in 2, 60 in 4)
+    // Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
+    // not so long that workgroups of their own pay (16 bits, heads 32 / 8 of 128: 64 new tokens over
+    // 8192 keys 49.0 us with one group and 8 splits, 41.1 with two; 16 of up to 64 over up to 4096
+    // 48.4 and 44.7; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 148).
+    // Splits: two workgroups' worth of waves a CU at once; more where sequences differ (8 bits: one
+    // of 512 new tokens over 8192 keys, 136 tiles, 282 us whole, 130 in 3, 107 in 4, 133 in 6).
+    const bool ragged = a->batch > 4;
     least = 256;
-    n = ((a->batch > 4 ? 1024 : 512) + groups - 1) / groups;
-  } else if (groups < 384 && keys >= 2048) {
-    // prompts see half their keys, the longest rows first: only long keys and few tiles gain (one of
-    // 4096 tokens, heads 8 / 2: 75 us whole, 57 in 3; one of 1000, 32 / 8, as many tiles: 25 and 33)
+    if (r.hd <= 128 && groups <= 256 && (keys <= 4096 || groups <= 32)) {
+      r.ks = 2;
+      n = std::min<int64_t>(((ragged ? 480 : 256) + groups - 1) / groups, std::max<int64_t>(1, keys / 1024));
+    } else {
+      n = ((ragged ? 1024 : 512) + groups - 1) / groups;
+    }
+  } else if (groups < 384 && keys >= 512) {
+    // Prompts see half their keys, the longest rows first: two groups, or splits, gain where tiles are
+    // few and keys long (heads 32 / 8 of 128: one of 1000 tokens, 250 tiles, 25.7 us with one group,
+    // 24.1 with two, 32.9 in 2 splits; of 300 13.0 and 14.7 with two.  Heads 8 / 2 of 64, one of 2361:
+    // 32.5, 26.9 with two groups, 22.0 in 2 splits as well; of 128, one of 4096, 256 tiles: 75.7,
+    // 62.4, 57.4 with one group in 3 splits).
     least = 512;
-    n = (768 + groups - 1) / groups;
+    if (r.hd <= 128 && groups <= (keys >= 2048 ? 160 : 256)) {
+      r.ks = 2;
+      n = keys >= 2048 ? 2 : 1;
+    } else if (keys >= 2048) {
+      n = (768 + groups - 1) / groups;
+    }
   }
   n = std::min<int64_t>(n, most_splits(bm));
   if (n > 1 && keys > least) {
@@ -172,11 +191,11 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
 
 hipError_t launch_tile_kernel(int dtype, const AttnPlan& r, dim3 grid, hipStream_t s) {
   if (dtype == CMPEXT3_F16) {
-    if (r.kind == kKvPacked) return launch_attention_tile_f16_packed(r.hd, r.p, grid, s);
-    return r.kind == kKvPaged16 ? launch_attention_tile_f16_paged16(r.hd, r.p, grid, s) : launch_attention_tile_f16_paged8(r.hd, r.p, grid, s);
+    if (r.kind == kKvPacked) return launch_attention_tile_f16_packed(r.hd, r.ks, r.p, grid, s);
+    return r.kind == kKvPaged16 ? launch_attention_tile_f16_paged16(r.hd, r.ks, r.p, grid, s) : launch_attention_tile_f16_paged8(r.hd, r.ks, r.p, grid, s);
   }
-  if (r.kind == kKvPacked) return launch_attention_tile_bf16_packed(r.hd, r.p, grid, s);
-  return r.kind == kKvPaged16 ? launch_attention_tile_bf16_paged16(r.hd, r.p, grid, s) : launch_attention_tile_bf16_paged8(r.hd, r.p, grid, s);
+  if (r.kind == kKvPacked) return launch_attention_tile_bf16_packed(r.hd, r.ks, r.p, grid, s);
+  return r.kind == kKvPaged16 ? launch_attention_tile_bf16_paged16(r.hd, r.ks, r.p, grid, s) : launch_attention_tile_bf16_paged8(r.hd, r.ks, r.p, grid, s);
 }
 
 hipError_t launch_few_kernel(int dtype, const AttnPlan& r, dim3 grid, hipStream_t s) {
@@ -221,8 +240,8 @@ extern "C" int cmpext3_attention_describe(const cmpext3_attention_args* args, ch
     if (r.empty)
       snprintf(buf, (size_t)buflen, "kernel=none");
     else
-      snprintf(buf, (size_t)buflen, "kernel=%s rows=%d keys=%s head=%d slots=%d splits=%d split_keys=%d",
-               r.blocks16 ? "attention_few" : "attention_tile", r.rows, kinds[r.kind], r.hd,
+      snprintf(buf, (size_t)buflen, "kernel=%s rows=%d groups=%d keys=%s head=%d slots=%d splits=%d split_keys=%d",
+               r.blocks16 ? "attention_few" : "attention_tile", r.rows, r.ks, kinds[r.kind], r.hd,
                r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0);
   }
   return CMPEXT3_OK;

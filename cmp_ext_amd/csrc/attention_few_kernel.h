@@ -352,7 +352,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : 
       *(u32x2*)(op + e) = u32x2{round2<T>(acc[0] * inv, acc[1] * inv), round2<T>(acc[2] * inv, acc[3] * inv)};
     }
   }
-  if (splits > 1) join_if_last<T>(p, sq, kvh, row0, min(S::BM, rows - row0), part, S::BM, splits, smem);
+  if (splits > 1) join_if_last<T, 64 * kFewWaves>(p, sq, kvh, row0, min(S::BM, rows - row0), part, S::BM, splits, smem);
 }
 
 template <typename T, int KIND, int MB>

@@ -33,18 +33,18 @@ __device__ __forceinline__ int splits_of(const AttnParams& p, int end) {
 
 // IT items (four elements of a row) of each thread, SP splits of each at a time: so many loads on
 // their way.  `share` threads take the splits of an item in turn (share > 1: all items at once).
-template <typename T, int IT, int SP>
+template <typename T, int IT, int SP, int THREADS>
 __device__ __forceinline__ void join_items(const AttnParams& p, const Seq& sq, int kvh, int row0, int rows, const float* part, int bm, int n,
                                            int share, const float* weight, const float* inv, f32x4* sums) {
   const int tid = threadIdx.x, quads = p.dim / 4, items = rows * quads;
   const int mine = share > 1 ? tid / items : 0;
-  for (int i0 = 0; i0 < items; i0 += 256 * IT) {
+  for (int i0 = 0; i0 < items; i0 += THREADS * IT) {
     f32x4 acc[IT];
     int r[IT], e[IT];
     bool busy[IT];
 #pragma unroll
     for (int t = 0; t < IT; ++t) {
-      const int i = share > 1 ? tid - mine * items : i0 + t * 256 + tid;
+      const int i = share > 1 ? tid - mine * items : i0 + t * THREADS + tid;
       busy[t] = i < items && mine < share;
       r[t] = busy[t] ? i / quads : 0;
       e[t] = busy[t] ? 4 * (i - r[t] * quads) : 0;
@@ -89,16 +89,16 @@ __device__ __forceinline__ void join_items(const AttnParams& p, const Seq& sq, i
   }
 }
 
-// Joins n > 1 splits of a tile's `rows` rows (of room for bm) and writes them out.  256 threads, all
-// of them here, with 4 KB + 4 bm (n + 1) bytes of LDS.
-template <typename T>
+// Joins n > 1 splits of a tile's `rows` rows (of room for bm) and writes them out.  The workgroup's
+// THREADS threads, all of them here, with 16 THREADS + 4 bm (n + 1) bytes of LDS.
+template <typename T, int THREADS>
 __device__ __forceinline__ void join_rows(const AttnParams& p, const Seq& sq, int kvh, int row0, int rows, const float* part, int bm,
                                           int n, unsigned char* lds) {
   const int tid = threadIdx.x;
   f32x4* sums = (f32x4*)lds;
-  float* inv = (float*)(sums + 256);  // 1 / the rows' sums
+  float* inv = (float*)(sums + THREADS);  // 1 / the rows' sums
   float* weight = inv + bm;           // [row][split]: 2^(m_s - m)
-  // the lanes of a row, a power of two up to a wave
+  // the lanes of a row, a power of two up to a wave: 256 threads at most
   const int lanes = rows <= 4 ? 64 : rows <= 8 ? 32 : rows <= 16 ? 16 : rows <= 32 ? 8 : rows <= 64 ? 4 : 2;
   const int r = tid / lanes;
   float m = -INFINITY, l = 0.f;
@@ -119,14 +119,14 @@ __device__ __forceinline__ void join_rows(const AttnParams& p, const Seq& sq, in
   if (r < rows && tid % lanes == 0) inv[r] = l > 0.f || l != l ? 1.f / l : 0.f;
   __syncthreads();
   const int items = rows * (p.dim / 4);
-  if (items <= 128)
-    join_items<T, 1, 16>(p, sq, kvh, row0, rows, part, bm, n, 256 / items, weight, inv, sums);
+  if (items <= THREADS / 2)
+    join_items<T, 1, 16, THREADS>(p, sq, kvh, row0, rows, part, bm, n, THREADS / items, weight, inv, sums);
   else
-    join_items<T, 4, 4>(p, sq, kvh, row0, rows, part, bm, n, 1, weight, inv, sums);
+    join_items<T, 4, 4, THREADS>(p, sq, kvh, row0, rows, part, bm, n, 1, weight, inv, sums);
 }
 
 // After a workgroup has stored its split: joins, if it is the last of its tile's n.
-template <typename T>
+template <typename T, int THREADS>
 __device__ __forceinline__ void join_if_last(const AttnParams& p, const Seq& sq, int kvh, int row0, int rows, const float* part, int bm,
                                              int n, unsigned char* lds) {
   if (p.sem == nullptr) return;
@@ -138,7 +138,7 @@ __device__ __forceinline__ void join_if_last(const AttnParams& p, const Seq& sq,
     last = __hip_atomic_fetch_add(count, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == (unsigned)(n - 1);
   __syncthreads();
   if (!last) return;
-  join_rows<T>(p, sq, kvh, row0, rows, part, bm, n, lds);
+  join_rows<T, THREADS>(p, sq, kvh, row0, rows, part, bm, n, lds);
   if (threadIdx.x == 0) __hip_atomic_store(count, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);  // for the next kernel
 }
 

@@ -12,7 +12,7 @@ __global__ void __launch_bounds__(256) attention_join_kernel(const AttnParams p,
   if (sq.b < 0) return;
   const int row0 = sq.tile * bm, rows = min(bm, sq.len_q * p.group - row0);
   const int n = splits_of(p, keys_end(p, sq, row0 + rows - 1));
-  if (n > 1) join_rows<T>(p, sq, kvh, row0, rows, part_of_tile(p, bm), bm, n, lds);
+  if (n > 1) join_rows<T, 256>(p, sq, kvh, row0, rows, part_of_tile(p, bm), bm, n, lds);
 }
 
 hipError_t launch_attention_join(int dtype, int bm, const AttnParams& p, hipStream_t s) {

@@ -53,13 +53,14 @@ struct AttnParams {
   unsigned int* sem;  // counters of the row tiles, or nullptr: joined by a second launch
 };
 
-// hd: 64, 128 or 256, the head padded (dim <= hd).  grid: slots * kv_heads, splits.
-hipError_t launch_attention_tile_f16_packed(int hd, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_tile_f16_paged16(int hd, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_tile_f16_paged8(int hd, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_tile_bf16_packed(int hd, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_tile_bf16_paged16(int hd, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_tile_bf16_paged8(int hd, const AttnParams& p, dim3 grid, hipStream_t s);
+// hd: 64, 128 or 256, the head padded (dim <= hd); ks: groups of waves of a workgroup, each with its
+// share of the keys, 1 or (hd up to 128) 2.  grid: slots * kv_heads, splits.
+hipError_t launch_attention_tile_f16_packed(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_tile_f16_paged16(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_tile_f16_paged8(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_tile_bf16_packed(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_tile_bf16_paged16(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_tile_bf16_paged8(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
 // blocks16: tiles of 16 rows a workgroup takes, 1 or 2.
 hipError_t launch_attention_few_f16_paged16(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_attention_few_f16_paged8(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);

@@ -1,7 +1,7 @@
 #include "attention_tile_kernel.h"
 
 namespace cmpext3 {
-hipError_t launch_attention_tile_f16_paged16(int hd, const AttnParams& p, dim3 grid, hipStream_t s) {
-  return launch_tile_hd<_Float16, kKvPaged16>(hd, p, grid, s);
+hipError_t launch_attention_tile_f16_paged16(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s) {
+  return launch_tile_hd<_Float16, kKvPaged16>(hd, ks, p, grid, s);
 }
 }  // namespace cmpext3

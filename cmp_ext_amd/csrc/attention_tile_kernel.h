@@ -7,6 +7,11 @@
 // (8192 tokens, 32 heads of 128 on MI355X: 520 us; eight waves over 256 rows, whose barriers bind
 // all waves of a CU together, 550; four waves of 64 rows with a SIMD to themselves 643.)
 //
+// Keys: where there are fewer tiles than CUs, a workgroup has two such groups of four waves (KS = 2),
+// one for the even steps and one for the odd ones, each with its own LDS, joined in LDS at the end:
+// two waves on every SIMD as with two workgroups, and half as many steps.  Beyond that the keys
+// are split over workgroups (attention_join.h).
+//
 // Products (32x32x16, fp32 sums) run transposed: S^T = K Q^T gives lane l the scores of row
 // l % 32 only (keys 8 (r / 4) + 4 (l / 32) + r % 4 of a block of 32), so the maximum, sum and
 // scale of a row are one register of a lane, joined over the two half-waves by one exchange;
@@ -74,15 +79,18 @@ __device__ __forceinline__ int v_place(int row, int byte_col) {
 }
 
 // Two waves share a SIMD's registers (packed heads up to 64: three; over 128: one has them all).
-template <typename T, int HD, int KIND, int NS>
-__global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && KIND == kKvPacked ? 3 : 2) attention_tile_kernel(const AttnParams p) {
+template <typename T, int HD, int KIND, int NS, int KS>
+__global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64 && KIND == kKvPacked && KS == 1 ? 3 : 2) attention_tile_kernel(const AttnParams p) {
   constexpr bool kPaged = KIND != kKvPacked, k8 = KIND == kKvPaged8;
   using S = TileShape<HD, kPaged, NS>;
   constexpr int KK = HD / 16, DB = HD / 32, NW = kTileWaves, BM = 32 * NW;
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[S::LDS];
+  __shared__ __attribute__((aligned(1024))) unsigned char all_smem[S::LDS * KS];
+  __shared__ int any_spoilt;
 
-  const int tid = threadIdx.x, lane = tid & 63;
+  const int tid = threadIdx.x & (64 * NW - 1), lane = tid & 63;  // of a group of four waves
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part_k = KS == 1 ? 0 : __builtin_amdgcn_readfirstlane((int)threadIdx.x / (64 * NW));  // which group
+  unsigned char* smem = all_smem + part_k * S::LDS;
   const int half = lane >> 5, col = lane & 31;
 
   // heads fastest: the workgroups of one kv head meet in the L2 of few XCDs
@@ -97,7 +105,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
   if (split >= splits) return;
   const int begin = split * p.split_keys;
   end = min(end, begin + p.split_keys);
-  const int steps = end > begin ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
+  // steps of this group, and of the group that has most: step j starts at key key_of(j)
+  const int all_steps = end > begin ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
+  const int steps = (all_steps - part_k + KS - 1) / KS, turns = (all_steps + KS - 1) / KS;
+  auto key_of = [&](int j) { return begin + (j * KS + part_k) * kTileKeys; };
 
   // ---- this lane's row ----
   const int last = min(sq.len_k, end) - 1;  // keys past `end` are another split's
@@ -146,7 +157,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
   const uint32_t lds0 = lds_addr(smem) + (uint32_t)(wave * S::DMA * 1024);
   // K or V of the step from key0 into a slot, zeros past the sequence and of steps past the last
   auto dma = [&](bool value, int step, int slot) {
-    const int key0 = begin + step * kTileKeys;
+    const int key0 = key_of(step);
     const i32x4 r = make_rsrc_sgpr(value ? vbase + (int64_t)key0 * p.kv.v_token : kbase + (int64_t)key0 * p.kv.k_token);
     const uint32_t dst = lds0 + (uint32_t)((value ? S::V0 : 0) + slot * S::BYTES);
     const int left = step < steps ? sq.len_k - key0 : 0;
@@ -267,7 +278,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
 
   // scores of step j, before their maximum is taken: scales of 8-bit keys, keys that are not seen
   auto finish_scores = [&](f32x16 (&s)[2], int j) {
-    const int key0 = begin + j * kTileKeys;
+    const int key0 = key_of(j);
     if constexpr (k8) {
       const float* sc = scales + (j & 3) * 2 * kTileKeys + 4 * half;
 #pragma unroll
@@ -381,8 +392,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
   };
   static_assert(N1 % AHEAD == 0, "the fragments' places go on from one phase to the other");
 
+  constexpr int STEP = KS * kTileKeys;  // keys from a step to the group's next one
   bool spoilt = false;
-  if (steps > 0) {
+  if (KS > 1 && threadIdx.x == 0) any_spoilt = 0;
+  if (turns > 0) {
     int page = -1;  // paged: of this thread's row, for the loads of the step after next
     if constexpr (!kPaged) {
       dma(false, 0, 0);
@@ -393,28 +406,28 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
       });
       ring_fence<(NS - 1) * 2 * S::DMA>();  // K of step 0
     } else {
-      const int key = begin + (tid & (kTileKeys - 1));
+      const int key = key_of(0) + (tid & (kTileKeys - 1));
       place_row(0, key, page_number(key));  // K and V of step 0
       store_scale(0, 0);
       __syncthreads();
       load_pieces(false, 0);
       store_pieces(false, 0);
       load_pieces(true, 0);
-      const int k1 = key + kTileKeys;
+      const int k1 = key + STEP;
       place_row(1, k1, page_number(k1));  // K of step 1 (and V's scales of it)
       store_scale(1, 1);
       store_pieces(true, 0);
       __syncthreads();
       load_pieces(false, 1);
-      const int k2 = value_row ? k1 : k1 + kTileKeys;
+      const int k2 = value_row ? k1 : k1 + STEP;
       place_row(0, k2, page_number(k2));  // K of step 2, V of step 1: for step 0's loads
       store_scale(2, 1);
-      page = page_number(k2 + kTileKeys);
+      page = page_number(k2 + STEP);
       store_pieces(false, 1);
       ring_fence<0>();
     }
     f32x16 s0[2], s1[2];
-    if (begin <= wave_any) {
+    if (key_of(0) <= wave_any) {
       s0[0] = s0[1] = f32x16{0};
 #pragma unroll
       for (int n = 0; n < N1; ++n) {
@@ -429,7 +442,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
     }
     auto whole_step = [&](int j, auto slotc, f32x16 (&sc)[2], f32x16 (&sn)[2]) {
       constexpr int slot = decltype(slotc)::value;
-      const int key0 = begin + j * kTileKeys;
+      const int key0 = key_of(j);
       // K of step j + 1 and V of step j are in LDS; K of step j and V of step j - 1 are read
       if constexpr (!kPaged) {
         ring_fence<(NS - 2) * 2 * S::DMA>();
@@ -439,12 +452,16 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
         ring_fence<0>();
         if (j + 1 < steps) load_pieces(false, slot);
       }
-      if (key0 + kTileKeys - 1 > tile_all) {
+      if (begin + (j + 1) * STEP - 1 > tile_all) {  // of any of the groups: all waves come here
         unsigned char* vs = smem + S::V0 + slot * S::BYTES;
-        if (any_not_finite<T>(vs, S::BYTES)) {  // all waves find the same
-          spoilt = true;
+        const bool bad = key0 + kTileKeys - 1 > tile_all && any_not_finite<T>(vs, S::BYTES);  // a group's waves find the same
+        if (KS > 1 || bad) {
           __syncthreads();
-          for (int i = 16 * tid; i < S::BYTES; i += 16 * 64 * NW) *(u32x4*)(vs + i) = finite_only<T>(*(const u32x4*)(vs + i));
+          if (bad) {
+            spoilt = true;
+            if (KS > 1) any_spoilt = 1;
+            for (int i = 16 * tid; i < S::BYTES; i += 16 * 64 * NW) *(u32x4*)(vs + i) = finite_only<T>(*(const u32x4*)(vs + i));
+          }
           __syncthreads();
         }
       }
@@ -455,9 +472,9 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
         if (j + 1 < steps) {
           store_pieces(false, slot);
           load_pieces(true, slot);
-          const int key = key0 + (value_row ? 2 : 3) * kTileKeys + (tid & (kTileKeys - 1));
+          const int key = key0 + (value_row ? 2 : 3) * STEP + (tid & (kTileKeys - 1));
           place_row(slot ^ 1, key, page);
-          page = page_number(key + kTileKeys);
+          page = page_number(key + STEP);
         }
       }
       if (active) second_phase(j, slotc, sc, sn, f);
@@ -468,10 +485,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
         }
       }
     };
-    for (int j = 0; j < steps; j += NS)
+    for (int j = 0; j < turns; j += NS)
       static_for<NS>([&](auto ic) {
         constexpr int i = decltype(ic)::value;
-        if (i == 0 || j + i < steps) {
+        if (i == 0 || j + i < turns) {
           if constexpr (i % 2 == 0) whole_step(j + i, ic, s0, s1);
           else whole_step(j + i, ic, s1, s0);
         }
@@ -480,10 +497,14 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
   }
   static_assert(NS % 2 == 0, "a step's scores change places with the next one's");
 
+  if (KS > 1) {
+    __syncthreads();
+    spoilt = any_spoilt != 0;
+  }
   if (spoilt) {  // add what was made zero (see any_not_finite)
-    for (int j = 0; j < steps; ++j) {
-      const int key0 = begin + j * kTileKeys;
-      if (key0 + kTileKeys - 1 <= tile_all) continue;
+    for (int j = 0; j < turns; ++j) {
+      const int key0 = key_of(j);
+      if (begin + (j + 1) * STEP - 1 <= tile_all) continue;
       ring_fence<0>();  // V's first slot is read
       if constexpr (!kPaged) {
         dma(true, j, 0);
@@ -495,6 +516,7 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
         store_pieces(true, 0);
       }
       ring_fence<0>();
+      if (key0 + kTileKeys - 1 <= tile_all) continue;  // this group's step was left as it is
       for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
@@ -512,11 +534,42 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
     }
   }
 
+  if constexpr (KS == 2) {  // the second group's sums to the first, lane by lane
+    f32x4* to = (f32x4*)all_smem;
+    float* ml = (float*)(to + DB * 4 * 64 * NW);
+    static_assert(S::LDS * KS >= DB * 4 * 64 * NW * 16 + 64 * NW * 8, "LDS");
+    __syncthreads();
+    if (part_k == 1) {
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4)
+          to[(4 * d + r / 4) * 64 * NW + tid] = f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]};
+      ml[tid] = m_ref;
+      ml[64 * NW + tid] = sum;
+    }
+    __syncthreads();
+    if (part_k == 0) {
+      const float m1 = ml[tid], m = fmaxf(m_ref, m1);
+      const float a0 = m_ref == m ? 1.f : exp2_hw((m_ref - m) * unit), a1 = m1 == m ? 1.f : exp2_hw((m1 - m) * unit);
+      sum = sum * a0 + ml[64 * NW + tid] * a1;
+      m_ref = m;
+#pragma unroll
+      for (int d = 0; d < DB; ++d)
+#pragma unroll
+        for (int r = 0; r < 16; r += 4) {
+          const f32x4 x = to[(4 * d + r / 4) * 64 * NW + tid];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) o[d][r + i] = o[d][r + i] * a0 + x[i] * a1;
+        }
+    }
+  }
+
   // ---- out: lane has row `row`, elements 32 d + 8 (r / 4) + 4 half + r % 4 ----
   sum += __shfl_xor(sum, 32);
   if (splits > 1) {
     float* part = part_of_tile(p, BM);
-    if (row < rows) {
+    if (row < rows && part_k == 0) {
       const uint32_t at = part_at(p, BM, split);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
@@ -528,10 +581,10 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
         }
       if (half == 0) store8_coherent(part, at + part_ml(p, BM, row - row0), m_ref * unit, sum);
     }
-    join_if_last<T>(p, sq, kvh, row0, min(BM, rows - row0), part, BM, splits, smem);
+    join_if_last<T, 64 * NW * KS>(p, sq, kvh, row0, min(BM, rows - row0), part, BM, splits, all_smem);
     return;
   }
-  if (row >= rows) return;
+  if (row >= rows || part_k != 0) return;
   const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
   T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
 #pragma unroll
@@ -544,13 +597,16 @@ __global__ void __launch_bounds__(64 * kTileWaves, HD == 256 ? 1 : HD == 64 && K
     }
 }
 
-// hd: the padded head.
+// hd: the padded head; ks: groups of a workgroup, 2 for hd up to 128 only.
 template <typename T, int KIND>
-hipError_t launch_tile_hd(int hd, const AttnParams& p, dim3 grid, hipStream_t s) {
-  const dim3 block(64 * kTileWaves);
-  if (hd == 64) return launch_kernel(attention_tile_kernel<T, 64, KIND, 2>, grid, block, 0, s, p);
-  if (hd == 128) return launch_kernel(attention_tile_kernel<T, 128, KIND, 2>, grid, block, 0, s, p);
-  return launch_kernel(attention_tile_kernel<T, 256, KIND, 2>, grid, block, 0, s, p);
+hipError_t launch_tile_hd(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s) {
+  const dim3 block(64 * kTileWaves * ks);
+  if (hd == 256) return launch_kernel(attention_tile_kernel<T, 256, KIND, 2, 1>, grid, block, 0, s, p);
+  if (ks == 2)
+    return hd == 64 ? launch_kernel(attention_tile_kernel<T, 64, KIND, 2, 2>, grid, block, 0, s, p)
+                    : launch_kernel(attention_tile_kernel<T, 128, KIND, 2, 2>, grid, block, 0, s, p);
+  return hd == 64 ? launch_kernel(attention_tile_kernel<T, 64, KIND, 2, 1>, grid, block, 0, s, p)
+                  : launch_kernel(attention_tile_kernel<T, 128, KIND, 2, 1>, grid, block, 0, s, p);
 }
 
 }  // namespace cmpext3

@@ -225,7 +225,7 @@ def test_plans():
         assert cabi.lib().cmpext3_attention_describe(ctypes.byref(attention_args(**kw)), buf, 256) == 0
         return buf.value.decode()
 
-    assert "attention_few rows=16 keys=paged16" in plan()
+    assert "attention_few rows=16 groups=1 keys=paged16" in plan()
     assert "attention_few rows=32" in plan(len_q=8)
     assert "attention_tile" in plan(len_q=64) and "splits=1 " in plan(len_q=64)
     assert "keys=paged8" in plan(cache=cache_args(kv_dtype=cabi.E4M3, k_scale=0x100, v_scale=0x200))

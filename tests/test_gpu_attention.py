@@ -115,6 +115,23 @@ def test_long_keys_are_split(causal):
         R.check(got[i], *R.attention(q[i], k[i], v[i], 128**-0.5, causal))
 
 
+@pytest.mark.parametrize("n", [511, 512, 700, 1100, 2100])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_few_tiles_share_their_keys(n, dim):
+    """Prompts with fewer row tiles than CUs: two groups of waves, and splits, over a tile's keys."""
+    packed(BF16, [n], [n], 2, 1, dim, True, seed=n)
+    packed(F16, [n, 5, 0, n - 300], [n, 70, 9, n], 2, 2, dim, False, seed=n)
+    def spoil(q, k, v):
+        k[n - 65 : n - 60] = float("nan")
+        v[n - 65 : n - 60] = float("inf")
+    q, k, v = (rand((n, 2, dim), BF16, s) for s in (1, 2, 3))
+    one = torch.tensor([0, n], dtype=torch.int32, device="cuda")
+    clean = cmpext3.attention(q.cuda(), k.cuda(), v.cuda(), one, one).cpu()
+    spoil(q, k, v)
+    got = cmpext3.attention(q.cuda(), k.cuda(), v.cuda(), one, one).cpu()
+    assert torch.equal(got[: n - 65], clean[: n - 65]) and not got[n - 60 :].isfinite().any()
+
+
 def test_large_scores():
     """Scores of some thousands, growing along the keys (the running maximum keeps moving), and a
     maximum that the first keys hold."""

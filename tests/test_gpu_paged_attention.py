@@ -102,6 +102,40 @@ def test_long_sequences_are_split(held, dim):
     paged(BF16, held, [40, 3, 70], [5000, 17, 2049], 8, 2, dim, 64, seed=2, spoil=True)
 
 
+@pytest.mark.parametrize("held", [BF16, F8])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("new,lens", [([64], [3000]), ([70, 1, 33, 9, 50], [700, 1, 1500, 40, 64]), ([100] * 6, [100, 1900, 130, 64, 65, 700]),
+                                      ([40], [9000]), ([300, 200], [9000, 400])])
+def test_chunks_share_their_keys(held, dim, new, lens):
+    """Chunks over few row tiles: groups of waves and splits of a tile's keys, joined in both ways."""
+    paged(BF16, held, new, lens, 4, 2, dim, 64, seed=sum(lens), spoil=True)
+    paged(BF16, held, new, lens, 4, 2, dim, 64, seed=sum(lens), spoil=True, causal=False)
+
+
+def test_a_long_cache_past_32_bits():
+    """Chunks and single tokens over pages whose elements lie past 2^32 bytes, both kinds of cache."""
+    page, heads, dim = 64, 8, 128
+    pages = (5 << 30) // (page * heads * dim * 2)
+    k = torch.empty(pages, page, heads, dim, dtype=F16, device="cuda")
+    k8, v8 = (torch.empty(2 * pages, page, heads, dim, dtype=F8, device="cuda") for _ in range(2))
+    ks, vs = (torch.empty(2 * pages, page, heads, device="cuda") for _ in range(2))
+    x, y = rand((2 * page, heads, dim), F16, 3), rand((2 * page, heads, dim), F16, 4)
+    table = torch.tensor([[pages - 1, pages - 3]], dtype=torch.int32)
+    table8 = torch.tensor([[2 * pages - 2, 2 * pages - 1]], dtype=torch.int32)
+    slots = (table[0].long()[:, None] * page + torch.arange(page)).flatten().cuda()
+    slots8 = (table8[0].long()[:, None] * page + torch.arange(page)).flatten().cuda()
+    cmpext3.kv_cache_write(x.cuda(), x.cuda(), k, k, slots)
+    cmpext3.kv_cache_write(x.cuda(), y.cuda(), k8, v8, slots8, ks, vs)
+    n = torch.tensor([2 * page - 3], dtype=torch.int32, device="cuda")
+    for new in (1, 90):
+        q = rand((new, heads, dim), F16, new)
+        cu = torch.tensor([0, new], dtype=torch.int32, device="cuda")
+        got = cmpext3.paged_attention(q.cuda(), k, k, table.cuda(), n, cu)
+        R.check(got, *R.attention(q, x[:-3], x[:-3], dim**-0.5, True))
+        got = cmpext3.paged_attention(q.cuda(), k8, v8, table8.cuda(), n, cu, k_scale=ks, v_scale=vs)
+        R.check(got, *R.attention(q, R.dequantise(*R.quantise(x))[:-3], R.dequantise(*R.quantise(y))[:-3], dim**-0.5, True))
+
+
 def test_empty_sequences():
     got = paged(BF16, BF16, [1, 1, 1], [0, 5, 0], 4, 2, 64, 16)
     assert not got[0].any() and not got[2].any() and got[1].any()
