@@ -17,7 +17,8 @@ using namespace cmpext3;
 namespace {
 
 constexpr int kMostDim = 256;  // of a head, in attention and cache
-constexpr int64_t kMostGrid = INT_MAX;
+constexpr int64_t kMostThreads = UINT32_MAX;  // of a grid, in one direction
+constexpr int kMostHeads = 0xffff;
 
 bool aligned(const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; }
 bool of8(int64_t a, int64_t b) { return a % 8 == 0 && b % 8 == 0; }
@@ -26,6 +27,7 @@ bool of8(int64_t a, int64_t b) { return a % 8 == 0 && b % 8 == 0; }
 int check_cache(const cmpext3_kv_cache& c, bool paged) {
   if (c.kv_dtype != CMPEXT3_F16 && c.kv_dtype != CMPEXT3_BF16 && c.kv_dtype != CMPEXT3_E4M3) return CMPEXT3_ERR_UNSUPPORTED;
   if (c.kv_heads <= 0 || c.dim <= 0) return CMPEXT3_ERR_INVALID_ARG;
+  if (c.kv_heads > kMostHeads) return CMPEXT3_ERR_TOO_LARGE;
   if (c.dim % 8 != 0 || c.dim > kMostDim) return CMPEXT3_ERR_UNSUPPORTED;
   // rows of 8 elements: 16 bytes, or 8 of codes
   const size_t row = c.kv_dtype == CMPEXT3_E4M3 ? 8 : 16;
@@ -74,6 +76,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   if (st != CMPEXT3_OK) return st;
   if (c.kv_dtype != a->dtype && !(paged && c.kv_dtype == CMPEXT3_E4M3)) return CMPEXT3_ERR_UNSUPPORTED;
   if (a->batch < 0 || a->heads <= 0 || a->heads % c.kv_heads != 0) return CMPEXT3_ERR_INVALID_ARG;
+  if (a->heads > kMostHeads) return CMPEXT3_ERR_TOO_LARGE;
   if (!(a->scale > 0.f) || !isfinite(a->scale)) return CMPEXT3_ERR_INVALID_ARG;
   const bool uniform_q = a->starts_q == nullptr;
   if (uniform_q ? a->len_q < 0 : a->total_q < 0) return CMPEXT3_ERR_INVALID_ARG;
@@ -128,7 +131,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   const int bm = r.rows = r.blocks16 ? 16 * r.blocks16 : 128;
   const int64_t slots = uniform_q ? (int64_t)a->batch * (((int64_t)a->len_q * group + bm - 1) / bm)
                                   : queries * group / bm + a->batch;
-  if (slots * c.kv_heads > kMostGrid) return CMPEXT3_ERR_TOO_LARGE;
+  if (slots * c.kv_heads * 512 > kMostThreads) return CMPEXT3_ERR_TOO_LARGE;
   p.slots = (int)slots;
   // Split the keys where the row tiles alone leave CUs idle.
   const int64_t groups = slots * c.kv_heads;
@@ -253,9 +256,9 @@ extern "C" int cmpext3_qk_norm_rope(const cmpext3_qk_norm_rope_args* a, void* st
   if (a->heads < 0 || a->kv_heads < 0 || a->tokens < 0 || a->dim <= 0 || a->table_rows < 0) return CMPEXT3_ERR_INVALID_ARG;
   if (a->rotary_dim < 0 || a->rotary_dim % 2 != 0 || a->rotary_dim > a->dim) return CMPEXT3_ERR_INVALID_ARG;
   if (a->dim > 1024) return CMPEXT3_ERR_UNSUPPORTED;
-  if (a->heads > 0xffff || a->kv_heads > 0xffff) return CMPEXT3_ERR_TOO_LARGE;
+  if (a->heads > kMostHeads || a->kv_heads > kMostHeads) return CMPEXT3_ERR_TOO_LARGE;
   const int64_t units = a->tokens * (a->heads + a->kv_heads);
-  if (a->tokens > INT64_MAX / (1 << 24) || units > kMostGrid) return CMPEXT3_ERR_TOO_LARGE;
+  if (a->tokens > INT64_MAX / (1 << 24) || units * 64 > kMostThreads) return CMPEXT3_ERR_TOO_LARGE;  // a wave per head
   if (units == 0) return CMPEXT3_OK;
   if ((a->heads > 0 && (a->q == nullptr || a->q_out == nullptr)) || (a->kv_heads > 0 && (a->k == nullptr || a->k_out == nullptr)) ||
       a->positions == nullptr || (a->rotary_dim > 0 && a->table_rows > 0 && (a->cos == nullptr || a->sin == nullptr)))
@@ -288,8 +291,7 @@ int cache_params(CacheParams& p, const cmpext3_kv_cache* cache, int dtype, int64
   const int st = check_cache(*cache, true);
   if (st != CMPEXT3_OK) return st;
   if (cache->kv_dtype != CMPEXT3_E4M3 && cache->kv_dtype != dtype) return CMPEXT3_ERR_UNSUPPORTED;
-  // one thread for 8 elements, at least 8 threads a row
-  if (tokens > INT_MAX || tokens * cache->kv_heads > (int64_t)INT_MAX * 2) return CMPEXT3_ERR_TOO_LARGE;
+  if (tokens > INT_MAX || tokens * cache->kv_heads * 32 > kMostThreads) return CMPEXT3_ERR_TOO_LARGE;  // 32 threads a row at most
   set_source(p.kv, *cache);
   p.kv_heads = cache->kv_heads;
   p.dim = cache->dim;

@@ -162,7 +162,8 @@ BAD, NOT, BIG = cabi.ERR_INVALID_ARG, cabi.ERR_UNSUPPORTED, cabi.ERR_TOO_LARGE
     (dict(scale=0.0), BAD), (dict(scale=-1.0), BAD), (dict(scale=float("inf")), BAD), (dict(scale=float("nan")), BAD),
     (dict(len_q=-1), BAD), (dict(q=None), BAD), (dict(out=None), BAD), (dict(q=0x10008), BAD), (dict(out=0x20004), BAD),
     (dict(q_token=511), BAD), (dict(q_head=60), BAD), (dict(out_token=510), BAD), (dict(table_pages=-1), BAD),
-    (dict(seq_lens=None), BAD), (dict(table_pages=1 << 28), BIG), (dict(len_q=1 << 30), BIG),
+    (dict(seq_lens=None), BAD), (dict(table_pages=1 << 28), BIG), (dict(len_q=1 << 30), BIG), (dict(heads=1 << 17), BIG),
+    (dict(batch=1 << 23), BIG),
 ])
 def test_attention_rejects_before_launch(kw, err):
     a = attention_args(**kw)
@@ -174,7 +175,7 @@ def test_attention_rejects_before_launch(kw, err):
     (dict(kv_dtype=cabi.BF16), NOT), (dict(kv_dtype=cabi.F32), NOT), (dict(kv_dtype=7), NOT), (dict(kv_heads=0), BAD),
     (dict(dim=0), BAD), (dict(dim=60), NOT), (dict(dim=264), NOT), (dict(k=0x1008), BAD), (dict(v=0x2004), BAD),
     (dict(k_page=2047), BAD), (dict(v_token=124), BAD), (dict(k_head=68), BAD), (dict(pages=-1), BAD), (dict(page_size=0), BAD),
-    (dict(k=None), BAD), (dict(kv_dtype=cabi.E4M3), BAD),
+    (dict(k=None), BAD), (dict(kv_dtype=cabi.E4M3), BAD), (dict(kv_heads=1 << 17), BIG),
 ])
 def test_caches_are_checked(kw, err):
     a = attention_args(cache=cache_args(**kw))
@@ -246,5 +247,5 @@ def test_qk_norm_rope_c_abi_rejects():
     for kw in (dict(dim=0), dict(tokens=-1), dict(heads=-1), dict(rotary_dim=66), dict(rotary_dim=3), dict(rotary_dim=-2), dict(q=None),
                dict(k_out=None), dict(positions=None), dict(cos=None), dict(table_rows=-1)):
         assert call(**kw) == BAD, kw
-    assert call(tokens=1 << 40) == BIG and call(heads=1 << 20) == BIG
+    assert call(tokens=1 << 40) == BIG and call(heads=1 << 20) == BIG and call(tokens=1 << 24) == BIG
     assert call(tokens=0, q=None) == 0 and call(heads=0, kv_heads=0) == 0
