@@ -335,7 +335,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
     pw[t / 4][t % 4] = w;
   };
 
-  constexpr int AHEAD = kPaged ? 2 : 4;    // fragments on their way from LDS
+  constexpr int AHEAD = 2;                 // fragments on their way from LDS (four, six: no faster)
   constexpr int N1 = 2 * KK, N2 = 4 * DB;  // products of the two phases
   constexpr int FIRST = 10;                // pairs of weights in the first phase (of 16), LEAD of them before
   constexpr int LEAD = 2;                  //   its first product, while that one's fragment arrives
