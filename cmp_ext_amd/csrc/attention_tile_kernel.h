@@ -4,8 +4,9 @@
 // Rows: a workgroup of four waves takes 128 rows of one sequence and one kv head, a row being one
 // query of one head of the group (row r: query r / group, head r % group), so that grouped heads
 // share each step's keys and values and short sequences fill their tiles.  A wave owns 32 rows.
-// (8192 tokens, 32 heads of 128 on MI355X: 520 us; eight waves over 256 rows, whose barriers bind
-// all waves of a CU together, 550; four waves of 64 rows with a SIMD to themselves 643.)
+// (8192 tokens, 32 heads of 128 and 8 of keys, bf16, on MI355X: 529 us, 1040 TFLOP/s of the products
+// that are not masked; eight waves over 256 rows, whose barriers bind all waves of a CU together, 548;
+// four waves of 64 rows with a SIMD to themselves 643.)
 //
 // Keys: where there are fewer tiles than CUs, a workgroup has two such groups of four waves (KS = 2),
 // one for the even steps and one for the odd ones, each with its own LDS, joined in LDS at the end:
@@ -26,15 +27,22 @@
 // a share of the vector work, kept in that order: the scores of step j + 1 beside the first
 // weights of step j, then the weighted values of step j beside its other weights and the maximum
 // of step j + 1.  The vector work (per score: scale, exponential at half the rate, sum, half a
-// conversion, half a maximum) is over half as long as the products.
+// conversion, half a maximum) is over half as long as the products.  On that prompt the matrix cores
+// are busy 53 % of the cycles and the vector units 45 %, and a wave waits for LDS or its barrier
+// 29 % of its time; with the loads into LDS left out it would take 463 us, with the exponentials left
+// out 503, with V's fragments 519, with K and V from L2 512: no single one of them bounds it.
 //
-// Keys and values of a step lie in LDS as rows of HD 16-bit elements in rings of NS slots, K
+// The weights are rounded once to 16 bits for the second product, their sum is of the unrounded
+// ones: the result is off by its own rounding and by one of the same size more.
+//
+// Keys and values of a step lie in LDS as rows of HD 16-bit elements in two slots each, K
 // with its 16-byte chunks and V with its 64-byte segments permuted by the row so that the reads
 // of both products hit all banks.  Packed ones come by LDS DMA, which zero fills what lies past
 // the sequence or the head; pages go through registers (any page size, 8-bit codes converted on
-// the way), their rows' addresses shared through LDS and their page numbers fetched steps ahead.
-// One barrier a step: K of step j + NS and V of step j + NS - 1 start to load behind it, into the
-// slots that the step before has read.
+// the way; one set of them, for K in the first phase and V in the second: with two, 93 spills made
+// chunks over 8 bits 206 us instead of 141), their rows' addresses shared through LDS and their page
+// numbers fetched steps ahead.  One barrier a step: K of step j + 2 and V of step j + 1 start to load
+// behind it, into the slots that the step before has read; they land well within a step.
 #pragma once
 
 #include "attention_join.h"
@@ -45,18 +53,19 @@ constexpr float kLazy = 8.0f;  // in powers of two
 
 constexpr int kTileWaves = 4;
 
-template <int HD, bool PAGED, int NS>
+constexpr int kSlots = 2;  // of K and of V
+
+template <int HD, bool PAGED>
 struct TileShape {
   static constexpr int ROW = HD * 2;             // bytes of a key's row in LDS
   static constexpr int BYTES = kTileKeys * ROW;  // K or V of a step
-  static constexpr int V0 = NS * BYTES;          // K's slots, then V's
-  static constexpr int ROWS_AT = 2 * NS * BYTES;    // paged: byte offsets of the rows of K and V, two steps'
+  static constexpr int V0 = kSlots * BYTES;          // K's slots, then V's
+  static constexpr int ROWS_AT = 2 * kSlots * BYTES;  // paged: byte offsets of the rows of K and V, two steps'
   static constexpr int SCALES = ROWS_AT + 2 * 2 * kTileKeys * 8;  // 8 bits: scales of K and V, four steps'
   static constexpr int LDS = PAGED ? SCALES + 4 * 2 * kTileKeys * 4 : ROWS_AT;
   static constexpr int DMA = BYTES / 1024 / kTileWaves;  // 1 KB LDS-DMA loads per wave of K, and of V
   static_assert(BYTES % (1024 * kTileWaves) == 0, "whole DMA loads per wave");
   static_assert(LDS <= 160 * 1024 && LDS >= kJoinBytes, "LDS budget");
-  static_assert(!PAGED || NS == 2, "pages are loaded one step ahead");
 };
 
 // Byte offset in a K slot of the 16-byte chunk `chunk` of row `row`: 16 rows at one chunk
@@ -79,10 +88,10 @@ __device__ __forceinline__ int v_place(int row, int byte_col) {
 }
 
 // Two waves share a SIMD's registers (packed heads up to 64: three; over 128: one has them all).
-template <typename T, int HD, int KIND, int NS, int KS>
+template <typename T, int HD, int KIND, int KS>
 __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64 && KIND == kKvPacked && KS == 1 ? 3 : 2) attention_tile_kernel(const AttnParams p) {
   constexpr bool kPaged = KIND != kKvPacked, k8 = KIND == kKvPaged8;
-  using S = TileShape<HD, kPaged, NS>;
+  using S = TileShape<HD, kPaged>;
   constexpr int KK = HD / 16, DB = HD / 32, NW = kTileWaves, BM = 32 * NW;
   __shared__ __attribute__((aligned(1024))) unsigned char all_smem[S::LDS * KS];
   __shared__ int any_spoilt;
@@ -342,7 +351,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   // step j: sc its scores, sn those of step j + 1 (past the last step whatever the slot holds, all
   // of it masked); f: fragments on their way
   auto first_phase = [&](int j, auto slotc, f32x16 (&sc)[2], f32x16 (&sn)[2], u32x4 (&f)[AHEAD]) {
-    constexpr int slot = decltype(slotc)::value, next = (slot + 1) % NS;
+    constexpr int slot = decltype(slotc)::value, next = slot ^ 1;
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) f[n] = k_frag(next, n);
     sn[0] = sn[1] = f32x16{0};
@@ -399,12 +408,9 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
     int page = -1;  // paged: of this thread's row, for the loads of the step after next
     if constexpr (!kPaged) {
       dma(false, 0, 0);
-      static_for<NS - 1>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        dma(false, i + 1, i + 1);
-        dma(true, i, i);
-      });
-      ring_fence<(NS - 1) * 2 * S::DMA>();  // K of step 0
+      dma(false, 1, 1);
+      dma(true, 0, 0);
+      ring_fence<2 * S::DMA>();  // K of step 0
     } else {
       const int key = key_of(0) + (tid & (kTileKeys - 1));
       place_row(0, key, page_number(key));  // K and V of step 0
@@ -444,12 +450,11 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       constexpr int slot = decltype(slotc)::value;
       const int key0 = key_of(j);
       // K of step j + 1 and V of step j are in LDS; K of step j and V of step j - 1 are read
+      ring_fence<0>();
       if constexpr (!kPaged) {
-        ring_fence<(NS - 2) * 2 * S::DMA>();
-        dma(false, j + NS, slot);
-        dma(true, j + NS - 1, (slot + NS - 1) % NS);
+        dma(false, j + 2, slot);
+        dma(true, j + 1, slot ^ 1);
       } else {
-        ring_fence<0>();
         if (j + 1 < steps) load_pieces(false, slot);
       }
       if (begin + (j + 1) * STEP - 1 > tile_all) {  // of any of the groups: all waves come here
@@ -485,17 +490,13 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
         }
       }
     };
-    for (int j = 0; j < turns; j += NS)
-      static_for<NS>([&](auto ic) {
-        constexpr int i = decltype(ic)::value;
-        if (i == 0 || j + i < turns) {
-          if constexpr (i % 2 == 0) whole_step(j + i, ic, s0, s1);
-          else whole_step(j + i, ic, s1, s0);
-        }
-      });
+    // a step's scores change places with the next one's
+    for (int j = 0; j < turns; j += 2) {
+      whole_step(j, std::integral_constant<int, 0>{}, s0, s1);
+      if (j + 1 < turns) whole_step(j + 1, std::integral_constant<int, 1>{}, s1, s0);
+    }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no LDS DMA may outlive its slot's use, or the workgroup
   }
-  static_assert(NS % 2 == 0, "a step's scores change places with the next one's");
 
   if (KS > 1) {
     __syncthreads();
@@ -601,12 +602,12 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
 template <typename T, int KIND>
 hipError_t launch_tile_hd(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s) {
   const dim3 block(64 * kTileWaves * ks);
-  if (hd == 256) return launch_kernel(attention_tile_kernel<T, 256, KIND, 2, 1>, grid, block, 0, s, p);
+  if (hd == 256) return launch_kernel(attention_tile_kernel<T, 256, KIND, 1>, grid, block, 0, s, p);
   if (ks == 2)
-    return hd == 64 ? launch_kernel(attention_tile_kernel<T, 64, KIND, 2, 2>, grid, block, 0, s, p)
-                    : launch_kernel(attention_tile_kernel<T, 128, KIND, 2, 2>, grid, block, 0, s, p);
-  return hd == 64 ? launch_kernel(attention_tile_kernel<T, 64, KIND, 2, 1>, grid, block, 0, s, p)
-                  : launch_kernel(attention_tile_kernel<T, 128, KIND, 2, 1>, grid, block, 0, s, p);
+    return hd == 64 ? launch_kernel(attention_tile_kernel<T, 64, KIND, 2>, grid, block, 0, s, p)
+                    : launch_kernel(attention_tile_kernel<T, 128, KIND, 2>, grid, block, 0, s, p);
+  return hd == 64 ? launch_kernel(attention_tile_kernel<T, 64, KIND, 1>, grid, block, 0, s, p)
+                  : launch_kernel(attention_tile_kernel<T, 128, KIND, 1>, grid, block, 0, s, p);
 }
 
 }  // namespace cmpext3
