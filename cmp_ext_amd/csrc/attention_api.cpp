@@ -88,15 +88,16 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
 
   AttnPlan r{};
   AttnParams& p = r.p;
-  const int64_t queries = uniform_q ? (int64_t)a->batch * a->len_q : a->batch > 0 ? a->total_q : 0;
+  const int64_t queries = uniform_q ? (int64_t)a->batch * a->len_q : a->total_q;
   r.empty = queries == 0;
   if (!r.empty && (a->q == nullptr || a->out == nullptr)) return CMPEXT3_ERR_INVALID_ARG;
   if (paged && (a->table_pages < 0 || (a->batch > 0 && a->seq_lens == nullptr))) return CMPEXT3_ERR_INVALID_ARG;
   const int64_t keys = paged ? (int64_t)a->table_pages * c.page_size : uniform_k ? a->len_k : a->total_k;
   if (!paged && keys > 0 && !r.empty && (c.k == nullptr || c.v == nullptr)) return CMPEXT3_ERR_INVALID_ARG;
   const int group = a->heads / c.kv_heads;
-  // rows and keys are counted in 32 bits, packed keys addressed within a step in 32
-  if (keys > INT_MAX - kTileKeys) return CMPEXT3_ERR_TOO_LARGE;
+  // rows and keys are counted in 32 bits, sums of two numbers of keys too; packed keys addressed
+  // within a step in 32
+  if (keys > INT_MAX / 2) return CMPEXT3_ERR_TOO_LARGE;
   if (queries * group > INT_MAX - 256) return CMPEXT3_ERR_TOO_LARGE;
   if (!paged && (c.k_token < 0 || c.v_token < 0 || std::max(c.k_token, c.v_token) > INT_MAX / (2 * kTileKeys) - kMostDim))
     return CMPEXT3_ERR_TOO_LARGE;
@@ -125,16 +126,17 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     *out = r;
     return CMPEXT3_OK;
   }
-  const int64_t mean_rows = queries * group / a->batch;  // of a sequence and kv head
+  const int64_t mean_rows = queries * group / std::max(a->batch, 1);  // of a sequence and kv head
   r.ks = 1;
   r.blocks16 = paged && mean_rows <= 32 ? (mean_rows <= 16 || r.hd == 256 ? 1 : 2) : 0;
   const int bm = r.rows = r.blocks16 ? 16 * r.blocks16 : 128;
-  const int64_t slots = uniform_q ? (int64_t)a->batch * (((int64_t)a->len_q * group + bm - 1) / bm)
+  const int64_t tiles = uniform_q ? (int64_t)a->batch * (((int64_t)a->len_q * group + bm - 1) / bm)
                                   : queries * group / bm + a->batch;
+  const int64_t slots = uniform_q ? tiles : tiles + 2;  // and the rows before and behind all sequences
   if (slots * c.kv_heads * 512 > kMostThreads) return CMPEXT3_ERR_TOO_LARGE;
   p.slots = (int)slots;
   // Split the keys where the row tiles alone leave CUs idle.
-  const int64_t groups = slots * c.kv_heads;
+  const int64_t groups = tiles * c.kv_heads;
   int64_t n = 1;  // splits of the longest sequence
   int least = 0;  // keys of a split at least
   if (r.blocks16) {
@@ -185,7 +187,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     if (splits > 1) {
       p.splits = (int)splits;
       p.split_keys = (int)per;
-      r.ws_bytes = groups * splits * bm * (c.dim + 2) * 4;
+      r.ws_bytes = slots * c.kv_heads * splits * bm * (c.dim + 2) * 4;
     }
   }
   *out = r;

@@ -12,7 +12,7 @@ struct Seq {
   int b;           // -1: none
   int q0, len_q;   // first row in the packed queries, number of queries
   int k0, len_k;
-  int tile;        // row tile of the sequence (or query, seq_of_slot)
+  int tile;        // row tile of the sequence
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -22,18 +22,19 @@ __device__ __forceinline__ int paged_keys(const AttnParams& p, int seq_len) {
   return (int)min((int64_t)max(seq_len, 0), (int64_t)p.kv.table_pages * p.kv.page_size);
 }
 
-// The sequence that holds row tile `slot` of the grid (rows > 0), or, with rows = 0, the packed
-// query `slot`; and which of its tiles of `rows` rows it is (a row is one query of one head of
-// the group).  With packed queries, sequence b owns the slots from starts_q[b] * group / rows + b
-// on: these grow by at least one per sequence and by no less than its tiles, so the grid needs no
-// lengths from the host; slots past a sequence's last tile have nothing to do (b = -1).  Each lane
-// looks at one sequence, 64 at a time, and loads all that is known of it at once: what follows
-// waits for one memory access, not for three in a row.
+// The sequence that holds row tile `slot` of the grid, and which of its tiles of `rows` rows that is
+// (a row is one query of one head of the group).  With packed queries, the rows before the first
+// sequence and those past the last one count as sequences without keys, e = 0 and batch + 1 (zeros
+// go out), sequence b as e = b + 1; e owns the slots from (its first query) * group / rows + e on: these
+// grow by at least one per sequence and by no less than its tiles, so the grid needs no lengths
+// from the host; slots past a sequence's last tile have nothing to do (b = -1).  Each lane looks
+// at one sequence, 64 at a time, and loads all that is known of it at once: what follows waits for
+// one memory access, not for three in a row.
 __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int rows) {
   Seq s;
   int start_k = 0, end_k = p.len_k;  // or, paged, the length as end_k
   if (p.starts_q == nullptr) {
-    const int tiles = rows > 0 ? (p.len_q * p.group + rows - 1) / rows : p.len_q;
+    const int tiles = (p.len_q * p.group + rows - 1) / rows;
     s.b = slot / tiles;
     s.tile = slot - s.b * tiles;
     s.q0 = 0;
@@ -47,33 +48,35 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
   } else {
     const int lane = threadIdx.x & 63;
     int at = -1, first = 0, q_from = 0, q_to = 0, k_from = 0, k_to = 0;
-    for (int b0 = 0; b0 < p.batch; b0 += 64) {
-      const int b = min(b0 + lane, p.batch - 1);
-      const int from = p.starts_q[b], to = p.starts_q[b + 1];
+    for (int e0 = 0; e0 < p.batch + 2; e0 += 64) {
+      const int e = min(e0 + lane, p.batch + 1), b = clampi(e - 1, 0, max(p.batch - 1, 0));
+      int from = p.starts_q[max(e - 1, 0)], to = p.starts_q[min(e, p.batch)];
       int kf = 0, kt = p.len_k;
-      if (p.kv.table != nullptr) {
-        kt = p.seq_lens[b];
-      } else if (p.starts_k != nullptr) {
-        kf = p.starts_k[b];
-        kt = p.starts_k[b + 1];
+      if (p.batch > 0) {
+        if (p.kv.table != nullptr) {
+          kt = p.seq_lens[b];
+        } else if (p.starts_k != nullptr) {
+          kf = p.starts_k[b];
+          kt = p.starts_k[b + 1];
+        }
       }
+      if (e == 0) from = 0, kf = kt = 0;
+      if (e == p.batch + 1) to = p.total_q, kf = kt = 0;
       const int q = clampi(from, 0, p.total_q);
-      const bool below = b0 + lane < p.batch && (rows > 0 ? q * p.group / rows + b : q) <= slot;
+      const bool below = e0 + lane < p.batch + 2 && q * p.group / rows + e <= slot;
       const unsigned long long m = __builtin_amdgcn_ballot_w64(below);
       const int n = __builtin_popcountll(m);
       if (n > 0) {
         at = n - 1;
-        first = b0;
+        first = e0;
         q_from = q, q_to = to, k_from = kf, k_to = kt;
       }
       if (n < 64) break;
     }
-    s.b = -1;
-    if (at < 0) return s;
-    s.b = first + at;
     s.q0 = __builtin_amdgcn_readlane(q_from, at);
     s.len_q = clampi(__builtin_amdgcn_readlane(q_to, at), s.q0, p.total_q) - s.q0;
-    s.tile = rows > 0 ? slot - (s.q0 * p.group / rows + s.b) : slot - s.q0;
+    s.tile = slot - (s.q0 * p.group / rows + first + at);
+    s.b = clampi(first + at - 1, 0, max(p.batch - 1, 0));
     start_k = __builtin_amdgcn_readlane(k_from, at);
     end_k = __builtin_amdgcn_readlane(k_to, at);
   }
@@ -81,12 +84,12 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
   s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
   s.len_q = __builtin_amdgcn_readfirstlane(s.len_q);
   s.tile = __builtin_amdgcn_readfirstlane(s.tile);
-  const int tiles = rows > 0 ? (s.len_q * p.group + rows - 1) / rows : s.len_q;
+  const int tiles = (s.len_q * p.group + rows - 1) / rows;
   if (s.tile < 0 || s.tile >= tiles) {
     s.b = -1;
     return s;
   }
-  if (rows > 0) s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
+  s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
   if (p.kv.table != nullptr) {
     s.k0 = 0;
     s.len_k = paged_keys(p, end_k);
@@ -95,7 +98,7 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
     s.len_k = clampi(end_k, s.k0, p.total_k) - s.k0;
   } else {
     s.k0 = 0;
-    s.len_k = p.len_k;
+    s.len_k = end_k;
   }
   s.k0 = __builtin_amdgcn_readfirstlane(s.k0);
   s.len_k = __builtin_amdgcn_readfirstlane(s.len_k);
@@ -105,6 +108,12 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
 // Keys that the sequence's row `row`, and all before it, may see end here.
 __device__ __forceinline__ int keys_end(const AttnParams& p, const Seq& s, int row) {
   return p.causal ? min(s.len_k, row / p.group + s.len_k - s.len_q + 1) : s.len_k;
+}
+
+// What a row's sum is multiplied by, with the weights' sum l: 1 / l, and 0 if the row sees no key (one
+// whose scores are all -inf sees keys, and has no largest one: infinity, which makes its zeros NaN).
+__device__ __forceinline__ float row_factor(const AttnParams& p, const Seq& s, int row, float l) {
+  return keys_end(p, s, row) > 0 ? 1.f / l : 0.f;
 }
 
 // The page of key `key` and its place in the page; -1 where the table names no page of the cache.

@@ -340,20 +340,18 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : 
     for (int w = 0; w < kFewWaves; ++w) m = fmaxf(m, ml[(w * S::BM + r) * 2]);
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
-    if (m != -INFINITY) {
 #pragma unroll
-      for (int w = 0; w < kFewWaves; ++w) {
-        const float f = exp2_hw(ml[(w * S::BM + r) * 2] - m);
-        l += f * ml[(w * S::BM + r) * 2 + 1];
-        acc += f * *(const f32x4*)((const float*)smem + (w * S::BM + r) * S::PITCH + e);
-      }
+    for (int w = 0; w < kFewWaves; ++w) {
+      const float f = m == -INFINITY ? 0.f : exp2_hw(ml[(w * S::BM + r) * 2] - m);  // times a sum of NaN: still NaN
+      l += f * ml[(w * S::BM + r) * 2 + 1];
+      acc += f * *(const f32x4*)((const float*)smem + (w * S::BM + r) * S::PITCH + e);
     }
     if (splits > 1) {
       store16_coherent(part, part_at(p, S::BM, split) + part_o(p, r) + 4 * e, acc);
       if (e == 0) store8_coherent(part, part_at(p, S::BM, split) + part_ml(p, S::BM, r), m, l);
     } else {
       const int tok = row / p.group, head = kvh * p.group + row - tok * p.group;
-      const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+      const float inv = row_factor(p, sq, row, l);
       T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
       *(u32x2*)(op + e) = u32x2{round2<T>(acc[0] * inv, acc[1] * inv), round2<T>(acc[2] * inv, acc[3] * inv)};
     }

@@ -116,7 +116,7 @@ __device__ __forceinline__ void join_rows(const AttnParams& p, const Seq& sq, in
       l += f * __uint_as_float(load8_coherent(part, part_at(p, bm, s) + part_ml(p, bm, r)).y);
     }
   for (int x = 1; x < lanes; x <<= 1) l += __shfl_xor(l, x);
-  if (r < rows && tid % lanes == 0) inv[r] = l > 0.f || l != l ? 1.f / l : 0.f;
+  if (r < rows && tid % lanes == 0) inv[r] = row_factor(p, sq, row0 + r, l);
   __syncthreads();
   const int items = rows * (p.dim / 4);
   if (items <= THREADS / 2)

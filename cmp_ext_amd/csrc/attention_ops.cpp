@@ -335,6 +335,7 @@ torch::Tensor paged_attention(const torch::Tensor& q_in, const torch::Tensor& k_
   a.causal = causal;
   if (given(cu_q)) {
     starts = index_vector(*cu_q, at::kInt, batch + 1, q, op, "cu_seqlens_q");
+    if (batch == 0) return out.zero_();
     a.starts_q = (const int32_t*)starts.data_ptr();
     a.total_q = checked_int(q.size(0), op, "tokens");
   } else {

@@ -112,6 +112,15 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   int end = keys_end(p, sq, min(row0 + BM, rows) - 1);  // of the keys any row of the tile sees
   const int splits = splits_of(p, end);
   if (split >= splits) return;
+  // what only the end of the kernel needs waits in LDS: the loop has no register to spare
+  __shared__ Seq kept_seq;
+  __shared__ int kept_kvh, kept_row0, kept_splits;
+  if (threadIdx.x == 0) {
+    kept_seq = sq;
+    kept_kvh = kvh;
+    kept_row0 = row0;
+    kept_splits = splits;
+  }
   const int begin = split * p.split_keys;
   end = min(end, begin + p.split_keys);
   // steps of this group, and of the group that has most: step j starts at key key_of(j)
@@ -143,7 +152,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   // packed: LDS-DMA loads i of this wave; where lane's 16 bytes of load i come from
   const T* kbase = nullptr;
   const T* vbase = nullptr;
-  uint32_t k_off[kPaged ? 1 : S::DMA], v_off[kPaged ? 1 : S::DMA];
+  uint32_t k_off[S::DMA], v_off[S::DMA];
   constexpr int ROWS1K = 1024 / S::ROW;  // rows of a DMA load
   const int dma_row = wave * S::DMA * ROWS1K + 16 * lane / S::ROW;
   if constexpr (!kPaged) {
@@ -192,7 +201,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   float* scales = (float*)(smem + S::SCALES);  // [step % 4][K, V][64]
   const int32_t* table = kPaged ? p.kv.table + sq.b * p.kv.table_row : nullptr;
   const bool value_row = tid >= kTileKeys;
-  u32x4 reg[kPaged ? PIECES : 1];  // of K in a step's first phase, of V in its second
+  u32x4 reg[PIECES];  // of K in a step's first phase, of V in its second
   float sreg = 0.f;
   auto page_number = [&](int key) -> int {  // of this thread's row
     if (tid >= 2 * kTileKeys || key >= sq.len_k) return -1;
@@ -566,28 +575,38 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
     }
   }
 
-  // ---- out: lane has row `row`, elements 32 d + 8 (r / 4) + 4 half + r % 4 ----
+  // ---- out: lane has row `out_row`, elements 32 d + 8 (r / 4) + 4 half + r % 4 ----
+  __syncthreads();
+  Seq os;
+  os.b = __builtin_amdgcn_readfirstlane(kept_seq.b);
+  os.q0 = __builtin_amdgcn_readfirstlane(kept_seq.q0);
+  os.len_q = __builtin_amdgcn_readfirstlane(kept_seq.len_q);
+  os.len_k = __builtin_amdgcn_readfirstlane(kept_seq.len_k);
+  const int out_kvh = __builtin_amdgcn_readfirstlane(kept_kvh), out_row0 = __builtin_amdgcn_readfirstlane(kept_row0);
+  const int out_splits = __builtin_amdgcn_readfirstlane(kept_splits);
+  const int out_row = out_row0 + wave * 32 + col, out_rows = os.len_q * p.group;
   sum += __shfl_xor(sum, 32);
-  if (splits > 1) {
+  if (out_splits > 1) {
     float* part = part_of_tile(p, BM);
-    if (row < rows && part_k == 0) {
-      const uint32_t at = part_at(p, BM, split);
+    if (out_row < out_rows && part_k == 0) {
+      const uint32_t at = part_at(p, BM, blockIdx.y);
 #pragma unroll
       for (int d = 0; d < DB; ++d)
 #pragma unroll
         for (int r = 0; r < 16; r += 4) {
           const int e = 32 * d + 8 * (r / 4) + 4 * half;
           if (e < p.dim)
-            store16_coherent(part, at + part_o(p, row - row0) + 4 * e, f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]});
+            store16_coherent(part, at + part_o(p, out_row - out_row0) + 4 * e, f32x4{o[d][r], o[d][r + 1], o[d][r + 2], o[d][r + 3]});
         }
-      if (half == 0) store8_coherent(part, at + part_ml(p, BM, row - row0), m_ref * unit, sum);
+      if (half == 0) store8_coherent(part, at + part_ml(p, BM, out_row - out_row0), m_ref * unit, sum);
     }
-    join_if_last<T, 64 * NW * KS>(p, sq, kvh, row0, min(BM, rows - row0), part, BM, splits, all_smem);
+    join_if_last<T, 64 * NW * KS>(p, os, out_kvh, out_row0, min(BM, out_rows - out_row0), part, BM, out_splits, all_smem);
     return;
   }
-  if (row >= rows || part_k != 0) return;
-  const float inv = sum > 0.f || sum != sum ? 1.f / sum : 0.f;
-  T* op = (T*)p.out + sq.b * p.out_batch + (int64_t)(sq.q0 + tok) * p.out_token + (int64_t)head * p.out_head;
+  if (out_row >= out_rows || part_k != 0) return;
+  const float inv = row_factor(p, os, out_row, sum);
+  const int out_tok = out_row / p.group, out_head = out_kvh * p.group + out_row - out_tok * p.group;
+  T* op = (T*)p.out + os.b * p.out_batch + (int64_t)(os.q0 + out_tok) * p.out_token + (int64_t)out_head * p.out_head;
 #pragma unroll
   for (int d = 0; d < DB; ++d)
 #pragma unroll

@@ -101,16 +101,16 @@ int cmpext3_kv_cache_read(const cmpext3_kv_cache* cache, const int32_t* block_ta
  * h / (heads / kv_heads)):
  *   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale * q_i . k_j)
  * over j < len_k, and with `causal` j <= i + len_k - len_q (the last query sees the last
- * key).  A query that sees no key gets zeros.  Products on the matrix cores with fp32 sums,
+ * key).  A query that sees no key gets zeros, one whose scores are all -inf NaN.  Products on the matrix cores with fp32 sums,
  * softmax statistics in fp32, the weights p rounded to the 16-bit type for the second product.
  *
  * Keys and values: packed (cache.k/v with k_token, k_head, ...; block_table NULL), where
  * cache.k_page is the stride between batch entries of uniform length; or paged (block_table
  * set).  cache.dim and cache.kv_heads always hold; cache.pages and page_size for pages only.
  * Lengths: starts_q NULL means batch entries of len_q queries each at a stride of q_batch,
- * else sequence b has rows starts_q[b] .. starts_q[b+1]-1 of total_q (out rows of no
- * sequence are left unwritten); the same for keys with starts_k, len_k, total_k when packed,
- * and seq_lens[b] keys when paged.
+ * else sequence b has rows starts_q[b] .. starts_q[b+1]-1 of total_q, starts_q not falling (rows
+ * before the first sequence and past the last get zeros); the same for keys with starts_k,
+ * len_k, total_k when packed, and seq_lens[b] keys when paged.
  */
 typedef struct cmpext3_attention_args {
   int32_t dtype; /* of q and out: CMPEXT3_F16 or CMPEXT3_BF16 */
