@@ -158,9 +158,16 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     // 48.4 and 44.7; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 148).
     // Splits: two workgroups' worth of waves a CU at once; more where sequences differ (8 bits: one
     // of 512 new tokens over 8192 keys, 136 tiles, 282 us whole, 130 in 3, 107 in 4, 133 in 6).
+    // Where tiles are many, those that see most keys go first, and no keys are split: 32 of up to 300 new
+    // tokens over up to 2000 keys, 1200 tiles, 150 us in the order of the sequences, 95 longest first (60
+    // of up to 100 over 1000, 960 tiles: 65.6 in splits, 42; but 60 of up to 60 over up to 4000, 752
+    // tiles: 131 in splits, 150).  Packed prompts gain nothing by that order (30 of up to 500: 51 and 63).
     const bool ragged = a->batch > 4;
     least = 256;
-    if (r.hd <= 128 && groups <= 256 && (keys <= 4096 || groups <= 32)) {
+    p.longest_first = !uniform_q && ragged && a->batch <= 62 && (groups >= 1024 || (groups >= 512 && keys <= 5 * groups));
+    if (p.longest_first) {
+      n = 1;
+    } else if (r.hd <= 128 && groups <= 256 && (keys <= 4096 || groups <= 32)) {
       r.ks = 2;
       n = std::min<int64_t>(((ragged ? 480 : 256) + groups - 1) / groups, std::max<int64_t>(1, keys / 1024));
     } else {
@@ -245,9 +252,9 @@ extern "C" int cmpext3_attention_describe(const cmpext3_attention_args* args, ch
     if (r.empty)
       snprintf(buf, (size_t)buflen, "kernel=none");
     else
-      snprintf(buf, (size_t)buflen, "kernel=%s rows=%d groups=%d keys=%s head=%d slots=%d splits=%d split_keys=%d",
+      snprintf(buf, (size_t)buflen, "kernel=%s rows=%d groups=%d keys=%s head=%d slots=%d splits=%d split_keys=%d%s",
                r.blocks16 ? "attention_few" : "attention_tile", r.rows, r.ks, kinds[r.kind], r.hd,
-               r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0);
+               r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0, r.p.longest_first ? " order=longest" : "");
   }
   return CMPEXT3_OK;
 }

@@ -22,6 +22,46 @@ __device__ __forceinline__ int paged_keys(const AttnParams& p, int seq_len) {
   return (int)min((int64_t)max(seq_len, 0), (int64_t)p.kv.table_pages * p.kv.page_size);
 }
 
+// Sum of x over this lane and those below it.
+__device__ __forceinline__ int sum_below(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, false);  // 1, 2, 4 and 8 lanes below, in rows of 16
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, false);
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 to row 1, 2 to 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the lower half to the upper
+  return x;
+}
+
+// Row tile `slot` in the order of the keys the tiles see, most first, over all of up to 62 sequences:
+// the sequence's entry e (seq_of_slot) and its tile; e = -1 past the last tile.  Lane e has entry e's
+// queries and keys.  With cost c(i) = max(0, i + 1 + off) of tile i of t (causal, off the keys before
+// its first query, in tiles; else the same for all), the tiles that cost L or more are
+//   n(L) = clamp(t + off - L + 1, 0, t)
+// of an entry; the wanted level is the last with more than `slot` of them in all.
+__device__ __forceinline__ int longest_first(const AttnParams& p, int slot, int rows, int len_q, int len_k, int& tile) {
+  const int lane = threadIdx.x & 63;
+  const int t = lane < p.batch + 2 ? (len_q * p.group + rows - 1) / rows : 0;
+  const int per = max(1, rows / p.group);  // queries of a tile
+  // the cost of the last tile
+  const int h = t == 0 || len_k == 0 ? 0 : p.causal ? t + (len_k - len_q) / per : len_k / per + 1;
+  auto at_least = [&](int level) { return level <= 0 ? t : p.causal ? clampi(h - level + 1, 0, t) : level <= h ? t : 0; };
+  if (__builtin_amdgcn_readlane(sum_below(t), 63) <= slot) return -1;
+  int low = 0;
+  for (int step = 1 << 30; step > 0; step >>= 1) {
+    if (__builtin_amdgcn_ballot_w64(h >= low + step) == 0) continue;
+    if (__builtin_amdgcn_readlane(sum_below(at_least(low + step)), 63) > slot) low += step;
+  }
+  const int above = at_least(low + 1), here = at_least(low) - above;
+  const int before = __builtin_amdgcn_readlane(sum_below(above), 63);
+  const int upto = before + sum_below(here);
+  const int e = __builtin_ctzll(__builtin_amdgcn_ballot_w64(upto > slot));
+  const int te = __builtin_amdgcn_readlane(t, e), he = __builtin_amdgcn_readlane(h, e);
+  const int r = slot - (__builtin_amdgcn_readlane(upto, e) - __builtin_amdgcn_readlane(here, e));
+  tile = clampi(low > 0 && p.causal ? low - 1 - he + te : r, 0, max(te - 1, 0));
+  return e;
+}
+
 // The sequence that holds row tile `slot` of the grid, and which of its tiles of `rows` rows that is
 // (a row is one query of one head of the group).  With packed queries, the rows before the first
 // sequence and those past the last one count as sequences without keys, e = 0 and batch + 1 (zeros
@@ -29,7 +69,8 @@ __device__ __forceinline__ int paged_keys(const AttnParams& p, int seq_len) {
 // grow by at least one per sequence and by no less than its tiles, so the grid needs no lengths
 // from the host; slots past a sequence's last tile have nothing to do (b = -1).  Each lane looks
 // at one sequence, 64 at a time, and loads all that is known of it at once: what follows waits for
-// one memory access, not for three in a row.
+// one memory access, not for three in a row.  SORTED: p.longest_first may be set (paged keys).
+template <bool SORTED = false>
 __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int rows) {
   Seq s;
   int start_k = 0, end_k = p.len_k;  // or, paged, the length as end_k
@@ -73,9 +114,16 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
       }
       if (n < 64) break;
     }
+    if constexpr (SORTED) {
+      if (p.longest_first) {
+        at = longest_first(p, slot, rows, clampi(q_to, q_from, p.total_q) - q_from, paged_keys(p, k_to), s.tile);
+        s.b = -1;
+        if (at < 0) return s;
+      }
+    }
     s.q0 = __builtin_amdgcn_readlane(q_from, at);
     s.len_q = clampi(__builtin_amdgcn_readlane(q_to, at), s.q0, p.total_q) - s.q0;
-    s.tile = slot - (s.q0 * p.group / rows + first + at);
+    if (!SORTED || !p.longest_first) s.tile = slot - (s.q0 * p.group / rows + first + at);
     s.b = clampi(first + at - 1, 0, max(p.batch - 1, 0));
     start_k = __builtin_amdgcn_readlane(k_from, at);
     end_k = __builtin_amdgcn_readlane(k_to, at);
@@ -89,7 +137,7 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
     s.b = -1;
     return s;
   }
-  s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
+  if (!SORTED || !p.longest_first) s.tile = tiles - 1 - s.tile;  // causal: the rows that see most keys come first
   if (p.kv.table != nullptr) {
     s.k0 = 0;
     s.len_k = paged_keys(p, end_k);

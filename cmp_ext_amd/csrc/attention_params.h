@@ -46,6 +46,7 @@ struct AttnParams {
   int batch, heads, kv_heads, group, dim;
   int causal;
   float scale_log2;  // scale * log2(e): the softmax runs on powers of two
+  int longest_first;  // packed queries, paged keys: row tiles in the order of the keys they see
   int slots;         // row tiles of the grid, for all sequences (see seq_of_slot)
   // split keys: split s of a sequence covers its keys [s * split_keys, (s + 1) * split_keys)
   int splits, split_keys;

@@ -104,7 +104,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
 
   // heads fastest: the workgroups of one kv head meet in the L2 of few XCDs
   const int kvh = blockIdx.x % p.kv_heads;
-  const Seq sq = seq_of_slot(p, blockIdx.x / p.kv_heads, BM);
+  const Seq sq = seq_of_slot<kPaged>(p, blockIdx.x / p.kv_heads, BM);
   if (sq.b < 0) return;
   const int split = blockIdx.y;
   const int shift = sq.len_k - sq.len_q;  // causal: query i sees keys up to i + shift

@@ -249,3 +249,27 @@ def test_qk_norm_rope_c_abi_rejects():
         assert call(**kw) == BAD, kw
     assert call(tokens=1 << 40) == BIG and call(heads=1 << 20) == BIG and call(tokens=1 << 24) == BIG
     assert call(tokens=0, q=None) == 0 and call(heads=0, kv_heads=0) == 0
+
+
+def test_plan_of_many_uneven_tiles():
+    """Chunks of up to 62 sequences whose row tiles fill the GPU go in the order of their keys, whole."""
+    def plan(**kw):
+        buf = ctypes.create_string_buffer(256)
+        a = attention_args(starts_q=0x1000, len_q=0, **kw)
+        assert cabi.lib().cmpext3_attention_describe(ctypes.byref(a), buf, 256) == 0
+        return buf.value.decode()
+
+    kv = attention_args().cache.kv_heads
+    for batch, tiles, pages, sorted_ in ((32, 1200, 8, True), (62, 1200, 4096, True), (63, 1200, 8, False), (4, 1200, 8, False),
+                                         (32, 560, 8, True), (32, 560, 4096, False), (32, 300, 8, False)):
+        rows = (tiles // kv - batch + 1) * 128  # of one kv head
+        a = attention_args()
+        got = plan(batch=batch, total_q=max(rows, 40 * batch) // (a.heads // kv), table_pages=pages)
+        assert ("order=longest" in got) == sorted_, (batch, tiles, pages, got)
+        assert not sorted_ or "splits=1 " in got
+
+
+def test_keys_counted_in_32_bits():
+    """Sums of two key numbers are taken in 32 bits: 2^30 keys of a sequence at most."""
+    assert size(attention_args(table_pages=2**30 // attention_args().cache.page_size)) == BIG
+    assert size(attention_args(table_pages=2**30 // attention_args().cache.page_size - 1)) >= 0

@@ -153,3 +153,44 @@ def test_no_sequence_at_all():
     cache = torch.ones(2, 16, 2, 64, dtype=F16, device="cuda")
     table = torch.zeros(0, 3, dtype=torch.int32, device="cuda")
     assert not cmpext3.paged_attention(q, cache, cache, table, none[:0], cu_seqlens_q=none).any()
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("count,most,longest,held", [(6, 700, 1500, BF16), (20, 200, 600, BF16), (62, 120, 300, F8), (63, 120, 300, BF16)])
+def test_many_tiles_of_uneven_sequences(causal, count, most, longest, held):
+    """Enough row tiles that those with most keys go first (up to 62 sequences): every row once, with
+    sequences of no token, of no key and of fewer keys than queries among them."""
+    heads, dim, page = 64, 8, 16
+    g = torch.Generator().manual_seed(count)
+    new = torch.randint(40, most, (count,), generator=g).tolist()
+    lens = [n + int(e) for n, e in zip(new, torch.randint(0, longest, (count,), generator=g))]
+    new[1] = 0
+    lens[2] = 0
+    lens[3] = new[3] // 2
+    need = [-(-n // page) for n in lens]
+    first = R.starts(need)
+    table = torch.full((count, max(need)), -1, dtype=torch.int32)
+    for i in range(count):
+        table[i, : need[i]] = torch.arange(first[i], first[i + 1])
+    caches, plain, scales = [], [], []
+    for name in range(2):
+        x = rand((int(first[-1]) * page, heads, dim), BF16, 30 + name)
+        if held == F8:
+            c, s = R.quantise(x)
+            plain.append(R.dequantise(c, s))
+            scales.append(s.unflatten(0, (-1, page)).cuda())
+            x = c
+        else:
+            plain.append(x)
+        caches.append(x.unflatten(0, (-1, page)).cuda())
+    cq = R.starts(new) + 5
+    q = rand((int(cq[-1]) + 9, heads, dim), BF16, 29)
+    junk = torch.full((4, *q.shape), math.nan, dtype=BF16, device="cuda")
+    del junk
+    print(f"new {new} lens {lens}", flush=True)
+    got = cmpext3.paged_attention(q.cuda(), *caches, table.cuda(), torch.tensor(lens, dtype=torch.int32).cuda(), cu_seqlens_q=cq.cuda(),
+                                  causal=causal, **(dict(k_scale=scales[0], v_scale=scales[1]) if scales else {})).cpu()
+    assert not got[:5].any() and not got[cq[-1] :].any()
+    for i in range(count):
+        a, b, c = cq[i], cq[i + 1], first[i] * page
+        R.check(got[a:b], *R.attention(q[a:b], plain[0][c : c + lens[i]], plain[1][c : c + lens[i]], dim**-0.5, causal), f"sequence {i}")
