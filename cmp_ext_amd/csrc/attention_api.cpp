@@ -61,6 +61,7 @@ struct AttnPlan {
   KvKind kind;
   int hd;        // padded head
   int blocks16;  // few-rows kernel: its tiles of 16 rows; 0: tile kernel
+  int waves;     // few-rows kernel: of a workgroup
   int ks;        // tile kernel: groups of waves that share a tile's keys
   int rows;      // of a workgroup
   bool empty;
@@ -151,6 +152,19 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     least = ragged ? 256 : 128;
     if (groups < 512) n = ((ragged ? 1024 : 512) + groups - 1) / groups;
     n = std::min<int64_t>(std::max<int64_t>(n, keys / 1024), 128);
+    // Short keys stay whole where a workgroup is through them sooner than splits are joined (4 of 250 keys
+    // 7.4 and 9.5 in two, 32 of up to 500 11.7 and 14.8, of up to 1000 18.2 and 20.5; but 16 of up to
+    // 1000, 128 tiles, 17.4 and 15.2).  Eight waves are through 8-bit keys in half the steps (4 of 500
+    // keys 8.5 us, 4 waves whole 10.0 and in splits 9.8; 32 of up to 500 9.3, 11.2 and 13.4, of up to 1000
+    // 13.7, 17.7 and 16.2; but 4 of 1000 11.6, in splits 10.3); of 16-bit keys a CU takes in no more
+    // bytes (4 of 1000 keys whole: 15.2 with eight waves, 16.0 with four).
+    r.waves = 4;
+    if (groups <= 256) {
+      if (r.kind == kKvPaged8 && r.blocks16 == 1 && r.hd <= 128 && keys > 128 && keys <= (groups >= 128 ? 1024 : 512))
+        r.waves = 8, n = 1;
+      else if (keys <= 256 || (ragged && keys <= 512) || (groups > 128 && keys <= 1024))
+        n = 1;
+    }
   } else if (paged) {
     // Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
     // not so long that workgroups of their own pay (16 bits, heads 32 / 8 of 128: 64 new tokens over
@@ -212,10 +226,10 @@ hipError_t launch_tile_kernel(int dtype, const AttnPlan& r, dim3 grid, hipStream
 
 hipError_t launch_few_kernel(int dtype, const AttnPlan& r, dim3 grid, hipStream_t s) {
   if (dtype == CMPEXT3_F16)
-    return r.kind == kKvPaged16 ? launch_attention_few_f16_paged16(r.hd, r.blocks16, r.p, grid, s)
-                                : launch_attention_few_f16_paged8(r.hd, r.blocks16, r.p, grid, s);
-  return r.kind == kKvPaged16 ? launch_attention_few_bf16_paged16(r.hd, r.blocks16, r.p, grid, s)
-                              : launch_attention_few_bf16_paged8(r.hd, r.blocks16, r.p, grid, s);
+    return r.kind == kKvPaged16 ? launch_attention_few_f16_paged16(r.hd, r.blocks16, r.waves, r.p, grid, s)
+                                : launch_attention_few_f16_paged8(r.hd, r.blocks16, r.waves, r.p, grid, s);
+  return r.kind == kKvPaged16 ? launch_attention_few_bf16_paged16(r.hd, r.blocks16, r.waves, r.p, grid, s)
+                              : launch_attention_few_bf16_paged8(r.hd, r.blocks16, r.waves, r.p, grid, s);
 }
 
 }  // namespace
@@ -253,7 +267,7 @@ extern "C" int cmpext3_attention_describe(const cmpext3_attention_args* args, ch
       snprintf(buf, (size_t)buflen, "kernel=none");
     else
       snprintf(buf, (size_t)buflen, "kernel=%s rows=%d groups=%d keys=%s head=%d slots=%d splits=%d split_keys=%d%s",
-               r.blocks16 ? "attention_few" : "attention_tile", r.rows, r.ks, kinds[r.kind], r.hd,
+               r.blocks16 ? (r.waves == 8 ? "attention_few8" : "attention_few") : "attention_tile", r.rows, r.ks, kinds[r.kind], r.hd,
                r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0, r.p.longest_first ? " order=longest" : "");
   }
   return CMPEXT3_OK;

@@ -1,7 +1,7 @@
 #include "attention_few_kernel.h"
 
 namespace cmpext3 {
-hipError_t launch_attention_few_bf16_paged16(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s) {
-  return blocks16 == 1 ? launch_few_hd<__bf16, kKvPaged16, 1>(hd, p, grid, s) : launch_few_hd<__bf16, kKvPaged16, 2>(hd, p, grid, s);
+hipError_t launch_attention_few_bf16_paged16(int hd, int blocks16, int waves, const AttnParams& p, dim3 grid, hipStream_t s) {
+  return blocks16 == 1 ? launch_few_hd<__bf16, kKvPaged16, 1>(hd, waves, p, grid, s) : launch_few_hd<__bf16, kKvPaged16, 2>(hd, waves, p, grid, s);
 }
 }  // namespace cmpext3

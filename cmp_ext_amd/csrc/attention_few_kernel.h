@@ -3,9 +3,9 @@
 //
 // Rows: a workgroup takes 16 MB rows of one sequence and one kv head (row r: query
 // r / group, head r % group), so that one pass over the cache serves the whole group of
-// heads, and one range of keys (split_keys of them); its four waves take steps of 32 keys in
-// turn, each with a running maximum and sum of its own, and are joined at the end in LDS.
-// The ranges are joined as attention_join.h says, if there is more than one.
+// heads, and one range of keys (split_keys of them); its four waves (eight for short 8-bit keys)
+// take steps of 32 keys in turn, each with a running maximum and sum of its own, and are joined at
+// the end in LDS.  The ranges are joined as attention_join.h says, if there is more than one.
 //
 // Products (16x16x32, fp32 sums) run transposed as in the tile kernel: S^T = K Q^T with the
 // keys' fragments loaded straight from the cache into registers (a lane's 16 bytes are one
@@ -27,16 +27,16 @@
 
 namespace cmpext3 {
 
-template <int HD, int MB>
+template <int HD, int MB, int NW>
 struct FewShape {
   static constexpr int BM = 16 * MB;
   static constexpr int V_BYTES = kWaveKeys * HD * 2;
   // V, the scales of K and V, the byte offsets of the keys' and values' rows in the cache
   static constexpr int WAVE = V_BYTES + 2 * kWaveKeys * 4 + 2 * kWaveKeys * 8;
   static constexpr int PITCH = HD + 4;                      // floats of a row of O in LDS
-  static constexpr int JOIN = kFewWaves * BM * PITCH * 4;
-  static constexpr int ML = kFewWaves * BM * 2 * 4;
-  static constexpr int BODY = WAVE * kFewWaves > JOIN ? WAVE * kFewWaves : JOIN;
+  static constexpr int JOIN = NW * BM * PITCH * 4;
+  static constexpr int ML = NW * BM * 2 * 4;
+  static constexpr int BODY = WAVE * NW > JOIN ? WAVE * NW : JOIN;
   static constexpr int LDS = BODY + ML > kJoinBytes ? BODY + ML : kJoinBytes;
 };
 
@@ -50,10 +50,11 @@ __device__ __forceinline__ int few_v_place(int row, int bc) {
     return row * HD * 2 + (((bc >> 6) ^ (row & 3)) << 6) + ((bc & 63) ^ (((row >> 2) & 1) << 5));
 }
 
-template <typename T, int HD, int KIND, int MB>
-__global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : HD == 64 ? 4 : KIND == kKvPaged8 ? 3 : 2) attention_few_kernel(const AttnParams p) {
+// The waves a SIMD holds at least: as many as have registers; of eight waves (NW) one workgroup is enough.
+template <typename T, int HD, int KIND, int MB, int NW>
+__global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 2 : HD == 64 ? 4 : KIND == kKvPaged8 ? 3 : 2) attention_few_kernel(const AttnParams p) {
   constexpr bool k8 = KIND == kKvPaged8;
-  using S = FewShape<HD, MB>;
+  using S = FewShape<HD, MB, NW>;
   constexpr int KK = HD / 32, DB = HD / 16;
   constexpr int EPP = k8 ? 16 : 8, ES = k8 ? 1 : 2;
   constexpr int KN = HD / (4 * EPP);              // 16-byte loads of a lane for a block of 16 keys
@@ -197,7 +198,7 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : 
     return u32x4{lo.x, lo.y, hi.x, hi.y};
   };
 
-  constexpr int STEP = kFewWaves * kWaveKeys;
+  constexpr int STEP = NW * kWaveKeys;
   bool spoilt = false;
   int key0 = begin + wave * kWaveKeys;
   int page = -1;
@@ -332,16 +333,16 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : 
   __syncthreads();
   constexpr int QUADS = HD / 4;
   float* part = part_of_tile(p, S::BM);
-  for (int n = tid; n < S::BM * QUADS; n += 64 * kFewWaves) {
+  for (int n = tid; n < S::BM * QUADS; n += 64 * NW) {
     const int r = n / QUADS, e = (n % QUADS) * 4, row = row0 + r;
     if (row >= rows || e >= p.dim) continue;
     float m = -INFINITY;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) m = fmaxf(m, ml[(w * S::BM + r) * 2]);
+    for (int w = 0; w < NW; ++w) m = fmaxf(m, ml[(w * S::BM + r) * 2]);
     f32x4 acc = f32x4{0.f, 0.f, 0.f, 0.f};
     float l = 0.f;
 #pragma unroll
-    for (int w = 0; w < kFewWaves; ++w) {
+    for (int w = 0; w < NW; ++w) {
       const float f = m == -INFINITY ? 0.f : exp2_hw(ml[(w * S::BM + r) * 2] - m);  // times a sum of NaN: still NaN
       l += f * ml[(w * S::BM + r) * 2 + 1];
       acc += f * *(const f32x4*)((const float*)smem + (w * S::BM + r) * S::PITCH + e);
@@ -356,15 +357,21 @@ __global__ void __launch_bounds__(64 * kFewWaves, HD == 256 ? 1 : MB == 2 ? 2 : 
       *(u32x2*)(op + e) = u32x2{round2<T>(acc[0] * inv, acc[1] * inv), round2<T>(acc[2] * inv, acc[3] * inv)};
     }
   }
-  if (splits > 1) join_if_last<T, 64 * kFewWaves>(p, sq, kvh, row0, min(S::BM, rows - row0), part, S::BM, splits, smem);
+  if (splits > 1) join_if_last<T, 64 * NW>(p, sq, kvh, row0, min(S::BM, rows - row0), part, S::BM, splits, smem);
 }
 
+// waves: 4, or 8 for 8 bits, 16 rows and hd up to 128.
 template <typename T, int KIND, int MB>
-hipError_t launch_few_hd(int hd, const AttnParams& p, dim3 grid, hipStream_t s) {
-  const dim3 block(64 * kFewWaves);
-  if (hd == 64) return launch_kernel(attention_few_kernel<T, 64, KIND, MB>, grid, block, 0, s, p);
-  if (hd == 128) return launch_kernel(attention_few_kernel<T, 128, KIND, MB>, grid, block, 0, s, p);
-  if constexpr (MB == 1) return launch_kernel(attention_few_kernel<T, 256, KIND, MB>, grid, block, 0, s, p);
+hipError_t launch_few_hd(int hd, int waves, const AttnParams& p, dim3 grid, hipStream_t s) {
+  const dim3 block(64 * waves);
+  if constexpr (MB == 1 && KIND == kKvPaged8) {
+    if (waves == 8)
+      return hd == 64 ? launch_kernel(attention_few_kernel<T, 64, KIND, 1, 8>, grid, block, 0, s, p)
+                      : launch_kernel(attention_few_kernel<T, 128, KIND, 1, 8>, grid, block, 0, s, p);
+  }
+  if (hd == 64) return launch_kernel(attention_few_kernel<T, 64, KIND, MB, 4>, grid, block, 0, s, p);
+  if (hd == 128) return launch_kernel(attention_few_kernel<T, 128, KIND, MB, 4>, grid, block, 0, s, p);
+  if constexpr (MB == 1) return launch_kernel(attention_few_kernel<T, 256, KIND, MB, 4>, grid, block, 0, s, p);
   return hipErrorInvalidValue;  // heads over 128 take 16 rows: two blocks' sums do not fit the registers
 }
 

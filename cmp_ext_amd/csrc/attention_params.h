@@ -12,7 +12,6 @@ enum KvKind : int { kKvPacked = 0, kKvPaged16 = 1, kKvPaged8 = 2 };
 // Keys per step of the tile kernel, and per step of one wave of the few-rows kernel.
 constexpr int kTileKeys = 64;
 constexpr int kWaveKeys = 32;
-constexpr int kFewWaves = 4;
 
 // LDS to join split keys in: a sum for each of 256 threads, a number for each row of a tile and one
 // for each of its splits, of which there are so many at most.
@@ -62,11 +61,12 @@ hipError_t launch_attention_tile_f16_paged8(int hd, int ks, const AttnParams& p,
 hipError_t launch_attention_tile_bf16_packed(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_attention_tile_bf16_paged16(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_attention_tile_bf16_paged8(int hd, int ks, const AttnParams& p, dim3 grid, hipStream_t s);
-// blocks16: tiles of 16 rows a workgroup takes, 1 or 2.
-hipError_t launch_attention_few_f16_paged16(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_few_f16_paged8(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_few_bf16_paged16(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
-hipError_t launch_attention_few_bf16_paged8(int hd, int blocks16, const AttnParams& p, dim3 grid, hipStream_t s);
+// blocks16: tiles of 16 rows a workgroup takes, 1 or 2; waves: of a workgroup, 4 or (8 bits,
+// one tile, hd up to 128) 8.
+hipError_t launch_attention_few_f16_paged16(int hd, int blocks16, int waves, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_few_f16_paged8(int hd, int blocks16, int waves, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_few_bf16_paged16(int hd, int blocks16, int waves, const AttnParams& p, dim3 grid, hipStream_t s);
+hipError_t launch_attention_few_bf16_paged8(int hd, int blocks16, int waves, const AttnParams& p, dim3 grid, hipStream_t s);
 // bm: rows of a row tile.
 hipError_t launch_attention_join(int dtype, int bm, const AttnParams& p, hipStream_t s);
 

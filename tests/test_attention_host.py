@@ -273,3 +273,20 @@ def test_keys_counted_in_32_bits():
     """Sums of two key numbers are taken in 32 bits: 2^30 keys of a sequence at most."""
     assert size(attention_args(table_pages=2**30 // attention_args().cache.page_size)) == BIG
     assert size(attention_args(table_pages=2**30 // attention_args().cache.page_size - 1)) >= 0
+
+
+def test_plan_of_short_keys():
+    """Few rows: whole keys up to some hundreds, with eight waves for 8 bits; longer ones in splits."""
+    def plan(held=cabi.F16, **kw):
+        buf = ctypes.create_string_buffer(256)
+        a = attention_args(cache=cache_args(kv_dtype=held, k_scale=0x100, v_scale=0x200), **kw)
+        assert cabi.lib().cmpext3_attention_describe(ctypes.byref(a), buf, 256) == 0
+        return buf.value.decode()
+
+    page = cache_args().page_size
+    assert "attention_few " in plan(table_pages=256 // page) and "splits=1 " in plan(table_pages=256 // page)
+    assert "splits=1 " not in plan(table_pages=512 // page) and "splits=1 " in plan(table_pages=512 // page, batch=8)
+    assert "attention_few8 " in plan(cabi.E4M3, table_pages=512 // page) and "attention_few " in plan(cabi.E4M3, table_pages=64 // page)
+    assert "attention_few " in plan(cabi.E4M3, table_pages=1024 // page) and "splits=1 " not in plan(cabi.E4M3, table_pages=1024 // page)
+    assert "attention_few8 " in plan(cabi.E4M3, table_pages=1024 // page, batch=128)
+    assert "attention_few " in plan(cabi.E4M3, table_pages=512 // page, batch=1000)

@@ -37,7 +37,7 @@ def run(dtype, held, new, lens, heads, kv_heads, dim, change, paged, causal=True
         table = torch.full((len(lens), max(need)), -1, dtype=torch.int32)
         caches, scales = [], []
         for x in (k, v):
-            c = torch.zeros(int(first[-1]) * page, kv_heads, dim, dtype=dtype)
+            c = torch.full((int(first[-1]) * page, kv_heads, dim), math.nan, dtype=dtype)
             for i, n in enumerate(lens):
                 table[i, : need[i]] = torch.arange(first[i], first[i + 1])
                 c[first[i] * page : first[i] * page + n] = x[ck[i] : ck[i + 1]]
@@ -194,3 +194,14 @@ def test_many_tiles_of_uneven_sequences(causal, count, most, longest, held):
     for i in range(count):
         a, b, c = cq[i], cq[i + 1], first[i] * page
         R.check(got[a:b], *R.attention(q[a:b], plain[0][c : c + lens[i]], plain[1][c : c + lens[i]], dim**-0.5, causal), f"sequence {i}")
+
+
+@pytest.mark.parametrize("dim", [24, 64, 128])
+@pytest.mark.parametrize("dtype,held", [(BF16, F8), (F16, F8), (F16, F16)])
+@pytest.mark.parametrize("new,lens", [([1, 1], [129, 250]), ([1] * 4, [512, 31, 257, 500]), ([1] * 9, [400, 1, 256, 130, 33, 512, 64, 255, 7]),
+                                      ([1] * 32, [1000 - 31 * i for i in range(32)]), ([2, 3, 1, 1, 2], [300, 200, 77, 1, 129])])
+def test_short_keys_stay_whole(dim, dtype, held, new, lens):
+    """Few rows over keys that no split is worth: four waves, or eight for 8 bits, each with its share."""
+    heads, kv_heads = (8, 4) if len(new) == 32 else (4, 2)
+    got, want, tol = run(dtype, held, new, lens, heads, kv_heads, dim, lambda q, k, v: None, True)
+    R.check(got, want, tol)
