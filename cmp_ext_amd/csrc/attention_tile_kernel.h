@@ -37,11 +37,13 @@
 //
 // Keys and values of a step lie in LDS as rows of HD 16-bit elements in two slots each, K
 // with its 16-byte chunks and V with its 64-byte segments permuted by the row so that the reads
-// of both products hit all banks.  Packed ones come by LDS DMA, which zero fills what lies past
-// the sequence or the head; pages go through registers (any page size, 8-bit codes converted on
-// the way; one set of them, for K in the first phase and V in the second: with two, 93 spills made
-// chunks over 8 bits 206 us instead of 141), their rows' addresses shared through LDS and their page
-// numbers fetched steps ahead.  One barrier a step: K of step j + 2 and V of step j + 1 start to load
+// of both products hit all banks.  16-bit ones come by LDS DMA, packed through a descriptor that
+// zero fills what lies past the sequence or the head, pages (of any size) from each lane's own
+// address or a piece of zeros (through registers instead: 6 chunks of up to 512 over up to 4000
+// keys, heads 16 / 4, 75.6 us for 67.0, one of 1024 over 4096, heads 32 / 8, 95.7 for 89.2).  8-bit codes are
+// converted on the way, in registers (one set of them, for K in the first phase and V in the
+// second: with two, 93 spills made chunks 206 us instead of 141).  The rows' addresses in the pages are
+// shared through LDS, their page numbers fetched steps ahead.  One barrier a step: K of step j + 2 and V of step j + 1 start to load
 // behind it, into the slots that the step before has read; they land well within a step.
 #pragma once
 
@@ -86,6 +88,9 @@ __device__ __forceinline__ int v_place(int row, int byte_col) {
   const int x = HD == 64 ? (row >> 1) & 1 : row & 3;
   return row * HD * 2 + (((byte_col >> 6) ^ x) << 6) + (byte_col & 63);
 }
+
+// What LDS-DMA reads for rows that are not there.
+static __device__ const uint32_t zero_piece[4] __attribute__((aligned(16))) = {0, 0, 0, 0};
 
 // Two waves share a SIMD's registers (packed heads up to 64: three; over 128: one has them all).
 template <typename T, int HD, int KIND, int KS>
@@ -149,13 +154,13 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   const int tile_all = p.causal ? min(row0 / p.group + shift, last) : last;
 
   // ---- loads: K or V of a step into a slot ----
-  // packed: LDS-DMA loads i of this wave; where lane's 16 bytes of load i come from
+  // 16 bits: LDS-DMA loads i of this wave; where lane's 16 bytes of load i come from (pages: in a row)
   const T* kbase = nullptr;
   const T* vbase = nullptr;
   uint32_t k_off[S::DMA], v_off[S::DMA];
   constexpr int ROWS1K = 1024 / S::ROW;  // rows of a DMA load
   const int dma_row = wave * S::DMA * ROWS1K + 16 * lane / S::ROW;
-  if constexpr (!kPaged) {
+  if constexpr (!k8) {
     kbase = (const T*)p.kv.k + sq.b * p.kv.k_page + (int64_t)sq.k0 * p.kv.k_token + (int64_t)kvh * p.kv.k_head;
     vbase = (const T*)p.kv.v + sq.b * p.kv.v_page + (int64_t)sq.k0 * p.kv.v_token + (int64_t)kvh * p.kv.v_head;
 #pragma unroll
@@ -166,10 +171,10 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
         c = ((at >> 4) ^ (row >> 1)) & 7;
       else
         c = ((at >> 4) & ~15) | (((at >> 4) ^ row) & 15);
-      k_off[i] = 8 * c < p.dim ? (uint32_t)(row * (int)p.kv.k_token + 8 * c) * 2u : kBufOOB;
+      k_off[i] = 8 * c < p.dim ? (uint32_t)((kPaged ? 0 : row * (int)p.kv.k_token) + 8 * c) * 2u : kBufOOB;
       const int x = HD == 64 ? (row >> 1) & 1 : row & 3;
       const int bc = (((at >> 6) ^ x) << 6) + (at & 63);
-      v_off[i] = bc < 2 * p.dim ? (uint32_t)(row * (int)p.kv.v_token * 2 + bc) : kBufOOB;
+      v_off[i] = bc < 2 * p.dim ? (uint32_t)((kPaged ? 0 : row * (int)p.kv.v_token * 2) + bc) : kBufOOB;
     }
   }
   const uint32_t lds0 = lds_addr(smem) + (uint32_t)(wave * S::DMA * 1024);
@@ -194,14 +199,14 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   };
   // paged: thread t < 64 looks after row t of a step of K, thread 64 + t after one of V: finds its
   // page, its byte offset in the cache (rows_at[step % 2][t], -1: zeros) and its scale
-  constexpr int EPP = k8 ? 16 : 8, ES = k8 ? 1 : 2;         // elements of a 16-byte piece, bytes of an element
+  constexpr int EPP = 16, ES = k8 ? 1 : 2;                  // 8 bits: elements of a 16-byte piece; bytes of an element
   constexpr int PIECES = kTileKeys * HD / EPP / (64 * NW);  // pieces a thread loads of K, and of V
   constexpr int PPR = HD / EPP;                             // pieces of a row
   int64_t* rows_at = (int64_t*)(smem + S::ROWS_AT);
   float* scales = (float*)(smem + S::SCALES);  // [step % 4][K, V][64]
   const int32_t* table = kPaged ? p.kv.table + sq.b * p.kv.table_row : nullptr;
   const bool value_row = tid >= kTileKeys;
-  u32x4 reg[PIECES];  // of K in a step's first phase, of V in its second
+  u32x4 reg[PIECES];  // 8 bits: of K in a step's first phase, of V in its second
   float sreg = 0.f;
   auto page_number = [&](int key) -> int {  // of this thread's row
     if (tid >= 2 * kTileKeys || key >= sq.len_k) return -1;
@@ -224,6 +229,32 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   auto store_scale = [&](int step_k, int step_v) {
     if (k8 && tid < 2 * kTileKeys) scales[((value_row ? step_v : step_k) & 3) * 2 * kTileKeys + tid] = sreg;
   };
+  // 16 bits: K or V of the step that rows_at[at] was found for, into a slot
+  auto dma_rows = [&](bool value, int at, int slot) {
+    const uint8_t* base = (const uint8_t*)(value ? p.kv.v : p.kv.k);
+    const uint32_t dst = lds0 + (uint32_t)((value ? S::V0 : 0) + slot * S::BYTES);
+    const int64_t* rows = rows_at + at * 2 * kTileKeys + (value ? kTileKeys : 0) + dma_row;
+    int64_t o[S::DMA];
+    bool all = p.dim == HD;
+#pragma unroll
+    for (int i = 0; i < S::DMA; ++i) {
+      o[i] = rows[i * ROWS1K];
+      all = all && o[i] >= 0;
+    }
+    if (__builtin_amdgcn_ballot_w64(!all) == 0) {
+      static_for<S::DMA>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        dma_load16_at(base + o[i] + (value ? v_off[i] : k_off[i]), dst, std::integral_constant<uint32_t, i * 1024>{});
+      });
+    } else {  // rows that are not there, and what lies past the head, are zeros
+      static_for<S::DMA>([&](auto ic) {
+        constexpr int i = decltype(ic)::value;
+        const uint32_t in_row = value ? v_off[i] : k_off[i];
+        const void* src = o[i] >= 0 && in_row != kBufOOB ? (const void*)(base + o[i] + in_row) : (const void*)zero_piece;
+        dma_load16_at(src, dst, std::integral_constant<uint32_t, i * 1024>{});
+      });
+    }
+  };
   auto load_pieces = [&](bool value, int at) {
     const uint8_t* base = (const uint8_t*)(value ? p.kv.v : p.kv.k);
     int64_t o[PIECES];
@@ -242,7 +273,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       for (int i = 0; i < PIECES; ++i) {
         reg[i] = u32x4{0, 0, 0, 0};
         if (o[i] < 0 || d >= p.dim) continue;
-        if (k8 && d + 8 >= p.dim) {  // the head ends in the middle of 16 codes
+        if (d + 8 >= p.dim) {  // the head ends in the middle of 16 codes
           const u32x2 h = *(const u32x2*)(base + o[i] + d);
           reg[i].x = h.x, reg[i].y = h.y;
         } else {
@@ -258,12 +289,8 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       const int n = i * 64 * NW + tid, r = n / PPR, c = (n % PPR) * (EPP / 8);
 #pragma unroll
       for (int h = 0; h < EPP / 8; ++h) {
-        u32x4 x = reg[i];
-        if constexpr (k8) {
-          const u32x2 a = e4m3x4<T>(reg[i][2 * h]), b = e4m3x4<T>(reg[i][2 * h + 1]);
-          x = u32x4{a.x, a.y, b.x, b.y};
-        }
-        *(u32x4*)(to + (value ? v_place<HD>(r, 16 * (c + h)) : k_place<HD>(r, c + h))) = x;
+        const u32x2 a = e4m3x4<T>(reg[i][2 * h]), b = e4m3x4<T>(reg[i][2 * h + 1]);
+        *(u32x4*)(to + (value ? v_place<HD>(r, 16 * (c + h)) : k_place<HD>(r, c + h))) = u32x4{a.x, a.y, b.x, b.y};
       }
     }
   };
@@ -425,20 +452,28 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       place_row(0, key, page_number(key));  // K and V of step 0
       store_scale(0, 0);
       __syncthreads();
-      load_pieces(false, 0);
-      store_pieces(false, 0);
-      load_pieces(true, 0);
+      if constexpr (k8) {
+        load_pieces(false, 0);
+        store_pieces(false, 0);
+        load_pieces(true, 0);
+      } else {
+        dma_rows(false, 0, 0);
+        dma_rows(true, 0, 0);
+      }
       const int k1 = key + STEP;
       place_row(1, k1, page_number(k1));  // K of step 1 (and V's scales of it)
       store_scale(1, 1);
-      store_pieces(true, 0);
+      if constexpr (k8) store_pieces(true, 0);
       __syncthreads();
-      load_pieces(false, 1);
+      if constexpr (k8)
+        load_pieces(false, 1);
+      else
+        dma_rows(false, 1, 1);
       const int k2 = value_row ? k1 : k1 + STEP;
       place_row(0, k2, page_number(k2));  // K of step 2, V of step 1: for step 0's loads
       store_scale(2, 1);
       page = page_number(k2 + STEP);
-      store_pieces(false, 1);
+      if constexpr (k8) store_pieces(false, 1);
       ring_fence<0>();
     }
     f32x16 s0[2], s1[2];
@@ -463,8 +498,14 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       if constexpr (!kPaged) {
         dma(false, j + 2, slot);
         dma(true, j + 1, slot ^ 1);
-      } else {
+      } else if constexpr (k8) {
         if (j + 1 < steps) load_pieces(false, slot);
+      } else {
+        asm volatile("" : "+v"(page));  // waited for here, not behind the loads that follow
+        if (j + 1 < steps) {
+          dma_rows(false, slot, slot);
+          dma_rows(true, slot, slot ^ 1);
+        }
       }
       if (begin + (j + 1) * STEP - 1 > tile_all) {  // of any of the groups: all waves come here
         unsigned char* vs = smem + S::V0 + slot * S::BYTES;
@@ -484,15 +525,17 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       if (active) first_phase(j, slotc, sc, sn, f);
       if constexpr (kPaged) {
         if (j + 1 < steps) {
-          store_pieces(false, slot);
-          load_pieces(true, slot);
+          if constexpr (k8) {
+            store_pieces(false, slot);
+            load_pieces(true, slot);
+          }
           const int key = key0 + (value_row ? 2 : 3) * STEP + (tid & (kTileKeys - 1));
           place_row(slot ^ 1, key, page);
           page = page_number(key + STEP);
         }
       }
       if (active) second_phase(j, slotc, sc, sn, f);
-      if constexpr (kPaged) {
+      if constexpr (k8) {
         if (j + 1 < steps) {
           store_pieces(true, slot ^ 1);
           store_scale(j + 3, j + 2);
@@ -522,8 +565,12 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
         const int key = key0 + (tid & (kTileKeys - 1));
         place_row(0, key, page_number(key));
         __syncthreads();
-        load_pieces(true, 0);
-        store_pieces(true, 0);
+        if constexpr (k8) {
+          load_pieces(true, 0);
+          store_pieces(true, 0);
+        } else {
+          dma_rows(true, 0, 0);
+        }
       }
       ring_fence<0>();
       if (key0 + kTileKeys - 1 <= tile_all) continue;  // this group's step was left as it is

@@ -97,6 +97,14 @@ __device__ __forceinline__ void dma_load4(i32x4 rsrc, uint32_t voff, uint32_t ld
                : "v"(voff), "s"(rsrc), "s"(lds_addr)
                : "memory", "m0");
 }
+// Same with 16 bytes from each lane's own 64-bit address.
+template <uint32_t DST>
+__device__ __forceinline__ void dma_load16_at(const void* src, uint32_t lds_base, std::integral_constant<uint32_t, DST> = {}) {
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+               :
+               : "v"(src), "s"(lds_base + DST)
+               : "memory", "m0");
+}
 #pragma clang diagnostic pop
 // Between the steps of a ring that LDS-DMA fills and the whole workgroup reads: at most
 // YOUNGER of this wave's loads are still on their way, its LDS reads are done (not only
