@@ -140,6 +140,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   const int64_t groups = tiles * c.kv_heads;
   int64_t n = 1;  // splits of the longest sequence
   int least = 0;  // keys of a split at least
+  int fit = 0;    // workgroups that splits should fit, found on the device
   if (r.blocks16) {
     // MI355X, one token for each sequence, heads 32 / 8 of 128: two workgroups a CU keep it busy;
     // sequences of one batch differ, so more of them want finer splits to even out (16 of up to
@@ -170,8 +171,11 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     // not so long that workgroups of their own pay (16 bits, heads 32 / 8 of 128: 64 new tokens over
     // 8192 keys 49.0 us with one group and 8 splits, 41.1 with two; 16 of up to 64 over up to 4096
     // 48.4 and 44.7; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 148).
-    // Splits: two workgroups' worth of waves a CU at once; more where sequences differ (8 bits: one
-    // of 512 new tokens over 8192 keys, 136 tiles, 282 us whole, 130 in 3, 107 in 4, 133 in 6).
+    // Splits: all at once, two workgroups a CU (8 bits: one of 512 new tokens over 8192 keys, 136 tiles,
+    // 282 us whole, 130 in 3, 107 in 4, 133 in 6).  How many keys that is follows from the lengths: up to 62
+    // sequences find it on the device (2 of up to 512 over up to 8000 130 us, in 4 splits by the number of
+    // tiles 158; 4 of up to 256 over up to 16000 182 and 227).  Many uneven tiles even out better in two
+    // rounds of splits (30 of up to 60 over up to 3000, 368 tiles, 74 and 84).
     // Where tiles are many, those that see most keys go first, and no keys are split: 32 of up to 300 new
     // tokens over up to 2000 keys, 1200 tiles, 150 us in the order of the sequences, 95 longest first (60
     // of up to 100 over 1000, 960 tiles: 65.6 in splits, 42; but 60 of up to 60 over up to 4000, 752
@@ -184,6 +188,9 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     } else if (r.hd <= 128 && groups <= 256 && (keys <= 4096 || groups <= 32)) {
       r.ks = 2;
       n = std::min<int64_t>(((ragged ? 480 : 256) + groups - 1) / groups, std::max<int64_t>(1, keys / 1024));
+    } else if (!uniform_q && a->batch <= 62 && (!ragged || groups <= 256)) {
+      fit = 512;
+      n = (1536 + groups - 1) / groups;
     } else {
       n = ((ragged ? 1024 : 512) + groups - 1) / groups;
     }
@@ -207,7 +214,8 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     const int64_t splits = (keys + per - 1) / per;
     if (splits > 1) {
       p.splits = (int)splits;
-      p.split_keys = (int)per;
+      p.split_keys = fit > 0 ? least : (int)per;
+      p.fit = fit;
       r.ws_bytes = slots * c.kv_heads * splits * bm * (c.dim + 2) * 4;
     }
   }
@@ -266,9 +274,9 @@ extern "C" int cmpext3_attention_describe(const cmpext3_attention_args* args, ch
     if (r.empty)
       snprintf(buf, (size_t)buflen, "kernel=none");
     else
-      snprintf(buf, (size_t)buflen, "kernel=%s rows=%d groups=%d keys=%s head=%d slots=%d splits=%d split_keys=%d%s",
+      snprintf(buf, (size_t)buflen, "kernel=%s rows=%d groups=%d keys=%s head=%d slots=%d splits=%d split_keys=%d fit=%d%s",
                r.blocks16 ? (r.waves == 8 ? "attention_few8" : "attention_few") : "attention_tile", r.rows, r.ks, kinds[r.kind], r.hd,
-               r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0, r.p.longest_first ? " order=longest" : "");
+               r.p.slots, r.p.splits, r.p.splits > 1 ? r.p.split_keys : 0, r.p.fit, r.p.longest_first ? " order=longest" : "");
   }
   return CMPEXT3_OK;
 }

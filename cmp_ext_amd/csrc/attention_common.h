@@ -13,6 +13,7 @@ struct Seq {
   int q0, len_q;   // first row in the packed queries, number of queries
   int k0, len_k;
   int tile;        // row tile of the sequence
+  int split_keys;  // keys of a split
 };
 
 __device__ __forceinline__ int clampi(int x, int lo, int hi) { return min(max(x, lo), hi); }
@@ -31,6 +32,34 @@ __device__ __forceinline__ int sum_below(int x) {
   x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row 0 to row 1, 2 to 3
   x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // the lower half to the upper
   return x;
+}
+
+// The largest x of all lanes.
+__device__ __forceinline__ int largest(int x) {
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x111, 0xf, 0xf, false));  // as in sum_below
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x112, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x114, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x118, 0xf, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x142, 0xa, 0xf, false));
+  x = max(x, __builtin_amdgcn_update_dpp(x, x, 0x143, 0xc, 0xf, false));
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+// Keys of a split, a multiple of 128, such that all tiles' splits are p.fit workgroups at most: the
+// least such number that p.split_keys and p.splits allow; all keys, if there is none.  Lane e has
+// entry e's queries and keys (seq_of_slot).  All workgroups find the same.
+__device__ __forceinline__ int fitting_split(const AttnParams& p, int rows, int len_q, int len_k) {
+  const int t = (threadIdx.x & 63) < p.batch + 2 && len_k > 0 ? (len_q * p.group + rows - 1) / rows : 0;
+  const int longest = (largest(t > 0 ? len_k : 0) + 127) / 128;
+  int low = max(p.split_keys / 128, (longest + p.splits - 1) / p.splits), high = max(longest, low);  // in 128 keys
+  while (low < high) {
+    const int mid = (low + high) / 2, keys = 128 * mid;
+    if (__builtin_amdgcn_readlane(sum_below(t * ((len_k + keys - 1) / keys)), 63) * p.kv_heads <= p.fit)
+      high = mid;
+    else
+      low = mid + 1;
+  }
+  return 128 * high;
 }
 
 // Row tile `slot` in the order of the keys the tiles see, most first, over all of up to 62 sequences:
@@ -73,6 +102,7 @@ __device__ __forceinline__ int longest_first(const AttnParams& p, int slot, int 
 template <bool SORTED = false>
 __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int rows) {
   Seq s;
+  s.split_keys = p.split_keys;
   int start_k = 0, end_k = p.len_k;  // or, paged, the length as end_k
   if (p.starts_q == nullptr) {
     const int tiles = (p.len_q * p.group + rows - 1) / rows;
@@ -115,6 +145,7 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
       if (n < 64) break;
     }
     if constexpr (SORTED) {
+      if (p.fit > 0) s.split_keys = fitting_split(p, rows, clampi(q_to, q_from, p.total_q) - q_from, paged_keys(p, k_to));
       if (p.longest_first) {
         at = longest_first(p, slot, rows, clampi(q_to, q_from, p.total_q) - q_from, paged_keys(p, k_to), s.tile);
         s.b = -1;
@@ -132,6 +163,7 @@ __device__ __forceinline__ Seq seq_of_slot(const AttnParams& p, int slot, int ro
   s.q0 = __builtin_amdgcn_readfirstlane(s.q0);
   s.len_q = __builtin_amdgcn_readfirstlane(s.len_q);
   s.tile = __builtin_amdgcn_readfirstlane(s.tile);
+  s.split_keys = __builtin_amdgcn_readfirstlane(s.split_keys);
   const int tiles = (s.len_q * p.group + rows - 1) / rows;
   if (s.tile < 0 || s.tile >= tiles) {
     s.b = -1;

@@ -71,7 +71,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
   const int shift = sq.len_k - sq.len_q;
   const int row0 = sq.tile * S::BM, rows = sq.len_q * p.group;
   int end = keys_end(p, sq, min(row0 + S::BM, rows) - 1);
-  const int splits = NW == 8 ? 1 : splits_of(p, end);  // eight waves take whole keys
+  const int splits = NW == 8 ? 1 : splits_of(p, sq, end);  // eight waves take whole keys
   if (split >= splits) return;
   const int begin = split * p.split_keys;
   end = min(end, begin + p.split_keys);

@@ -27,8 +27,8 @@ __device__ __forceinline__ uint32_t part_o(const AttnParams& p, int r) { return 
 __device__ __forceinline__ uint32_t part_ml(const AttnParams& p, int bm, int r) { return (uint32_t)(bm * p.dim + 2 * r) * 4u; }
 
 // Splits that a row tile has: those that hold a key before `end`, at least one.
-__device__ __forceinline__ int splits_of(const AttnParams& p, int end) {
-  return p.splits == 1 ? 1 : min(p.splits, max(1, (end + p.split_keys - 1) / p.split_keys));
+__device__ __forceinline__ int splits_of(const AttnParams& p, const Seq& s, int end) {
+  return p.splits == 1 ? 1 : min(p.splits, max(1, (end + s.split_keys - 1) / s.split_keys));
 }
 
 // IT items (four elements of a row) of each thread, SP splits of each at a time: so many loads on

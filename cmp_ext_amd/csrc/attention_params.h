@@ -49,6 +49,8 @@ struct AttnParams {
   int slots;         // row tiles of the grid, for all sequences (see seq_of_slot)
   // split keys: split s of a sequence covers its keys [s * split_keys, (s + 1) * split_keys)
   int splits, split_keys;
+  int fit;            // packed queries, paged keys: split_keys is the least, the kernel takes the number of
+                      // keys whose splits are at most so many workgroups (fitting_split); 0: it is the number
   float* part;        // sums of the splits (attention_join.h)
   unsigned int* sem;  // counters of the row tiles, or nullptr: joined by a second launch
 };

@@ -115,7 +115,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   const int shift = sq.len_k - sq.len_q;  // causal: query i sees keys up to i + shift
   const int row0 = sq.tile * BM, rows = sq.len_q * p.group;
   int end = keys_end(p, sq, min(row0 + BM, rows) - 1);  // of the keys any row of the tile sees
-  const int splits = splits_of(p, end);
+  const int splits = splits_of(p, sq, end);
   if (split >= splits) return;
   // what only the end of the kernel needs waits in LDS: the loop has no register to spare
   __shared__ Seq kept_seq;
@@ -126,8 +126,8 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
     kept_row0 = row0;
     kept_splits = splits;
   }
-  const int begin = split * p.split_keys;
-  end = min(end, begin + p.split_keys);
+  const int begin = split * sq.split_keys;
+  end = min(end, begin + sq.split_keys);
   // steps of this group, and of the group that has most: step j starts at key key_of(j)
   const int all_steps = end > begin ? (end - begin + kTileKeys - 1) / kTileKeys : 0;
   const int steps = (all_steps - part_k + KS - 1) / KS, turns = (all_steps + KS - 1) / KS;

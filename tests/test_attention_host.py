@@ -290,3 +290,18 @@ def test_plan_of_short_keys():
     assert "attention_few " in plan(cabi.E4M3, table_pages=1024 // page) and "splits=1 " not in plan(cabi.E4M3, table_pages=1024 // page)
     assert "attention_few8 " in plan(cabi.E4M3, table_pages=1024 // page, batch=128)
     assert "attention_few " in plan(cabi.E4M3, table_pages=512 // page, batch=1000)
+
+
+def test_plan_of_splits_found_on_the_device():
+    """Chunks over long keys: the splits of up to 62 sequences follow from their lengths."""
+    def plan(**kw):
+        buf = ctypes.create_string_buffer(256)
+        a = attention_args(starts_q=0x1000, len_q=0, **kw)
+        assert cabi.lib().cmpext3_attention_describe(ctypes.byref(a), buf, 256) == 0
+        return buf.value.decode()
+
+    page = cache_args().page_size
+    assert "fit=512" in plan(batch=4, total_q=1500, table_pages=8192 // page) and "splits=1 " not in plan(batch=4, total_q=1500, table_pages=8192 // page)
+    assert "fit=0" in plan(batch=40, total_q=6000, table_pages=65536 // page)
+    assert "fit=0" in plan(batch=63, total_q=3000, table_pages=8192 // page)
+    assert "fit=0" in plan(batch=4, total_q=1500, table_pages=2048 // page) and "groups=2" in plan(batch=4, total_q=1500, table_pages=2048 // page)

@@ -205,3 +205,41 @@ def test_short_keys_stay_whole(dim, dtype, held, new, lens):
     heads, kv_heads = (8, 4) if len(new) == 32 else (4, 2)
     got, want, tol = run(dtype, held, new, lens, heads, kv_heads, dim, lambda q, k, v: None, True)
     R.check(got, want, tol)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("held", [BF16, F8])
+@pytest.mark.parametrize("new,lens,heads,kv_heads,dim", [
+    ([300, 1, 200, 0, 3], [5000, 300, 4200, 7, 1], 8, 8, 64), ([200], [4500], 16, 8, 128), ([90, 300], [1500, 700], 2, 1, 256),
+    ([70, 65, 129], [4200, 0, 60], 16, 16, 64)])
+def test_splits_that_follow_from_the_lengths(causal, held, new, lens, heads, kv_heads, dim):
+    got, want, tol = run(BF16, held, new, lens, heads, kv_heads, dim, lambda q, k, v: None, True, causal=causal)
+    R.check(got, want, tol)
+
+
+def test_splits_found_on_the_device_in_a_graph():
+    """Joined by a second launch, which finds the same splits: the same result, with the lengths of each replay."""
+    heads, kv_heads, dim, page, pages = 8, 8, 64, 64, 200
+    q, k, v = (rand(s, BF16, i).cuda() for i, s in enumerate(((400, heads, dim), (pages, page, kv_heads, dim), (pages, page, kv_heads, dim))))
+    table = torch.arange(160, dtype=torch.int32).view(2, 80).cuda()
+    cu, lens = torch.tensor([0, 300, 400], dtype=torch.int32).cuda(), torch.tensor([5000, 4100], dtype=torch.int32).cuda()
+    call = lambda: cmpext3.paged_attention(q, k, v, table, lens, cu_seqlens_q=cu)  # noqa: E731
+    eager = call()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        call()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = call()
+    for n in (5000, 700, 4999, 5000):
+        lens[0] = n
+        want = call()
+        torch.cuda.synchronize()
+        out.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), n
+    assert torch.equal(want, eager)
