@@ -476,6 +476,10 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       if constexpr (k8) store_pieces(false, 1);
       ring_fence<0>();
     }
+    // the queries are here: else the compiler, which sees a path without their use, waits for them in
+    // every step, and with them for the loads that the step has begun
+#pragma unroll
+    for (int kk = 0; kk < KK; ++kk) asm volatile("" : "+v"(q[kk]));
     f32x16 s0[2], s1[2];
     if (key_of(0) <= wave_any) {
       s0[0] = s0[1] = f32x16{0};
