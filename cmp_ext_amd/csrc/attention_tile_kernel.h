@@ -4,9 +4,9 @@
 // Rows: a workgroup of four waves takes 128 rows of one sequence and one kv head, a row being one
 // query of one head of the group (row r: query r / group, head r % group), so that grouped heads
 // share each step's keys and values and short sequences fill their tiles.  A wave owns 32 rows.
-// (8192 tokens, 32 heads of 128 and 8 of keys, bf16, on MI355X: 529 us, 1040 TFLOP/s of the products
-// that are not masked; eight waves over 256 rows, whose barriers bind all waves of a CU together, 548;
-// four waves of 64 rows with a SIMD to themselves 643.)
+// (8192 tokens, 32 heads of 128 and 8 of keys, bf16, on MI355X: 503 us, 1093 TFLOP/s of the products
+// that are not masked.  Where four waves of 32 rows took 529, eight over 256 rows, whose barriers bind all
+// waves of a CU together, took 548, and four of 64 rows with a SIMD to themselves 643.)
 //
 // Keys: where there are fewer tiles than CUs, a workgroup has two such groups of four waves (KS = 2),
 // one for the even steps and one for the odd ones, each with its own LDS, joined in LDS at the end:
@@ -28,9 +28,9 @@
 // weights of step j, then the weighted values of step j beside its other weights and the maximum
 // of step j + 1.  The vector work (per score: scale, exponential at half the rate, sum, half a
 // conversion, half a maximum) is over half as long as the products.  On that prompt the matrix cores
-// are busy 53 % of the cycles and the vector units 45 %, and a wave waits for LDS or its barrier
-// 29 % of its time; with the loads into LDS left out it would take 463 us, with the exponentials left
-// out 503, with V's fragments 519, with K and V from L2 512: no single one of them bounds it.
+// are busy 57 % of the cycles and the vector units 50 %, a wave waits for LDS or its barrier 23 % of its
+// time, and the clock is 1.85 GHz: power bounds it as well (more fragments on their way, or other shares
+// of the vector work in the two phases, change nothing).
 //
 // The weights are rounded once to 16 bits for the second product, their sum is of the unrounded
 // ones: the result is off by its own rounding and by one of the same size more.
