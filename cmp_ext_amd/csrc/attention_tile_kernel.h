@@ -42,7 +42,8 @@
 // address or a piece of zeros (through registers instead: 6 chunks of up to 512 over up to 4000
 // keys, heads 16 / 4, 75.6 us for 67.0, one of 1024 over 4096, heads 32 / 8, 95.7 for 89.2).  8-bit codes are
 // converted on the way, in registers (one set of them, for K in the first phase and V in the
-// second: with two, 93 spills made chunks 206 us instead of 141).  The rows' addresses in the pages are
+// second: with two, 93 spills made chunks 206 us instead of 141; 126 with what followed, 4 of up to 512
+// over up to 8100 keys, heads 32 / 8).  The rows' addresses in the pages are
 // shared through LDS, their page numbers fetched steps ahead.  One barrier a step: K of step j + 2 and V of step j + 1 start to load
 // behind it, into the slots that the step before has read; they land well within a step.
 #pragma once
@@ -205,15 +206,15 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   int64_t* rows_at = (int64_t*)(smem + S::ROWS_AT);
   float* scales = (float*)(smem + S::SCALES);  // [step % 4][K, V][64]
   const int32_t* table = kPaged ? p.kv.table + sq.b * p.kv.table_row : nullptr;
-  const bool value_row = tid >= kTileKeys;
+  const bool value_row = wave > 0;  // of the first two waves, which find the rows
   u32x4 reg[PIECES];  // 8 bits: of K in a step's first phase, of V in its second
   float sreg = 0.f;
   auto page_number = [&](int key) -> int {  // of this thread's row
-    if (tid >= 2 * kTileKeys || key >= sq.len_k) return -1;
+    if (wave > 1 || key >= sq.len_k) return -1;
     return table[p.kv.page_shift >= 0 ? key >> p.kv.page_shift : key / p.kv.page_size];
   };
   auto place_row = [&](int at, int key, int page) {
-    if (tid >= 2 * kTileKeys) return;
+    if (wave > 1) return;
     const int place = p.kv.page_shift >= 0 ? key & (p.kv.page_size - 1) : key % p.kv.page_size;
     const bool there = (unsigned)page < (unsigned)p.kv.pages;
     const int64_t o = value_row ? page * p.kv.v_page + place * p.kv.v_token + kvh * p.kv.v_head
@@ -223,11 +224,11 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       sreg = 0.f;
       if (there)
         sreg = value_row ? p.kv.v_scale[page * p.kv.vs_page + place * p.kv.vs_token + kvh * p.kv.vs_head]
-                         : p.kv.k_scale[page * p.kv.ks_page + place * p.kv.ks_token + kvh * p.kv.ks_head] * p.scale_log2;
+                         : p.kv.k_scale[page * p.kv.ks_page + place * p.kv.ks_token + kvh * p.kv.ks_head];
     }
   };
   auto store_scale = [&](int step_k, int step_v) {
-    if (k8 && tid < 2 * kTileKeys) scales[((value_row ? step_v : step_k) & 3) * 2 * kTileKeys + tid] = sreg;
+    if (k8 && wave < 2) scales[((value_row ? step_v : step_k) & 3) * 2 * kTileKeys + tid] = sreg;
   };
   // 16 bits: K or V of the step that rows_at[at] was found for, into a slot
   auto dma_rows = [&](bool value, int at, int slot) {
@@ -318,7 +319,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   for (int d = 0; d < DB; ++d) o[d] = f32x16{0};
   float m_ref = -INFINITY, sum = 0.f;
   float base = 0.f;                             // what is subtracted, in powers of two (0 for no key yet)
-  const float unit = k8 ? 1.f : p.scale_log2;   // scores times this are powers of two
+  const float unit = p.scale_log2;              // scores times this are powers of two
   u32x4 pw[4];                                  // weights of 16 keys each
 
   // scores of step j, before their maximum is taken: scales of 8-bit keys, keys that are not seen
@@ -361,14 +362,8 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   // pair t of a step's weights
   auto weigh = [&](f32x16 (&s)[2], int j, auto tc) {
     constexpr int t = decltype(tc)::value, b = t / 8, r = t % 8 * 2;
-    float w0, w1;
-    if constexpr (k8) {
-      w0 = exp2_hw(s[b][r] - base);
-      w1 = exp2_hw(s[b][r + 1] - base);
-    } else {
-      w0 = exp2_hw(__builtin_fmaf(s[b][r], unit, -base));
-      w1 = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -base));
-    }
+    float w0 = exp2_hw(__builtin_fmaf(s[b][r], unit, -base));
+    float w1 = exp2_hw(__builtin_fmaf(s[b][r + 1], unit, -base));
     sum += w0 + w1;
     if constexpr (k8) {
       const float* sc = scales + (j & 3) * 2 * kTileKeys + kTileKeys + 4 * half + 32 * b + 8 * (r / 4) + r % 4;
