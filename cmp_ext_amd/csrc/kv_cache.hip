@@ -133,7 +133,8 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(const CacheParams p)
   const int per_row = p.dim / EPL, per_token = p.kv_heads * per_row;
   const int64_t unit0 = (int64_t)blockIdx.x * 256;
   const int64_t token0 = unit0 / per_token;
-  // the last sequence that starts at or before the workgroup's first token, -1 if none does
+  // the last sequence that starts at or before the workgroup's first token, -1 if none does; starts that
+  // fall can name one that begins later, so the row's own place in it is looked at below
   int b = -1;
   for (int i = 0; i < p.batch; i += 64) {
     const bool below = i + lane < p.batch && p.starts[min(i + lane, p.batch - 1)] <= token0;
@@ -153,7 +154,7 @@ __global__ void __launch_bounds__(256) kv_cache_read_kernel(const CacheParams p)
   if (b >= 0 && token < p.starts[b + 1]) {
     const int64_t key = token - p.starts[b];
     int place, page = -1;
-    if (key < (int64_t)p.kv.table_pages * p.kv.page_size)
+    if (key >= 0 && key < (int64_t)p.kv.table_pages * p.kv.page_size)
       page = page_of(p.kv, p.kv.table + b * p.kv.table_row, (int)key, place);
     if (page >= 0) {
       float ks = 1.f, vs = 1.f;

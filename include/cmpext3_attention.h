@@ -90,7 +90,8 @@ int cmpext3_kv_cache_write(const cmpext3_kv_cache* cache, int dtype, const void*
  * Reads the sequences' tokens back as packed rows k_out, v_out ([total, kv_heads, dim]
  * contiguous, of `dtype`): rows starts[b] .. starts[b+1]-1 are tokens 0, 1, ... of sequence
  * b, found through block_table[b * table_row + token / page_size].  Rows in no sequence, past
- * the table's table_pages columns or with a page number outside the cache are zeros.
+ * the table's table_pages columns or with a page number outside the cache are zeros.  Starts that
+ * fall leave it undefined which sequence a row is taken from.
  */
 int cmpext3_kv_cache_read(const cmpext3_kv_cache* cache, const int32_t* block_table, int64_t table_row,
                           int32_t table_pages, const int32_t* starts, int32_t batch, int64_t total, int dtype,
