@@ -99,7 +99,7 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   // rows and keys are counted in 32 bits, sums of two numbers of keys too; packed keys addressed
   // within a step in 32
   if (keys > INT_MAX / 2) return CMPEXT3_ERR_TOO_LARGE;
-  if (queries * group > INT_MAX - 256) return CMPEXT3_ERR_TOO_LARGE;
+  if (queries > (INT_MAX - 256) / group) return CMPEXT3_ERR_TOO_LARGE;  // their product may pass 64 bits
   if (!paged && (c.k_token < 0 || c.v_token < 0 || std::max(c.k_token, c.v_token) > INT_MAX / (2 * kTileKeys) - kMostDim))
     return CMPEXT3_ERR_TOO_LARGE;
 
@@ -289,9 +289,9 @@ extern "C" int cmpext3_qk_norm_rope(const cmpext3_qk_norm_rope_args* a, void* st
   if (a->rotary_dim < 0 || a->rotary_dim % 2 != 0 || a->rotary_dim > a->dim) return CMPEXT3_ERR_INVALID_ARG;
   if (a->dim > 1024) return CMPEXT3_ERR_UNSUPPORTED;
   if (a->heads > kMostHeads || a->kv_heads > kMostHeads) return CMPEXT3_ERR_TOO_LARGE;
-  const int64_t units = a->tokens * (a->heads + a->kv_heads);
-  if (a->tokens > INT64_MAX / (1 << 24) || units * 64 > kMostThreads) return CMPEXT3_ERR_TOO_LARGE;  // a wave per head
-  if (units == 0) return CMPEXT3_OK;
+  const int64_t per_token = a->heads + a->kv_heads;
+  if (a->tokens == 0 || per_token == 0) return CMPEXT3_OK;
+  if (a->tokens > kMostThreads / 64 / per_token) return CMPEXT3_ERR_TOO_LARGE;  // a wave per head
   if ((a->heads > 0 && (a->q == nullptr || a->q_out == nullptr)) || (a->kv_heads > 0 && (a->k == nullptr || a->k_out == nullptr)) ||
       a->positions == nullptr || (a->rotary_dim > 0 && a->table_rows > 0 && (a->cos == nullptr || a->sin == nullptr)))
     return CMPEXT3_ERR_INVALID_ARG;
