@@ -236,6 +236,13 @@ __device__ __forceinline__ float max_halves(float x) {
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
 
+// fp16 numbers lose bits below 2^-14 and are zero below 2^-25, so fp16 weights are taken times a power of two
+// that puts the largest of a row near the type's end, not at 1: the sums get the same factor and it cancels.
+// With it the other keys keep their weights where one key stands far above them (its score 16 above, of 600
+// keys: off by 3e-4 of the result, without it by 4e-2).
+template <typename T>
+constexpr bool kHalf = std::is_same<T, _Float16>::value;
+
 // 2^x, the hardware's (relative error about 2^-23; 0 for -infinity).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
 

@@ -174,6 +174,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
     for (int d = 0; d < DB; ++d) o[mb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float unit = k8 ? 1.f : p.scale_log2;
+  constexpr float TOP = kHalf<T> && !k8 ? 15.f : 0.f;  // the largest weight is 2^TOP (see kHalf)
 
   // V of a step into this wave's LDS, and its fragments from there: keys 4 G .. and 16 + 4 G ..
   auto store_v = [&]() {
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
 #pragma unroll
         for (int d = 0; d < DB; ++d) o[mb][d] *= alpha;
       }
-      const float base = m_ref[mb] == -INFINITY ? 0.f : m_ref[mb] * unit;
+      const float base = m_ref[mb] == -INFINITY ? 0.f : m_ref[mb] * unit - TOP;
       float w[8];
 #pragma unroll
       for (int b = 0; b < 2; ++b)

@@ -20,8 +20,9 @@
 // product take the keys in the order the lane has them: the transposing LDS reads of V then
 // fetch rows 16 g + 4 (l / 32) and + 8 instead of 8 consecutive ones.  No weight crosses lanes.
 //
-// The maximum a row subtracts is only raised when a score exceeds it by more than 2^8
-// (kLazy): the sums stay far from overflow and the accumulators are rarely rescaled.
+// The maximum a row subtracts is only raised when a score exceeds it by more than 2^8 (2^4 in fp16,
+// where the weights begin at 2^10: see kHalf): the sums stay far from overflow and the accumulators are
+// rarely rescaled.
 //
 // Pipeline: step j (64 keys) has two phases, each a sequence of slots of one matrix product with
 // a share of the vector work, kept in that order: the scores of step j + 1 beside the first
@@ -51,8 +52,6 @@
 #include "attention_join.h"
 
 namespace cmpext3 {
-
-constexpr float kLazy = 8.0f;  // in powers of two
 
 constexpr int kTileWaves = 4;
 
@@ -320,6 +319,8 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   float m_ref = -INFINITY, sum = 0.f;
   float base = 0.f;                             // what is subtracted, in powers of two (0 for no key yet)
   const float unit = p.scale_log2;              // scores times this are powers of two
+  // a weight is 2^TOP at the reference, and 2^(TOP + LAZY) at most before the reference is raised
+  constexpr float TOP = kHalf<T> && !k8 ? 10.f : 0.f, LAZY = kHalf<T> && !k8 ? 4.f : 8.f;
   u32x4 pw[4];                                  // weights of 16 keys each
 
   // scores of step j, before their maximum is taken: scales of 8-bit keys, keys that are not seen
@@ -347,11 +348,11 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   // with the maximum of a step's scores (of this lane's keys): the reference is raised
   auto raise = [&](float mx) {
     mx = max_halves(mx);
-    if (__builtin_amdgcn_ballot_w64((mx - m_ref) * unit > kLazy)) {  // -inf - -inf is no reason
+    if (__builtin_amdgcn_ballot_w64((mx - m_ref) * unit > LAZY)) {  // -inf - -inf is no reason
       const float m_new = fmaxf(m_ref, mx);
       const float alpha = m_new == m_ref ? 1.f : exp2_hw((m_ref - m_new) * unit);
       m_ref = m_new;
-      base = m_new == -INFINITY ? 0.f : m_new * unit;
+      base = m_new == -INFINITY ? 0.f : m_new * unit - TOP;
       sum *= alpha;
 #pragma unroll
       for (int d = 0; d < DB; ++d)
