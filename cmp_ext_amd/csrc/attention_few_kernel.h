@@ -14,7 +14,10 @@
 // transposing reads.  Each step's loads start when the step before has used its registers, and
 // its page numbers, one per lane, are fetched another step ahead.  A weight is taken as the sum
 // of two 16-bit numbers (the second product twice): there is time for it under the loads (188.5 us
-// below with and without), and the result is then off by its own rounding only.
+// below with and without), and the result is then off by its own rounding only.  Over codes the
+// weight carries its value's scale, which may be any float: the two numbers are bf16 there whatever
+// the queries are (16 bits of a weight together, and codes fit bf16 as well), as fp16 ends at 2^-25
+// (4096 keys with values of size 1e-3: off by 6e-4, which is the result's own rounding, in fp16 by 1e-2).
 //
 // MI355X, heads 32 / 8 of 128: 64 sequences of up to 8192 keys in 16 bits, 875 MB, 188 us (4.65 TB/s;
 // a large copy moves 5.25): two workgroups a CU, 16 KB of each wave on their way.  One of 65537 keys
@@ -54,6 +57,7 @@ __device__ __forceinline__ int few_v_place(int row, int bc) {
 template <typename T, int HD, int KIND, int MB, int NW>
 __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 2 : HD == 64 ? 4 : KIND == kKvPaged8 ? 3 : 2) attention_few_kernel(const AttnParams p) {
   constexpr bool k8 = KIND == kKvPaged8;
+  using W = std::conditional_t<k8, __bf16, T>;  // the second product's operands
   using S = FewShape<HD, MB, NW>;
   constexpr int KK = HD / 32, DB = HD / 16;
   constexpr int EPP = k8 ? 16 : 8, ES = k8 ? 1 : 2;
@@ -174,7 +178,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
     for (int d = 0; d < DB; ++d) o[mb][d] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
   const float unit = k8 ? 1.f : p.scale_log2;
-  constexpr float TOP = kHalf<T> && !k8 ? 15.f : 0.f;  // the largest weight is 2^TOP (see kHalf)
+  constexpr float TOP = kHalf<W> ? 15.f : 0.f;  // the largest weight is 2^TOP (see kHalf)
 
   // V of a step into this wave's LDS, and its fragments from there: keys 4 G .. and 16 + 4 G ..
   auto store_v = [&]() {
@@ -184,7 +188,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
       if constexpr (k8) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const u32x2 a = e4m3x4<T>(vr[i][2 * h]), b = e4m3x4<T>(vr[i][2 * h + 1]);
+          const u32x2 a = e4m3x4<W>(vr[i][2 * h]), b = e4m3x4<W>(vr[i][2 * h + 1]);
           *(u32x4*)(vs + few_v_place<HD>(r, c + 16 * h)) = u32x4{a.x, a.y, b.x, b.y};
         }
       } else {
@@ -278,19 +282,19 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
         }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        pw[mb][i] = round2<T>(w[2 * i], w[2 * i + 1]);
-        pl[mb][i] = round2<T>(w[2 * i] - from_bits<T>((uint16_t)pw[mb][i]), w[2 * i + 1] - from_bits<T>((uint16_t)(pw[mb][i] >> 16)));
+        pw[mb][i] = round2<W>(w[2 * i], w[2 * i + 1]);
+        pl[mb][i] = round2<W>(w[2 * i] - from_bits<W>((uint16_t)pw[mb][i]), w[2 * i + 1] - from_bits<W>((uint16_t)(pw[mb][i] >> 16)));
       }
     }
-    if (key0 + kWaveKeys - 1 > all && any_not_finite<T>(vs, S::V_BYTES)) {
+    if (key0 + kWaveKeys - 1 > all && any_not_finite<W>(vs, S::V_BYTES)) {
       spoilt = true;
-      for (int i = 16 * lane; i < S::V_BYTES; i += 1024) *(u32x4*)(vs + i) = finite_only<T>(*(const u32x4*)(vs + i));
+      for (int i = 16 * lane; i < S::V_BYTES; i += 1024) *(u32x4*)(vs + i) = finite_only<W>(*(const u32x4*)(vs + i));
     }
 #pragma unroll
     for (int d = 0; d < DB; ++d) {
       const u32x4 v = v_frag(d);
 #pragma unroll
-      for (int mb = 0; mb < MB; ++mb) o[mb][d] = Mfma<T>::mma(v, pl[mb], Mfma<T>::mma(v, pw[mb], o[mb][d]));
+      for (int mb = 0; mb < MB; ++mb) o[mb][d] = Mfma<W>::mma(v, pl[mb], Mfma<W>::mma(v, pw[mb], o[mb][d]));
       if (d % 4 == 3) __builtin_amdgcn_sched_barrier(0);
     }
   }
@@ -303,11 +307,11 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {
           const int key = key0 + 4 * G, most = min(limit[mb], end - 1);
-          const u32x4 seen = {ones_up_to<T>(key, most), ones_up_to<T>(key + 2, most), ones_up_to<T>(key + 16, most),
-                              ones_up_to<T>(key + 18, most)};
+          const u32x4 seen = {ones_up_to<W>(key, most), ones_up_to<W>(key + 2, most), ones_up_to<W>(key + 16, most),
+                              ones_up_to<W>(key + 18, most)};
 #pragma unroll
           for (int d = 0; d < DB; ++d) {
-            const f32x4 hit = Mfma<T>::mma(kind_ones<T>(v_frag(d), kind), seen, f32x4{0.f, 0.f, 0.f, 0.f});
+            const f32x4 hit = Mfma<W>::mma(kind_ones<W>(v_frag(d), kind), seen, f32x4{0.f, 0.f, 0.f, 0.f});
 #pragma unroll
             for (int i = 0; i < 4; ++i) o[mb][d][i] += hit[i] > 0.f ? kind_value(kind) : 0.f;
           }
