@@ -64,7 +64,8 @@ struct TileShape {
   static constexpr int V0 = kSlots * BYTES;          // K's slots, then V's
   static constexpr int ROWS_AT = 2 * kSlots * BYTES;  // paged: byte offsets of the rows of K and V, two steps'
   static constexpr int SCALES = ROWS_AT + 2 * 2 * kTileKeys * 8;  // 8 bits: scales of K and V, four steps'
-  static constexpr int LDS = PAGED ? SCALES + 4 * 2 * kTileKeys * 4 : ROWS_AT;
+  static constexpr int UNITS = SCALES + 4 * 2 * kTileKeys * 4;    // and the unit of V's, four steps'
+  static constexpr int LDS = PAGED ? UNITS + 4 * 4 : ROWS_AT;
   static constexpr int DMA = BYTES / 1024 / kTileWaves;  // 1 KB LDS-DMA loads per wave of K, and of V
   static_assert(BYTES % (1024 * kTileWaves) == 0, "whole DMA loads per wave");
   static_assert(LDS <= 160 * 1024 && LDS >= kJoinBytes, "LDS budget");
@@ -204,6 +205,14 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   constexpr int PPR = HD / EPP;                             // pieces of a row
   int64_t* rows_at = (int64_t*)(smem + S::ROWS_AT);
   float* scales = (float*)(smem + S::SCALES);  // [step % 4][K, V][64]
+  // fp16: V's scales of a step are held in a power of two of their own size, 2^(unit - 127), and so are the
+  // sums: weights that carry them stay where fp16 has its bits (see kHalf) whatever the values' size.
+  // The unit is raised to the largest of a step, and lowered to it if that is over 2^4 smaller.  (4 of up to
+  // 512 over up to 8100 keys, heads 32 / 8 of 128: 130 us for 127 without; found by the wave that stores the
+  // scales, which has most to do, 134.)
+  constexpr bool UNITS = k8 && kHalf<T>;
+  int* units = (int*)(smem + S::UNITS);  // [step % 4]
+  int unit_found = 127, most_found = 1;  // the wave that finds it: of the last step, the largest of all
   const int32_t* table = kPaged ? p.kv.table + sq.b * p.kv.table_row : nullptr;
   const bool value_row = wave > 0;  // of the first two waves, which find the rows
   u32x4 reg[PIECES];  // 8 bits: of K in a step's first phase, of V in its second
@@ -228,6 +237,20 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   };
   auto store_scale = [&](int step_k, int step_v) {
     if (k8 && wave < 2) scales[((value_row ? step_v : step_k) & 3) * 2 * kTileKeys + tid] = sreg;
+  };
+  auto find_unit = [&](int step) {  // the last wave, which finds no rows, behind a barrier after the scales were stored
+    if constexpr (UNITS) {
+      if (wave != NW - 1) return;
+      float* mine = scales + (step & 3) * 2 * kTileKeys + kTileKeys + lane;
+      const int bits = __float_as_int(fabsf(*mine)), e = bits < 0x7F800000 ? bits >> 23 : 0;
+      if (__builtin_amdgcn_ballot_w64(e > unit_found) != 0 || __builtin_amdgcn_ballot_w64(e >= unit_found - 4) == 0) {
+        const int most = largest(e);  // 0: only zeros, nothing to go by
+        most_found = max(most_found, most);
+        if (most > 0) unit_found = max(most, most_found - 60);  // not so far below that sums of the largest leave the floats
+      }
+      *mine = __builtin_ldexpf(*mine, 127 - unit_found);
+      if (lane == 0) units[step & 3] = unit_found;
+    }
   };
   // 16 bits: K or V of the step that rows_at[at] was found for, into a slot
   auto dma_rows = [&](bool value, int at, int slot) {
@@ -320,7 +343,9 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   float base = 0.f;                             // what is subtracted, in powers of two (0 for no key yet)
   const float unit = p.scale_log2;              // scores times this are powers of two
   // a weight is 2^TOP at the reference, and 2^(TOP + LAZY) at most before the reference is raised
-  constexpr float TOP = kHalf<T> && !k8 ? 10.f : 0.f, LAZY = kHalf<T> && !k8 ? 4.f : 8.f;
+  // (twice that with V's scale)
+  constexpr float TOP = kHalf<T> ? 10.f : 0.f, LAZY = kHalf<T> ? 4.f : 8.f;
+  int sum_unit = 127, step_unit = 127;  // of o, as `units`, and of the step's values
   u32x4 pw[4];                                  // weights of 16 keys each
 
   // scores of step j, before their maximum is taken: scales of 8-bit keys, keys that are not seen
@@ -386,6 +411,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
     constexpr int slot = decltype(slotc)::value, next = slot ^ 1;
 #pragma unroll
     for (int n = 0; n < AHEAD; ++n) f[n] = k_frag(next, n);
+    if constexpr (UNITS) step_unit = units[j & 3];
     sn[0] = sn[1] = f32x16{0};
     static_for<LEAD>([&](auto t) { weigh(sc, j, t); });
     __builtin_amdgcn_sched_barrier(0);
@@ -406,6 +432,17 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   auto second_phase = [&](int j, auto slotc, f32x16 (&sc)[2], f32x16 (&sn)[2], u32x4 (&f)[AHEAD]) {
     constexpr int slot = decltype(slotc)::value;
     float mx = 0.f;
+    if constexpr (UNITS) {
+      const int to = __builtin_amdgcn_readfirstlane(step_unit);
+      if (to != sum_unit) {
+        const float by = __builtin_ldexpf(1.f, sum_unit - to);
+        sum_unit = to;
+#pragma unroll
+        for (int d = 0; d < DB; ++d)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) o[d][r] *= by;
+      }
+    }
     __builtin_amdgcn_sched_barrier(0);
     // the other weights in the first half (groups 2 and 3 of 16 keys are used in the second), the
     // maximum in the second
@@ -448,6 +485,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       place_row(0, key, page_number(key));  // K and V of step 0
       store_scale(0, 0);
       __syncthreads();
+      find_unit(0);
       if constexpr (k8) {
         load_pieces(false, 0);
         store_pieces(false, 0);
@@ -526,6 +564,7 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       if constexpr (kPaged) {
         if (j + 1 < steps) {
           if constexpr (k8) {
+            find_unit(j + 1);
             store_pieces(false, slot);
             load_pieces(true, slot);
           }
@@ -548,6 +587,12 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       if (j + 1 < turns) whole_step(j + 1, std::integral_constant<int, 1>{}, s1, s0);
     }
     asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no LDS DMA may outlive its slot's use, or the workgroup
+  }
+  if constexpr (UNITS) {
+#pragma unroll
+    for (int d = 0; d < DB; ++d)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) o[d][r] = __builtin_ldexpf(o[d][r], sum_unit - 127);
   }
 
   if (KS > 1) {

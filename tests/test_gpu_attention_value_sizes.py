@@ -19,7 +19,10 @@ def _gpu():
 FEW = [  # new tokens, lengths, heads, kv heads, dim: whole keys with four waves and eight, splits, 32 rows, heads of 256
     ([1, 1], [100, 1], 4, 1, 128), ([1, 1], [300, 250], 4, 2, 64), ([1, 1], [3000, 500], 8, 2, 128), ([4, 9], [3000, 500], 4, 2, 64),
     ([1], [2000], 4, 2, 256)]
-WAYS = FEW
+TILE = [  # chunks: one group of waves, two, splits, heads of 256
+    ([300, 90], [700, 500], 64, 16, 64), ([64], [3000], 8, 2, 128), ([300, 40], [9000, 400], 4, 2, 64), ([90, 30], [200, 64], 2, 1, 256),
+    ([70, 1, 40], [150, 65, 40], 4, 2, 128)]
+WAYS = FEW + TILE
 
 
 def sizes(kind, tokens):
