@@ -55,7 +55,8 @@ __device__ __forceinline__ void join_items(const AttnParams& p, const Seq& sq, i
     for (int s0 = mine; s0 < n; s0 += SP * share) {
       f32x4 x[IT][SP];
       float w[IT][SP];
-      // past the last split the last one again, with no weight: no load waits behind a branch
+      // past the last split the last one again: no load waits behind a branch.  It is its sum that is made
+      // zero, not its weight, which would make NaN of an infinite one.
 #pragma unroll
       for (int t = 0; t < IT; ++t)
 #pragma unroll
@@ -64,15 +65,12 @@ __device__ __forceinline__ void join_items(const AttnParams& p, const Seq& sq, i
 #pragma unroll
       for (int t = 0; t < IT; ++t)
 #pragma unroll
-        for (int j = 0; j < SP; ++j) {
-          const float y = weight[r[t] * n + min(s0 + j * share, n - 1)];
-          w[t][j] = s0 + j * share < n ? y : 0.f;
-        }
+        for (int j = 0; j < SP; ++j) w[t][j] = weight[r[t] * n + min(s0 + j * share, n - 1)];
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int t = 0; t < IT; ++t)
 #pragma unroll
-        for (int j = 0; j < SP; ++j) acc[t] += w[t][j] * x[t][j];
+        for (int j = 0; j < SP; ++j) acc[t] += w[t][j] * (s0 + j * share < n ? x[t][j] : f32x4{0.f, 0.f, 0.f, 0.f});
     }
     if (share > 1) {  // uniform
       sums[tid] = acc[0];
