@@ -307,6 +307,17 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
     r[j] = ((v[j] & e) == e ? 0u : v[j] & 0xFFFFu) | ((v[j] >> 16 & e) == e ? 0u : v[j] & 0xFFFF0000u);
   return r;
 }
+// A scale of 8-bit values that is no finite number acts as such values do: in steps that some row sees only
+// part of it is made zero, and in the second pass the row in LDS gets what its codes are with it.
+__device__ __forceinline__ bool not_finite(float x) { return !__builtin_isfinite(x); }
+template <typename T>
+__device__ __forceinline__ u32x4 times(u32x4 v, float scale) {
+  u32x4 r;
+#pragma unroll
+  for (int j = 0; j < 4; ++j)
+    r[j] = round2<T>(from_bits<T>((uint16_t)v[j]) * scale, from_bits<T>((uint16_t)(v[j] >> 16)) * scale);
+  return r;
+}
 // Two 16-bit ones, for keys `key` and `key` + 1 up to `limit`.
 template <typename T>
 __device__ __forceinline__ uint32_t ones_up_to(int key, int limit) {

@@ -213,7 +213,14 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
   }
   for (; key0 < end; key0 += STEP) {
     store_v();
-    if constexpr (k8) sc[lane] = sr;
+    if constexpr (k8) {
+      const bool bad = value && not_finite(sr);
+      if (key0 + kWaveKeys - 1 > all && __builtin_amdgcn_ballot_w64(bad) != 0) {
+        spoilt = true;
+        if (bad) sr = 0.f;
+      }
+      sc[lane] = sr;
+    }
     __builtin_amdgcn_sched_barrier(0);  // V's registers are free
     f32x4 s[MB][2];
 #pragma unroll
@@ -303,6 +310,14 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
       if (key0 + kWaveKeys - 1 <= all) continue;
       load(key0, page_number(key0));
       store_v();
+      if constexpr (k8) {
+        const unsigned long long bad = __builtin_amdgcn_ballot_w64(value && not_finite(sr)) >> kWaveKeys;
+        sc[lane] = sr;
+        for (int i = 16 * lane; bad != 0 && i < S::V_BYTES; i += 1024) {
+          const int r = i / (2 * HD);  // few_v_place keeps to its row
+          if (bad >> r & 1) *(u32x4*)(vs + i) = times<W>(*(const u32x4*)(vs + i), sc[kWaveKeys + r]);
+        }
+      }
       for (int kind = 0; kind < 3; ++kind)
 #pragma unroll
         for (int mb = 0; mb < MB; ++mb) {

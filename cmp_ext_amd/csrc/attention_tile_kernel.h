@@ -238,10 +238,11 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   auto store_scale = [&](int step_k, int step_v) {
     if (k8 && wave < 2) scales[((value_row ? step_v : step_k) & 3) * 2 * kTileKeys + tid] = sreg;
   };
+  auto value_scales = [&](int step) { return scales + (step & 3) * 2 * kTileKeys + kTileKeys; };
   auto find_unit = [&](int step) {  // the last wave, which finds no rows, behind a barrier after the scales were stored
     if constexpr (UNITS) {
       if (wave != NW - 1) return;
-      float* mine = scales + (step & 3) * 2 * kTileKeys + kTileKeys + lane;
+      float* mine = value_scales(step) + lane;
       const int bits = __float_as_int(fabsf(*mine)), e = bits < 0x7F800000 ? bits >> 23 : 0;
       if (__builtin_amdgcn_ballot_w64(e > unit_found) != 0 || __builtin_amdgcn_ballot_w64(e >= unit_found - 4) == 0) {
         const int most = largest(e);  // 0: only zeros, nothing to go by
@@ -547,13 +548,18 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
       }
       if (begin + (j + 1) * STEP - 1 > tile_all) {  // of any of the groups: all waves come here
         unsigned char* vs = smem + S::V0 + slot * S::BYTES;
-        const bool bad = key0 + kTileKeys - 1 > tile_all && any_not_finite<T>(vs, S::BYTES);  // a group's waves find the same
+        bool bad = false;  // a group's waves find the same
+        if (key0 + kTileKeys - 1 > tile_all) {
+          bad = any_not_finite<T>(vs, S::BYTES);
+          if constexpr (k8) bad = bad || __builtin_amdgcn_ballot_w64(not_finite(value_scales(j)[lane])) != 0;
+        }
         if (KS > 1 || bad) {
           __syncthreads();
           if (bad) {
             spoilt = true;
             if (KS > 1) any_spoilt = 1;
             for (int i = 16 * tid; i < S::BYTES; i += 16 * 64 * NW) *(u32x4*)(vs + i) = finite_only<T>(*(const u32x4*)(vs + i));
+            if (k8 && wave == 0 && not_finite(value_scales(j)[lane])) value_scales(j)[lane] = 0.f;
           }
           __syncthreads();
         }
@@ -608,11 +614,32 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
         dma(true, j, 0);
       } else {
         const int key = key0 + (tid & (kTileKeys - 1));
-        place_row(0, key, page_number(key));
+        const int page = page_number(key);
+        place_row(0, key, page);
+        if constexpr (k8) {
+          if (wave == 1) {
+            // where the scales are is read again: kept through the loop for this, it costs registers (129.5 us for
+            // 125.9, 4 chunks of up to 512 over up to 8100 keys, heads 32 / 8 of 128)
+            auto args = (const __attribute__((address_space(4))) AttnParams*)__builtin_amdgcn_kernarg_segment_ptr();
+            asm("" : "+s"(args));
+            const int place = key % args->kv.page_size;
+            float s = 0.f;
+            if ((unsigned)page < (unsigned)args->kv.pages)
+              s = args->kv.v_scale[page * args->kv.vs_page + place * args->kv.vs_token + kvh * args->kv.vs_head];
+            value_scales(0)[lane] = s;
+          }
+        }
         __syncthreads();
         if constexpr (k8) {
           load_pieces(true, 0);
           store_pieces(true, 0);
+          __syncthreads();
+          const float* sc = value_scales(0);
+          for (int i = 16 * tid; i < S::BYTES; i += 16 * 64 * NW) {
+            const int r = i / S::ROW;  // v_place keeps to its row
+            u32x4* at = (u32x4*)(smem + S::V0 + i);
+            if (not_finite(sc[r])) *at = times<T>(*at, sc[r]);
+          }
         } else {
           dma_rows(true, 0, 0);
         }
