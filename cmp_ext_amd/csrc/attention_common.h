@@ -218,12 +218,39 @@ __device__ __forceinline__ u32x2 e4m3x4(uint32_t c) {
   return r;
 }
 
+// fp16 numbers lose bits below 2^-14 and are zero below 2^-25, so fp16 weights are taken times a power of two
+// that puts the largest of a row near the type's end, not at 1: the sums get the same factor and it cancels.
+// With it the other keys keep their weights where one key stands far above them (its score 16 above, of 600
+// keys: off by 3e-4 of the result, without it by 4e-2).
+template <typename T>
+constexpr bool kHalf = std::is_same<T, _Float16>::value;
+
+typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 // Two floats rounded to nearest even, as one instruction.
 template <typename T>
 __device__ __forceinline__ uint32_t round2(float lo, float hi) {
   typedef float f32x2 __attribute__((ext_vector_type(2)));
   typedef T t2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2{lo, hi}), t2));
+}
+
+// Two floats cut to 16 bits towards zero.
+template <typename T>
+__device__ __forceinline__ uint32_t cut2(float lo, float hi) {
+  if constexpr (kHalf<T>)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pkrtz(lo, hi));
+  else
+    return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
+}
+// What cutting two weights to `cut` has left.  Not zero unless the first part is, and of its sign: a value of
+// infinity times both is infinity, where 0 or a second part below zero would make it NaN.  (What is put for
+// zero, the least number of fp16 or the least normal one of bf16, is 2^-39 of the largest weight, or less.)
+template <typename T>
+__device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t cut) {
+  const float a = lo - from_bits<T>((uint16_t)cut), b = hi - from_bits<T>((uint16_t)(cut >> 16));
+  constexpr unsigned short least = kHalf<T> ? 0x0001 : 0x0080;
+  const u16x2 some = __builtin_elementwise_min(__builtin_bit_cast(u16x2, cut), u16x2{least, least});
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, round2<T>(a, b)), some));
 }
 
 // The larger of two, NaN if one is: two of them are one instruction of three operands, while
@@ -235,13 +262,6 @@ __device__ __forceinline__ float max_halves(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-
-// fp16 numbers lose bits below 2^-14 and are zero below 2^-25, so fp16 weights are taken times a power of two
-// that puts the largest of a row near the type's end, not at 1: the sums get the same factor and it cancels.
-// With it the other keys keep their weights where one key stands far above them (its score 16 above, of 600
-// keys: off by 3e-4 of the result, without it by 4e-2).
-template <typename T>
-constexpr bool kHalf = std::is_same<T, _Float16>::value;
 
 // 2^x, the hardware's (relative error about 2^-23; 0 for -infinity).
 __device__ __forceinline__ float exp2_hw(float x) { return __builtin_amdgcn_exp2f(x); }
@@ -265,7 +285,6 @@ __device__ __forceinline__ u32x2 lds_read_tr(const unsigned char* q) {
 template <typename T>
 constexpr uint32_t kExponents = std::is_same<T, _Float16>::value ? 0x7C007C00u : 0x7F807F80u;
 
-typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
 // Whether the stretch of `bytes` of LDS (a multiple of 1024) holds one; the same for all lanes.
 template <typename T>
 __device__ __forceinline__ bool any_not_finite(const unsigned char* lds, int bytes) {
@@ -307,8 +326,9 @@ __device__ __forceinline__ u32x4 finite_only(u32x4 v) {
     r[j] = ((v[j] & e) == e ? 0u : v[j] & 0xFFFFu) | ((v[j] >> 16 & e) == e ? 0u : v[j] & 0xFFFF0000u);
   return r;
 }
-// A scale of 8-bit values that is no finite number acts as such values do: in steps that some row sees only
-// part of it is made zero, and in the second pass the row in LDS gets what its codes are with it.
+// A scale of 8-bit values that is no finite number acts as such values do: it is made zero (in the tile
+// kernel in steps that some row sees only part of), and in the second pass the row in LDS gets what its
+// codes are with it.
 __device__ __forceinline__ bool not_finite(float x) { return !__builtin_isfinite(x); }
 template <typename T>
 __device__ __forceinline__ u32x4 times(u32x4 v, float scale) {

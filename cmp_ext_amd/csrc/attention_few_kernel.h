@@ -204,6 +204,9 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
   };
 
   constexpr int STEP = NW * kWaveKeys;
+  // values that are not finite are looked for in steps with keys past this, and added in a second pass over those
+  // (all of them once a scale is not finite: what a step has had already it gets again, infinity or NaN)
+  int whole = all;
   bool spoilt = false;
   int key0 = begin + wave * kWaveKeys;
   int page = -1;
@@ -215,8 +218,9 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
     store_v();
     if constexpr (k8) {
       const bool bad = value && not_finite(sr);
-      if (key0 + kWaveKeys - 1 > all && __builtin_amdgcn_ballot_w64(bad) != 0) {
+      if (__builtin_amdgcn_ballot_w64(bad) != 0) {
         spoilt = true;
+        whole = -1;
         if (bad) sr = 0.f;
       }
       sc[lane] = sr;
@@ -252,7 +256,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
         vsc[b] = *(const f32x4*)(sc + 32 + 16 * b + 4 * G);
       }
     }
-    u32x4 pw[MB], pl[MB];  // weights, and what their rounding left
+    u32x4 pw[MB], pl[MB];  // weights, and what cutting them left
 #pragma unroll
     for (int mb = 0; mb < MB; ++mb) {
       float mx = -INFINITY;
@@ -289,11 +293,11 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
         }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        pw[mb][i] = round2<W>(w[2 * i], w[2 * i + 1]);
-        pl[mb][i] = round2<W>(w[2 * i] - from_bits<W>((uint16_t)pw[mb][i]), w[2 * i + 1] - from_bits<W>((uint16_t)(pw[mb][i] >> 16)));
+        pw[mb][i] = cut2<W>(w[2 * i], w[2 * i + 1]);
+        pl[mb][i] = rest2<W>(w[2 * i], w[2 * i + 1], pw[mb][i]);
       }
     }
-    if (key0 + kWaveKeys - 1 > all && any_not_finite<W>(vs, S::V_BYTES)) {
+    if (key0 + kWaveKeys - 1 > whole && any_not_finite<W>(vs, S::V_BYTES)) {
       spoilt = true;
       for (int i = 16 * lane; i < S::V_BYTES; i += 1024) *(u32x4*)(vs + i) = finite_only<W>(*(const u32x4*)(vs + i));
     }
@@ -307,7 +311,7 @@ __global__ void __launch_bounds__(64 * NW, HD == 256 ? 1 : MB == 2 || NW == 8 ? 
   }
   if (spoilt) {  // add what was made zero (see any_not_finite)
     for (key0 = begin + wave * kWaveKeys; key0 < end; key0 += STEP) {
-      if (key0 + kWaveKeys - 1 <= all) continue;
+      if (key0 + kWaveKeys - 1 <= whole) continue;
       load(key0, page_number(key0));
       store_v();
       if constexpr (k8) {
