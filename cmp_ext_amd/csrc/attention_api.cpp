@@ -144,21 +144,23 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   if (r.blocks16) {
     // MI355X, one token for each sequence, heads 32 / 8 of 128: two workgroups a CU keep it busy;
     // sequences of one batch differ, so more of them want finer splits to even out (16 of up to
-    // 2000 keys: 512 workgroups 20.7 us, 1024 15.9; 64 of up to 8192 in 8 bits: splits of 8192 keys
-    // 154, 2048 130, 1024 123), but not below 256 keys, and none where the tiles fill the GPU (64 of
-    // up to 1000: 27.2 whole, 31.3 in splits of 512).  A few short ones are latency: 128 keys, one
-    // step of each wave (4 of 1000 keys: 10.3 us, in splits of 512 14.4).  Over 128 splits joining
-    // them costs more than they save (one of 65536, heads 8 / 2: 128 splits 22.3 us, 256 26.7).
+    // 2000 keys: 512 workgroups 20.1 us, 1024 16.0, 2048 20.3; 64 of up to 8192 in 8 bits: splits of 8192
+    // keys 153, 2048 130, 1024 124, 512 130), but not below 256 keys, and none where the tiles fill the GPU
+    // (64 of up to 1000: 26.1 whole, 31.0 in splits of 512).  A few short ones are latency: 128 keys, one
+    // step of each wave (4 of up to 1000 keys: 10.4 us, in splits of 512 14.3).  Over 128 splits joining
+    // them costs more than they save (one of 65536, heads 8 / 2: 128 splits 22.2 us, 256 26.9).
+    // (`keys` is what the table has room for: with one for 131072 keys splits have 1024, and 64 of up to 8192
+    // take 256 us for 189, 4 of up to 4000 21.4 for 15.4.)
     const bool ragged = a->batch > 4;
     least = ragged ? 256 : 128;
     if (groups < 512) n = ((ragged ? 1024 : 512) + groups - 1) / groups;
     n = std::min<int64_t>(std::max<int64_t>(n, keys / 1024), 128);
-    // Short keys stay whole where a workgroup is through them sooner than splits are joined (4 of 250 keys
-    // 7.4 and 9.5 in two, 32 of up to 500 11.7 and 14.8, of up to 1000 18.2 and 20.5; but 16 of up to
-    // 1000, 128 tiles, 17.4 and 15.2).  Eight waves are through 8-bit keys in half the steps (4 of 500
-    // keys 8.5 us, 4 waves whole 10.0 and in splits 9.8; 32 of up to 500 9.3, 11.2 and 13.4, of up to 1000
-    // 13.7, 17.7 and 16.2; but 4 of 1000 11.6, in splits 10.3); of 16-bit keys a CU takes in no more
-    // bytes (4 of 1000 keys whole: 15.2 with eight waves, 16.0 with four).
+    // Short keys stay whole where a workgroup is through them sooner than splits are joined (4 of up to 250
+    // keys 7.6 and 9.6 in two, 32 of up to 500 11.8 and 15.1, of up to 1000 18.0 and 20.9; but 16 of up to
+    // 1000, 128 tiles, 17.1 and 15.4).  Eight waves are through 8-bit keys in half the steps (4 of up to 500
+    // keys 8.6 us, 4 waves whole 10.3 and in splits 10.0; 32 of up to 500 9.4, 11.4 and 13.5, of up to 1000
+    // 13.9, 18.1 and 16.4; but 4 of up to 1000 11.7, in splits 10.4); of 16-bit keys a CU takes in no more
+    // bytes (4 of up to 1000 keys whole: 15.2 with eight waves, when they were tried, 15.9 with four).
     r.waves = 4;
     if (groups <= 256) {
       if (r.kind == kKvPaged8 && r.blocks16 == 1 && r.hd <= 128 && keys > 128 && keys <= (groups >= 128 ? 1024 : 512))
@@ -167,20 +169,21 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
         n = 1;
     }
   } else if (paged) {
-    // (Times of the tile kernel here and for prompts are from before its last steps, which took 5 to 12 %
-    // off either side.)  Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
+    // Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
     // not so long that workgroups of their own pay (16 bits, heads 32 / 8 of 128: 64 new tokens over
-    // 8192 keys 49.0 us with one group and 8 splits, 41.1 with two; 16 of up to 64 over up to 4096
-    // 48.4 and 44.7; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 148).
+    // 8192 keys 43.0 us with one group and 8 splits, 37.4 with two; 16 of up to 64 over up to 4096
+    // 50.7 and 42.4; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 129).  (The rule's limits are on
+    // the safe side: one of 1024 over 4096, counted as 264 tiles, 90 in two splits, 78 with two groups.)
     // Splits: all at once, two workgroups a CU (8 bits: one of 512 new tokens over 8192 keys, 136 tiles,
-    // 282 us whole, 130 in 3, 107 in 4, 133 in 6).  How many keys that is follows from the lengths: up to 62
-    // sequences find it on the device (2 of up to 512 over up to 8000 130 us, in 4 splits by the number of
-    // tiles 158; 4 of up to 256 over up to 16000 182 and 227).  Many uneven tiles even out better in two
-    // rounds of splits (30 of up to 60 over up to 3000, 368 tiles, 74 and 84).
+    // 255 us whole, 125 in 3, 103 in 4, 125 in 6).  How many keys that is follows from the lengths: up to 62
+    // sequences find it on the device (2 of up to 512 over up to 8000 123 us, in 4 splits by the number of
+    // tiles 152; 4 of up to 256 over up to 16000 176, in 3 splits 216, in 4 172).  Many uneven tiles even out
+    // better in two rounds of splits (30 of up to 60 over up to 3000, 368 tiles, 70.6 and 78.7).
     // Where tiles are many, those that see most keys go first, and no keys are split: 32 of up to 300 new
-    // tokens over up to 2000 keys, 1200 tiles, 150 us in the order of the sequences, 95 longest first (60
-    // of up to 100 over 1000, 960 tiles: 65.6 in splits, 42; but 60 of up to 60 over up to 4000, 752
-    // tiles: 131 in splits, 150).  Packed prompts gain nothing by that order (30 of up to 500: 51 and 63).
+    // tokens over up to 2000 16-bit keys, 1200 tiles, 118 us in the order of the sequences, 84.5 longest first
+    // (60 of up to 100 over 1000, 960 tiles: 68.8 in splits, 41.5; but 60 of up to 60 over up to 4000, 752
+    // tiles: 117 in splits, 123).  Packed prompts gained nothing by that order when it was tried (30 of up to
+    // 500: 51 us, 63 with it).
     const bool ragged = a->batch > 4;
     least = 256;
     p.longest_first = !uniform_q && ragged && a->batch <= 62 && (groups >= 1024 || (groups >= 512 && keys <= 5 * groups));
@@ -198,9 +201,9 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
   } else if (groups < 384 && keys >= 512) {
     // Prompts see half their keys, the longest rows first: two groups, or splits, gain where tiles are
     // few and keys long (heads 32 / 8 of 128: one of 1000 tokens, 250 tiles, 25.7 us with one group,
-    // 24.1 with two, 32.9 in 2 splits; of 300 13.0 and 14.7 with two.  Heads 8 / 2 of 64, one of 2361:
-    // 32.5, 26.9 with two groups, 22.0 in 2 splits as well; of 128, one of 4096, 256 tiles: 75.7,
-    // 62.4, 57.4 with one group in 3 splits).
+    // 24.6 with two, 33.4 in 2 splits; of 700 19.8 and 20.1, of 300 13.1 and 14.9.  Heads 8 / 2 of 64, one of
+    // 2361: 33.1, 27.1 with two groups, 22.1 in 2 splits as well; of 128, one of 4096, 256 tiles: 72.9,
+    // 62.5, 58.9 with one group in 3 splits).
     least = 512;
     if (r.hd <= 128 && groups <= (keys >= 2048 ? 160 : 256)) {
       r.ks = 2;

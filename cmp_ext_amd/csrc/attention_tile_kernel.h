@@ -4,8 +4,8 @@
 // Rows: a workgroup of four waves takes 128 rows of one sequence and one kv head, a row being one
 // query of one head of the group (row r: query r / group, head r % group), so that grouped heads
 // share each step's keys and values and short sequences fill their tiles.  A wave owns 32 rows.
-// (8192 tokens, 32 heads of 128 and 8 of keys, bf16, on MI355X: 503 us, 1093 TFLOP/s of the products
-// that are not masked.  Where four waves of 32 rows took 529, eight over 256 rows, whose barriers bind all
+// (8192 tokens, 32 heads of 128 and 8 of keys, bf16, on MI355X: 512 us, 503 to 520 on different boxes,
+// 1074 TFLOP/s of the products that are not masked.  When four waves of 32 rows took 529, eight over 256 rows, whose barriers bind all
 // waves of a CU together, took 548, and four of 64 rows with a SIMD to themselves 643.)
 //
 // Keys: where there are fewer tiles than CUs, a workgroup has two such groups of four waves (KS = 2),
@@ -29,12 +29,14 @@
 // weights of step j, then the weighted values of step j beside its other weights and the maximum
 // of step j + 1.  The vector work (per score: scale, exponential at half the rate, sum, half a
 // conversion, half a maximum) is over half as long as the products.  On that prompt the matrix cores
-// are busy 57 % of the cycles and the vector units 50 %, a wave waits for LDS or its barrier 23 % of its
-// time, and the clock is 1.85 GHz: power bounds it as well (more fragments on their way, or other shares
-// of the vector work in the two phases, change nothing).
+// are busy 56 % of the cycles and the vector units 49 %, a wave waits for LDS or its barrier 23 % of its
+// time, and power bounds it as well: 1339 W of the board's 1400, at 1.79 GHz (2.4 under the other kernels
+// here).  More fragments on their way, or other shares of the vector work in the two phases, changed nothing.
 //
 // The weights are rounded once to 16 bits for the second product, their sum is of the unrounded
-// ones: the result is off by its own rounding and by one of the same size more.
+// ones: the result is off by its own rounding and by one of the same size more (in fp16 for weights down to
+// 2^-24 of the row's largest; over codes, down to 2^-20 of the largest times the largest scale among the 64 keys
+// of a step; below that a weight is off by up to 2^-35, or 2^-31, of that).
 //
 // Keys and values of a step lie in LDS as rows of HD 16-bit elements in two slots each, K
 // with its 16-byte chunks and V with its 64-byte segments permuted by the row so that the reads

@@ -1,7 +1,7 @@
 // Norms of queries and keys for each head with the position rotation, in one pass over both:
 //   y = x * rsqrt(mean(x^2) + eps) * weight,  pairs (a, b) -> (a cos - b sin, b cos + a sin).
-// Bound by reading and writing every element once: 8192 tokens of 40 heads of 128 in 36 us on MI355X,
-// 4.75 TB/s (a large copy moves 5.25); a few tokens by the launch, 3 us, and the call from the host, 5.
+// Bound by reading and writing every element once: 8192 tokens of 40 heads of 128 in 37 us on MI355X,
+// 4.7 TB/s (a large copy moves 5.25), in fp32 71.5; a few tokens by the launch, 4 us, and the call from the host, 5.
 //
 // Vector kernel (rows of 16-byte pieces): a head belongs to dim / 16 neighbouring lanes (rounded
 // up to a power of two), and a lane holds the two pieces of 8 elements whose elements pair up
@@ -9,7 +9,8 @@
 // that only the sum of squares crosses lanes.  (Two or four heads a lane, with one row of the tables:
 // no faster.)  The tables are read as fp32, one row per token,
 // shared by its heads through the caches.
-// General kernel (any dim, alignment): one wave per head, an element at a time.
+// General kernel (any dim, alignment): one wave per head, an element at a time, its partner read again: 200 us
+// for those tokens with heads of 100 (26 for their bytes at the copy's rate).
 #include "attention_params.h"
 #include "device_common.h"
 

@@ -26,7 +26,10 @@ def rope_table(max_positions: int, rotary_dim: int, base: float = 10000.0, *, sc
       "yarn"    frequencies that turn more than beta_fast times within original_positions stay, those
                 that turn less than beta_slow times are divided by factor, those between are mixed
                 linearly by their turns, and both tables are multiplied by attention_factor
-                (0.1 ln(factor) + 1 unless given).
+                (0.1 ln(factor) + 1 unless given).  Implementations that mix linearly over the
+                index i instead, between the indices of the two bounds, turn those between by other
+                frequencies (up to a factor of 3 for 128, factor 16 and 4096 positions): a model
+                that was trained with one needs its own tables, which `qk_norm_rope` takes as well.
     """
     if max_positions < 0:
         raise ValueError(f"rope_table: max_positions must not be negative, got {max_positions}")

@@ -102,8 +102,14 @@ int cmpext3_kv_cache_read(const cmpext3_kv_cache* cache, const int32_t* block_ta
  * h / (heads / kv_heads)):
  *   out_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = exp(scale * q_i . k_j)
  * over j < len_k, and with `causal` j <= i + len_k - len_q (the last query sees the last
- * key).  A query that sees no key gets zeros, one whose scores are all -inf NaN.  Products on the matrix cores with fp32 sums,
- * softmax statistics in fp32, the weights p rounded to the 16-bit type for the second product.
+ * key).  A query that sees no key gets zeros, one whose scores are all -inf NaN; keys, values and
+ * scales that a query does not see take no part in its row, NaN and infinity among them.
+ * Products on the matrix cores with fp32 sums, softmax statistics in fp32.  For the second
+ * product the weights p (times their values' scales) are held
+ *   pages, up to 32 rows of a sequence and kv head on average: as two 16-bit numbers each (over
+ *     e4m3 both bf16), so that the result is off by its own rounding only;
+ *   otherwise: rounded to the type of q.  In fp16, which ends at 2^-25, a row's largest weight is
+ *     taken as 2^10 to 2^14, and the scales of each 64 values in a power of two of their own size.
  *
  * Keys and values: packed (cache.k/v with k_token, k_head, ...; block_table NULL), where
  * cache.k_page is the stride between batch entries of uniform length; or paged (block_table
