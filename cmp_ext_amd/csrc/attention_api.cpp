@@ -172,8 +172,8 @@ int plan_attention(const cmpext3_attention_args* a, AttnPlan* out) {
     // Two groups of waves share a tile's keys where the tiles do not fill the CUs and the keys are
     // not so long that workgroups of their own pay (16 bits, heads 32 / 8 of 128: 64 new tokens over
     // 8192 keys 43.0 us with one group and 8 splits, 37.4 with two; 16 of up to 64 over up to 4096
-    // 50.7 and 42.4; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 129).  (The rule's limits are on
-    // the safe side: one of 1024 over 4096, counted as 264 tiles, 90 in two splits, 78 with two groups.)
+    // 50.7 and 42.4; but 4 of up to 512 over up to 8100, 240 tiles, 114 and 129).  (The limits
+    // do not take the best everywhere: one of 1024 over 4096, counted as 264 tiles, 90 in two splits, 78 with two groups.)
     // Splits: all at once, two workgroups a CU (8 bits: one of 512 new tokens over 8192 keys, 136 tiles,
     // 255 us whole, 125 in 3, 103 in 4, 125 in 6).  How many keys that is follows from the lengths: up to 62
     // sequences find it on the device (2 of up to 512 over up to 8000 123 us, in 4 splits by the number of

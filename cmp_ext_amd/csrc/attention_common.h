@@ -242,9 +242,10 @@ __device__ __forceinline__ uint32_t cut2(float lo, float hi) {
   else
     return __builtin_amdgcn_perm(__float_as_uint(hi), __float_as_uint(lo), 0x07060302u);
 }
-// What cutting two weights to `cut` has left.  Not zero unless the first part is, and of its sign: a value of
-// infinity times both is infinity, where 0 or a second part below zero would make it NaN.  (What is put for
-// zero, the least number of fp16 or the least normal one of bf16, is 2^-39 of the largest weight, or less.)
+// What cutting two weights (not negative) to `cut` has left.  Not zero unless the first part is: a value of
+// infinity times both is infinity, where 0 or a second part below zero, as rounding leaves, would make it NaN.
+// (What is put for zero, the least number of fp16 or the least normal one of bf16, is 2^-39 of the largest
+// weight, or less.)
 template <typename T>
 __device__ __forceinline__ uint32_t rest2(float lo, float hi, uint32_t cut) {
   const float a = lo - from_bits<T>((uint16_t)cut), b = hi - from_bits<T>((uint16_t)(cut >> 16));

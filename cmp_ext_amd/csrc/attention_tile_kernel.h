@@ -5,8 +5,8 @@
 // query of one head of the group (row r: query r / group, head r % group), so that grouped heads
 // share each step's keys and values and short sequences fill their tiles.  A wave owns 32 rows.
 // (8192 tokens, 32 heads of 128 and 8 of keys, bf16, on MI355X: 512 us, 503 to 520 on different boxes,
-// 1074 TFLOP/s of the products that are not masked.  When four waves of 32 rows took 529, eight over 256 rows, whose barriers bind all
-// waves of a CU together, took 548, and four of 64 rows with a SIMD to themselves 643.)
+// 1074 TFLOP/s of the products that are not masked.  When four waves of 32 rows took 529, eight over 256 rows,
+// whose barriers bind all waves of a CU together, took 548, and four of 64 rows with a SIMD to themselves 643.)
 //
 // Keys: where there are fewer tiles than CUs, a workgroup has two such groups of four waves (KS = 2),
 // one for the even steps and one for the odd ones, each with its own LDS, joined in LDS at the end:
@@ -210,8 +210,8 @@ __global__ void __launch_bounds__(64 * kTileWaves * KS, HD == 256 ? 1 : HD == 64
   // fp16: V's scales of a step are held in a power of two of their own size, 2^(unit - 127), and so are the
   // sums: weights that carry them stay where fp16 has its bits (see kHalf) whatever the values' size.
   // The unit is raised to the largest of a step, and lowered to it if that is over 2^4 smaller.  (4 of up to
-  // 512 over up to 8100 keys, heads 32 / 8 of 128: 130 us for 127 without; found by the wave that stores the
-  // scales, which has most to do, 134.)
+  // 512 over up to 8100 keys, heads 32 / 8 of 128: 130 us for 127 without, of 64: 104 for 99; found by the wave that
+  // stores the scales, which has most to do, 134 for heads of 128.)
   constexpr bool UNITS = k8 && kHalf<T>;
   int* units = (int*)(smem + S::UNITS);  // [step % 4]
   int unit_found = 127, most_found = 1;  // the wave that finds it: of the last step, the largest of all
