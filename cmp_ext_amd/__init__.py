@@ -1,4 +1,4 @@
-"""cmpext3 operators for AMD Instinct MI355X (gfx950): dense GEMM, and the attention layer next to it.
+"""cmpext3 operators for AMD Instinct MI355X (gfx950): dense GEMM, and the attention layer and feed-forward block next to it.
 
 Python surface (same names and argument meaning as the reference extension's
 GEMM entry points, src/main.cpp:1594-1602, plus the dtype-specific matmuls):
@@ -25,6 +25,15 @@ What stands between an attention layer's projections when it serves a model (for
     paged_attention(q, k_cache, v_cache, block_table, seq_lens, cu_seqlens_q=None, k_scale=None,
                     v_scale=None, causal=True, scale=None)     new tokens over a paged cache
 
+The projections of a feed-forward block:
+
+    gated_linear(x, w_gate, w_up, activation="silu")           act(x @ w_gate.T) * (x @ w_up.T), with its backward pass
+    quantize_int8(x)                                           rows as int8 codes with a scale for each
+    int8_linear(x, weight, weight_scale, bias=None, x_scale=None, dtype=None)
+                                                               x @ weight.T in 8-bit integers (forward only)
+    int8_gated_linear(x, w_gate, w_up, gate_scale, up_scale, activation="silu", x_scale=None, dtype=None)
+                                                               the gated one in 8-bit integers (forward only)
+
 Every call runs the hand-written gfx950 kernels of lib/libcmpext3_gemm.so on
 PyTorch's current stream.  There is no fallback: if the compiled extension is
 missing, every operator access (and `import cmpext3`) raises ImportError; only
@@ -33,8 +42,10 @@ the `build` submodule stays usable.
 import torch  # noqa: F401  (loads PyTorch's HIP runtime before the extension binds to it)
 
 __all__ = ["fp16_matmul", "bf16_matmul", "fp32_matmul", "linear", "bmm", "conv2d", "plan", "last_plan",
-           "qk_norm_rope", "kv_cache_write", "kv_cache_read", "attention", "paged_attention", "rope_table", "version"]
+           "qk_norm_rope", "kv_cache_write", "kv_cache_read", "attention", "paged_attention", "rope_table",
+           "gated_linear", "quantize_int8", "int8_linear", "int8_gated_linear", "version"]
 
+from .gated import gated_linear  # noqa: E402
 from .rope import rope_table  # noqa: E402
 
 try:
@@ -61,9 +72,13 @@ if _ext is not None:
     kv_cache_read = _ext.kv_cache_read
     attention = _ext.attention
     paged_attention = _ext.paged_attention
+    quantize_int8 = _ext.quantize_int8
+    int8_linear = _ext.int8_linear
+    int8_gated_linear = _ext.int8_gated_linear
     version = _ext.version
     extension_path = _ext.__file__
 else:
+    del gated_linear  # needs the extension: raises at access, as the others do
 
     def __getattr__(name):
         # The submodule `cmp_ext_amd.build` stays importable so that an unbuilt tree can be

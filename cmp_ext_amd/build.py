@@ -2,7 +2,7 @@
 
 Outputs (git-ignored, shipped to the GPU box with the tree):
   cmp_ext_amd/lib/libcmpext3_gemm.so   HIP kernels + C ABI (include/cmpext3_gemm.h,
-                                       include/cmpext3_attention.h)
+                                       include/cmpext3_attention.h, include/cmpext3_projection.h)
   cmp_ext_amd/_cmpext3<EXT_SUFFIX>      pybind11 module `cmpext3` (links the above)
 
 The kernels are compiled with hipcc for gfx950 only; the host-only sources
@@ -31,9 +31,10 @@ HIP_SOURCES = [f"tile_{t}_{lay}_{k}.hip" for t in ("f16", "bf16") for lay in ("k
     ["skinny.hip", "tall.hip", "stream.hip", "stream_nk.hip", "f32.hip", "generic.hip", "pad.hip", "noalloc.hip", "sem.hip"] + \
     [f"attention_tile_{t}_{k}.hip" for t in ("f16", "bf16") for k in ("packed", "paged16", "paged8")] + \
     [f"attention_few_{t}_{k}.hip" for t in ("f16", "bf16") for k in ("paged16", "paged8")] + \
-    ["attention_join.hip", "qk_norm_rope.hip", "kv_cache.hip"]
-HOST_SOURCES = ["selector.cpp", "api.cpp", "attention_api.cpp"]
-BINDING_SOURCES = ["main.cpp", "attention_ops.cpp"]
+    ["attention_join.hip", "qk_norm_rope.hip", "kv_cache.hip"] + \
+    ["projection_any.hip", "quantize.hip", "gated_grad.hip"]
+HOST_SOURCES = ["selector.cpp", "api.cpp", "attention_api.cpp", "projection_api.cpp"]
+BINDING_SOURCES = ["main.cpp", "attention_ops.cpp", "projection_ops.cpp"]
 
 HIP_FLAGS = [
     "--offload-arch=gfx950",

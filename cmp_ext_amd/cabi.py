@@ -1,5 +1,5 @@
-"""ctypes view of the C ABI in include/cmpext3_gemm.h and include/cmpext3_attention.h
-(libcmpext3_gemm.so).
+"""ctypes view of the C ABI in include/cmpext3_gemm.h, include/cmpext3_attention.h and
+include/cmpext3_projection.h (libcmpext3_gemm.so).
 
 Used by the tests and the benchmark to drive the kernels through the same
 boundary a non-Python caller would bind.  PyTorch is imported first so that
@@ -15,7 +15,8 @@ import torch  # noqa: F401
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "lib", "libcmpext3_gemm.so")
 
-F16, BF16, F32, E4M3 = 0, 1, 2, 3
+F16, BF16, F32, E4M3, I8 = 0, 1, 2, 3, 4
+ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_RELU = 0, 1, 2, 3
 B_KN, B_NK = 0, 1
 OK, ERR_INVALID_ARG, ERR_UNSUPPORTED, ERR_TOO_LARGE, ERR_WORKSPACE, ERR_SCRATCH = 0, -1, -2, -3, -4, -5
 SCRATCH_BYTES = 64 << 20
@@ -82,6 +83,33 @@ ATTENTION_SIGNATURES = {
     "cmpext3_attention_describe": (_i, [_p, _cp, _i]),
 }
 
+
+# The structures of include/cmpext3_projection.h.
+class QuantizeInt8Args(ctypes.Structure):
+    _fields_ = _fields("i32: dtype cols; i64: rows; ptr: x; i64: x_row; ptr: codes; i64: codes_row; ptr: scale")
+
+
+class ProjectionArgs(ctypes.Structure):
+    _fields_ = _fields("""i32: dtype out_dtype activation M N K; ptr: x; i64: x_row; ptr: x_scale w_gate; i64: gate_row; ptr: gate_scale w_up;
+                          i64: up_row; ptr: up_scale bias out; i64: out_row; ptr: gate_out up_out; i64: pre_row""")
+
+
+class GatedBackwardArgs(ctypes.Structure):
+    _fields_ = _fields("""i32: dtype activation M N K; ptr: grad_out; i64: grad_row; ptr: gate up; i64: pre_row; ptr: x; i64: x_row;
+                          ptr: w_gate; i64: gate_row; ptr: w_up; i64: up_row; ptr: dx; i64: dx_row; ptr: dw_gate; i64: dgate_row;
+                          ptr: dw_up; i64: dup_row""")
+
+
+# Exported symbols of include/cmpext3_projection.h.
+PROJECTION_SIGNATURES = {
+    "cmpext3_quantize_int8": (_i, [_p, _p]),
+    "cmpext3_projection_workspace_size": (_i64, [_p]),
+    "cmpext3_projection": (_i, [_p, _p, _i64, _p]),
+    "cmpext3_projection_describe": (_i, [_p, _cp, _i]),
+    "cmpext3_gated_backward_workspace_size": (_i64, [_p]),
+    "cmpext3_gated_backward": (_i, [_p, _p, _i64, _p]),
+}
+
 _lib = None
 
 
@@ -91,7 +119,7 @@ def lib() -> ctypes.CDLL:
         if not os.path.exists(LIB_PATH):
             raise OSError(f"{LIB_PATH} not built; run `python -m cmp_ext_amd.build`")
         l = ctypes.CDLL(LIB_PATH)
-        for name, (res, args) in {**SIGNATURES, **ATTENTION_SIGNATURES}.items():
+        for name, (res, args) in {**SIGNATURES, **ATTENTION_SIGNATURES, **PROJECTION_SIGNATURES}.items():
             f = getattr(l, name)
             f.restype = res
             f.argtypes = args

@@ -15,6 +15,7 @@
 
 #include "../../include/cmpext3_gemm.h"
 #include "attention_ops.h"
+#include "projection_ops.h"
 
 namespace {
 
@@ -381,5 +382,6 @@ PYBIND11_MODULE(_cmpext3, m) {
         "Describe the kernel(s) the last operator call on this thread ran (its actual pointers, pitches and "
         "workspace)");
   register_attention_ops(m);
+  register_projection_ops(m);
   m.def("version", []() { return std::string(cmpext3_version()); });
 }

@@ -1,0 +1,154 @@
+"""The feed-forward operators without a GPU: what the Python surface and the C ABI refuse before any launch."""
+import ctypes
+import os
+import re
+
+import pytest
+import torch
+
+import cmpext3
+from cmp_ext_amd import cabi
+
+HEADER = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include", "cmpext3_projection.h")
+BAD, NOT, BIG, WORK = cabi.ERR_INVALID_ARG, cabi.ERR_UNSUPPORTED, cabi.ERR_TOO_LARGE, cabi.ERR_WORKSPACE
+
+
+def header():
+    return re.sub(r"/\*.*?\*/", "", open(HEADER).read(), flags=re.S)
+
+
+def test_exports_match_the_header():
+    declared = set(re.findall(r"\b(cmpext3_\w+)\s*\(", header()))
+    assert declared == set(cabi.PROJECTION_SIGNATURES)
+    for name in declared:
+        assert hasattr(cabi.lib(), name)
+
+
+def test_structures_match_the_header():
+    kinds = {"int32_t": ctypes.c_int32, "int64_t": ctypes.c_int64, "float": ctypes.c_float}
+    for cls, name in ((cabi.QuantizeInt8Args, "cmpext3_quantize_int8_args"), (cabi.ProjectionArgs, "cmpext3_projection_args"),
+                      (cabi.GatedBackwardArgs, "cmpext3_gated_backward_args")):
+        body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), header(), re.S).group(1)
+        want = []
+        for line in body.split(";"):
+            m = re.match(r"\s*(const )?(\w+)(\*?)\s+(.*)", line.strip(), re.S)
+            if not m:
+                continue
+            for field in m.group(4).split(","):
+                pointer = m.group(3) or field.strip().startswith("*")
+                want.append((field.strip().lstrip("*"), ctypes.c_void_p if pointer else kinds[m.group(2)]))
+        assert [tuple(f) for f in cls._fields_] == want
+
+
+def test_constants_match_the_header():
+    for name, value in re.findall(r"#define CMPEXT3_(ACT_\w+|I8) (\d+)", header()):
+        assert getattr(cabi, name) == int(value)
+
+
+def refuses(match, fn, *args, **kw):
+    with pytest.raises(RuntimeError, match=match):
+        fn(*args, **kw)
+
+
+def test_python_refusals():
+    h, c = torch.zeros(3, 16, dtype=torch.float16), torch.zeros(5, 16, dtype=torch.int8)
+    s = torch.ones(5)
+    refuses("on a GPU", cmpext3.quantize_int8, h)
+    refuses("unsupported dtype", cmpext3.quantize_int8, h.double())
+    refuses("unsupported dtype", cmpext3.quantize_int8, c)
+    refuses("at least one dimension", cmpext3.quantize_int8, h[0, 0])
+    refuses("on a GPU", cmpext3.int8_linear, h, c, s)
+    refuses("at least one dimension", cmpext3.int8_linear, h[0, 0], c, s)
+    refuses("on a GPU", cmpext3.int8_gated_linear, h, c, c, s, s)
+    refuses("unknown activation 'swish'", cmpext3.int8_gated_linear, h, c, c, s, s, "swish")
+    refuses("on a GPU", cmpext3.gated_linear, h, c.half(), c.half())
+
+
+def projection(**kw):
+    a = cabi.ProjectionArgs(dtype=cabi.BF16, out_dtype=cabi.BF16, activation=cabi.ACT_SILU, M=8, N=64, K=128, x=0x1000, x_row=128,
+                            w_gate=0x2000, gate_row=128, w_up=0x3000, up_row=128, out=0x4000, out_row=64)
+    if kw.get("dtype") == cabi.I8:
+        a.x_scale, a.gate_scale, a.up_scale = 0x5000, 0x6000, 0x7000
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def size(a):
+    return cabi.lib().cmpext3_projection_workspace_size(ctypes.byref(a))
+
+
+def test_projection_c_abi_rejects():
+    i8 = dict(dtype=cabi.I8)
+    assert size(projection()) >= 0 and size(projection(**i8)) >= 0 and size(projection(out_dtype=cabi.F32, **i8)) >= 0
+    assert size(projection(w_up=None, bias=0x8000, **i8)) >= 0
+    assert cabi.lib().cmpext3_projection_workspace_size(None) == BAD
+    for kw in (dict(dtype=cabi.F32), dict(dtype=cabi.E4M3), dict(out_dtype=cabi.F32), dict(out_dtype=cabi.F16), dict(w_up=None),
+               dict(activation=4), dict(activation=-1), dict(bias=0x8000), dict(out_dtype=cabi.I8, **i8),
+               dict(gate_out=0x100, up_out=0x200, pre_row=64, **i8)):
+        assert size(projection(**kw)) == NOT, kw
+    for kw in (dict(M=-1), dict(N=-1), dict(K=-1), dict(x=None), dict(w_gate=None), dict(out=None), dict(x_row=127), dict(gate_row=127),
+               dict(up_row=100), dict(out_row=63), dict(x=0x1001), dict(out=0x4001), dict(gate_out=0x100, pre_row=64),
+               dict(gate_out=0x100, up_out=0x200, pre_row=63), dict(x_scale=None, **i8), dict(gate_scale=None, **i8),
+               dict(up_scale=None, **i8), dict(x_scale=0x5002, **i8), dict(out=0x4002, out_dtype=cabi.F32, **i8),
+               dict(w_up=None, bias=0x8001, **i8)):
+        assert size(projection(**kw)) == BAD, kw
+    for kw in (dict(K=131072, x_row=131072, gate_row=131072, up_row=131072, **i8), dict(x_row=1 << 31), dict(gate_row=1 << 40),
+               dict(M=2**31 - 1), dict(N=2**31 - 1, out_row=2**31 - 1), dict(out_row=1 << 31)):
+        assert size(projection(**kw)) == BIG, kw
+    assert size(projection(M=0, x=None, out=None)) == 0 and size(projection(N=0, w_gate=None)) == 0
+    assert size(projection(K=131071, x_row=131071, gate_row=131071, up_row=131071, **i8)) >= 0
+    lib = cabi.lib()
+    assert lib.cmpext3_projection(ctypes.byref(projection(M=0)), None, 0, None) == 0
+    assert lib.cmpext3_projection(ctypes.byref(projection(M=-1)), None, 0, None) == BAD
+    assert lib.cmpext3_projection_describe(ctypes.byref(projection(M=-1)), None, 0) == BAD
+
+
+def backward(**kw):
+    a = cabi.GatedBackwardArgs(dtype=cabi.F16, activation=cabi.ACT_GELU, M=8, N=64, K=128, grad_out=0x1000, grad_row=64, gate=0x2000,
+                               up=0x3000, pre_row=64, x=0x4000, x_row=128, w_gate=0x5000, gate_row=128, w_up=0x6000, up_row=128,
+                               dx=0x7000, dx_row=128, dw_gate=0x8000, dgate_row=128, dw_up=0x9000, dup_row=128)
+    for name, value in kw.items():
+        setattr(a, name, value)
+    return a
+
+
+def test_gated_backward_c_abi_rejects():
+    lib = cabi.lib()
+
+    def need(a):
+        return lib.cmpext3_gated_backward_workspace_size(ctypes.byref(a))
+
+    assert need(backward()) >= 2 * 2 * 8 * 64
+    assert lib.cmpext3_gated_backward_workspace_size(None) == BAD
+    for kw in (dict(dtype=cabi.F32), dict(dtype=cabi.I8), dict(activation=4), dict(activation=-1)):
+        assert need(backward(**kw)) == NOT, kw
+    for kw in (dict(M=-1), dict(N=-1), dict(K=-1), dict(grad_out=None), dict(gate=None), dict(up=None), dict(x=None), dict(w_gate=None),
+               dict(w_up=None), dict(grad_row=63), dict(pre_row=63), dict(x_row=127), dict(gate_row=127), dict(up_row=127), dict(dx_row=127),
+               dict(dgate_row=127), dict(dup_row=127), dict(dx=0x7001)):
+        assert need(backward(**kw)) == BAD, kw
+    for kw in (dict(M=2**31 - 1), dict(x_row=1 << 31), dict(M=1 << 25)):
+        assert need(backward(**kw)) == BIG, kw
+    # what is not asked for needs no operands
+    assert need(backward(dx=None, w_gate=None, w_up=None)) >= 0
+    assert need(backward(dw_gate=None, dw_up=None, x=None)) >= 0
+    a = backward()
+    assert lib.cmpext3_gated_backward(ctypes.byref(a), None, 0, None) == WORK
+    assert lib.cmpext3_gated_backward(ctypes.byref(a), 0x10000, need(a) - 1, None) == WORK
+    assert lib.cmpext3_gated_backward(ctypes.byref(a), 0x10008, need(a), None) == WORK
+
+
+def test_quantize_c_abi_rejects():
+    def call(**kw):
+        a = cabi.QuantizeInt8Args(dtype=cabi.F16, cols=64, rows=3, x=0x1000, x_row=64, codes=0x2000, codes_row=64, scale=0x3000)
+        for name, value in kw.items():
+            setattr(a, name, value)
+        return cabi.lib().cmpext3_quantize_int8(ctypes.byref(a), None)
+
+    assert cabi.lib().cmpext3_quantize_int8(None, None) == BAD
+    assert call(dtype=cabi.I8) == NOT and call(dtype=cabi.E4M3) == NOT
+    for kw in (dict(rows=-1), dict(cols=-1), dict(x=None), dict(codes=None), dict(scale=None), dict(x_row=63), dict(codes_row=63),
+               dict(x=0x1001), dict(scale=0x3002)):
+        assert call(**kw) == BAD, kw
+    assert call(rows=1 << 40) == BIG
+    assert call(rows=0) == 0
