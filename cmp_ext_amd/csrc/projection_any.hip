@@ -48,7 +48,7 @@ __global__ void __launch_bounds__(256) projection_any_kernel(const ProjParams p)
     for (int i = 0; i < 4; ++i) acc[q][i >> 1][i & 1] = Prod<T>::zero();
 #pragma unroll
   for (int part = 0; part < (MODE == kProjSum ? 2 : 1); ++part) {
-    const E* a = (const E*)p.a[part] + blockIdx.z * p.batch_a;
+    const E* a = (const E*)p.a[MODE == kProjSum ? part : blockIdx.z];
     for (int k0 = 0; k0 < p.K; k0 += KS) {
       __syncthreads();
       any_load<E, A_KM>(sa, a, p.lda, p.M, m0, p.K, k0);
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(256) projection_any_kernel(const ProjParams p)
       } else if (p.bias != nullptr) {
         y += load_elem(p.bias, n, p.out_dtype);
       }
-      store_elem(p.out, blockIdx.z * p.batch_out + m * p.ldo + n, p.out_dtype, y);
+      store_elem(p.out[blockIdx.z], m * p.ldo[blockIdx.z] + n, p.out_dtype, y);
     }
   }
 }
@@ -114,7 +114,7 @@ hipError_t launch16(ProjMode mode, bool a_km, bool b_kn, const ProjParams& p, di
 }  // namespace
 
 hipError_t launch_projection_any(int dtype, ProjMode mode, bool a_km, bool b_kn, const ProjParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)((p.M + kAnyTile - 1) / kAnyTile), (unsigned)((p.N + kAnyTile - 1) / kAnyTile), 1);
+  const dim3 grid((unsigned)((p.M + kAnyTile - 1) / kAnyTile), (unsigned)((p.N + kAnyTile - 1) / kAnyTile), (unsigned)p.batch);
   if (dtype == kF16) return launch16<_Float16>(mode, a_km, b_kn, p, grid, s);
   if (dtype == kBF16) return launch16<__bf16>(mode, a_km, b_kn, p, grid, s);
   if (mode == kProjPlain) return launch_kernel((projection_any_kernel<int8_t, kProjPlain, false, false>), grid, dim3(256), 0, s, p);

@@ -4,11 +4,14 @@
 #include <limits.h>
 #include <stdint.h>
 #include <stdio.h>
+#include <stdlib.h>
+#include <string.h>
 
 #include <algorithm>
 
 #include "../../include/cmpext3_projection.h"
 #include "gemm_params.h"
+#include "kernels.h"
 #include "projection_params.h"
 
 using namespace cmpext3;
@@ -85,6 +88,142 @@ int check_projection(const cmpext3_projection_args* a) {
   return CMPEXT3_OK;
 }
 
+// A matrix with rows along k that the tiles read: as it is, or as a copy in the workspace whose rows are whole
+// 16 bytes, zero past the matrix.
+struct Operand {
+  const void* p;
+  int64_t ld;
+  int rows, cols;
+  int64_t copy_at;  // in the workspace, or -1
+  int64_t copy_ld;
+};
+
+bool rows_of_16(const Operand& o, size_t esz) {
+  return aligned(o.p, 16) && (o.rows <= 1 || o.ld * (int64_t)esz % 16 == 0) && o.cols * (int64_t)esz % 16 == 0;
+}
+
+// Takes `bytes` of the workspace, in whole 256 bytes.
+int64_t take(int64_t* used, int64_t bytes) {
+  const int64_t at = *used;
+  *used += cdiv(bytes, 256) * 256;
+  return at;
+}
+
+void plan_copy(Operand* o, size_t esz, int64_t* used) {
+  o->copy_at = -1;
+  if (rows_of_16(*o, esz)) return;
+  o->copy_ld = cdiv(o->cols * (int64_t)esz, 16) * 16 / (int64_t)esz;
+  o->copy_at = take(used, (int64_t)o->rows * o->copy_ld * (int64_t)esz);
+}
+
+// Makes the copy; afterwards the operand is the copy.
+hipError_t run_copy(Operand* o, size_t esz, char* ws, hipStream_t s) {
+  if (o->copy_at < 0) return hipSuccess;
+  void* dst = ws + o->copy_at;
+  const hipError_t e = launch_pad_copy(o->p, o->ld, 0, o->rows, o->cols, dst, o->copy_ld, 0, o->rows, (int)o->copy_ld, 1, (int)esz, s);
+  o->p = dst;
+  o->ld = o->copy_ld;
+  return e;
+}
+
+// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|tile128x128|tile256x256>[,splits=<s>]" replaces
+// the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan, ignored where malformed.
+struct Override {
+  char kernel[32];
+  int splits;
+};
+Override read_override() {
+  Override o{};
+  const char* env = getenv("CMPEXT3_PROJECTION_CONFIG");
+  if (env != nullptr && sscanf(env, "kernel=%31[^,],splits=%d", o.kernel, &o.splits) < 1) o.kernel[0] = 0;
+  return o;
+}
+
+struct TilePlan {
+  int bm;    // 256, 128, or 0: the kernel for any alignment
+  bool deep;
+  int splits, ksplit;
+};
+
+// Which tiles, and in how many splits of the steps of 128 bytes of k, for M x N results (of `products` products)
+// in `batch` entries.  Modelled microseconds (MI355X).
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch) {
+  const Override o = read_override();
+  const int64_t bn256 = 256 / products, bn128 = 128 / products;
+  const int64_t rounds = cdiv(cdiv(M, 256) * cdiv(N, bn256) * batch, 256);
+  TilePlan best{256, false, 1, (int)steps};
+  double least = (double)rounds * (steps * 1.6 + 6.0);
+  const int64_t tiles = cdiv(M, 128) * cdiv(N, bn128) * batch;
+  if (strcmp(o.kernel, "tile256x256") == 0) return best;
+  const bool forced = strcmp(o.kernel, "tile128x128") == 0;
+  if (forced) least = 1e30;
+  for (int64_t s = 1; s <= 16 && (s == 1 || s * 4 <= steps); ++s) {
+    const int64_t each = cdiv(steps, s);
+    if (s > 1 && (s - 1) * each >= steps) continue;  // an empty split
+    if (forced && o.splits > 0 && s != o.splits) continue;
+    const int64_t wgs = tiles * s;
+    if (wgs * batch > INT_MAX / 256) break;
+    const bool deep = wgs <= 256 && each >= 8;
+    const int64_t full = wgs / 512, rest = wgs % 512;
+    double t = (double)full * (each * 0.98 + 5.0);
+    if (rest > 256) t += each * 0.98 + 5.0;
+    else if (rest > 0) t += each * (deep ? 0.46 : 0.70) + 4.0;
+    if (s > 1) t += 4.0 + (double)s * batch * M * N * products * 8.0 / 5e6;
+    if (t < least) {
+      least = t;
+      best = TilePlan{128, deep, (int)s, (int)each};
+    }
+  }
+  return best;
+}
+
+int64_t partial_pitch(int64_t N) { return cdiv(N, 4) * 4; }
+int64_t partial_bytes(const TilePlan& t, int64_t M, int64_t N, int products, int64_t batch) {
+  return t.splits > 1 ? (int64_t)t.splits * batch * products * M * partial_pitch(N) * 4 : 0;
+}
+
+bool tile_grid_fits(int64_t M, int64_t N, int products, int64_t batch) {
+  return cdiv(M, 128) * cdiv(N, 128 / products) * batch <= kMostThreads / 512;
+}
+
+// Sets the tiles' grid in p and launches them, and the join of their splits.
+hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* launch, const TilePlan& t, ProjParams& p, void* partials, hipStream_t s) {
+  const int products = mode == kProjGated ? 2 : 1;
+  p.tiles_m = (int)cdiv(p.M, t.bm);
+  p.tiles_n = (int)cdiv(p.N, t.bm / products);
+  p.group_m = 4;
+  p.splits = t.splits;
+  p.ksplit = t.ksplit;
+  p.partials = partials;
+  p.ld_part = partial_pitch(p.N);
+  const hipError_t e = launch(p, t.bm, t.deep, s);
+  return e != hipSuccess || t.splits == 1 ? e : launch_projection_join(dtype, mode, p, s);
+}
+
+struct ProjPlan {
+  Operand x, w[2];
+  TilePlan tile;
+  int64_t partials_at, ws_bytes;
+};
+
+int plan_projection(const cmpext3_projection_args* a, ProjPlan* q) {
+  const int st = check_projection(a);
+  if (st != CMPEXT3_OK) return st;
+  *q = ProjPlan{};
+  if (a->M == 0 || a->N == 0) return CMPEXT3_OK;
+  const size_t esz = elem_size(a->dtype);
+  const int products = a->w_up != nullptr ? 2 : 1;
+  q->x = Operand{a->x, a->x_row, a->M, a->K, -1, 0};
+  q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
+  q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
+  if (a->K == 0 || strcmp(read_override().kernel, "any64x64") == 0 || !tile_grid_fits(a->M, a->N, products, 1)) return CMPEXT3_OK;  // tile.bm = 0
+  plan_copy(&q->x, esz, &q->ws_bytes);
+  for (int i = 0; i < products; ++i) plan_copy(&q->w[i], esz, &q->ws_bytes);
+  q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1);
+  q->partials_at = take(&q->ws_bytes, partial_bytes(q->tile, a->M, a->N, products, 1));
+  return CMPEXT3_OK;
+}
+
 ProjParams params_of(const cmpext3_projection_args* a) {
   ProjParams p{};
   p.a[0] = p.a[1] = a->x;
@@ -97,14 +236,16 @@ ProjParams params_of(const cmpext3_projection_args* a) {
   p.b_scale[0] = a->gate_scale;
   p.b_scale[1] = a->up_scale;
   p.bias = a->bias;
-  p.out = a->out;
-  p.ldo = a->out_row;
+  p.out[0] = a->out;
+  p.ldo[0] = a->out_row;
   p.out_dtype = a->out_dtype;
   p.pre[0] = a->gate_out;
   p.pre[1] = a->up_out;
   p.ld_pre = a->pre_row;
+  p.pre_vec = a->pre_row % 4 == 0 && aligned(a->gate_out, 16) && aligned(a->up_out, 16);
   p.act = a->activation;
   p.M = a->M, p.N = a->N, p.K = a->K;
+  p.batch = p.splits = 1;
   return p;
 }
 
@@ -132,6 +273,39 @@ int check_gated_backward(const cmpext3_gated_backward_args* a) {
 // Elements of a row of the held gradients: whole 16 bytes.
 int64_t grad_pitch(int N) { return cdiv(N, 8) * 8; }
 
+struct BackwardPlan {
+  int64_t d_at[2];
+  Operand w[2], x;  // [K, N] operands of the products: rows across k
+  TilePlan dx, dw;
+  int64_t partials_at, ws_bytes;
+};
+
+int plan_backward(const cmpext3_gated_backward_args* a, BackwardPlan* q) {
+  const int st = check_gated_backward(a);
+  if (st != CMPEXT3_OK) return st;
+  *q = BackwardPlan{};
+  const int64_t held = (int64_t)a->M * grad_pitch(a->N) * 2;
+  for (int64_t& at : q->d_at) at = take(&q->ws_bytes, held);
+  q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
+  q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
+  q->x = Operand{a->x, a->x_row, a->M, a->K, -1, 0};
+  if (a->M == 0 || a->N == 0 || a->K == 0 || strcmp(read_override().kernel, "any64x64") == 0) return CMPEXT3_OK;
+  const int64_t batch = (a->dw_gate != nullptr) + (a->dw_up != nullptr);
+  int64_t partials = 0;
+  if (a->dx != nullptr && tile_grid_fits(a->M, a->K, 1, 1)) {
+    for (Operand& w : q->w) plan_copy(&w, 2, &q->ws_bytes);
+    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1);
+    partials = partial_bytes(q->dx, a->M, a->K, 1, 1);
+  }
+  if (batch > 0 && tile_grid_fits(a->N, a->K, 1, batch)) {
+    plan_copy(&q->x, 2, &q->ws_bytes);
+    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch);
+    partials = std::max(partials, partial_bytes(q->dw, a->N, a->K, 1, batch));
+  }
+  q->partials_at = take(&q->ws_bytes, partials);
+  return CMPEXT3_OK;
+}
+
 }  // namespace
 
 extern "C" int cmpext3_quantize_int8(const cmpext3_quantize_int8_args* a, void* stream) {
@@ -157,37 +331,68 @@ extern "C" int cmpext3_quantize_int8(const cmpext3_quantize_int8_args* a, void* 
   return (int)launch_quantize_int8(a->dtype, p, (hipStream_t)stream);
 }
 
-extern "C" int64_t cmpext3_projection_workspace_size(const cmpext3_projection_args* a) { return check_projection(a); }
+extern "C" int64_t cmpext3_projection_workspace_size(const cmpext3_projection_args* a) {
+  ProjPlan q;
+  const int st = plan_projection(a, &q);
+  return st != CMPEXT3_OK ? st : q.ws_bytes;
+}
 
 extern "C" int cmpext3_projection(const cmpext3_projection_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
-  const int64_t need = cmpext3_projection_workspace_size(a);
-  const int st = check_workspace(need, workspace, workspace_bytes);
+  ProjPlan q;
+  int st = plan_projection(a, &q);
+  if (st == CMPEXT3_OK) st = check_workspace(q.ws_bytes, workspace, workspace_bytes);
   if (st != CMPEXT3_OK) return st;
   if (a->M == 0 || a->N == 0) return CMPEXT3_OK;
+  const hipStream_t s = (hipStream_t)stream;
   const ProjMode mode = a->w_up != nullptr ? kProjGated : kProjPlain;
-  return (int)launch_projection_any(a->dtype, mode, false, false, params_of(a), (hipStream_t)stream);
+  ProjParams p = params_of(a);
+  if (q.tile.bm == 0) return (int)launch_projection_any(a->dtype, mode, false, false, p, s);
+  const size_t esz = elem_size(a->dtype);
+  for (Operand* o : {&q.x, &q.w[0], &q.w[1]}) {
+    const hipError_t e = run_copy(o, esz, (char*)workspace, s);
+    if (e != hipSuccess) return (int)e;
+  }
+  p.a[0] = p.a[1] = q.x.p;
+  p.lda = q.x.ld;
+  for (int i = 0; i < 2; ++i) p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
+  p.K = (int)(cdiv(a->K * (int64_t)esz, 16) * 16 / (int64_t)esz);  // copies hold zeros up to there
+  ProjTileLaunch* launch = a->dtype == CMPEXT3_F16    ? launch_projection_tile_gated_f16
+                           : a->dtype == CMPEXT3_BF16 ? launch_projection_tile_gated_bf16
+                           : mode == kProjGated       ? launch_projection_tile_int8_gated
+                                                      : launch_projection_tile_int8_plain;
+  return (int)run_tiles(a->dtype, mode, launch, q.tile, p, (char*)workspace + q.partials_at, s);
 }
 
 extern "C" int cmpext3_projection_describe(const cmpext3_projection_args* a, char* buf, int buflen) {
-  const int st = check_projection(a);
+  ProjPlan q;
+  const int st = plan_projection(a, &q);
   if (st != CMPEXT3_OK) return st;
-  if (buf != nullptr && buflen > 0) snprintf(buf, (size_t)buflen, "kernel=any64x64");
+  if (buf == nullptr || buflen <= 0) return CMPEXT3_OK;
+  if (a->M == 0 || a->N == 0)
+    snprintf(buf, (size_t)buflen, "kernel=none");
+  else if (q.tile.bm == 0)
+    snprintf(buf, (size_t)buflen, "kernel=any64x64");
+  else
+    snprintf(buf, (size_t)buflen, "kernel=tile%dx%d%s splits=%d copies=%d", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.splits,
+             (q.x.copy_at >= 0) + (q.w[0].copy_at >= 0) + (q.w[1].copy_at >= 0));
   return CMPEXT3_OK;
 }
 
 extern "C" int64_t cmpext3_gated_backward_workspace_size(const cmpext3_gated_backward_args* a) {
-  const int st = check_gated_backward(a);
-  if (st != CMPEXT3_OK) return st;
-  return 2 * 2 * (int64_t)a->M * grad_pitch(a->N);
+  BackwardPlan q;
+  const int st = plan_backward(a, &q);
+  return st != CMPEXT3_OK ? st : q.ws_bytes;
 }
 
 extern "C" int cmpext3_gated_backward(const cmpext3_gated_backward_args* a, void* workspace, int64_t workspace_bytes, void* stream) {
-  const int64_t need = cmpext3_gated_backward_workspace_size(a);
-  const int st = check_workspace(need, workspace, workspace_bytes);
+  BackwardPlan q;
+  int st = plan_backward(a, &q);
+  if (st == CMPEXT3_OK) st = check_workspace(q.ws_bytes, workspace, workspace_bytes);
   if (st != CMPEXT3_OK) return st;
   const hipStream_t s = (hipStream_t)stream;
+  char* ws = (char*)workspace;
   const int64_t pitch = grad_pitch(a->N);
-  uint16_t* d[2] = {(uint16_t*)workspace, (uint16_t*)workspace + (int64_t)a->M * pitch};
+  uint16_t* d[2] = {(uint16_t*)(ws + q.d_at[0]), (uint16_t*)(ws + q.d_at[1])};
   hipError_t e = hipSuccess;
   if (a->M > 0 && a->N > 0) {
     GatedGradParams g{};
@@ -202,31 +407,43 @@ extern "C" int cmpext3_gated_backward(const cmpext3_gated_backward_args* a, void
     e = launch_gated_grad(a->dtype, g, s);
     if (e != hipSuccess) return (int)e;
   }
+  const bool f16 = a->dtype == CMPEXT3_F16;
   ProjParams p{};
   p.out_dtype = a->dtype;
   p.lda = pitch;
+  p.a[0] = d[0], p.a[1] = d[1];
+  p.batch = p.splits = 1;
   if (a->dx != nullptr && a->M > 0 && a->K > 0) {
-    p.a[0] = d[0], p.a[1] = d[1];
-    p.b[0] = a->w_gate, p.b[1] = a->w_up;
-    p.ldb[0] = a->gate_row, p.ldb[1] = a->up_row;
-    p.out = a->dx;
-    p.ldo = a->dx_row;
+    for (int i = 0; i < 2; ++i) {
+      e = run_copy(&q.w[i], 2, ws, s);
+      if (e != hipSuccess) return (int)e;
+      p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
+    }
+    p.out[0] = a->dx;
+    p.ldo[0] = a->dx_row;
     p.M = a->M, p.N = a->K, p.K = a->N;
-    e = launch_projection_any(a->dtype, kProjSum, false, true, p, s);
+    e = q.dx.bm == 0 ? launch_projection_any(a->dtype, kProjSum, false, true, p, s)
+                     : run_tiles(a->dtype, kProjSum, f16 ? launch_projection_tile_sum_f16 : launch_projection_tile_sum_bf16, q.dx, p,
+                                 ws + q.partials_at, s);
     if (e != hipSuccess) return (int)e;
   }
+  // the weights' gradients that are asked for, as one batch
+  p.batch = 0;
   void* dw[2] = {a->dw_gate, a->dw_up};
   const int64_t dw_row[2] = {a->dgate_row, a->dup_row};
   for (int i = 0; i < 2; ++i) {
-    if (dw[i] == nullptr || a->N == 0 || a->K == 0) continue;
-    p.a[0] = d[i];
-    p.b[0] = a->x;
-    p.ldb[0] = a->x_row;
-    p.out = dw[i];
-    p.ldo = dw_row[i];
-    p.M = a->N, p.N = a->K, p.K = a->M;
-    e = launch_projection_any(a->dtype, kProjPlain, true, true, p, s);
-    if (e != hipSuccess) return (int)e;
+    if (dw[i] == nullptr) continue;
+    p.a[p.batch] = d[i];
+    p.out[p.batch] = dw[i];
+    p.ldo[p.batch] = dw_row[i];
+    ++p.batch;
   }
-  return CMPEXT3_OK;
+  if (p.batch == 0 || a->N == 0 || a->K == 0) return CMPEXT3_OK;
+  e = run_copy(&q.x, 2, ws, s);
+  if (e != hipSuccess) return (int)e;
+  p.b[0] = q.x.p, p.ldb[0] = q.x.ld;
+  p.M = a->N, p.N = a->K, p.K = a->M;
+  return (int)(q.dw.bm == 0 ? launch_projection_any(a->dtype, kProjPlain, true, true, p, s)
+                            : run_tiles(a->dtype, kProjPlain, f16 ? launch_projection_tile_wgrad_f16 : launch_projection_tile_wgrad_bf16,
+                                        q.dw, p, ws + q.partials_at, s));
 }

@@ -18,24 +18,40 @@ enum ProjMode : int {
 };
 
 struct ProjParams {
-  const void* a[2];  // kProjSum: both; otherwise a[0]
+  const void* a[2];  // kProjSum: both terms'; otherwise of each entry of the batch
   const void* b[2];  // kProjPlain: b[0]
   int64_t lda, ldb[2];
   const float* a_scale;     // 8-bit codes: of a row of a,
   const float* b_scale[2];  // of a row of b
   const void* bias;         // kProjPlain: [N] of the output's type, or nullptr
-  void* out;
-  int64_t ldo;
+  void* out[2];  // of each entry of the batch
+  int64_t ldo[2];
   int out_dtype;  // kF16, kBF16, kF32
   float* pre[2];  // kProjGated: both products, or nullptr
   int64_t ld_pre;
+  int pre_vec;    // their rows are aligned to 16 bytes
   int act;
   int M, N, K;
-  int64_t batch_a, batch_out;  // grid.z: what a further product adds to a (elements) and out
+  int batch;  // products with the same b (weight gradients: 2), else 1
+  // tiles: their grid, rows of tiles of an ordering group, and splits of the steps of K (ksplit steps
+  // each), whose sums go to partials [split][batch][product][M][ld_part]
+  int tiles_m, tiles_n, group_m, splits, ksplit;
+  void* partials;
+  int64_t ld_part;
 };
 
 // Any pitch and alignment; a is [M, K] or, a_km, [K, M]; b is [N, K] or, b_kn, [K, N].
 hipError_t launch_projection_any(int dtype, ProjMode mode, bool a_km, bool b_kn, const ProjParams& p, hipStream_t s);
+
+// Tiles of bm = 256 or 128 rows; `deep`: alone on a CU, with a ring of four steps.  Operands have rows of
+// whole 16 bytes.  (One translation unit for each element type and mode.)
+using ProjTileLaunch = hipError_t(const ProjParams& p, int bm, bool deep, hipStream_t s);
+ProjTileLaunch launch_projection_tile_gated_f16, launch_projection_tile_gated_bf16;
+ProjTileLaunch launch_projection_tile_sum_f16, launch_projection_tile_sum_bf16;
+ProjTileLaunch launch_projection_tile_wgrad_f16, launch_projection_tile_wgrad_bf16;
+ProjTileLaunch launch_projection_tile_int8_plain, launch_projection_tile_int8_gated;
+// Adds the splits' sums in their order and finishes the results as an unsplit kernel does.
+hipError_t launch_projection_join(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
 
 struct QuantParams {
   const void* x;
