@@ -126,7 +126,7 @@ hipError_t run_copy(Operand* o, size_t esz, char* ws, hipStream_t s) {
   return e;
 }
 
-// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|tile128x128|tile256x256>[,splits=<s>]" replaces
+// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows_any|rows|tile128x128|tile256x256>[,splits=<s>]" replaces
 // the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan, ignored where malformed.
 struct Override {
   char kernel[32];
@@ -200,7 +200,11 @@ hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* launch, const Til
   return e != hipSuccess || t.splits == 1 ? e : launch_projection_join(dtype, mode, p, s);
 }
 
+enum ProjKernel { kAny, kRows, kRowsAny, kTile };
+const char* kernel_name(ProjKernel k) { return k == kAny ? "any64x64" : k == kRows ? "rows" : k == kRowsAny ? "rows_any" : "tile"; }
+
 struct ProjPlan {
+  ProjKernel kernel;
   Operand x, w[2];
   TilePlan tile;
   int64_t partials_at, ws_bytes;
@@ -216,7 +220,18 @@ int plan_projection(const cmpext3_projection_args* a, ProjPlan* q) {
   q->x = Operand{a->x, a->x_row, a->M, a->K, -1, 0};
   q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
   q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
-  if (a->K == 0 || strcmp(read_override().kernel, "any64x64") == 0 || !tile_grid_fits(a->M, a->N, products, 1)) return CMPEXT3_OK;  // tile.bm = 0
+  const Override o = read_override();
+  const bool tiles_fit = tile_grid_fits(a->M, a->N, products, 1);
+  const bool whole = rows_of_16(q->x, esz) && rows_of_16(q->w[0], esz) && (products == 1 || rows_of_16(q->w[1], esz));
+  q->kernel = kAny;
+  if (a->K == 0 || strcmp(o.kernel, "any64x64") == 0) return CMPEXT3_OK;
+  if (a->M <= kFewRows && strncmp(o.kernel, "tile", 4) != 0 && (int64_t)a->K * (int64_t)esz >= 16) {
+    // few rows: bound by reading the weights, once
+    q->kernel = whole && strcmp(o.kernel, "rows_any") != 0 ? kRows : kRowsAny;
+    return CMPEXT3_OK;
+  }
+  if (!tiles_fit) return CMPEXT3_OK;
+  q->kernel = kTile;
   plan_copy(&q->x, esz, &q->ws_bytes);
   for (int i = 0; i < products; ++i) plan_copy(&q->w[i], esz, &q->ws_bytes);
   q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1);
@@ -266,7 +281,7 @@ int check_gated_backward(const cmpext3_gated_backward_args* a) {
   if (st == CMPEXT3_OK && a->dw_up != nullptr) st = check_matrix(a->dw_up, a->N, a->K, a->dup_row, t);
   if (st != CMPEXT3_OK) return st;
   if (!any_grid_fits(a->M, a->K) || !any_grid_fits(a->N, a->K)) return CMPEXT3_ERR_TOO_LARGE;
-  if (a->M * (int64_t)256 > kMostThreads || cdiv(a->N, 256) >= kMostGridY) return CMPEXT3_ERR_TOO_LARGE;
+  if (a->M * cdiv(a->N, 2048) * 256 > kMostThreads) return CMPEXT3_ERR_TOO_LARGE;
   return CMPEXT3_OK;
 }
 
@@ -346,7 +361,9 @@ extern "C" int cmpext3_projection(const cmpext3_projection_args* a, void* worksp
   const hipStream_t s = (hipStream_t)stream;
   const ProjMode mode = a->w_up != nullptr ? kProjGated : kProjPlain;
   ProjParams p = params_of(a);
-  if (q.tile.bm == 0) return (int)launch_projection_any(a->dtype, mode, false, false, p, s);
+  if (q.kernel == kAny) return (int)launch_projection_any(a->dtype, mode, false, false, p, s);
+  if (q.kernel == kRows) return (int)launch_projection_rows(a->dtype, mode, p, s);
+  if (q.kernel == kRowsAny) return (int)launch_projection_rows_any(a->dtype, mode, p, s);
   const size_t esz = elem_size(a->dtype);
   for (Operand* o : {&q.x, &q.w[0], &q.w[1]}) {
     const hipError_t e = run_copy(o, esz, (char*)workspace, s);
@@ -370,8 +387,8 @@ extern "C" int cmpext3_projection_describe(const cmpext3_projection_args* a, cha
   if (buf == nullptr || buflen <= 0) return CMPEXT3_OK;
   if (a->M == 0 || a->N == 0)
     snprintf(buf, (size_t)buflen, "kernel=none");
-  else if (q.tile.bm == 0)
-    snprintf(buf, (size_t)buflen, "kernel=any64x64");
+  else if (q.kernel != kTile)
+    snprintf(buf, (size_t)buflen, "kernel=%s", kernel_name(q.kernel));
   else
     snprintf(buf, (size_t)buflen, "kernel=tile%dx%d%s splits=%d copies=%d", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.splits,
              (q.x.copy_at >= 0) + (q.w[0].copy_at >= 0) + (q.w[1].copy_at >= 0));

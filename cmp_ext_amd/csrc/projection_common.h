@@ -41,4 +41,60 @@ __device__ __forceinline__ float load_elem(const void* base, int64_t i, int dtyp
   return dtype == kF16 ? from_bits<_Float16>(h) : from_bits<__bf16>(h);
 }
 
+// Workgroup w runs on XCD w % 8: gives each XCD a contiguous range of the `total` strips of a matrix's rows,
+// so that neighbouring rows are read from one XCD at a time (x[16, 8192] by 8192 rows of codes, 32 a strip: 19.2
+// -> 12.4 us; x[1, 4096] by 4096 rows, 16 a strip: 6.1 -> 4.6).
+__device__ __forceinline__ int strip_of(int w, int total) {
+  const int xcd = w & 7, base = total >> 3, rem = total & 7;
+  return xcd * base + (xcd < rem ? xcd : rem) + (w >> 3);
+}
+
+// LDS-DMA of dma_load16_m0 with the non-temporal policy, for what is read once.
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+template <uint32_t DST>
+__device__ __forceinline__ void dma_load16_m0_once(i32x4 rsrc, uint32_t voff, uint32_t soff, uint32_t lds_base,
+                                                   std::integral_constant<uint32_t, DST> = {}) {
+  asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen nt lds"
+               :
+               : "v"(voff), "s"(rsrc), "s"(lds_base + DST), "s"(soff)
+               : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// The end of the kernels for few rows: adds the sums of WAVES waves, [wave][16 MB rows of x][PITCH] of which the
+// first 16 NB are a strip's rows (gated: 16 of w_gate, 16 of w_up, ..), and finishes and stores the results.
+template <typename T, int MODE, int MB, int NB, int WAVES, int PITCH>
+__device__ __forceinline__ void finish_rows(const ProjParams& p, const void* red, int n0) {
+  using E = typename std::conditional<sizeof(T) == 1, int, float>::type;
+  constexpr bool GATED = MODE == kProjGated;
+  constexpr int COLS = GATED ? 8 * NB : 16 * NB;
+  const E* sums = (const E*)red;
+  for (int o = threadIdx.x; o < 16 * MB * COLS; o += 64 * WAVES) {
+    const int64_t m = o / COLS, n = n0 + o % COLS;
+    if (m >= p.M || n >= p.N) continue;
+    float v[2];
+#pragma unroll
+    for (int q = 0; q < (GATED ? 2 : 1); ++q) {
+      const int c = GATED ? 32 * ((o % COLS) / 16) + 16 * q + o % 16 : o % COLS;
+      E s = 0;
+#pragma unroll
+      for (int i = 0; i < WAVES; ++i) s += sums[((i * MB * 16) + (int)m) * PITCH + c];
+      v[q] = (float)s;
+      if (sizeof(T) == 1) v[q] = v[q] * p.a_scale[m] * p.b_scale[q][n];
+    }
+    float y = v[0];
+    if constexpr (GATED) {
+      if (p.pre[0] != nullptr) {
+        p.pre[0][m * p.ld_pre + n] = v[0];
+        p.pre[1][m * p.ld_pre + n] = v[1];
+      }
+      with_act(p.act, [&](auto act) { y = act_value<decltype(act)::value>(v[0]) * v[1]; });
+    } else if (p.bias != nullptr) {
+      y += load_elem(p.bias, n, p.out_dtype);
+    }
+    store_elem(p.out[0], m * p.ldo[0] + n, p.out_dtype, y);
+  }
+}
+
 }  // namespace cmpext3

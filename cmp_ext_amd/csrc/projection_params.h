@@ -43,6 +43,11 @@ struct ProjParams {
 // Any pitch and alignment; a is [M, K] or, a_km, [K, M]; b is [N, K] or, b_kn, [K, N].
 hipError_t launch_projection_any(int dtype, ProjMode mode, bool a_km, bool b_kn, const ProjParams& p, hipStream_t s);
 
+// Up to kFewRows rows of a, b as [N, K]: rows of whole 16 bytes, or (_any) of any alignment and at least 16 bytes.
+constexpr int kFewRows = 64;
+hipError_t launch_projection_rows(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
+hipError_t launch_projection_rows_any(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
+
 // Tiles of bm = 256 or 128 rows; `deep`: alone on a CU, with a ring of four steps.  Operands have rows of
 // whole 16 bytes.  (One translation unit for each element type and mode.)
 using ProjTileLaunch = hipError_t(const ProjParams& p, int bm, bool deep, hipStream_t s);

@@ -1,61 +1,166 @@
-// Rows as 8-bit codes with a scale for each: a = max(max |x|, 2^-100), code = round(127 x / a),
-// scale = a / 127.  A workgroup takes a row: once for its largest value, once more for the codes.
+// Rows as 8-bit codes with a scale for each: a = max(max |x|, 2^-100), code = round(127 x / a), scale = a / 127.
+//
+// Bound by reading x and writing the codes.  A wave takes a row of up to 2048 elements, a workgroup one of up to
+// 16384, and holds it in registers between the search for its largest value and the codes, so that it
+// is read once; longer rows are read twice (the second time mostly from the caches).  Pieces of 8 elements are loaded
+// and stored whole at any alignment, but for a row's last.
 #include "projection_common.h"
 
 namespace cmpext3 {
 namespace {
 
+// Eight elements as they are held between the passes.
 template <typename T>
-__device__ __forceinline__ float as_float(const T* x, int64_t i) {
-  return (float)x[i];
-}
+struct Piece {
+  typedef u32x4 Any __attribute__((aligned(2)));
+  u32x4 v;
+  __device__ __forceinline__ void load(const T* x, int left) {
+    if (left >= 8) {
+      v = *(const Any*)x;
+    } else {
+      v = u32x4{0, 0, 0, 0};
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) v[i >> 1] |= (uint32_t)((const uint16_t*)x)[i] << (16 * (i & 1));
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return from_bits<T>((uint16_t)(v[i >> 1] >> (16 * (i & 1)))); }
+};
+template <>
+struct Piece<float> {
+  typedef f32x4 Any __attribute__((aligned(4)));
+  f32x4 v[2];
+  __device__ __forceinline__ void load(const float* x, int left) {
+    if (left >= 8) {
+      v[0] = *(const Any*)x;
+      v[1] = *(const Any*)(x + 4);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i >> 2][i & 3] = i < left ? x[i] : 0.f;
+    }
+  }
+  __device__ __forceinline__ float at(int i) const { return v[i >> 2][i & 3]; }
+};
 
-// round(127 x / a) for |x| <= a, inverse = 1 / a: a quotient by the inverse, corrected by what is left of
-// 127 x (exactly, so that a quotient halfway between two codes is seen as that).
-__device__ __forceinline__ int8_t code_of(float x, float a, float inverse) {
-  const float t = 127.f * x;
-  const float y = t * inverse;
-  return (int8_t)(int)rintf(fmaf(fmaf(-y, a, t), inverse, y));
-}
-
+// The bits of the largest |x|: absolute values are ordered as their bits, infinity and NaN above all numbers.
 template <typename T>
-__global__ void __launch_bounds__(256) quantize_int8_kernel(const QuantParams p) {
-  __shared__ uint32_t most[4];
-  const int64_t row = blockIdx.x;
-  const T* x = (const T*)p.x + row * p.ldx;
-  // absolute values are ordered as their bits, with infinity and NaN above all numbers
-  uint32_t a = 0;
-  for (int i = threadIdx.x; i < p.cols; i += 256) {
-    const uint32_t b = __float_as_uint(as_float(x, i)) & 0x7fffffffu;
+__device__ __forceinline__ uint32_t most_of(const Piece<T>& p, uint32_t a) {
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t b = __float_as_uint(p.at(i)) & 0x7fffffffu;
     a = a > b ? a : b;
+  }
+  return a;
+}
+
+// Codes of four elements: round(127 x / a), a quotient by the inverse of a, corrected by what is left of 127 x
+// (exactly, so that a quotient halfway between two codes is seen as that).  Adding 1.5 * 2^23 rounds to whole
+// numbers, ties to even, and leaves them in the low bits.
+template <typename T>
+__device__ __forceinline__ uint32_t four_codes(const Piece<T>& p, int first, float up, float a, float inverse) {
+  uint32_t c[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float t = up * p.at(first + i), y = t * inverse;
+    c[i] = __float_as_uint(fmaf(fmaf(-y, a, t), inverse, y) + 12582912.f);
+  }
+  const uint32_t lo = __builtin_amdgcn_perm(c[1], c[0], 0x0c0c0400u), hi = __builtin_amdgcn_perm(c[3], c[2], 0x04000c0cu);
+  return lo | hi;
+}
+
+// LANES: of a row, 64 or 256; PER: pieces of 8 elements that a lane holds, 0: the row is read twice.
+template <typename T, int LANES, int PER>
+__global__ void __launch_bounds__(256) quantize_int8_kernel(const QuantParams p) {
+  const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+  const int t = threadIdx.x % LANES;
+  if (LANES == 64 && row >= p.rows) return;  // whole waves
+  const T* x = (const T*)p.x + row * p.ldx;
+  const int pieces = (p.cols + 7) / 8;
+  Piece<T> held[PER > 0 ? PER : 1];
+  uint32_t most = 0;
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) {
+      const int at = t + LANES * i;
+      held[i].load(x + 8 * (int64_t)at, at < pieces ? p.cols - 8 * at : 0);
+    }
+#pragma unroll
+    for (int i = 0; i < PER; ++i) most = most_of(held[i], most);
+  } else {
+    for (int at = t; at < pieces; at += LANES) {
+      held[0].load(x + 8 * (int64_t)at, p.cols - 8 * at);
+      most = most_of(held[0], most);
+    }
   }
 #pragma unroll
   for (int d = 32; d > 0; d >>= 1) {
-    const uint32_t b = __shfl_xor(a, d);
-    a = a > b ? a : b;
+    const uint32_t b = __shfl_xor(most, d);
+    most = most > b ? most : b;
   }
-  if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = a;
-  __syncthreads();
-  a = most[0];
+  if constexpr (LANES == 256) {
+    __shared__ uint32_t waves[4];
+    if ((t & 63) == 0) waves[t >> 6] = most;
+    __syncthreads();
+    most = waves[0];
 #pragma unroll
-  for (int i = 1; i < 4; ++i) a = a > most[i] ? a : most[i];
-  const bool finite = a < 0x7f800000u;
-  const float amax = fmaxf(__uint_as_float(a), 0x1p-100f);
+    for (int i = 1; i < 4; ++i) most = most > waves[i] ? most : waves[i];
+  }
+  const bool finite = most < 0x7f800000u;
+  const float amax = fmaxf(__uint_as_float(most), 0x1p-100f);
   // 127 x must not overflow: rows of large values are taken 2^-16 as large
   const float unit = amax > 0x1p100f ? 0x1p-16f : 1.f;
-  const float most_x = amax * unit, inverse = 1.f / most_x;
-  if (threadIdx.x == 0) p.scale[row] = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
+  const float a = amax * unit, inverse = 1.f / a, up = 127.f * unit;
+  if (t == 0) p.scale[row] = finite ? amax / 127.f : __uint_as_float(0x7fc00000u);
+  const uint32_t mask = finite ? ~0u : 0u;
   int8_t* codes = p.codes + row * p.ldc;
-  for (int i = threadIdx.x; i < p.cols; i += 256) codes[i] = finite ? code_of(as_float(x, i) * unit, most_x, inverse) : (int8_t)0;
+  typedef u32x2 Any __attribute__((aligned(1)));
+  auto store = [&](const Piece<T>& h, int at) {
+    const u32x2 c = {four_codes(h, 0, up, a, inverse) & mask, four_codes(h, 4, up, a, inverse) & mask};
+    const int left = p.cols - 8 * at;
+    int8_t* dst = codes + 8 * (int64_t)at;
+    if (left >= 8) {
+      *(Any*)dst = c;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (i < left) dst[i] = (int8_t)(c[i >> 2] >> (8 * (i & 3)));
+    }
+  };
+  if constexpr (PER > 0) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i)
+      if (t + LANES * i < pieces) store(held[i], t + LANES * i);
+  } else {
+    for (int at = t; at < pieces; at += LANES) {
+      held[0].load(x + 8 * (int64_t)at, p.cols - 8 * at);
+      store(held[0], at);
+    }
+  }
+}
+
+template <typename T>
+hipError_t launch(const QuantParams& p, hipStream_t s) {
+  const dim3 block(256), rows1((unsigned)p.rows), rows4((unsigned)((p.rows + 3) / 4));
+  const int pieces = (p.cols + 7) / 8;
+  // a wave a row where rows are short, but a workgroup where they are few: its loads are all on their way at once
+  if (p.rows >= 1024 || pieces <= 64) {
+    if (pieces <= 64) return launch_kernel((quantize_int8_kernel<T, 64, 1>), rows4, block, 0, s, p);
+    if (pieces <= 128) return launch_kernel((quantize_int8_kernel<T, 64, 2>), rows4, block, 0, s, p);
+    if (pieces <= 256) return launch_kernel((quantize_int8_kernel<T, 64, 4>), rows4, block, 0, s, p);
+  }
+  if (pieces <= 256) return launch_kernel((quantize_int8_kernel<T, 256, 1>), rows1, block, 0, s, p);
+  if (pieces <= 512) return launch_kernel((quantize_int8_kernel<T, 256, 2>), rows1, block, 0, s, p);
+  if (pieces <= 1024) return launch_kernel((quantize_int8_kernel<T, 256, 4>), rows1, block, 0, s, p);
+  if (pieces <= 2048) return launch_kernel((quantize_int8_kernel<T, 256, 8>), rows1, block, 0, s, p);
+  return launch_kernel((quantize_int8_kernel<T, 256, 0>), rows1, block, 0, s, p);
 }
 
 }  // namespace
 
 hipError_t launch_quantize_int8(int dtype, const QuantParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)p.rows), block(256);
-  if (dtype == kF16) return launch_kernel(quantize_int8_kernel<_Float16>, grid, block, 0, s, p);
-  if (dtype == kBF16) return launch_kernel(quantize_int8_kernel<__bf16>, grid, block, 0, s, p);
-  return launch_kernel(quantize_int8_kernel<float>, grid, block, 0, s, p);
+  if (dtype == kF16) return launch<_Float16>(p, s);
+  if (dtype == kBF16) return launch<__bf16>(p, s);
+  return launch<float>(p, s);
 }
 
 }  // namespace cmpext3
