@@ -45,7 +45,6 @@ __all__ = ["fp16_matmul", "bf16_matmul", "fp32_matmul", "linear", "bmm", "conv2d
            "qk_norm_rope", "kv_cache_write", "kv_cache_read", "attention", "paged_attention", "rope_table",
            "gated_linear", "quantize_int8", "int8_linear", "int8_gated_linear", "version"]
 
-from .gated import gated_linear  # noqa: E402
 from .rope import rope_table  # noqa: E402
 
 try:
@@ -72,13 +71,13 @@ if _ext is not None:
     kv_cache_read = _ext.kv_cache_read
     attention = _ext.attention
     paged_attention = _ext.paged_attention
+    gated_linear = _ext.gated_linear
     quantize_int8 = _ext.quantize_int8
     int8_linear = _ext.int8_linear
     int8_gated_linear = _ext.int8_gated_linear
     version = _ext.version
     extension_path = _ext.__file__
 else:
-    del gated_linear  # needs the extension: raises at access, as the others do
 
     def __getattr__(name):
         # The submodule `cmp_ext_amd.build` stays importable so that an unbuilt tree can be

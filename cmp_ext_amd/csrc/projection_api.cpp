@@ -126,11 +126,14 @@ hipError_t run_copy(Operand* o, size_t esz, char* ws, hipStream_t s) {
   return e;
 }
 
-// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows_any|rows|tile128x128|tile256x256>[,splits=<s>]" replaces
-// the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan, ignored where malformed.
+// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows|small64x64|tile128x128|tile256x256>[,splits=<s>]"
+// replaces the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan,
+// ignored where malformed.
 struct Override {
   char kernel[32];
   int splits;
+  bool is(const char* name) const { return strcmp(kernel, name) == 0; }
+  bool tiles() const { return is("small64x64") || is("tile128x128") || is("tile256x256"); }
 };
 Override read_override() {
   Override o{};
@@ -140,40 +143,59 @@ Override read_override() {
 }
 
 struct TilePlan {
-  int bm;    // 256, 128, or 0: the kernel for any alignment
+  int bm;  // 256, 128, 64 (no copies of operands), or 0: the kernel for any size
   bool deep;
   int splits, ksplit;
 };
 
 // Which tiles, and in how many splits of the steps of 128 bytes of k, for M x N results (of `products` products)
-// in `batch` entries.  Modelled microseconds (MI355X).
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch) {
+// in `batch` entries; copy_us: what the large tiles' copies of operands take (0: none).  Modelled microseconds, fitted
+// to timings of 27 shapes with every tile and 1, 2, 4 and 8 splits (MI355X): a round of workgroups takes its steps
+// and some start and end, but no less than reading the operands once; splits add their sums' way to memory and back
+// and a launch.  64 x 64 tiles run three to a CU, and read operands of odd rows (every line twice) at 0.9 us
+// a step for 0.65: x[1000, 2001], two of 4001 rows, 90 us, in copies 67; x[333, 2050] by 1001 rows of codes 11.4 and 26.6,
+// x[100, 1024], two of 1024, 8.5 for 10.0.
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch, double copy_us, bool small_ok) {
   const Override o = read_override();
-  const int64_t bn256 = 256 / products, bn128 = 128 / products;
-  const int64_t rounds = cdiv(cdiv(M, 256) * cdiv(N, bn256) * batch, 256);
-  TilePlan best{256, false, 1, (int)steps};
-  double least = (double)rounds * (steps * 1.6 + 6.0);
-  const int64_t tiles = cdiv(M, 128) * cdiv(N, bn128) * batch;
-  if (strcmp(o.kernel, "tile256x256") == 0) return best;
-  const bool forced = strcmp(o.kernel, "tile128x128") == 0;
-  if (forced) least = 1e30;
-  for (int64_t s = 1; s <= 16 && (s == 1 || s * 4 <= steps); ++s) {
-    const int64_t each = cdiv(steps, s);
-    if (s > 1 && (s - 1) * each >= steps) continue;  // an empty split
-    if (forced && o.splits > 0 && s != o.splits) continue;
-    const int64_t wgs = tiles * s;
-    if (wgs * batch > INT_MAX / 256) break;
-    const bool deep = wgs <= 256 && each >= 8;
-    const int64_t full = wgs / 512, rest = wgs % 512;
-    double t = (double)full * (each * 0.98 + 5.0);
-    if (rest > 256) t += each * 0.98 + 5.0;
-    else if (rest > 0) t += each * (deep ? 0.46 : 0.70) + 4.0;
-    if (s > 1) t += 4.0 + (double)s * batch * M * N * products * 8.0 / 5e6;
-    if (t < least) {
-      least = t;
-      best = TilePlan{128, deep, (int)s, (int)each};
+  TilePlan best{0, false, 1, (int)steps};
+  double least = 1e30;
+  auto consider = [&](int bm) {
+    if ((bm == 64 && !small_ok) || (o.tiles() && atoi(strchr(o.kernel, 'x') - (bm == 64 ? 2 : 3)) != bm)) return;
+    const int64_t tiles = cdiv(M, bm) * cdiv(N, bm / products) * batch;
+    for (int64_t s = 1; s <= 16 && (s == 1 || (s * 4 <= steps && bm < 256)); ++s) {
+      const int64_t each = cdiv(steps, s);
+      if (s > 1 && (s - 1) * each >= steps) continue;  // an empty split
+      if (o.tiles() && o.splits > 0 && s != o.splits) continue;
+      const int64_t wgs = tiles * s;
+      if (wgs > kMostThreads / 512) break;
+      bool deep = false;
+      double t = 0;
+      if (bm == 256) {
+        t += (double)cdiv(wgs, 256) * (each * 1.6 + 6.0);
+      } else if (bm == 128) {
+        deep = wgs <= 256 && each >= 8;
+        const int64_t full = wgs / 512, rest = wgs % 512;
+        t += (double)full * (each * 0.98 + 5.0);
+        if (rest > 256) t += each * 0.98 + 5.0;
+        else if (rest > 0) t += each * (deep ? 0.46 : 0.70) + 4.0;
+      } else {
+        const int64_t full = wgs / 768, rest = wgs % 768;
+        const double busy = copy_us > 0 ? 0.9 : 0.65;
+        t += (double)full * (each * busy + 4.0);
+        if (rest > 0) t += each * (rest > 512 ? busy : rest > 256 ? 0.5 : 0.36) + 4.0;
+      }
+      t = std::max(t, (double)batch * (M + N * products) * steps * 128 / 4.5e6);
+      if (bm > 64) t += copy_us;
+      if (s > 1) t += 4.0 + (double)s * batch * M * N * products * 8.0 / 5e6;
+      if (t < least) {
+        least = t;
+        best = TilePlan{bm, deep, (int)s, (int)each};
+      }
     }
-  }
+  };
+  consider(256);
+  consider(128);
+  consider(64);
   return best;
 }
 
@@ -182,12 +204,11 @@ int64_t partial_bytes(const TilePlan& t, int64_t M, int64_t N, int products, int
   return t.splits > 1 ? (int64_t)t.splits * batch * products * M * partial_pitch(N) * 4 : 0;
 }
 
-bool tile_grid_fits(int64_t M, int64_t N, int products, int64_t batch) {
-  return cdiv(M, 128) * cdiv(N, 128 / products) * batch <= kMostThreads / 512;
-}
+// Microseconds of a zero-padded copy of an operand, 0 where none is needed.
+double copy_us(const Operand& o, size_t esz) { return rows_of_16(o, esz) ? 0.0 : 4.0 + (double)o.rows * o.cols * (int)esz * 2.0 / 4e6; }
 
 // Sets the tiles' grid in p and launches them, and the join of their splits.
-hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* launch, const TilePlan& t, ProjParams& p, void* partials, hipStream_t s) {
+hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* large, const TilePlan& t, ProjParams& p, void* partials, hipStream_t s) {
   const int products = mode == kProjGated ? 2 : 1;
   p.tiles_m = (int)cdiv(p.M, t.bm);
   p.tiles_n = (int)cdiv(p.N, t.bm / products);
@@ -196,12 +217,14 @@ hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* launch, const Til
   p.ksplit = t.ksplit;
   p.partials = partials;
   p.ld_part = partial_pitch(p.N);
-  const hipError_t e = launch(p, t.bm, t.deep, s);
+  ProjSmallLaunch* small = dtype == CMPEXT3_F16    ? launch_projection_small_f16
+                           : dtype == CMPEXT3_BF16 ? launch_projection_small_bf16
+                                                   : launch_projection_small_int8;
+  const hipError_t e = t.bm == 64 ? small(mode, p, s) : large(p, t.bm, t.deep, s);
   return e != hipSuccess || t.splits == 1 ? e : launch_projection_join(dtype, mode, p, s);
 }
 
-enum ProjKernel { kAny, kRows, kRowsAny, kTile };
-const char* kernel_name(ProjKernel k) { return k == kAny ? "any64x64" : k == kRows ? "rows" : k == kRowsAny ? "rows_any" : "tile"; }
+enum ProjKernel { kAny, kRows, kTile };
 
 struct ProjPlan {
   ProjKernel kernel;
@@ -221,20 +244,26 @@ int plan_projection(const cmpext3_projection_args* a, ProjPlan* q) {
   q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
   q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
   const Override o = read_override();
-  const bool tiles_fit = tile_grid_fits(a->M, a->N, products, 1);
   const bool whole = rows_of_16(q->x, esz) && rows_of_16(q->w[0], esz) && (products == 1 || rows_of_16(q->w[1], esz));
   q->kernel = kAny;
-  if (a->K == 0 || strcmp(o.kernel, "any64x64") == 0) return CMPEXT3_OK;
-  if (a->M <= kFewRows && strncmp(o.kernel, "tile", 4) != 0 && (int64_t)a->K * (int64_t)esz >= 16) {
-    // few rows: bound by reading the weights, once
-    q->kernel = whole && strcmp(o.kernel, "rows_any") != 0 ? kRows : kRowsAny;
+  if ((int64_t)a->K * (int64_t)esz < 16 || o.is("any64x64")) return CMPEXT3_OK;
+  // Few rows: bound by reading the weights, once.  Above 32 rows the 64 x 64 tiles are as fast where they fill the CUs
+  // (codes, 64 x 4096 x 14336: 16.1 us for 20.5; but 64 x 4096 x 4096 14.9 for 10.1), and weights of odd rows go
+  // there too (4 or 16 rows by 14336 of 4099 codes 16 and 19 us; a kernel that loads them into registers took 25 and 33).
+  const bool rows = whole && (a->M <= 32 || (a->M <= kFewRows && (int64_t)a->N * products <= 8192));
+  if (o.is("rows") ? whole && a->M <= kFewRows : rows && !o.tiles()) {
+    q->kernel = kRows;
     return CMPEXT3_OK;
   }
-  if (!tiles_fit) return CMPEXT3_OK;
+  double copies = copy_us(q->x, esz);
+  for (int i = 0; i < products; ++i) copies += copy_us(q->w[i], esz);
+  q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1, copies, true);
+  if (q->tile.bm == 0) return CMPEXT3_OK;
   q->kernel = kTile;
-  plan_copy(&q->x, esz, &q->ws_bytes);
-  for (int i = 0; i < products; ++i) plan_copy(&q->w[i], esz, &q->ws_bytes);
-  q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1);
+  if (q->tile.bm > 64) {
+    plan_copy(&q->x, esz, &q->ws_bytes);
+    for (int i = 0; i < products; ++i) plan_copy(&q->w[i], esz, &q->ws_bytes);
+  }
   q->partials_at = take(&q->ws_bytes, partial_bytes(q->tile, a->M, a->N, products, 1));
   return CMPEXT3_OK;
 }
@@ -304,17 +333,20 @@ int plan_backward(const cmpext3_gated_backward_args* a, BackwardPlan* q) {
   q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
   q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
   q->x = Operand{a->x, a->x_row, a->M, a->K, -1, 0};
-  if (a->M == 0 || a->N == 0 || a->K == 0 || strcmp(read_override().kernel, "any64x64") == 0) return CMPEXT3_OK;
+  if (a->M == 0 || a->N == 0 || a->K == 0 || read_override().is("any64x64")) return CMPEXT3_OK;
   const int64_t batch = (a->dw_gate != nullptr) + (a->dw_up != nullptr);
   int64_t partials = 0;
-  if (a->dx != nullptr && tile_grid_fits(a->M, a->K, 1, 1)) {
-    for (Operand& w : q->w) plan_copy(&w, 2, &q->ws_bytes);
-    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1);
+  // the small tiles read 16 bytes of a row at least: of x and the weights, and of dgate's and dup's N
+  const bool rows16 = a->K >= 8 && a->N >= 8;
+  if (a->dx != nullptr) {
+    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1, copy_us(q->w[0], 2) + copy_us(q->w[1], 2), rows16);
+    if (q->dx.bm > 64)
+      for (Operand& w : q->w) plan_copy(&w, 2, &q->ws_bytes);
     partials = partial_bytes(q->dx, a->M, a->K, 1, 1);
   }
-  if (batch > 0 && tile_grid_fits(a->N, a->K, 1, batch)) {
-    plan_copy(&q->x, 2, &q->ws_bytes);
-    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch);
+  if (batch > 0) {
+    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch, copy_us(q->x, 2), rows16);
+    if (q->dw.bm > 64) plan_copy(&q->x, 2, &q->ws_bytes);
     partials = std::max(partials, partial_bytes(q->dw, a->N, a->K, 1, batch));
   }
   q->partials_at = take(&q->ws_bytes, partials);
@@ -363,7 +395,6 @@ extern "C" int cmpext3_projection(const cmpext3_projection_args* a, void* worksp
   ProjParams p = params_of(a);
   if (q.kernel == kAny) return (int)launch_projection_any(a->dtype, mode, false, false, p, s);
   if (q.kernel == kRows) return (int)launch_projection_rows(a->dtype, mode, p, s);
-  if (q.kernel == kRowsAny) return (int)launch_projection_rows_any(a->dtype, mode, p, s);
   const size_t esz = elem_size(a->dtype);
   for (Operand* o : {&q.x, &q.w[0], &q.w[1]}) {
     const hipError_t e = run_copy(o, esz, (char*)workspace, s);
@@ -372,7 +403,7 @@ extern "C" int cmpext3_projection(const cmpext3_projection_args* a, void* worksp
   p.a[0] = p.a[1] = q.x.p;
   p.lda = q.x.ld;
   for (int i = 0; i < 2; ++i) p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
-  p.K = (int)(cdiv(a->K * (int64_t)esz, 16) * 16 / (int64_t)esz);  // copies hold zeros up to there
+  if (q.tile.bm > 64) p.K = (int)(cdiv(a->K * (int64_t)esz, 16) * 16 / (int64_t)esz);  // copies hold zeros up to there
   ProjTileLaunch* launch = a->dtype == CMPEXT3_F16    ? launch_projection_tile_gated_f16
                            : a->dtype == CMPEXT3_BF16 ? launch_projection_tile_gated_bf16
                            : mode == kProjGated       ? launch_projection_tile_int8_gated
@@ -388,9 +419,9 @@ extern "C" int cmpext3_projection_describe(const cmpext3_projection_args* a, cha
   if (a->M == 0 || a->N == 0)
     snprintf(buf, (size_t)buflen, "kernel=none");
   else if (q.kernel != kTile)
-    snprintf(buf, (size_t)buflen, "kernel=%s", kernel_name(q.kernel));
+    snprintf(buf, (size_t)buflen, "kernel=%s", q.kernel == kRows ? "rows" : "any64x64");
   else
-    snprintf(buf, (size_t)buflen, "kernel=tile%dx%d%s splits=%d copies=%d", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.splits,
+    snprintf(buf, (size_t)buflen, "kernel=%s%dx%d%s splits=%d copies=%d", q.tile.bm == 64 ? "small" : "tile", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.splits,
              (q.x.copy_at >= 0) + (q.w[0].copy_at >= 0) + (q.w[1].copy_at >= 0));
   return CMPEXT3_OK;
 }

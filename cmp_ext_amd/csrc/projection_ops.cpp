@@ -340,8 +340,9 @@ std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& grad, const Tens
 // Under graph capture the gradient of a leaf is added on the stream that its accumulating node was
 // made on.  A node that an eager graph on another stream keeps alive would pull that stream into the
 // capture, which ends the process from autograd's thread: refused here, before anything is recorded.
-void check_capture(const std::vector<Tensor>& leaves) {
-  for (const Tensor& t : leaves) {
+void check_capture(std::initializer_list<const Tensor*> leaves) {
+  for (const Tensor* leaf : leaves) {
+    const Tensor& t = *leaf;
     if (!t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
     const auto stream = c10::hip::getCurrentHIPStream(t.get_device());
     hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
@@ -355,6 +356,34 @@ void check_capture(const std::vector<Tensor>& leaves) {
   }
 }
 
+// gated_linear with its gradients.  Saved for the backward pass: the inputs and, in fp32, both products.
+struct GatedLinear : torch::autograd::Function<GatedLinear> {
+  static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
+                        const std::string& activation) {
+    Tensor out, gate, up;
+    std::tie(out, gate, up) = gated_forward(x, w_gate, w_up, activation, true);
+    ctx->save_for_backward({x, w_gate, w_up, gate, up});
+    ctx->saved_data["activation"] = activation;
+    return out;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
+    const auto saved = ctx->get_saved_variables();
+    Tensor dx, dgate, dup;
+    std::tie(dx, dgate, dup) = gated_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+                                              ctx->saved_data["activation"].toStringRef(), ctx->needs_input_grad(0),
+                                              ctx->needs_input_grad(1), ctx->needs_input_grad(2));
+    return {dx, dgate, dup, Tensor()};
+  }
+};
+
+Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const std::string& activation) {
+  if (!at::GradMode::is_enabled() || !(x.requires_grad() || w_gate.requires_grad() || w_up.requires_grad()))
+    return std::get<0>(gated_forward(x, w_gate, w_up, activation, false));
+  check_capture({&x, &w_gate, &w_up});
+  return GatedLinear::apply(x, w_gate, w_up, activation);
+}
+
 }  // namespace
 
 void register_projection_ops(py::module& m) {
@@ -364,7 +393,14 @@ void register_projection_ops(py::module& m) {
   m.def("int8_gated_linear", &int8_gated_linear, "act(x @ w_gate.T) * (x @ w_up.T) for int8 codes with scales", py::arg("x"),
         py::arg("w_gate"), py::arg("w_up"), py::arg("gate_scale"), py::arg("up_scale"), py::arg("activation") = "silu",
         py::arg("x_scale") = py::none(), py::arg("dtype") = py::none());
-  m.def("_gated_forward", &gated_forward);
-  m.def("_gated_backward", &gated_backward);
-  m.def("_check_capture", &check_capture);
+  m.def("gated_linear", &gated_linear,
+        R"(act(x @ w_gate.T) * (x @ w_up.T) in one kernel: x [..., K], weights [N, K], all float16 or all bfloat16; sums
+and the activation in fp32, rounded once.
+
+activation: "silu", "gelu" (by the error function), "gelu_tanh" or "relu".
+
+Differentiable once in all three tensors.  For the backward pass x, the weights and both products (in float32,
+8 bytes for each result) are kept; where no input needs a gradient nothing is.  Weights may be the two halves of one
+tensor.  Under graph capture the inputs' leaves must not be held by a graph of another stream (refused).)",
+        py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("activation") = "silu");
 }

@@ -43,10 +43,9 @@ struct ProjParams {
 // Any pitch and alignment; a is [M, K] or, a_km, [K, M]; b is [N, K] or, b_kn, [K, N].
 hipError_t launch_projection_any(int dtype, ProjMode mode, bool a_km, bool b_kn, const ProjParams& p, hipStream_t s);
 
-// Up to kFewRows rows of a, b as [N, K]: rows of whole 16 bytes, or (_any) of any alignment and at least 16 bytes.
+// Up to kFewRows rows of a, b as [N, K], rows of whole 16 bytes.
 constexpr int kFewRows = 64;
 hipError_t launch_projection_rows(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
-hipError_t launch_projection_rows_any(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
 
 // Tiles of bm = 256 or 128 rows; `deep`: alone on a CU, with a ring of four steps.  Operands have rows of
 // whole 16 bytes.  (One translation unit for each element type and mode.)
@@ -55,6 +54,10 @@ ProjTileLaunch launch_projection_tile_gated_f16, launch_projection_tile_gated_bf
 ProjTileLaunch launch_projection_tile_sum_f16, launch_projection_tile_sum_bf16;
 ProjTileLaunch launch_projection_tile_wgrad_f16, launch_projection_tile_wgrad_bf16;
 ProjTileLaunch launch_projection_tile_int8_plain, launch_projection_tile_int8_gated;
+// Tiles of 64 x 64, operands of any alignment whose rows have at least 16 bytes (sum and plain: see the modes' layouts
+// above; gradients have a across k or b as [K, N] as the large tiles do).
+using ProjSmallLaunch = hipError_t(ProjMode mode, const ProjParams& p, hipStream_t s);
+ProjSmallLaunch launch_projection_small_f16, launch_projection_small_bf16, launch_projection_small_int8;
 // Adds the splits' sums in their order and finishes the results as an unsplit kernel does.
 hipError_t launch_projection_join(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
 

@@ -1,0 +1,10 @@
+// Small tiles of a gated block and its gradients, bf16.
+#include "projection_small_kernel.h"
+
+namespace cmpext3 {
+hipError_t launch_projection_small_bf16(ProjMode mode, const ProjParams& p, hipStream_t s) {
+  if (mode == kProjGated) return launch_projection_small<__bf16, kProjGated, false, false>(p, s);
+  if (mode == kProjSum) return launch_projection_small<__bf16, kProjSum, false, true>(p, s);
+  return launch_projection_small<__bf16, kProjPlain, true, true>(p, s);
+}
+}  // namespace cmpext3
