@@ -90,7 +90,7 @@ class QuantizeInt8Args(ctypes.Structure):
 
 
 class ProjectionArgs(ctypes.Structure):
-    _fields_ = _fields("""i32: dtype out_dtype activation M N K; ptr: x; i64: x_row; ptr: x_scale w_gate; i64: gate_row; ptr: gate_scale w_up;
+    _fields_ = _fields("""i32: dtype x_dtype out_dtype activation M N K; ptr: x; i64: x_row; ptr: x_scale w_gate; i64: gate_row; ptr: gate_scale w_up;
                           i64: up_row; ptr: up_scale bias out; i64: out_row; ptr: gate_out up_out; i64: pre_row""")
 
 

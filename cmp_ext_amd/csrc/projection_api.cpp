@@ -60,6 +60,7 @@ int check_projection(const cmpext3_projection_args* a) {
   if (a == nullptr) return CMPEXT3_ERR_INVALID_ARG;
   const bool i8 = a->dtype == CMPEXT3_I8, gated = a->w_up != nullptr;
   if (!i8 && !is16(a->dtype)) return CMPEXT3_ERR_UNSUPPORTED;
+  if (a->x_dtype != a->dtype && !(i8 && (is16(a->x_dtype) || a->x_dtype == CMPEXT3_F32))) return CMPEXT3_ERR_UNSUPPORTED;
   if (!is16(a->out_dtype) && !(i8 && a->out_dtype == CMPEXT3_F32)) return CMPEXT3_ERR_UNSUPPORTED;
   if (!i8 && (a->out_dtype != a->dtype || !gated)) return CMPEXT3_ERR_UNSUPPORTED;
   if (gated && (a->activation < CMPEXT3_ACT_SILU || a->activation > CMPEXT3_ACT_RELU)) return CMPEXT3_ERR_UNSUPPORTED;
@@ -70,7 +71,7 @@ int check_projection(const cmpext3_projection_args* a) {
   if (st != CMPEXT3_OK) return st;
   if (i8 && a->K > CMPEXT3_I8_MAX_K) return CMPEXT3_ERR_TOO_LARGE;
   if (a->M == 0 || a->N == 0) return CMPEXT3_OK;
-  st = first_of({check_matrix(a->x, a->M, a->K, a->x_row, a->dtype), check_matrix(a->w_gate, a->N, a->K, a->gate_row, a->dtype),
+  st = first_of({check_matrix(a->x, a->M, a->K, a->x_row, a->x_dtype), check_matrix(a->w_gate, a->N, a->K, a->gate_row, a->dtype),
                  gated ? check_matrix(a->w_up, a->N, a->K, a->up_row, a->dtype) : CMPEXT3_OK,
                  check_matrix(a->out, a->M, a->N, a->out_row, a->out_dtype)});
   if (st != CMPEXT3_OK) return st;
@@ -79,7 +80,8 @@ int check_projection(const cmpext3_projection_args* a) {
     if (st != CMPEXT3_OK) return st;
   }
   if (i8) {
-    if (a->x_scale == nullptr || !aligned(a->x_scale, 4)) return CMPEXT3_ERR_INVALID_ARG;
+    if ((a->x_scale != nullptr) != (a->x_dtype == CMPEXT3_I8) || !aligned(a->x_scale, 4)) return CMPEXT3_ERR_INVALID_ARG;
+    if (a->x_dtype != CMPEXT3_I8 && a->M > kMostThreads / 256) return CMPEXT3_ERR_TOO_LARGE;
     if (a->gate_scale == nullptr || !aligned(a->gate_scale, 4)) return CMPEXT3_ERR_INVALID_ARG;
     if (gated && (a->up_scale == nullptr || !aligned(a->up_scale, 4))) return CMPEXT3_ERR_INVALID_ARG;
   }
@@ -228,6 +230,9 @@ enum ProjKernel { kAny, kRows, kTile };
 
 struct ProjPlan {
   ProjKernel kernel;
+  bool make;         // x's codes are made in the workspace first, in rows of whole 16 bytes with zeros behind x's,
+  bool make_inside;  // or by the kernel
+  int64_t codes_at, scale_at;
   Operand x, w[2];
   TilePlan tile;
   int64_t partials_at, ws_bytes;
@@ -243,6 +248,20 @@ int plan_projection(const cmpext3_projection_args* a, ProjPlan* q) {
   q->x = Operand{a->x, a->x_row, a->M, a->K, -1, 0};
   q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
   q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
+  q->make = a->x_dtype != a->dtype;
+  if (q->make) {
+    const int pitch = (int)(cdiv(a->K, 16) * 16);
+    const bool few = is16(a->x_dtype) && a->M <= kRowsCodesRows && (int64_t)a->M * a->K <= kRowsCodesMost && a->K % kRowsCodesUnit == 0 && a->K > 0 &&
+                     rows_of_16(q->x, elem_size(a->x_dtype));
+    q->make_inside = few && rows_of_16(q->w[0], 1) && (products == 1 || rows_of_16(q->w[1], 1)) && read_override().kernel[0] == 0;
+    if (q->make_inside) {
+      q->kernel = kRows;
+      return CMPEXT3_OK;
+    }
+    q->codes_at = take(&q->ws_bytes, (int64_t)a->M * pitch);
+    q->scale_at = take(&q->ws_bytes, (int64_t)a->M * 4);
+    q->x = Operand{nullptr, pitch, a->M, pitch, -1, 0};  // an address of 16 bytes: the workspace's
+  }
   const Override o = read_override();
   const bool whole = rows_of_16(q->x, esz) && rows_of_16(q->w[0], esz) && (products == 1 || rows_of_16(q->w[1], esz));
   q->kernel = kAny;
@@ -374,7 +393,7 @@ extern "C" int cmpext3_quantize_int8(const cmpext3_quantize_int8_args* a, void* 
   p.ldc = a->codes_row;
   p.scale = a->scale;
   p.rows = a->rows;
-  p.cols = a->cols;
+  p.cols = p.written = a->cols;
   return (int)launch_quantize_int8(a->dtype, p, (hipStream_t)stream);
 }
 
@@ -393,6 +412,21 @@ extern "C" int cmpext3_projection(const cmpext3_projection_args* a, void* worksp
   const hipStream_t s = (hipStream_t)stream;
   const ProjMode mode = a->w_up != nullptr ? kProjGated : kProjPlain;
   ProjParams p = params_of(a);
+  if (q.make_inside) return (int)launch_projection_rows_codes(a->x_dtype, mode, p, s);
+  if (q.make) {
+    QuantParams c{};
+    c.x = a->x;
+    c.ldx = a->x_row;
+    c.codes = (int8_t*)workspace + q.codes_at;
+    c.ldc = c.written = (int)q.x.ld;
+    c.scale = (float*)((char*)workspace + q.scale_at);
+    c.rows = a->M, c.cols = a->K;
+    const hipError_t e = launch_quantize_int8(a->x_dtype, c, s);
+    if (e != hipSuccess) return (int)e;
+    q.x.p = p.a[0] = p.a[1] = c.codes;
+    p.lda = c.ldc;
+    p.a_scale = c.scale;
+  }
   if (q.kernel == kAny) return (int)launch_projection_any(a->dtype, mode, false, false, p, s);
   if (q.kernel == kRows) return (int)launch_projection_rows(a->dtype, mode, p, s);
   const size_t esz = elem_size(a->dtype);
@@ -419,7 +453,7 @@ extern "C" int cmpext3_projection_describe(const cmpext3_projection_args* a, cha
   if (a->M == 0 || a->N == 0)
     snprintf(buf, (size_t)buflen, "kernel=none");
   else if (q.kernel != kTile)
-    snprintf(buf, (size_t)buflen, "kernel=%s", q.kernel == kRows ? "rows" : "any64x64");
+    snprintf(buf, (size_t)buflen, "kernel=%s%s", q.kernel == kRows ? "rows" : "any64x64", q.make_inside ? " codes=inside" : "");
   else
     snprintf(buf, (size_t)buflen, "kernel=%s%dx%d%s splits=%d copies=%d", q.tile.bm == 64 ? "small" : "tile", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.splits,
              (q.x.copy_at >= 0) + (q.w[0].copy_at >= 0) + (q.w[1].copy_at >= 0));

@@ -64,8 +64,9 @@ __device__ __forceinline__ void dma_load16_m0_once(i32x4 rsrc, uint32_t voff, ui
 
 // The end of the kernels for few rows: adds the sums of WAVES waves, [wave][16 MB rows of x][PITCH] of which the
 // first 16 NB are a strip's rows (gated: 16 of w_gate, 16 of w_up, ..), and finishes and stores the results.
+// a_scale: of x's rows, in memory or LDS.
 template <typename T, int MODE, int MB, int NB, int WAVES, int PITCH>
-__device__ __forceinline__ void finish_rows(const ProjParams& p, const void* red, int n0) {
+__device__ __forceinline__ void finish_rows(const ProjParams& p, const void* red, int n0, const float* a_scale) {
   using E = typename std::conditional<sizeof(T) == 1, int, float>::type;
   constexpr bool GATED = MODE == kProjGated;
   constexpr int COLS = GATED ? 8 * NB : 16 * NB;
@@ -81,7 +82,7 @@ __device__ __forceinline__ void finish_rows(const ProjParams& p, const void* red
 #pragma unroll
       for (int i = 0; i < WAVES; ++i) s += sums[((i * MB * 16) + (int)m) * PITCH + c];
       v[q] = (float)s;
-      if (sizeof(T) == 1) v[q] = v[q] * p.a_scale[m] * p.b_scale[q][n];
+      if (sizeof(T) == 1) v[q] = v[q] * a_scale[m] * p.b_scale[q][n];
     }
     float y = v[0];
     if constexpr (GATED) {

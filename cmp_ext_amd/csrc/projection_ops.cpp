@@ -103,7 +103,8 @@ Tensor float_vector(const Tensor& t, int64_t size, const Tensor& like, const cha
   return t.contiguous();
 }
 
-std::tuple<Tensor, Tensor> quantize(const Tensor& x, const char* op) {
+std::tuple<Tensor, Tensor> quantize_int8(const Tensor& x) {
+  const char* op = "quantize_int8";
   TORCH_CHECK(x.dim() >= 1, "cmpext3.", op, ": the input needs at least one dimension");
   TORCH_CHECK(is16(x) || x.scalar_type() == at::kFloat, "cmpext3.", op, ": unsupported dtype ", x.scalar_type(),
               " (float16, bfloat16 or float32)");
@@ -124,8 +125,6 @@ std::tuple<Tensor, Tensor> quantize(const Tensor& x, const char* op) {
   check_status(cmpext3_quantize_int8(&a, current_stream(x)), op);
   return {codes, scale};
 }
-
-std::tuple<Tensor, Tensor> quantize_int8(const Tensor& x) { return quantize(x, "quantize_int8"); }
 
 // What all projections check: x's and the weights' shapes and devices.
 void check_operands(const Tensor& x, std::initializer_list<const Tensor*> weights, const char* op) {
@@ -191,23 +190,18 @@ Tensor int8_projection(const Tensor& x, const Tensor& w_gate, const Tensor& gate
     check_device(*bias, x, op, "bias");
     bias_c = bias->contiguous();
   }
-  Tensor xq = x, xs;
-  if (codes) {
-    xs = float_vector(*x_scale, x.size(-1) == 0 ? x_scale->numel() : x.numel() / x.size(-1), x, op, "x_scale");
-  } else {
-    std::tie(xq, xs) = quantize(x, op);
-  }
-  const Rows rx = rows_of(xq), rg = rows_of(w_gate), ru = gated ? rows_of(w_up) : rg;
-  TORCH_CHECK(xs.numel() == rx.rows, "cmpext3.", op, ": x_scale must have ", rx.rows, " elements, got ", xs.numel());
+  const Rows rx = rows_of(x), rg = rows_of(w_gate), ru = gated ? rows_of(w_up) : rg;
+  const Tensor xs = codes ? float_vector(*x_scale, rx.rows, x, op, "x_scale") : Tensor();
   Tensor out = torch::empty(with_last(x, N), x.options().dtype(out_type));
   cmpext3_projection_args a{};
   a.dtype = CMPEXT3_I8;
+  a.x_dtype = dtype_code(x.scalar_type());
   a.out_dtype = dtype_code(out_type);
   a.activation = act;
   set_sizes(a, rx, w_gate, op);
   a.x = rx.t.data_ptr();
   a.x_row = rx.pitch;
-  a.x_scale = (const float*)xs.data_ptr();
+  if (codes) a.x_scale = (const float*)xs.data_ptr();
   a.w_gate = rg.t.data_ptr();
   a.gate_row = rg.pitch;
   a.gate_scale = (const float*)gs.data_ptr();
@@ -256,7 +250,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& 
   const int64_t N = w_gate.size(0);
   Tensor out = torch::empty(with_last(x, N), x.options()), gate, up;
   cmpext3_projection_args a{};
-  a.dtype = a.out_dtype = dtype_code(x.scalar_type());
+  a.dtype = a.x_dtype = a.out_dtype = dtype_code(x.scalar_type());
   a.activation = act;
   set_sizes(a, rx, w_gate, op);
   a.x = rx.t.data_ptr();

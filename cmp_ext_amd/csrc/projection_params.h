@@ -46,6 +46,9 @@ hipError_t launch_projection_any(int dtype, ProjMode mode, bool a_km, bool b_kn,
 // Up to kFewRows rows of a, b as [N, K], rows of whole 16 bytes.
 constexpr int kFewRows = 64;
 hipError_t launch_projection_rows(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
+// The same for few elements of x in 16 bits, which every workgroup makes codes of (lda: of x; a_scale: none).
+constexpr int kRowsCodesRows = 16, kRowsCodesMost = 4096, kRowsCodesUnit = 512;  // rows, elements, of a row a multiple of
+hipError_t launch_projection_rows_codes(int x_dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
 
 // Tiles of bm = 256 or 128 rows; `deep`: alone on a CU, with a ring of four steps.  Operands have rows of
 // whole 16 bytes.  (One translation unit for each element type and mode.)
@@ -69,6 +72,7 @@ struct QuantParams {
   float* scale;
   int64_t rows;
   int cols;
+  int written;  // codes of a row: cols, or more, those past cols zeros
 };
 hipError_t launch_quantize_int8(int dtype, const QuantParams& p, hipStream_t s);
 

@@ -56,18 +56,20 @@ int cmpext3_quantize_int8(const cmpext3_quantize_int8_args* args, void* stream);
  *   plain (w_up NULL; dtype CMPEXT3_I8):  out = p(w) + bias
  *   gated (both weights):                 out = act(p(w_gate)) * p(w_up)
  * where p(w)[m, n] is the sum over k of x[m, k] * w[n, k]: F16 or BF16 with fp32 sums, or I8
- * with exact 32-bit integer sums times x_scale[m] * w_scale[n].  out [M, N] has out_dtype (F16,
+ * with exact 32-bit integer sums times x_scale[m] * w_scale[n].  x has x_dtype: that of the
+ * weights, or, with I8 weights, F16, BF16 or F32: it is then taken as cmpext3_quantize_int8 would
+ * give it (x_scale NULL).  out [M, N] has out_dtype (F16,
  * BF16, F32; that of x where it is not I8), rounded once.  In the plain form the weight is
  * w_gate, its scale gate_scale; bias [N] has out_dtype, or is NULL.  gate_out and up_out
  * (gated F16 / BF16 only; both or neither): p(w_gate) and p(w_up) as fp32, for the backward pass.
  * K = 0 gives sums of zero; K of I8 up to CMPEXT3_I8_MAX_K.
  */
 typedef struct cmpext3_projection_args {
-  int32_t dtype, out_dtype, activation;
+  int32_t dtype, x_dtype, out_dtype, activation; /* dtype: of the weights */
   int32_t M, N, K;
   const void* x;
   int64_t x_row;
-  const float* x_scale; /* [M], I8 only */
+  const float* x_scale; /* [M], x of I8 only */
   const void* w_gate;
   int64_t gate_row;
   const float* gate_scale; /* [N], I8 only */

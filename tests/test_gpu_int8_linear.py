@@ -120,7 +120,8 @@ def test_int8_largest_sums(m, n, k):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("m,n,k", [(1, 128, 512), (16, 300, 136), (77, 500, 1001), (300, 520, 2048)])
+@pytest.mark.parametrize("m,n,k", [(1, 128, 512), (1, 4096, 4096), (1, 9000, 16384), (3, 70, 512), (4, 520, 4096), (16, 100, 1024), (8, 33, 2048),
+                                   (17, 64, 512), (16, 300, 136), (77, 500, 1001), (300, 520, 2048), (5, 40, 15), (40, 1000, 100)])
 def test_int8_linear_quantises_its_input(dtype, m, n, k):
     import cmpext3
 
@@ -132,6 +133,26 @@ def test_int8_linear_quantises_its_input(dtype, m, n, k):
     R.check(y, R.int8_linear(q, s, w, ws, None, dtype))
     y32 = cmpext3.int8_linear(x, w, ws, dtype=torch.float32)
     R.check(y32, R.int8_linear(q, s, w, ws, None, torch.float32))
+    z = cmpext3.int8_gated_linear(x, w, w.flip(0), ws * 0.1, ws, "gelu")
+    assert torch.equal(z, cmpext3.int8_gated_linear(q, w, w.flip(0), ws * 0.1, ws, "gelu", x_scale=s, dtype=dtype))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_int8_linear_of_few_rows_that_are_not_finite(dtype):
+    import cmpext3
+
+    x = rand(6, 1024, dtype=dtype)
+    x[1, 1000], x[4, 0] = math.nan, math.inf
+    w, ws = rand_codes(50, 1024, seed=2), scales(50, 4)
+    y = cmpext3.int8_linear(x, w, ws)
+    assert torch.isnan(y[1]).all() and torch.isnan(y[4]).all()
+    x[1, 1000], x[4, 0] = 0, 0
+    z = cmpext3.int8_linear(x, w, ws)
+    assert torch.equal(y[[0, 2, 3, 5]], z[[0, 2, 3, 5]])
+    big = torch.zeros(2, 512, dtype=dtype, device=DEV)
+    big[0, 0], big[0, 1] = torch.finfo(dtype).max, torch.finfo(dtype).max / 2
+    q, s = cmpext3.quantize_int8(big)
+    assert torch.equal(cmpext3.int8_linear(big, w[:, :512], ws), cmpext3.int8_linear(q, w[:, :512], ws, x_scale=s, dtype=dtype))
 
 
 @pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh", "relu"])

@@ -65,7 +65,8 @@ def test_python_refusals():
 
 
 def projection(**kw):
-    a = cabi.ProjectionArgs(dtype=cabi.BF16, out_dtype=cabi.BF16, activation=cabi.ACT_SILU, M=8, N=64, K=128, x=0x1000, x_row=128,
+    dtype = kw.get("dtype", cabi.BF16)
+    a = cabi.ProjectionArgs(dtype=dtype, x_dtype=dtype, out_dtype=cabi.BF16, activation=cabi.ACT_SILU, M=8, N=64, K=128, x=0x1000, x_row=128,
                             w_gate=0x2000, gate_row=128, w_up=0x3000, up_row=128, out=0x4000, out_row=64)
     if kw.get("dtype") == cabi.I8:
         a.x_scale, a.gate_scale, a.up_scale = 0x5000, 0x6000, 0x7000
@@ -82,14 +83,16 @@ def test_projection_c_abi_rejects():
     i8 = dict(dtype=cabi.I8)
     assert size(projection()) >= 0 and size(projection(**i8)) >= 0 and size(projection(out_dtype=cabi.F32, **i8)) >= 0
     assert size(projection(w_up=None, bias=0x8000, **i8)) >= 0
+    assert all(size(projection(x_dtype=t, x_scale=None, **i8)) >= 0 for t in (cabi.F16, cabi.BF16, cabi.F32))
     assert cabi.lib().cmpext3_projection_workspace_size(None) == BAD
     for kw in (dict(dtype=cabi.F32), dict(dtype=cabi.E4M3), dict(out_dtype=cabi.F32), dict(out_dtype=cabi.F16), dict(w_up=None),
-               dict(activation=4), dict(activation=-1), dict(bias=0x8000), dict(out_dtype=cabi.I8, **i8),
+               dict(activation=4), dict(activation=-1), dict(bias=0x8000), dict(out_dtype=cabi.I8, **i8), dict(x_dtype=cabi.F16),
+               dict(x_dtype=cabi.I8), dict(x_dtype=cabi.E4M3, **i8),
                dict(gate_out=0x100, up_out=0x200, pre_row=64, **i8)):
         assert size(projection(**kw)) == NOT, kw
     for kw in (dict(M=-1), dict(N=-1), dict(K=-1), dict(x=None), dict(w_gate=None), dict(out=None), dict(x_row=127), dict(gate_row=127),
                dict(up_row=100), dict(out_row=63), dict(x=0x1001), dict(out=0x4001), dict(gate_out=0x100, pre_row=64),
-               dict(gate_out=0x100, up_out=0x200, pre_row=63), dict(x_scale=None, **i8), dict(gate_scale=None, **i8),
+               dict(gate_out=0x100, up_out=0x200, pre_row=63), dict(x_scale=None, **i8), dict(x_dtype=cabi.F16, **i8), dict(gate_scale=None, **i8),
                dict(up_scale=None, **i8), dict(x_scale=0x5002, **i8), dict(out=0x4002, out_dtype=cabi.F32, **i8),
                dict(w_up=None, bias=0x8001, **i8)):
         assert size(projection(**kw)) == BAD, kw
