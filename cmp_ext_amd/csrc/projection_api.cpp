@@ -128,25 +128,26 @@ hipError_t run_copy(Operand* o, size_t esz, char* ws, hipStream_t s) {
   return e;
 }
 
-// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows|small64x64|tile128x128|tile256x256>[,splits=<s>]"
-// replaces the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan,
+// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows|small64x64|tile128x128|tile256x256>[,splits=<s>
+// [,groups=<g>]]" replaces the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan,
 // ignored where malformed.
 struct Override {
   char kernel[32];
-  int splits;
+  int splits, groups;
   bool is(const char* name) const { return strcmp(kernel, name) == 0; }
   bool tiles() const { return is("small64x64") || is("tile128x128") || is("tile256x256"); }
 };
 Override read_override() {
   Override o{};
   const char* env = getenv("CMPEXT3_PROJECTION_CONFIG");
-  if (env != nullptr && sscanf(env, "kernel=%31[^,],splits=%d", o.kernel, &o.splits) < 1) o.kernel[0] = 0;
+  if (env != nullptr && sscanf(env, "kernel=%31[^,],splits=%d,groups=%d", o.kernel, &o.splits, &o.groups) < 1) o.kernel[0] = 0;
   return o;
 }
 
 struct TilePlan {
   int bm;  // 256, 128, 64 (no copies of operands), or 0: the kernel for any size
   bool deep;
+  int groups;  // of four waves that share a 64 x 64 tile's steps
   int splits, ksplit;
 };
 
@@ -156,10 +157,12 @@ struct TilePlan {
 // and some start and end, but no less than reading the operands once; splits add their sums' way to memory and back
 // and a launch.  64 x 64 tiles run three to a CU, and read operands of odd rows (every line twice) at 0.9 us
 // a step for 0.65: x[1000, 2001], two of 4001 rows, 90 us, in copies 67; x[333, 2050] by 1001 rows of codes 11.4 and 26.6,
-// x[100, 1024], two of 1024, 8.5 for 10.0.
+// x[100, 1024], two of 1024, 8.5 for 10.0.  Where they are alone on their CUs two groups of waves share a tile's steps (256 x
+// 4096 x 4096 of codes 14.8 -> 12.5 us, 128 x 4096 x 4096 14.1 -> 11.7, dx[64, 1024] 17.4 -> 14.6; four groups: no faster; but
+// 8 steps 8.9 -> 11.9, and 2 tiles on some CUs no longer fit at once).
 TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch, double copy_us, bool small_ok) {
   const Override o = read_override();
-  TilePlan best{0, false, 1, (int)steps};
+  TilePlan best{0, false, 1, 1, (int)steps};
   double least = 1e30;
   auto consider = [&](int bm) {
     if ((bm == 64 && !small_ok) || (o.tiles() && atoi(strchr(o.kernel, 'x') - (bm == 64 ? 2 : 3)) != bm)) return;
@@ -171,6 +174,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t b
       const int64_t wgs = tiles * s;
       if (wgs > kMostThreads / 512) break;
       bool deep = false;
+      int groups = 1;
       double t = 0;
       if (bm == 256) {
         t += (double)cdiv(wgs, 256) * (each * 1.6 + 6.0);
@@ -179,19 +183,21 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t b
         const int64_t full = wgs / 512, rest = wgs % 512;
         t += (double)full * (each * 0.98 + 5.0);
         if (rest > 256) t += each * 0.98 + 5.0;
-        else if (rest > 0) t += each * (deep ? 0.46 : 0.70) + 4.0;
+        else if (rest > 0) t += each * (!deep ? 0.70 : rest > 128 ? 0.40 : 0.33) + 5.0;
       } else {
+        groups = wgs <= 256 && each >= 16 ? 2 : 1;
+        if (o.groups > 0) groups = o.groups == 2 ? 2 : 1;
         const int64_t full = wgs / 768, rest = wgs % 768;
         const double busy = copy_us > 0 ? 0.9 : 0.65;
         t += (double)full * (each * busy + 4.0);
-        if (rest > 0) t += each * (rest > 512 ? busy : rest > 256 ? 0.5 : 0.36) + 4.0;
+        if (rest > 0) t += each * (rest > 512 ? busy : rest > 256 ? 0.47 : groups == 2 ? 0.21 : 0.28) + 4.0;
       }
       t = std::max(t, (double)batch * (M + N * products) * steps * 128 / 4.5e6);
       if (bm > 64) t += copy_us;
       if (s > 1) t += 4.0 + (double)s * batch * M * N * products * 8.0 / 5e6;
       if (t < least) {
         least = t;
-        best = TilePlan{bm, deep, (int)s, (int)each};
+        best = TilePlan{bm, deep, groups, (int)s, (int)each};
       }
     }
   };
@@ -222,7 +228,7 @@ hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* large, const Tile
   ProjSmallLaunch* small = dtype == CMPEXT3_F16    ? launch_projection_small_f16
                            : dtype == CMPEXT3_BF16 ? launch_projection_small_bf16
                                                    : launch_projection_small_int8;
-  const hipError_t e = t.bm == 64 ? small(mode, p, s) : large(p, t.bm, t.deep, s);
+  const hipError_t e = t.bm == 64 ? small(mode, p, t.groups, s) : large(p, t.bm, t.deep, s);
   return e != hipSuccess || t.splits == 1 ? e : launch_projection_join(dtype, mode, p, s);
 }
 
@@ -455,7 +461,7 @@ extern "C" int cmpext3_projection_describe(const cmpext3_projection_args* a, cha
   else if (q.kernel != kTile)
     snprintf(buf, (size_t)buflen, "kernel=%s%s", q.kernel == kRows ? "rows" : "any64x64", q.make_inside ? " codes=inside" : "");
   else
-    snprintf(buf, (size_t)buflen, "kernel=%s%dx%d%s splits=%d copies=%d", q.tile.bm == 64 ? "small" : "tile", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.splits,
+    snprintf(buf, (size_t)buflen, "kernel=%s%dx%d%s groups=%d splits=%d copies=%d", q.tile.bm == 64 ? "small" : "tile", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.groups, q.tile.splits,
              (q.x.copy_at >= 0) + (q.w[0].copy_at >= 0) + (q.w[1].copy_at >= 0));
   return CMPEXT3_OK;
 }

@@ -59,7 +59,8 @@ ProjTileLaunch launch_projection_tile_wgrad_f16, launch_projection_tile_wgrad_bf
 ProjTileLaunch launch_projection_tile_int8_plain, launch_projection_tile_int8_gated;
 // Tiles of 64 x 64, operands of any alignment whose rows have at least 16 bytes (sum and plain: see the modes' layouts
 // above; gradients have a across k or b as [K, N] as the large tiles do).
-using ProjSmallLaunch = hipError_t(ProjMode mode, const ProjParams& p, hipStream_t s);
+// groups: 1 or 2 of four waves share a tile's steps.
+using ProjSmallLaunch = hipError_t(ProjMode mode, const ProjParams& p, int groups, hipStream_t s);
 ProjSmallLaunch launch_projection_small_f16, launch_projection_small_bf16, launch_projection_small_int8;
 // Adds the splits' sums in their order and finishes the results as an unsplit kernel does.
 hipError_t launch_projection_join(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);

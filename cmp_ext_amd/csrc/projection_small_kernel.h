@@ -24,85 +24,74 @@ __device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
   return __builtin_bit_cast(u32x4, x);
 }
 
-// One operand's share of a thread: two 16-byte pieces of each step.
+// One operand's share of a thread: two 16-byte pieces of each step, in rows r and r + 32 of its tile (of the
+// step, across).  Addresses are a scalar base that moves with the steps and 32-bit offsets within the tile.
 template <int ESZ, bool ACROSS>
 struct SmallOperand {
-  const char* row[2];  // along k: the piece's row; across: the operand's start
-  int64_t ld;          // bytes of a row
-  int64_t length;      // bytes of a row that are the operand's
-  int K;
-  uint32_t lds[2];
-  int at[2];    // bytes within a row: along k, of the step; across, of the row
-  int k[2];     // across: row of the step
-  bool edge;    // across: the tile reaches past the last column
+  const char* base;  // along k: the tile's first row; across: the operand
+  int64_t ld;        // bytes of a row
+  int length, K;     // bytes of a row that are the operand's; its k
+  uint32_t off[2];   // along k: of the pieces' rows
+  int r, at;         // across: row of the step; bytes within a row: along k, of the step
+  uint32_t lds;
+  bool edge;  // across: the tile reaches past the last column
 
+  __device__ __forceinline__ void place(const char* first_row, int64_t pitch, int length_, int K_) {
+    base = first_row;
+    ld = pitch * ESZ;
+    length = length_;
+    K = K_;
+    r = (threadIdx.x % 256) >> 3;
+    at = 16 * (threadIdx.x & 7);
+    lds = ACROSS ? kn128_off(r, at) : lds_off128(r, at >> 4);  // 32 rows on: 4096 bytes
+    edge = false;
+  }
   // rows: of the operand along k, or its columns across it; first: the tile's first one
   __device__ __forceinline__ void init(const void* p, int64_t pitch, int rows, int first, int K_) {
-    ld = pitch * ESZ;
-    K = K_;
-    edge = false;
+    if constexpr (ACROSS) {
+      place((const char*)p, pitch, rows * ESZ, K_);
+      at += first * ESZ;  // 64 columns of 2 bytes: 128 bytes
+      edge = first + kSmallTile > rows;
+    } else {
+      place((const char*)p + first * (pitch * ESZ), pitch, K_ * ESZ, K_);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = threadIdx.x + 256 * i, r = q >> 3, chunk = q & 7;
-      if constexpr (ACROSS) {
-        length = (int64_t)rows * ESZ;
-        row[i] = (const char*)p;
-        k[i] = r;
-        at[i] = first * ESZ + 16 * chunk;  // 64 columns of 2 bytes: 128 bytes
-        lds[i] = kn128_off(r, 16 * chunk);
-        edge = first + kSmallTile > rows;
-      } else {
-        length = (int64_t)K * ESZ;
-        row[i] = (const char*)p + (int64_t)min(first + r, rows - 1) * ld;
-        k[i] = 0;
-        at[i] = 16 * chunk;
-        lds[i] = lds_off128(r, chunk);
-      }
+      for (int i = 0; i < 2; ++i) off[i] = (uint32_t)(min(r + 32 * i, rows - 1 - first) * ld);
     }
   }
-  // gated: rows 0..15 of every 32 of the tile are of the first weight, the others the same rows of the second
-  __device__ __forceinline__ void init_pair(const ProjParams& p, int first) {
+  // gated: rows 0..15 of every 32 of the tile are of the first weight (waves 0 and 1), the others the same rows of
+  // the second
+  __device__ __forceinline__ void init_pair(const ProjParams& p, int first, int wave) {
     static_assert(!ACROSS, "weights along k");
-    K = p.K;
-    length = (int64_t)K * ESZ;
-    edge = false;
+    const int which = wave >> 1;
+    place((const char*)p.b[which] + first * (p.ldb[which] * ESZ), p.ldb[which], p.K * ESZ, p.K);
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int q = threadIdx.x + 256 * i, r = q >> 3, chunk = q & 7;
-      const bool second = (r >> 4) & 1;
-      const int64_t n = min(first + (r >> 5) * 16 + (r & 15), p.N - 1);
-      row[i] = (const char*)(second ? p.b[1] : p.b[0]) + n * (second ? p.ldb[1] : p.ldb[0]) * ESZ;
-      k[i] = 0;
-      at[i] = 16 * chunk;
-      lds[i] = lds_off128(r, chunk);
-    }
+    for (int i = 0; i < 2; ++i) off[i] = (uint32_t)(min((r & 15) + 16 * i, p.N - 1 - first) * ld);
   }
   __device__ __forceinline__ void load(u32x4* v, int step) const {
+    if constexpr (ACROSS) {
+      const int k0 = step * (128 / ESZ);
+      const char* row0 = base + k0 * ld;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      if constexpr (ACROSS) {
-        const int64_t kk = min((int64_t)step * (128 / ESZ) + k[i], (int64_t)K - 1);
-        v[i] = *(const u32x4_any*)(row[i] + kk * ld + min((int64_t)at[i], length - 16));
-      } else {
-        v[i] = *(const u32x4_any*)(row[i] + min((int64_t)step * 128 + at[i], length - 16));
-      }
+      for (int i = 0; i < 2; ++i)
+        v[i] = *(const u32x4_any*)(row0 + (uint32_t)(min(r + 32 * i, K - 1 - k0) * (int)ld + min(at, length - 16)));
+    } else {
+      const uint32_t from = (uint32_t)min(step * 128 + at, length - 16);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] = *(const u32x4_any*)(base + (off[i] + from));
     }
   }
   // whether pieces of the step run past their row or the last k (the same for the whole workgroup)
-  __device__ __forceinline__ bool cut(int step) const {
-    return edge || (step + 1) * (int64_t)(128 / ESZ) > K;
-  }
+  __device__ __forceinline__ bool cut(int step) const { return edge || (step + 1) * (128 / ESZ) > K; }
   template <bool CUT>
   __device__ __forceinline__ void store(unsigned char* slot, const u32x4* v, int step) const {
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       u32x4 x = v[i];
       if constexpr (CUT) {
-        const int64_t from = (ACROSS ? 0 : (int64_t)step * 128) + at[i];
-        x = drop_bytes(x, (int)min(max(from + 16 - length, (int64_t)0), (int64_t)16));
-        if (ACROSS && (int64_t)step * (128 / ESZ) + k[i] >= K) x = u32x4{0, 0, 0, 0};
+        x = drop_bytes(x, min(max((ACROSS ? 0 : step * 128) + at + 16 - length, 0), 16));
+        if (ACROSS && step * (128 / ESZ) + r + 32 * i >= K) x = u32x4{0, 0, 0, 0};
       }
-      *(u32x4*)(slot + lds[i]) = x;
+      *(u32x4*)(slot + lds + 4096 * i) = x;
     }
   }
 };
@@ -124,15 +113,18 @@ __device__ __forceinline__ void store_four(void* out, int64_t row_at, int n, int
     if (n + e < N) store_elem(out, row_at + n + e, dtype, y[e]);
 }
 
-template <typename T, int MODE, bool AKM, bool BKN, int DEPTH, bool SPLITK>
-__global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams p) {
+// GROUPS: of four waves, which take a tile's steps in turn; their sums are added at the end.
+template <typename T, int MODE, bool AKM, bool BKN, int DEPTH, int GROUPS, bool SPLITK>
+__global__ void __launch_bounds__(256 * GROUPS) projection_small_kernel(const ProjParams p) {
   using Acc = typename Prod<T>::Acc;
   constexpr bool GATED = MODE == kProjGated, SUM = MODE == kProjSum;
   constexpr int ESZ = sizeof(T), BK = 128 / ESZ;
   constexpr int COLS = GATED ? 32 : 64;  // of results
-  __shared__ __attribute__((aligned(1024))) unsigned char smem[2][2][kSmallTile * 128];
+  __shared__ __attribute__((aligned(1024))) unsigned char slots[GROUPS][2][2][kSmallTile * 128];
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int group = GROUPS > 1 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 8) : 0;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  auto& smem = slots[group];
   const int r16 = lane & 15, G = lane >> 4;
   const int wm = 32 * (wave >> 1), wn = 32 * (wave & 1);
   int tm, tn, bzi;
@@ -149,7 +141,7 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
   SmallOperand<ESZ, BKN> b[SUM ? 2 : 1];
   a[0].init(p.a[SUM ? 0 : bz], p.lda, p.M, m0, p.K);
   if constexpr (GATED)
-    b[0].init_pair(p, n0);
+    b[0].init_pair(p, n0, wave);
   else
     b[0].init(p.b[0], p.ldb[0], p.N, n0, p.K);
   if constexpr (SUM) {
@@ -167,14 +159,15 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
       b[0].load(vb[d], step);
     }
   };
-  auto store = [&](int d, int kt) {  // both parts' rows lie alike
+  auto store = [&](int d, int r) {  // both parts' rows lie alike
+    const int kt = GROUPS * r + group;
     const int step = SUM && first + kt >= part_steps ? first + kt - part_steps : first + kt;
     if (a[0].cut(step) || b[0].cut(step)) {
-      a[0].template store<true>(smem[kt & 1][0], va[d], step);
-      b[0].template store<true>(smem[kt & 1][1], vb[d], step);
+      a[0].template store<true>(smem[r & 1][0], va[d], step);
+      b[0].template store<true>(smem[r & 1][1], vb[d], step);
     } else {
-      a[0].template store<false>(smem[kt & 1][0], va[d], step);
-      b[0].template store<false>(smem[kt & 1][1], vb[d], step);
+      a[0].template store<false>(smem[r & 1][0], va[d], step);
+      b[0].template store<false>(smem[r & 1][1], vb[d], step);
     }
   };
 
@@ -206,9 +199,9 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
   Acc acc[2][2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = Prod<T>::zero();
-  auto multiply = [&](int kt) {
-    const unsigned char* ta = smem[kt & 1][0];
-    const unsigned char* tb = smem[kt & 1][1];
+  auto multiply = [&](int r) {
+    const unsigned char* ta = smem[r & 1][0];
+    const unsigned char* tb = smem[r & 1][1];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       u32x4 fa[2], fb[2];
@@ -221,30 +214,58 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
       for (int i = 0; i < 4; ++i) acc[i >> 1][i & 1] = Prod<T>::mma(fb[i & 1], fa[i >> 1], acc[i >> 1][i & 1]);
     }
   };
-  // past the end the last step is loaded again and not used: a load under a condition would make the compiler
-  // wait for all that are on their way
+  // Round r is step GROUPS r + group.  Past the end the last step is loaded again and not used: a load under a
+  // condition would make the compiler wait for all that are on their way.
+  auto load_round = [&](int d, int r) { load(d, min(GROUPS * r + group, nk - 1)); };
   if (nk > 0) {
 #pragma unroll
     for (int d = 0; d < DEPTH; ++d) {
-      load(d, min(d, nk - 1));
+      load_round(d, d);
       __builtin_amdgcn_sched_barrier(0);  // in this order, as the loop waits for them
     }
   }
-  auto step = [&](int d, int kt, auto more) {
-    store(d, kt);
-    if constexpr (decltype(more)::value) load(d, min(kt + DEPTH, nk - 1));
+  auto fence = [] {
     // this wave's part of the slot is written; every wave is past its reads of the slot before
     asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" : : : "memory");
-    multiply(kt);
   };
-  int kt = 0;
-  for (; kt + DEPTH <= nk; kt += DEPTH) {
+  const int whole = nk / GROUPS, rounds = (nk + GROUPS - 1) / GROUPS;  // whole: every group has a step
+  int r = 0;
+  for (; r + DEPTH <= whole; r += DEPTH) {
 #pragma unroll
-    for (int d = 0; d < DEPTH; ++d) step(d, kt + d, std::true_type{});
+    for (int d = 0; d < DEPTH; ++d) {
+      store(d, r + d);
+      load_round(d, r + d + DEPTH);
+      fence();
+      multiply(r + d);
+    }
   }
 #pragma unroll
-  for (int d = 0; d < DEPTH - 1; ++d)
-    if (kt + d < nk) step(d, kt + d, std::false_type{});
+  for (int d = 0; d < DEPTH; ++d) {
+    if (r + d >= rounds) break;
+    const bool mine = GROUPS * (r + d) + group < nk;
+    if (mine) store(d, r + d);
+    fence();
+    if (mine) multiply(r + d);
+  }
+
+  // ---- sums of the groups, in their order: group g < 2 then holds rows 16g .. of the wave's block ----
+  constexpr int I = GROUPS > 1 ? 1 : 2;  // row blocks that a group finishes
+  if constexpr (GROUPS > 1) {
+    Acc* sums = (Acc*)slots;  // [group][block][wave][lane]
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < 4; ++x) sums[((group * 4 + x) * 4 + wave) * 64 + lane] = acc[x >> 1][x & 1];
+    __syncthreads();
+    if (group >= 2) return;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+      Acc sum = sums[((2 * group + j) * 4 + wave) * 64 + lane];
+#pragma unroll
+      for (int g = 1; g < GROUPS; ++g) sum += sums[((g * 4 + 2 * group + j) * 4 + wave) * 64 + lane];
+      acc[0][j] = sum;
+    }
+  }
+  const int i0 = GROUPS > 1 ? group : 0;
 
   // ---- acc[i][j][e]: row 16i + r16, B tile row 16j + 4G + e of the wave's block ----
   const int nw = n0 + (GATED ? wn / 2 : wn) + 4 * G;
@@ -252,8 +273,8 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
     constexpr int NP = GATED ? 2 : 1;
     uint32_t* part = (uint32_t*)p.partials + ((int64_t)ks * p.batch + bz) * NP * p.M * p.ld_part;
 #pragma unroll
-    for (int x = 0; x < 4; ++x) {
-      const int64_t m = m0 + wm + 16 * (x >> 1) + r16;
+    for (int x = 0; x < 2 * I; ++x) {
+      const int64_t m = m0 + wm + 16 * (i0 + (x >> 1)) + r16;
       const int n = nw + (GATED ? 0 : 16 * (x & 1));
       if (m < p.M && n < p.N)
         *(u32x4*)(part + ((GATED ? (x & 1) * (int64_t)p.M : 0) + m) * p.ld_part + n) = __builtin_bit_cast(u32x4, acc[x >> 1][x & 1]);
@@ -261,8 +282,8 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
     return;
   }
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int64_t m = m0 + wm + 16 * i + r16;
+  for (int i = 0; i < I; ++i) {
+    const int64_t m = m0 + wm + 16 * (i0 + i) + r16;
     if (m >= p.M) continue;
     const float as = ESZ == 1 ? p.a_scale[m] : 1.f;
     f32x4 v[2];
@@ -298,10 +319,14 @@ __global__ void __launch_bounds__(256) projection_small_kernel(const ProjParams 
 }
 
 template <typename T, int MODE, bool AKM, bool BKN>
-hipError_t launch_projection_small(const ProjParams& p, hipStream_t s) {
-  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)(p.batch * p.splits)), block(256);
-  if (p.splits > 1) return launch_kernel((projection_small_kernel<T, MODE, AKM, BKN, 3, true>), grid, block, 0, s, p);
-  return launch_kernel((projection_small_kernel<T, MODE, AKM, BKN, 3, false>), grid, block, 0, s, p);
+hipError_t launch_projection_small(const ProjParams& p, int groups, hipStream_t s) {
+  const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)(p.batch * p.splits)), block(256 * groups);
+  if (p.splits > 1) {
+    if (groups == 2) return launch_kernel((projection_small_kernel<T, MODE, AKM, BKN, 3, 2, true>), grid, block, 0, s, p);
+    return launch_kernel((projection_small_kernel<T, MODE, AKM, BKN, 3, 1, true>), grid, block, 0, s, p);
+  }
+  if (groups == 2) return launch_kernel((projection_small_kernel<T, MODE, AKM, BKN, 3, 2, false>), grid, block, 0, s, p);
+  return launch_kernel((projection_small_kernel<T, MODE, AKM, BKN, 3, 1, false>), grid, block, 0, s, p);
 }
 
 }  // namespace cmpext3
