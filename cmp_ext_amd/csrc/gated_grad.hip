@@ -24,9 +24,9 @@ __global__ void __launch_bounds__(256) gated_grad_kernel(const GatedGradParams p
   u32x4 d = {0, 0, 0, 0};
   f32x4 g[2], u[2];
   if (n + 8 <= p.N) {
-    d = *(const u32x4_e*)grad;
+    d = __builtin_nontemporal_load((const u32x4_e*)grad);
 #pragma unroll
-    for (int h = 0; h < 2; ++h) g[h] = *(const f32x4_e*)(gate + 4 * h), u[h] = *(const f32x4_e*)(up + 4 * h);
+    for (int h = 0; h < 2; ++h) g[h] = __builtin_nontemporal_load((const f32x4_e*)(gate + 4 * h)), u[h] = __builtin_nontemporal_load((const f32x4_e*)(up + 4 * h));
   } else {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {

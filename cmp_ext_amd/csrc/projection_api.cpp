@@ -128,14 +128,14 @@ hipError_t run_copy(Operand* o, size_t esz, char* ws, hipStream_t s) {
   return e;
 }
 
-// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows|small64x64|tile128x128|tile256x256>[,splits=<s>
+// Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows|small64x64|tile128x128|tile256x128|tile256x256>[,splits=<s>
 // [,groups=<g>]]" replaces the plan's choice wherever that kernel can run.  For sweeps and tests: read on every plan,
 // ignored where malformed.
 struct Override {
   char kernel[32];
   int splits, groups;
   bool is(const char* name) const { return strcmp(kernel, name) == 0; }
-  bool tiles() const { return is("small64x64") || is("tile128x128") || is("tile256x256"); }
+  bool tiles() const { return is("small64x64") || is("tile128x128") || is("tile256x128") || is("tile256x256"); }
 };
 Override read_override() {
   Override o{};
@@ -145,14 +145,14 @@ Override read_override() {
 }
 
 struct TilePlan {
-  int bm;  // 256, 128, 64 (no copies of operands), or 0: the kernel for any size
+  int bm, bn;  // 256 x 256, 256 x 128, 128 x 128, 64 x 64 (no copies of operands), or 0: the kernel for any size
   bool deep;
   int groups;  // of four waves that share a 64 x 64 tile's steps
   int splits, ksplit;
 };
 
 // Which tiles, and in how many splits of the steps of 128 bytes of k, for M x N results (of `products` products)
-// in `batch` entries; copy_us: what the large tiles' copies of operands take (0: none).  Modelled microseconds, fitted
+// in `batch` entries; copy_us: what the large tiles' copies of operands take (0: none); along: both operands along k.  Modelled microseconds, fitted
 // to timings of 27 shapes with every tile and 1, 2, 4 and 8 splits (MI355X): a round of workgroups takes its steps
 // and some start and end, but no less than reading the operands once; splits add their sums' way to memory and back
 // and a launch.  64 x 64 tiles run three to a CU, and read operands of odd rows (every line twice) at 0.9 us
@@ -160,13 +160,13 @@ struct TilePlan {
 // x[100, 1024], two of 1024, 8.5 for 10.0.  Where they are alone on their CUs two groups of waves share a tile's steps (256 x
 // 4096 x 4096 of codes 14.8 -> 12.5 us, 128 x 4096 x 4096 14.1 -> 11.7, dx[64, 1024] 17.4 -> 14.6; four groups: no faster; but
 // 8 steps 8.9 -> 11.9, and 2 tiles on some CUs no longer fit at once).
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch, double copy_us, bool small_ok) {
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch, double copy_us, bool small_ok, bool along) {
   const Override o = read_override();
-  TilePlan best{0, false, 1, 1, (int)steps};
+  TilePlan best{0, 0, false, 1, 1, (int)steps};
   double least = 1e30;
-  auto consider = [&](int bm) {
-    if ((bm == 64 && !small_ok) || (o.tiles() && atoi(strchr(o.kernel, 'x') - (bm == 64 ? 2 : 3)) != bm)) return;
-    const int64_t tiles = cdiv(M, bm) * cdiv(N, bm / products) * batch;
+  auto consider = [&](int bm, int bn, const char* name) {
+    if ((bm == 64 && !small_ok) || (bm != bn && !along) || (o.tiles() && !o.is(name))) return;
+    const int64_t tiles = cdiv(M, bm) * cdiv(N, bn / products) * batch;
     for (int64_t s = 1; s <= 16 && (s == 1 || (s * 4 <= steps && bm < 256)); ++s) {
       const int64_t each = cdiv(steps, s);
       if (s > 1 && (s - 1) * each >= steps) continue;  // an empty split
@@ -177,7 +177,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t b
       int groups = 1;
       double t = 0;
       if (bm == 256) {
-        t += (double)cdiv(wgs, 256) * (each * 1.6 + 6.0);
+        t += (double)cdiv(wgs, 256) * (bn == 256 ? each * 1.6 + 6.0 : each * 0.66 + 4.0);
       } else if (bm == 128) {
         deep = wgs <= 256 && each >= 8;
         const int64_t full = wgs / 512, rest = wgs % 512;
@@ -192,18 +192,19 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t b
         t += (double)full * (each * busy + 4.0);
         if (rest > 0) t += each * (rest > 512 ? busy : rest > 256 ? 0.47 : groups == 2 ? 0.21 : 0.28) + 4.0;
       }
-      t = std::max(t, (double)batch * (M + N * products) * steps * 128 / 4.5e6);
+      t = std::max(t, (double)batch * (M + N * products) * steps * 128 / (bm == bn ? 4.5e6 : 3.7e6));
       if (bm > 64) t += copy_us;
       if (s > 1) t += 4.0 + (double)s * batch * M * N * products * 8.0 / 5e6;
       if (t < least) {
         least = t;
-        best = TilePlan{bm, deep, groups, (int)s, (int)each};
+        best = TilePlan{bm, bn, deep, groups, (int)s, (int)each};
       }
     }
   };
-  consider(256);
-  consider(128);
-  consider(64);
+  consider(256, 256, "tile256x256");
+  consider(256, 128, "tile256x128");
+  consider(128, 128, "tile128x128");
+  consider(64, 64, "small64x64");
   return best;
 }
 
@@ -219,7 +220,7 @@ double copy_us(const Operand& o, size_t esz) { return rows_of_16(o, esz) ? 0.0 :
 hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* large, const TilePlan& t, ProjParams& p, void* partials, hipStream_t s) {
   const int products = mode == kProjGated ? 2 : 1;
   p.tiles_m = (int)cdiv(p.M, t.bm);
-  p.tiles_n = (int)cdiv(p.N, t.bm / products);
+  p.tiles_n = (int)cdiv(p.N, t.bn / products);
   p.group_m = 4;
   p.splits = t.splits;
   p.ksplit = t.ksplit;
@@ -228,7 +229,7 @@ hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* large, const Tile
   ProjSmallLaunch* small = dtype == CMPEXT3_F16    ? launch_projection_small_f16
                            : dtype == CMPEXT3_BF16 ? launch_projection_small_bf16
                                                    : launch_projection_small_int8;
-  const hipError_t e = t.bm == 64 ? small(mode, p, t.groups, s) : large(p, t.bm, t.deep, s);
+  const hipError_t e = t.bm == 64 ? small(mode, p, t.groups, s) : large(p, t.bm, t.bn, t.deep, s);
   return e != hipSuccess || t.splits == 1 ? e : launch_projection_join(dtype, mode, p, s);
 }
 
@@ -282,7 +283,7 @@ int plan_projection(const cmpext3_projection_args* a, ProjPlan* q) {
   }
   double copies = copy_us(q->x, esz);
   for (int i = 0; i < products; ++i) copies += copy_us(q->w[i], esz);
-  q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1, copies, true);
+  q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1, copies, true, true);
   if (q->tile.bm == 0) return CMPEXT3_OK;
   q->kernel = kTile;
   if (q->tile.bm > 64) {
@@ -364,13 +365,13 @@ int plan_backward(const cmpext3_gated_backward_args* a, BackwardPlan* q) {
   // the small tiles read 16 bytes of a row at least: of x and the weights, and of dgate's and dup's N
   const bool rows16 = a->K >= 8 && a->N >= 8;
   if (a->dx != nullptr) {
-    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1, copy_us(q->w[0], 2) + copy_us(q->w[1], 2), rows16);
+    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1, copy_us(q->w[0], 2) + copy_us(q->w[1], 2), rows16, false);
     if (q->dx.bm > 64)
       for (Operand& w : q->w) plan_copy(&w, 2, &q->ws_bytes);
     partials = partial_bytes(q->dx, a->M, a->K, 1, 1);
   }
   if (batch > 0) {
-    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch, copy_us(q->x, 2), rows16);
+    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch, copy_us(q->x, 2), rows16, false);
     if (q->dw.bm > 64) plan_copy(&q->x, 2, &q->ws_bytes);
     partials = std::max(partials, partial_bytes(q->dw, a->N, a->K, 1, batch));
   }
@@ -461,7 +462,7 @@ extern "C" int cmpext3_projection_describe(const cmpext3_projection_args* a, cha
   else if (q.kernel != kTile)
     snprintf(buf, (size_t)buflen, "kernel=%s%s", q.kernel == kRows ? "rows" : "any64x64", q.make_inside ? " codes=inside" : "");
   else
-    snprintf(buf, (size_t)buflen, "kernel=%s%dx%d%s groups=%d splits=%d copies=%d", q.tile.bm == 64 ? "small" : "tile", q.tile.bm, q.tile.bm, q.tile.deep ? " ring=4" : "", q.tile.groups, q.tile.splits,
+    snprintf(buf, (size_t)buflen, "kernel=%s%dx%d%s groups=%d splits=%d copies=%d", q.tile.bm == 64 ? "small" : "tile", q.tile.bm, q.tile.bn, q.tile.deep ? " ring=4" : "", q.tile.groups, q.tile.splits,
              (q.x.copy_at >= 0) + (q.w[0].copy_at >= 0) + (q.w[1].copy_at >= 0));
   return CMPEXT3_OK;
 }

@@ -230,14 +230,9 @@ Tensor int8_gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_
   return int8_projection(x, w_gate, gate_scale, w_up, up_scale, c10::nullopt, x_scale, dtype, activation_code(activation, op), op);
 }
 
-// fp32 rows of whole 32 bytes, of which the first n elements are the tensor: kernels store and read
-// them in pieces of 16 wherever n itself is odd.
-Tensor padded_rows(int64_t rows, int64_t n, const Tensor& like) {
-  return torch::empty({rows, (n + 7) / 8 * 8}, like.options().dtype(at::kFloat)).narrow(1, 0, n);
-}
-
-// act(x w_gate^T) * (x w_up^T), and both products where `keep` asks for them.
-std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const std::string& activation,
+// act(x w_gate^T) * (x w_up^T), and both products where `keep` asks for them: [2, rows, N rounded up to 8], so that
+// kernels store and read whole pieces wherever N itself is odd.
+std::tuple<Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const std::string& activation,
                                                  bool keep) {
   const char* op = "gated_linear";
   check_operands(x, {&w_gate, &w_up}, op);
@@ -248,7 +243,7 @@ std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& 
   c10::DeviceGuard guard(x.device());
   const Rows rx = rows_of(x), rg = rows_of(w_gate), ru = rows_of(w_up);
   const int64_t N = w_gate.size(0);
-  Tensor out = torch::empty(with_last(x, N), x.options()), gate, up;
+  Tensor out = torch::empty(with_last(x, N), x.options()), pre;
   cmpext3_projection_args a{};
   a.dtype = a.x_dtype = a.out_dtype = dtype_code(x.scalar_type());
   a.activation = act;
@@ -263,30 +258,28 @@ std::tuple<Tensor, Tensor, Tensor> gated_forward(const Tensor& x, const Tensor& 
   a.out = out.data_ptr();
   a.out_row = std::max<int64_t>(N, 1);
   if (keep) {
-    gate = padded_rows(rx.rows, N, x);
-    up = padded_rows(rx.rows, N, x);
-    a.gate_out = (float*)gate.data_ptr();
-    a.up_out = (float*)up.data_ptr();
-    a.pre_row = std::max<int64_t>(gate.stride(0), 1);
+    const int64_t pitch = (N + 7) / 8 * 8;
+    pre = torch::empty({2, rx.rows, pitch}, x.options().dtype(at::kFloat));
+    a.gate_out = (float*)pre.data_ptr();
+    a.up_out = a.gate_out + rx.rows * pitch;
+    a.pre_row = pitch;
   }
   if (out.numel() > 0) run_projection(a, x, op);
-  return {out, gate, up};
+  return {out, pre};
 }
 
 // Gradients of x and of both weights, each only where asked for.
 std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& grad, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
-                                                  const Tensor& gate, const Tensor& up, const std::string& activation, bool want_x,
-                                                  bool want_gate, bool want_up) {
+                                                  const Tensor& pre, const std::string& activation, bool want_x, bool want_gate,
+                                                  bool want_up) {
   const char* op = "gated_linear (backward)";
   check_operands(x, {&w_gate, &w_up}, op);
   check_device(grad, x, op, "gradient");
   TORCH_CHECK(grad.scalar_type() == x.scalar_type(), "cmpext3.", op, ": dtype mismatch of the gradient, ", grad.scalar_type());
   c10::DeviceGuard guard(x.device());
   const Rows rx = rows_of(x), rd = rows_of(grad), rg = rows_of(w_gate), ru = rows_of(w_up);
-  const Rows pg = rows_of(gate), pu = rows_of(up);
   const int64_t N = w_gate.size(0), K = w_gate.size(1);
-  TORCH_CHECK(rd.rows == rx.rows && rd.cols == N && pg.rows == rx.rows && pg.cols == N && pu.rows == rx.rows && pu.cols == N &&
-                  gate.scalar_type() == at::kFloat && up.scalar_type() == at::kFloat && (rx.rows <= 1 || pg.pitch == pu.pitch),
+  TORCH_CHECK(rd.rows == rx.rows && rd.cols == N,
               "cmpext3.", op, ": shape mismatch of the gradient ", grad.sizes());
   Tensor dx, dgate, dup;
   cmpext3_gated_backward_args a{};
@@ -297,9 +290,9 @@ std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& grad, const Tens
   a.K = checked_int(K, op, "the row length");
   a.grad_out = rd.t.data_ptr();
   a.grad_row = rd.pitch;
-  a.gate = (const float*)pg.t.data_ptr();
-  a.up = (const float*)pu.t.data_ptr();
-  a.pre_row = pg.pitch;
+  a.gate = (const float*)pre.data_ptr();
+  a.up = a.gate + rx.rows * pre.size(2);
+  a.pre_row = pre.size(2);
   a.x = rx.t.data_ptr();
   a.x_row = rx.pitch;
   a.w_gate = rg.t.data_ptr();
@@ -354,9 +347,9 @@ void check_capture(std::initializer_list<const Tensor*> leaves) {
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static Tensor forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& w_gate, const Tensor& w_up,
                         const std::string& activation) {
-    Tensor out, gate, up;
-    std::tie(out, gate, up) = gated_forward(x, w_gate, w_up, activation, true);
-    ctx->save_for_backward({x, w_gate, w_up, gate, up});
+    Tensor out, pre;
+    std::tie(out, pre) = gated_forward(x, w_gate, w_up, activation, true);
+    ctx->save_for_backward({x, w_gate, w_up, pre});
     ctx->saved_data["activation"] = activation;
     return out;
   }
@@ -364,7 +357,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     if (!grads[0].defined()) return {Tensor(), Tensor(), Tensor(), Tensor()};
     const auto saved = ctx->get_saved_variables();
     Tensor dx, dgate, dup;
-    std::tie(dx, dgate, dup) = gated_backward(grads[0], saved[0], saved[1], saved[2], saved[3], saved[4],
+    std::tie(dx, dgate, dup) = gated_backward(grads[0], saved[0], saved[1], saved[2], saved[3],
                                               ctx->saved_data["activation"].toStringRef(), ctx->needs_input_grad(0),
                                               ctx->needs_input_grad(1), ctx->needs_input_grad(2));
     return {dx, dgate, dup, Tensor()};

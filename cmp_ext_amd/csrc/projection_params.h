@@ -50,9 +50,9 @@ hipError_t launch_projection_rows(int dtype, ProjMode mode, const ProjParams& p,
 constexpr int kRowsCodesRows = 16, kRowsCodesMost = 4096, kRowsCodesUnit = 512;  // rows, elements, of a row a multiple of
 hipError_t launch_projection_rows_codes(int x_dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
 
-// Tiles of bm = 256 or 128 rows; `deep`: alone on a CU, with a ring of four steps.  Operands have rows of
+// Tiles of bm x bn = 256 x 256, 256 x 128 or 128 x 128; `deep` (128 x 128): alone on a CU, with a ring of four steps.  Operands have rows of
 // whole 16 bytes.  (One translation unit for each element type and mode.)
-using ProjTileLaunch = hipError_t(const ProjParams& p, int bm, bool deep, hipStream_t s);
+using ProjTileLaunch = hipError_t(const ProjParams& p, int bm, int bn, bool deep, hipStream_t s);
 ProjTileLaunch launch_projection_tile_gated_f16, launch_projection_tile_gated_bf16;
 ProjTileLaunch launch_projection_tile_sum_f16, launch_projection_tile_sum_bf16;
 ProjTileLaunch launch_projection_tile_wgrad_f16, launch_projection_tile_wgrad_bf16;

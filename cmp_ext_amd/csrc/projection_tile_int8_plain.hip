@@ -2,9 +2,9 @@
 #include "projection_tile_kernel.h"
 
 namespace cmpext3 {
-hipError_t launch_projection_tile_int8_plain(const ProjParams& p, int bm, bool deep, hipStream_t s) {
-  if (p.out_dtype == kF16) return launch_projection_tile<int8_t, _Float16, kProjPlain, false, false>(p, bm, deep, s);
-  if (p.out_dtype == kBF16) return launch_projection_tile<int8_t, __bf16, kProjPlain, false, false>(p, bm, deep, s);
-  return launch_projection_tile<int8_t, float, kProjPlain, false, false>(p, bm, deep, s);
+hipError_t launch_projection_tile_int8_plain(const ProjParams& p, int bm, int bn, bool deep, hipStream_t s) {
+  if (p.out_dtype == kF16) return launch_projection_tile<int8_t, _Float16, kProjPlain, false, false>(p, bm, bn, deep, s);
+  if (p.out_dtype == kBF16) return launch_projection_tile<int8_t, __bf16, kProjPlain, false, false>(p, bm, bn, deep, s);
+  return launch_projection_tile<int8_t, float, kProjPlain, false, false>(p, bm, bn, deep, s);
 }
 }  // namespace cmpext3

@@ -33,10 +33,11 @@ struct ProjTileShape {
   static constexpr int DMA = A_DMA + B_DMA;
   static_assert(WTM % 16 == 0 && WTN % 32 == 0, "16-row blocks, pairs of 16-column blocks");
   static_assert(A_BYTES % (1024 * NW) == 0 && B_BYTES % (1024 * NW) == 0, "whole DMA loads per wave");
-  static_assert(B_DMA % 4 == 0, "a wave's loads alternate between both weights the same way");
+  static_assert(B_DMA % 4 == 0 || B_DMA == 2, "pairs of a wave's loads alternate between both weights, or the waves do");
   static_assert(LDS <= 160 * 1024, "LDS budget");
   static_assert(NS >= 2 && (NS - 1) * DMA <= 63, "vmcnt range");
-  static_assert((NS - 1) * A_BYTES + (AKM ? 36 * A_PITCH : (FM - 1) * 2048) <= 65535 &&
+  // (a ring of three has a second base for its last slot)
+  static_assert(NS == 3 || (NS - 1) * A_BYTES + (AKM ? 36 * A_PITCH : (FM - 1) * 2048) <= 65535 &&
                     (NS - 1) * B_BYTES + (BKN ? 36 * B_PITCH : (FN - 1) * 2048) <= 65535,
                 "immediate LDS offsets");
 };
@@ -110,7 +111,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
       dma128_geom(wave * S::B_DMA + i, lane, row, chunk);
       // gated: rows 0..15 of every 32 are of w_gate, the others the same rows of w_up
       const int col = GATED ? (row >> 5) * 16 + (row & 15) : row;
-      const int64_t ldb = p.ldb[GATED ? (i >> 1) & 1 : 0];
+      const int64_t ldb = p.ldb[GATED ? (S::B_DMA == 2 ? wave & 1 : (i >> 1) & 1) : 0];
       b_off[i] = n0 + col < N ? (uint32_t)(col * ldb + E16 * chunk) * (uint32_t)sizeof(T) : kBufOOB;
       b_kx[i] = E16 * chunk;
     }
@@ -128,6 +129,14 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
   }
   const uint32_t lds_a = lds_addr(smem) + (uint32_t)(wave * S::A_DMA * 1024);
   const uint32_t lds_b = lds_addr(smem) + (uint32_t)(S::B_REGION + wave * S::B_DMA * 1024);
+  // gated: the weight that a wave's loads 0 and 1, and 2 and 3, are of
+  i32x4 rsrc_pair[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    rsrc_pair[i] = make_rsrc_sgpr(Bbase[S::B_DMA == 2 ? wave & 1 : i]);
+    rsrc_pair[i][0] = __builtin_amdgcn_readfirstlane(rsrc_pair[i][0]);
+    rsrc_pair[i][1] = __builtin_amdgcn_readfirstlane(rsrc_pair[i][1]);
+  }
   // LDS-DMA load d (A pieces first, then B) of step kt into ring slot `slot`.  Operands along k keep a
   // descriptor at the tile's base and advance through the scalar offset, operands across it get one per step;
   // a step past the end loads through a descriptor of no records (zeros, no memory read).
@@ -146,12 +155,16 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
       dma_load16_m0(r, voff, AKM ? 0u : (uint32_t)k0 * (uint32_t)sizeof(T), lds_a, std::integral_constant<uint32_t, dst>{});
     } else {
       constexpr int i = d - S::A_DMA;
-      constexpr int which = GATED ? (i >> 1) & 1 : 0;
       constexpr uint32_t dst = (uint32_t)(slot * S::B_BYTES + i * 1024);
       const uint32_t in = SUM && second ? b_off1[SUM ? i : 0] : b_off[i];
       const uint32_t voff = !KCHECK || b_kx[i] < p.K - k0 ? in : kBufOOB;
-      const T* base = second ? Bbase[1] : Bbase[which];
-      i32x4 r = make_rsrc_sgpr(BKN ? base + (int64_t)(live ? k0 : 0) * (second ? p.ldb[1] : p.ldb[0]) : base);
+      i32x4 r;
+      if constexpr (GATED) {
+        r = rsrc_pair[(i >> 1) & 1];
+      } else {
+        const T* base = second ? Bbase[1] : Bbase[0];
+        r = make_rsrc_sgpr(BKN ? base + (int64_t)(live ? k0 : 0) * (second ? p.ldb[1] : p.ldb[0]) : base);
+      }
       r[2] = live ? (int)kBufRecords : 0;
       dma_load16_m0(r, voff, BKN ? 0u : (uint32_t)k0 * (uint32_t)sizeof(T), lds_b, std::integral_constant<uint32_t, dst>{});
     }
@@ -400,9 +413,15 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
 }
 
 // Tiles: 256 x 256 with 8 waves, one workgroup per CU; 128 x 128 with 4 waves, two per CU, or one with
-// a ring of four steps where no CU gets a second (see the plan).
+// a ring of four steps where no CU gets a second (see the plan); and, along k, 256 x 128 with 8 waves and a ring
+// of three steps, for some hundred rows whose weights come from HBM: the time is that of loads on their way (x[256,
+// 4096], two weights of 14336 rows, bf16: 256 x 256 101 us, 128 x 128 85, 256 x 128 with a ring of two 84, of three 68).
 template <typename T, typename O, int MODE, bool AKM, bool BKN, bool KCHECK>
-hipError_t launch_projection_tile_k(const ProjParams& p, int bm, bool deep, dim3 grid, hipStream_t s) {
+hipError_t launch_projection_tile_k(const ProjParams& p, int bm, int bn, bool deep, dim3 grid, hipStream_t s) {
+  if constexpr (!AKM && !BKN) {
+    if (bn == 128 && bm == 256)
+      return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 128, 4, 2, 1, 3, KCHECK, false>), grid, dim3(512), 0, s, p);
+  }
   if (bm == 256)
     return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 256, 4, 2, 1, 2, KCHECK, false>), grid, dim3(512), 0, s, p);
   if (p.splits > 1) {
@@ -416,11 +435,11 @@ hipError_t launch_projection_tile_k(const ProjParams& p, int bm, bool deep, dim3
 }
 
 template <typename T, typename O, int MODE, bool AKM, bool BKN>
-hipError_t launch_projection_tile(const ProjParams& p, int bm, bool deep, hipStream_t s) {
+hipError_t launch_projection_tile(const ProjParams& p, int bm, int bn, bool deep, hipStream_t s) {
   const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), 1, (unsigned)(p.batch * p.splits));
   constexpr int BK = 128 / sizeof(T);
-  if (p.K % BK != 0) return launch_projection_tile_k<T, O, MODE, AKM, BKN, true>(p, bm, deep, grid, s);
-  return launch_projection_tile_k<T, O, MODE, AKM, BKN, false>(p, bm, deep, grid, s);
+  if (p.K % BK != 0) return launch_projection_tile_k<T, O, MODE, AKM, BKN, true>(p, bm, bn, deep, grid, s);
+  return launch_projection_tile_k<T, O, MODE, AKM, BKN, false>(p, bm, bn, deep, grid, s);
 }
 
 }  // namespace cmpext3
