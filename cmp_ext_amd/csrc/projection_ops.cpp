@@ -7,6 +7,8 @@
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+
 #include <string>
 #include <tuple>
 #include <vector>
@@ -360,7 +362,15 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     std::tie(dx, dgate, dup) = gated_backward(grads[0], saved[0], saved[1], saved[2], saved[3],
                                               ctx->saved_data["activation"].toStringRef(), ctx->needs_input_grad(0),
                                               ctx->needs_input_grad(1), ctx->needs_input_grad(2));
-    return {dx, dgate, dup, Tensor()};
+    torch::autograd::variable_list out = {dx, dgate, dup};
+    if (at::GradMode::is_enabled()) {
+      // asked for a graph of the gradients: they have none, and say so when one is taken through them
+      for (Tensor& t : out)
+        if (t.defined()) t = t.detach().requires_grad_();
+      out = (*std::make_shared<torch::autograd::DelayedError>("cmpext3.gated_linear: differentiable once only", 3))(std::move(out));
+    }
+    out.emplace_back();
+    return out;
   }
 };
 

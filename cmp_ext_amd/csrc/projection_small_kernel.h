@@ -248,7 +248,8 @@ __global__ void __launch_bounds__(256 * GROUPS) projection_small_kernel(const Pr
     if (mine) multiply(r + d);
   }
 
-  // ---- sums of the groups, in their order: group g < 2 then holds rows 16g .. of the wave's block ----
+  // ---- sums of the groups, in their order: group g then holds rows 16g .. of the wave's block ----
+  static_assert(GROUPS <= 2, "a group for each of the wave's two row blocks");
   constexpr int I = GROUPS > 1 ? 1 : 2;  // row blocks that a group finishes
   if constexpr (GROUPS > 1) {
     Acc* sums = (Acc*)slots;  // [group][block][wave][lane]
@@ -256,7 +257,6 @@ __global__ void __launch_bounds__(256 * GROUPS) projection_small_kernel(const Pr
 #pragma unroll
     for (int x = 0; x < 4; ++x) sums[((group * 4 + x) * 4 + wave) * 64 + lane] = acc[x >> 1][x & 1];
     __syncthreads();
-    if (group >= 2) return;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
       Acc sum = sums[((2 * group + j) * 4 + wave) * 64 + lane];

@@ -10,10 +10,10 @@
 namespace cmpext3 {
 namespace {
 
-// LANES: of a row, 64 or 256; PER: pieces of 8 elements that a lane holds, 0: the row is read twice.
+// LANES: of a row, 64, 256 or 1024; PER: pieces of 8 elements that a lane holds, 0: the row is read twice.
 template <typename T, int LANES, int PER>
-__global__ void __launch_bounds__(256) quantize_int8_kernel(const QuantParams p) {
-  const int64_t row = (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES;
+__global__ void __launch_bounds__(LANES < 256 ? 256 : LANES) quantize_int8_kernel(const QuantParams p) {
+  const int64_t row = LANES < 256 ? (int64_t)blockIdx.x * (256 / LANES) + threadIdx.x / LANES : blockIdx.x;
   const int t = threadIdx.x % LANES;
   if (LANES == 64 && row >= p.rows) return;  // whole waves
   const T* x = (const T*)p.x + row * p.ldx;
@@ -39,13 +39,13 @@ __global__ void __launch_bounds__(256) quantize_int8_kernel(const QuantParams p)
     const uint32_t b = __shfl_xor(most, d);
     most = most > b ? most : b;
   }
-  if constexpr (LANES == 256) {
-    __shared__ uint32_t waves[4];
+  if constexpr (LANES > 64) {
+    __shared__ uint32_t waves[LANES / 64];
     if ((t & 63) == 0) waves[t >> 6] = most;
     __syncthreads();
     most = waves[0];
 #pragma unroll
-    for (int i = 1; i < 4; ++i) most = most > waves[i] ? most : waves[i];
+    for (int i = 1; i < LANES / 64; ++i) most = most > waves[i] ? most : waves[i];
   }
   const RowScale r(most);
   if (t == 0) p.scale[row] = r.scale;
@@ -84,6 +84,10 @@ hipError_t launch(const QuantParams& p, hipStream_t s) {
     if (pieces <= 64) return launch_kernel((quantize_int8_kernel<T, 64, 1>), rows4, block, 0, s, p);
     if (pieces <= 128) return launch_kernel((quantize_int8_kernel<T, 64, 2>), rows4, block, 0, s, p);
     if (pieces <= 256) return launch_kernel((quantize_int8_kernel<T, 64, 4>), rows4, block, 0, s, p);
+  }
+  if (p.rows <= 256 && pieces > 512) {  // rows of few workgroups: every piece has a lane
+    if (pieces <= 1024) return launch_kernel((quantize_int8_kernel<T, 1024, 1>), rows1, dim3(1024), 0, s, p);
+    if (pieces <= 2048) return launch_kernel((quantize_int8_kernel<T, 1024, 2>), rows1, dim3(1024), 0, s, p);
   }
   if (pieces <= 256) return launch_kernel((quantize_int8_kernel<T, 256, 1>), rows1, block, 0, s, p);
   if (pieces <= 512) return launch_kernel((quantize_int8_kernel<T, 256, 2>), rows1, block, 0, s, p);

@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-import projection_ref as R
+from tests import projection_ref as R
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16]
@@ -87,14 +87,12 @@ def test_formula_against_autograd_and_differences(act):
         assert abs(((loss(*plus) - loss(*minus)) / (2 * h) - (formula[i] * v).sum()).item()) < 1e-6 * (1 + (formula[i] * v).sum().abs().item())
 
 
-@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("act", [a for a in ACTS if a != "relu"])  # which has no third derivative at 0
 def test_gradient_against_differences_of_the_result(act):
     """Directional differences of the operator's own result: a step of 2^-4 along v, where rounding (2^-11 of
     each result) and the third derivative (below 2, times h^2 / 6) both stay below 2 % of the sizes summed."""
     import cmpext3
 
-    if act == "relu":
-        pytest.skip("no third derivative at 0")
     x, wg, wu = operands(64, 96, 128, torch.float16, seed=3)
     grad = rand(64, 96, seed=4, dtype=torch.float16)
     leaves = [t.clone().requires_grad_() for t in (x, wg, wu)]

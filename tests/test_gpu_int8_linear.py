@@ -4,7 +4,7 @@ import math
 import pytest
 import torch
 
-import projection_ref as R
+from tests import projection_ref as R
 
 pytestmark = pytest.mark.gpu
 DTYPES = [torch.float16, torch.bfloat16, torch.float32]
