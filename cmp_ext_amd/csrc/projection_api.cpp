@@ -177,7 +177,7 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t b
       int groups = 1;
       double t = 0;
       if (bm == 256) {
-        t += (double)cdiv(wgs, 256) * (bn == 256 ? each * 1.6 + 6.0 : each * 0.66 + 4.0);
+        t += (double)cdiv(wgs, 256) * (bn == 256 ? each * 1.6 + 6.0 : wgs <= 224 ? each * 0.66 + 4.0 : each * 0.88 + 5.0);
       } else if (bm == 128) {
         deep = wgs <= 256 && each >= 8;
         const int64_t full = wgs / 512, rest = wgs % 512;
