@@ -39,7 +39,7 @@ hipError_t launch_skinny_reduce(DType dt, const GemmParams& p, const float* ws, 
 hipError_t launch_stream(DType dt, BLayout lay, const GemmParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_f32(KernelId id, BLayout lay, bool dma16, const GemmParams& p, dim3 grid, hipStream_t s);
 hipError_t launch_generic(DType dt, BLayout lay, const GemmParams& p, dim3 grid, hipStream_t s);
-// dst[b][r][c] = src[b][r][c] (elements of esz = 1, 2 or 4 bytes) for r < rows, c < cols,
+// dst[b][r][c] = src[b][r][c] (elements of esz = 2 or 4 bytes) for r < rows, c < cols,
 // zero elsewhere in dst_rows x dst_cols; dst_ld == dst_cols, rows of a multiple of 16
 // bytes, dst 16-byte aligned.
 hipError_t launch_pad_copy(const void* src, int64_t src_ld, int64_t src_stride, int rows, int cols, void* dst,

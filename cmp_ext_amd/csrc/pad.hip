@@ -1,7 +1,7 @@
 // Zero-padded copies of operands whose rows are not 16-byte aligned (odd K,
 // odd N, offset views), so that the 16-byte LDS-DMA kernels can run on them:
 // dst[b][r][c] = src[b][r][c] for r < rows, c < cols, and 0 elsewhere in the
-// dst_rows x dst_cols block.  Elements of 1 byte (8-bit codes), 2 (f16/bf16) or 4 (fp32).  dst
+// dst_rows x dst_cols block.  Elements of 2 bytes (f16/bf16) or 4 (fp32).  dst
 // is dense (dst_ld == dst_cols, a multiple of 16 bytes) and 16-byte aligned;
 // src may have any pitch and offset.  No counterpart in the reference, whose kernels read
 // misaligned rows element by element (bf16_matmul.cu:31-38).
@@ -54,7 +54,7 @@ __global__ void __launch_bounds__(256) pad_copy_kernel(const E* __restrict__ src
 hipError_t launch_pad_copy(const void* src, int64_t src_ld, int64_t src_stride, int rows, int cols, void* dst,
                            int64_t dst_ld, int64_t dst_stride, int dst_rows, int dst_cols, int64_t batch,
                            int esz, hipStream_t s) {
-  if (esz != 1 && esz != 2 && esz != 4) return hipErrorInvalidValue;
+  if (esz != 2 && esz != 4) return hipErrorInvalidValue;
   if (dst_ld != dst_cols || dst_cols % (16 / esz) != 0) return hipErrorInvalidValue;  // dst is a dense block
   constexpr int64_t kMaxZ = 65535;
   const dim3 block(256);
@@ -63,11 +63,7 @@ hipError_t launch_pad_copy(const void* src, int64_t src_ld, int64_t src_stride, 
     const int64_t nb = batch - b0 < kMaxZ ? batch - b0 : kMaxZ;
     const dim3 grid((unsigned)((total + kChunk - 1) / kChunk), 1, (unsigned)nb);
     hipError_t e;
-    if (esz == 1)
-      e = launch_kernel(pad_copy_kernel<uint8_t>, grid, block, 0, s, (const uint8_t*)src + b0 * src_stride,
-                         src_ld, src_stride, rows, cols, (uint8_t*)dst + b0 * dst_stride, dst_stride, dst_rows,
-                         dst_cols);
-    else if (esz == 2)
+    if (esz == 2)
       e = launch_kernel(pad_copy_kernel<uint16_t>, grid, block, 0, s, (const uint16_t*)src + b0 * src_stride,
                          src_ld, src_stride, rows, cols, (uint16_t*)dst + b0 * dst_stride, dst_stride, dst_rows,
                          dst_cols);

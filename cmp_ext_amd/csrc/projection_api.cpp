@@ -11,7 +11,6 @@
 
 #include "../../include/cmpext3_projection.h"
 #include "gemm_params.h"
-#include "kernels.h"
 #include "projection_params.h"
 
 using namespace cmpext3;
@@ -118,14 +117,17 @@ void plan_copy(Operand* o, size_t esz, int64_t* used) {
   o->copy_at = take(used, (int64_t)o->rows * o->copy_ld * (int64_t)esz);
 }
 
-// Makes the copy; afterwards the operand is the copy.
-hipError_t run_copy(Operand* o, size_t esz, char* ws, hipStream_t s) {
-  if (o->copy_at < 0) return hipSuccess;
-  void* dst = ws + o->copy_at;
-  const hipError_t e = launch_pad_copy(o->p, o->ld, 0, o->rows, o->cols, dst, o->copy_ld, 0, o->rows, (int)o->copy_ld, 1, (int)esz, s);
-  o->p = dst;
-  o->ld = o->copy_ld;
-  return e;
+// Makes the operands' copies; afterwards the operands are the copies.
+hipError_t run_copies(std::initializer_list<Operand*> operands, size_t esz, char* ws, hipStream_t s) {
+  PadParams p{};
+  int count = 0;
+  for (Operand* o : operands) {
+    if (o->copy_at < 0) continue;
+    p.m[count++] = PadParams::Matrix{o->p, ws + o->copy_at, o->ld * (int64_t)esz, o->copy_ld * (int64_t)esz, o->rows, (int)(o->cols * (int64_t)esz)};
+    o->p = ws + o->copy_at;
+    o->ld = o->copy_ld;
+  }
+  return launch_projection_pad(p, count, s);
 }
 
 // Tuning override: CMPEXT3_PROJECTION_CONFIG="kernel=<any64x64|rows|small64x64|tile128x128|tile256x128|tile256x256>[,splits=<s>
@@ -152,7 +154,8 @@ struct TilePlan {
 };
 
 // Which tiles, and in how many splits of the steps of 128 bytes of k, for M x N results (of `products` products)
-// in `batch` entries; copy_us: what the large tiles' copies of operands take (0: none); along: both operands along k.  Modelled microseconds, fitted
+// in `batch` entries; copy_us: what the large tiles' copies of operands take (0: none); rows16:
+// operands' rows have 16 bytes, which copies and 64 x 64 tiles need; along: both operands along k.  Modelled microseconds, fitted
 // to timings of 27 shapes with every tile and 1, 2, 4 and 8 splits (MI355X): a round of workgroups takes its steps
 // and some start and end, but no less than reading the operands once; splits add their sums' way to memory and back
 // and a launch.  64 x 64 tiles run three to a CU, and read operands of odd rows (every line twice) at 0.9 us
@@ -160,12 +163,12 @@ struct TilePlan {
 // x[100, 1024], two of 1024, 8.5 for 10.0.  Where they are alone on their CUs two groups of waves share a tile's steps (256 x
 // 4096 x 4096 of codes 14.8 -> 12.5 us, 128 x 4096 x 4096 14.1 -> 11.7, dx[64, 1024] 17.4 -> 14.6; four groups: no faster; but
 // 8 steps 8.9 -> 11.9, and 2 tiles on some CUs no longer fit at once).
-TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch, double copy_us, bool small_ok, bool along) {
+TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t batch, double copy_us, bool rows16, bool along) {
   const Override o = read_override();
   TilePlan best{0, 0, false, 1, 1, (int)steps};
   double least = 1e30;
   auto consider = [&](int bm, int bn, const char* name) {
-    if ((bm == 64 && !small_ok) || (bm != bn && !along) || (o.tiles() && !o.is(name))) return;
+    if (((bm == 64 || copy_us > 0) && !rows16) || (bm != bn && !along) || (o.tiles() && !o.is(name))) return;
     const int64_t tiles = cdiv(M, bm) * cdiv(N, bn / products) * batch;
     for (int64_t s = 1; s <= 16 && (s == 1 || (s * 4 <= steps && bm < 256)); ++s) {
       const int64_t each = cdiv(steps, s);
@@ -213,8 +216,13 @@ int64_t partial_bytes(const TilePlan& t, int64_t M, int64_t N, int products, int
   return t.splits > 1 ? (int64_t)t.splits * batch * products * M * partial_pitch(N) * 4 : 0;
 }
 
-// Microseconds of a zero-padded copy of an operand, 0 where none is needed.
-double copy_us(const Operand& o, size_t esz) { return rows_of_16(o, esz) ? 0.0 : 4.0 + (double)o.rows * o.cols * (int)esz * 2.0 / 4e6; }
+// Microseconds of the zero-padded copies of operands, in one launch, 0 where none is needed.
+double copy_us(std::initializer_list<const Operand*> operands, size_t esz) {
+  double us = 0;
+  for (const Operand* o : operands)
+    if (!rows_of_16(*o, esz)) us += (double)o->rows * o->cols * (int)esz * 2.0 / 4e6;
+  return us > 0 ? us + 4.0 : 0.0;
+}
 
 // Sets the tiles' grid in p and launches them, and the join of their splits.
 hipError_t run_tiles(int dtype, ProjMode mode, ProjTileLaunch* large, const TilePlan& t, ProjParams& p, void* partials, hipStream_t s) {
@@ -281,8 +289,7 @@ int plan_projection(const cmpext3_projection_args* a, ProjPlan* q) {
     q->kernel = kRows;
     return CMPEXT3_OK;
   }
-  double copies = copy_us(q->x, esz);
-  for (int i = 0; i < products; ++i) copies += copy_us(q->w[i], esz);
+  const double copies = products == 2 ? copy_us({&q->x, &q->w[0], &q->w[1]}, esz) : copy_us({&q->x, &q->w[0]}, esz);
   q->tile = plan_tiles(a->M, a->N, cdiv(a->K * (int64_t)esz, 128), products, 1, copies, true, true);
   if (q->tile.bm == 0) return CMPEXT3_OK;
   q->kernel = kTile;
@@ -365,13 +372,13 @@ int plan_backward(const cmpext3_gated_backward_args* a, BackwardPlan* q) {
   // the small tiles read 16 bytes of a row at least: of x and the weights, and of dgate's and dup's N
   const bool rows16 = a->K >= 8 && a->N >= 8;
   if (a->dx != nullptr) {
-    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1, copy_us(q->w[0], 2) + copy_us(q->w[1], 2), rows16, false);
+    q->dx = plan_tiles(a->M, a->K, 2 * cdiv(a->N, 64), 1, 1, copy_us({&q->w[0], &q->w[1]}, 2), rows16, false);
     if (q->dx.bm > 64)
       for (Operand& w : q->w) plan_copy(&w, 2, &q->ws_bytes);
     partials = partial_bytes(q->dx, a->M, a->K, 1, 1);
   }
   if (batch > 0) {
-    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch, copy_us(q->x, 2), rows16, false);
+    q->dw = plan_tiles(a->N, a->K, cdiv(a->M, 64), 1, batch, copy_us({&q->x}, 2), rows16, false);
     if (q->dw.bm > 64) plan_copy(&q->x, 2, &q->ws_bytes);
     partials = std::max(partials, partial_bytes(q->dw, a->N, a->K, 1, batch));
   }
@@ -437,10 +444,8 @@ extern "C" int cmpext3_projection(const cmpext3_projection_args* a, void* worksp
   if (q.kernel == kAny) return (int)launch_projection_any(a->dtype, mode, false, false, p, s);
   if (q.kernel == kRows) return (int)launch_projection_rows(a->dtype, mode, p, s);
   const size_t esz = elem_size(a->dtype);
-  for (Operand* o : {&q.x, &q.w[0], &q.w[1]}) {
-    const hipError_t e = run_copy(o, esz, (char*)workspace, s);
-    if (e != hipSuccess) return (int)e;
-  }
+  const hipError_t e = run_copies({&q.x, &q.w[0], &q.w[1]}, esz, (char*)workspace, s);
+  if (e != hipSuccess) return (int)e;
   p.a[0] = p.a[1] = q.x.p;
   p.lda = q.x.ld;
   for (int i = 0; i < 2; ++i) p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
@@ -497,17 +502,15 @@ extern "C" int cmpext3_gated_backward(const cmpext3_gated_backward_args* a, void
     if (e != hipSuccess) return (int)e;
   }
   const bool f16 = a->dtype == CMPEXT3_F16;
+  e = run_copies({&q.w[0], &q.w[1], &q.x}, 2, ws, s);
+  if (e != hipSuccess) return (int)e;
   ProjParams p{};
   p.out_dtype = a->dtype;
   p.lda = pitch;
   p.a[0] = d[0], p.a[1] = d[1];
   p.batch = p.splits = 1;
   if (a->dx != nullptr && a->M > 0 && a->K > 0) {
-    for (int i = 0; i < 2; ++i) {
-      e = run_copy(&q.w[i], 2, ws, s);
-      if (e != hipSuccess) return (int)e;
-      p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
-    }
+    for (int i = 0; i < 2; ++i) p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
     p.out[0] = a->dx;
     p.ldo[0] = a->dx_row;
     p.M = a->M, p.N = a->K, p.K = a->N;
@@ -528,8 +531,6 @@ extern "C" int cmpext3_gated_backward(const cmpext3_gated_backward_args* a, void
     ++p.batch;
   }
   if (p.batch == 0 || a->N == 0 || a->K == 0) return CMPEXT3_OK;
-  e = run_copy(&q.x, 2, ws, s);
-  if (e != hipSuccess) return (int)e;
   p.b[0] = q.x.p, p.ldb[0] = q.x.ld;
   p.M = a->N, p.N = a->K, p.K = a->M;
   return (int)(q.dw.bm == 0 ? launch_projection_any(a->dtype, kProjPlain, true, true, p, s)

@@ -28,6 +28,22 @@ struct Prod<int8_t> {
   }
 };
 
+// 16 bytes at any address.
+typedef u32x4 u32x4_any __attribute__((aligned(1)));
+
+// v without its first `bytes` bytes (0 to 16), zeros behind.  In steps of 32 bits: a 64-bit shift by an amount that the
+// compiler puts into the last register a wave has (v15 of 16) shifted some waves' data by other amounts here, now and
+// then, right after memory was mapped.
+__device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
+  const int words = bytes >> 2;
+  if (words & 1) v = u32x4{v.y, v.z, v.w, 0};
+  if (words & 2) v = u32x4{v.z, v.w, 0, 0};
+  if (words & 4) v = u32x4{0, 0, 0, 0};
+  const uint32_t by = (uint32_t)bytes & 3;
+  return u32x4{__builtin_amdgcn_alignbyte(v.y, v.x, by), __builtin_amdgcn_alignbyte(v.z, v.y, by), __builtin_amdgcn_alignbyte(v.w, v.z, by),
+               __builtin_amdgcn_alignbyte(0u, v.w, by)};
+}
+
 // One element of the given type (kF16, kBF16, kF32), rounded to nearest even.
 __device__ __forceinline__ void store_elem(void* base, int64_t i, int dtype, float v) {
   if (dtype == kF32)

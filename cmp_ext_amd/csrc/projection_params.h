@@ -65,6 +65,17 @@ ProjSmallLaunch launch_projection_small_f16, launch_projection_small_bf16, launc
 // Adds the splits' sums in their order and finishes the results as an unsplit kernel does.
 hipError_t launch_projection_join(int dtype, ProjMode mode, const ProjParams& p, hipStream_t s);
 
+// Rows copied to rows of whole 16 bytes, zeros behind row_bytes (16 at least); dst aligned to 16 bytes.
+struct PadParams {
+  struct Matrix {
+    const void* src;
+    void* dst;
+    int64_t src_row, dst_row;  // bytes
+    int rows, row_bytes;
+  } m[3];
+};
+hipError_t launch_projection_pad(const PadParams& p, int count, hipStream_t s);
+
 struct QuantParams {
   const void* x;
   int64_t ldx;

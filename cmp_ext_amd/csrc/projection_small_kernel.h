@@ -15,15 +15,6 @@ namespace cmpext3 {
 
 constexpr int kSmallTile = 64;
 
-typedef u32x4 u32x4_any __attribute__((aligned(1)));
-
-// v without its first `bytes` bytes (0 to 16), zeros behind.
-__device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
-  unsigned __int128 x = __builtin_bit_cast(unsigned __int128, v);
-  x = bytes >= 16 ? 0 : x >> (8 * bytes);
-  return __builtin_bit_cast(u32x4, x);
-}
-
 // One operand's share of a thread: two 16-byte pieces of each step, in rows r and r + 32 of its tile (of the
 // step, across).  Addresses are a scalar base that moves with the steps and 32-bit offsets within the tile.
 template <int ESZ, bool ACROSS>

@@ -180,3 +180,26 @@ def test_gradients_have_no_gradient():
     (d,) = torch.autograd.grad(y.float().square().sum(), (x,), create_graph=True)
     with pytest.raises(RuntimeError, match="differentiable once only"):
         d.sum().backward()
+
+
+@pytest.mark.parametrize("kernel", ["tile128x128,splits=1", "small64x64"])
+def test_odd_rows_while_memory_is_mapped(monkeypatch, kernel):
+    """Rows that are shifted into place, beside allocations that come and go: every call gives the same bits."""
+    import cmpext3
+
+    monkeypatch.setenv("CMPEXT3_PROJECTION_CONFIG", "kernel=" + kernel)
+    x, w, u = rand_codes(300, 1000, seed=1), rand_codes(500, 1000, seed=2), rand_codes(500, 1000, seed=3)
+    xs, ws = scales(300, 3), scales(500, 4)
+    want = None
+    for i in range(150):
+        t = torch.empty(1 << (20 + i % 5), device=DEV)
+        t.fill_(1.0)
+        noise = torch.empty(170000, device=DEV, dtype=torch.float64).normal_()
+        del t, noise
+        if i % 25 == 0:
+            torch.cuda.empty_cache()
+        y = cmpext3.int8_gated_linear(x, w, u, ws * 0.01, ws, x_scale=xs, dtype=torch.float32)
+        if want is None:
+            want = y.clone()
+            R.check(y, R.int8_gated(x, xs, w, ws * 0.01, u, ws, "silu", torch.float32))
+        assert torch.equal(y, want), i
