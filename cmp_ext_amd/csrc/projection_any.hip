@@ -1,4 +1,5 @@
-// Products of the feed-forward operators for any size, pitch and alignment, an element at a time.
+// Products of the feed-forward operators for any size, pitch and alignment, an element at a time: for what the others
+// cannot take, rows of less than 16 bytes, no k at all, and grids beyond theirs.  (Codes, 4096 x 4096 x 14336: 2031 us.)
 //
 // One workgroup of four waves sums a 64 x 64 block of results in steps of 64 bytes of k (32
 // 16-bit elements, 64 codes).  Operands go through registers into LDS rows of one row's (or

@@ -1,7 +1,7 @@
 // Copies of operands whose rows are not whole 16 bytes, for the large tiles: rows of whole 16 bytes, zeros behind
 // each row's end.  Bound by reading and writing them: a thread moves 16 bytes from any address; the last of a row are
 // loaded from where they end with it and shifted.  All operands of a product in one launch: x[1000, 2001] and two
-// weights of 4001 rows of bf16 PAD_US.
+// weights of 4001 rows of bf16 13.4 us (2 x 36 MB: 5.4 TB/s).
 #include "projection_common.h"
 
 namespace cmpext3 {

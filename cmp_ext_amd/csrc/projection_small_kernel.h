@@ -7,6 +7,10 @@
 // across k (B as [K, N], A as [K, M]) as [k][64 columns] for the transposing reads (kn128_off).  Where 16 bytes
 // would run past their row they are loaded from where they end with it, and shifted.  Rows past the last one
 // are read as the last one (their results are not stored), steps of k past the end are zeros.
+//
+// What bounds it: the chain of a step (0.2 to 0.28 us where a workgroup is alone on its CU: store, barrier, read,
+// multiply), and LDS at full CUs (0.65 us a step of three workgroups).  MI355X: codes x[333, 2050] by 1001 rows 10.7 us, gated
+// fp16 x[77, 1001], two of 2731, 10.2, gated codes x[100, 1000], two of 4099, 8.5; 128 x 128 tiles on copies 18.7, 20 and 28.
 #pragma once
 
 #include "projection_common.h"

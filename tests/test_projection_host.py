@@ -107,6 +107,50 @@ def test_projection_c_abi_rejects():
     assert lib.cmpext3_projection_describe(ctypes.byref(projection(M=-1)), None, 0) == BAD
 
 
+def plan(**kw):
+    buf = ctypes.create_string_buffer(256)
+    assert cabi.lib().cmpext3_projection_describe(ctypes.byref(projection(**kw)), buf, 256) == 0
+    return buf.value.decode()
+
+
+def sized(m, n, k, **kw):
+    return dict(M=m, N=n, K=k, x_row=k, gate_row=k, up_row=k, out_row=n, **kw)
+
+
+def test_plans(monkeypatch):
+    """Which kernel a call takes, by its sizes, types and alignment."""
+    monkeypatch.delenv("CMPEXT3_PROJECTION_CONFIG", raising=False)
+    i8 = dict(dtype=cabi.I8)
+    assert plan(M=0) == "kernel=none" and plan(**sized(8, 64, 7)) == "kernel=any64x64" and plan(**sized(8, 64, 0)) == "kernel=any64x64"
+    assert plan(**sized(16, 14336, 4096)) == "kernel=rows" and plan(**sized(64, 4096, 4096)) == "kernel=rows"
+    assert plan(**sized(64, 14336, 4096)) != "kernel=rows"  # fills the CUs: tiles are as fast
+    assert "small64x64" in plan(**sized(16, 4099, 1001))  # odd rows: no strips of 16 bytes
+    assert "small64x64" in plan(x=0x1002, **sized(16, 4096, 1024))
+    assert "tile256x256" in plan(**sized(4096, 14336, 4096)) and "copies=0" in plan(**sized(4096, 14336, 4096))
+    assert "copies=3" in plan(**sized(4096, 14336, 4097)) and "tile256x256" in plan(**sized(4096, 14336, 4097))
+    assert "tile256x128" in plan(**sized(256, 14336, 4096))
+    assert "groups=2" in plan(w_up=None, **sized(256, 4096, 4096, **i8)) and "splits=1 " not in plan(**sized(100, 512, 16384))
+    codes = dict(x_scale=None, x_dtype=cabi.BF16, w_up=None, **i8)
+    assert plan(**sized(1, 4096, 4096, **codes)) == "kernel=rows codes=inside"
+    assert plan(**sized(2, 4096, 4096, **codes)) == "kernel=rows"
+    assert plan(**sized(1, 4096, 4000, **codes)) == "kernel=rows" and "codes=inside" in plan(**sized(8, 4096, 512, **codes))
+    monkeypatch.setenv("CMPEXT3_PROJECTION_CONFIG", "kernel=tile128x128,splits=3")
+    assert "tile128x128" in plan(**sized(256, 4096, 4096)) and "splits=3" in plan(**sized(256, 4096, 4096))
+    monkeypatch.setenv("CMPEXT3_PROJECTION_CONFIG", "kernel=nothing")
+    assert plan(**sized(16, 14336, 4096)) == "kernel=rows"
+
+
+def test_workspace_covers_what_a_plan_needs(monkeypatch):
+    monkeypatch.delenv("CMPEXT3_PROJECTION_CONFIG", raising=False)
+    assert size(projection(**sized(4096, 14336, 4096))) == 0
+    pitch = 4104 * 2  # of 4097 elements in whole 16 bytes
+    assert size(projection(**sized(4096, 14336, 4097))) >= pitch * (4096 + 2 * 14336)
+    i8 = dict(dtype=cabi.I8, x_dtype=cabi.F32, x_scale=None)
+    assert size(projection(**sized(100, 512, 1000, **i8))) >= 100 * 1008 + 100 * 4
+    a = projection(**sized(100, 512, 1000, **i8))
+    assert cabi.lib().cmpext3_projection(ctypes.byref(a), None, 0, None) == WORK
+
+
 def backward(**kw):
     a = cabi.GatedBackwardArgs(dtype=cabi.F16, activation=cabi.ACT_GELU, M=8, N=64, K=128, grad_out=0x1000, grad_row=64, gate=0x2000,
                                up=0x3000, pre_row=64, x=0x4000, x_row=128, w_gate=0x5000, gate_row=128, w_up=0x6000, up_row=128,
