@@ -156,7 +156,7 @@ struct TilePlan {
 // Which tiles, and in how many splits of the steps of 128 bytes of k, for M x N results (of `products` products)
 // in `batch` entries; copy_us: what the large tiles' copies of operands take (0: none); rows16:
 // operands' rows have 16 bytes, which copies and 64 x 64 tiles need; along: both operands along k.  Modelled microseconds, fitted
-// to timings of 27 shapes with every tile and 1, 2, 4 and 8 splits (MI355X): a round of workgroups takes its steps
+// to timings of some 60 shapes with every tile and 1, 2, 4 and 8 splits (MI355X): a round of workgroups takes its steps
 // and some start and end, but no less than reading the operands once; splits add their sums' way to memory and back
 // and a launch.  64 x 64 tiles run three to a CU, and read operands of odd rows (every line twice) at 0.9 us
 // a step for 0.65: x[1000, 2001], two of 4001 rows, 90 us, in copies 67; x[333, 2050] by 1001 rows of codes 11.4 and 26.6,
@@ -180,12 +180,12 @@ TilePlan plan_tiles(int64_t M, int64_t N, int64_t steps, int products, int64_t b
       int groups = 1;
       double t = 0;
       if (bm == 256) {
-        t += (double)cdiv(wgs, 256) * (bn == 256 ? each * 1.6 + 6.0 : wgs <= 224 ? each * 0.66 + 4.0 : each * 0.88 + 5.0);
+        t += (double)cdiv(wgs, 256) * (bn == 256 ? each * 1.5 + 6.0 : wgs <= 224 ? each * 0.66 + 4.0 : each * 0.88 + 5.0);
       } else if (bm == 128) {
         deep = wgs <= 256 && each >= 8;
         const int64_t full = wgs / 512, rest = wgs % 512;
-        t += (double)full * (each * 0.98 + 5.0);
-        if (rest > 256) t += each * 0.98 + 5.0;
+        t += (double)full * (each * 0.94 + 5.0);
+        if (rest > 256) t += each * 0.94 + 5.0;
         else if (rest > 0) t += each * (!deep ? 0.70 : rest > 128 ? 0.40 : 0.33) + 5.0;
       } else {
         groups = wgs <= 256 && each >= 16 ? 2 : 1;

@@ -15,17 +15,18 @@
 //     reads that B as [K, N] has there.
 //
 // What bounds it at prompts and training batches: the board's power limit, as for the plain products.  MI355X, 256 x
-// 256 tiles: gated bf16 4096 x 4096, two of 14336: 698 us, 1.38 PFLOP/s; with both products stored in fp32 (470 MB more,
-// which every CU stores at the end of its tile, all at once) 805; dx 4096 x 28672 x 4096 702..728, dw 2 x 14336 x
-// 4096 x 4096 727..734 (1.32 PFLOP/s, matrix units busy 71..73 % of the active cycles); codes, 4096 x 14336 x 4096:
-// 175, 2.75 POP/s, gated 2048 x 4096, two of 11008: 162.
+// 256 tiles: gated bf16 4096 x 4096, two of 14336: 650 us, 1.48 PFLOP/s; dx 4096 x 28672 x 4096 650, dw 2 x 14336 x
+// 4096 x 4096 681 (1.41 PFLOP/s); codes, 4096 x 14336 x 4096: 163, 2.95 POP/s, gated 2048 x 4096, two of 11008: 149.
+// Both products stored in fp32 for the backward pass (470 MB more, which every CU stores at the end of its tile, all at
+// once) cost some 100 us of the first.
 #pragma once
 
 #include "projection_common.h"
 
 namespace cmpext3 {
 
-template <int BM, int BN, bool AKM, bool BKN, int WM, int WN, int NS>
+// NSA, NSB: ring slots of A and of B, a step each.
+template <int BM, int BN, bool AKM, bool BKN, int WM, int WN, int NSA, int NSB>
 struct ProjTileShape {
   static constexpr int ROW = 128;  // bytes of k of a step
   static constexpr int NW = WM * WN;
@@ -33,26 +34,26 @@ struct ProjTileShape {
   static constexpr int FM = WTM / 16, FN = WTN / 16;
   static constexpr int A_PITCH = AKM ? BM * 2 : ROW, B_PITCH = BKN ? BN * 2 : ROW;
   static constexpr int A_BYTES = BM * ROW, B_BYTES = BN * ROW;  // 64 k either way
-  static constexpr int B_REGION = NS * A_BYTES;
-  static constexpr int LDS = NS * (A_BYTES + B_BYTES);
+  static constexpr int B_REGION = NSA * A_BYTES;
+  static constexpr int LDS = NSA * A_BYTES + NSB * B_BYTES;
   static constexpr int A_DMA = A_BYTES / 1024 / NW, B_DMA = B_BYTES / 1024 / NW;
   static constexpr int DMA = A_DMA + B_DMA;
   static_assert(WTM % 16 == 0 && WTN % 32 == 0, "16-row blocks, pairs of 16-column blocks");
   static_assert(A_BYTES % (1024 * NW) == 0 && B_BYTES % (1024 * NW) == 0, "whole DMA loads per wave");
   static_assert(B_DMA % 4 == 0 || B_DMA == 2, "pairs of a wave's loads alternate between both weights, or the waves do");
   static_assert(LDS <= 160 * 1024, "LDS budget");
-  static_assert(NS >= 2 && (NS - 1) * DMA <= 63, "vmcnt range");
-  // (a ring of three has a second base for its last slot)
-  static_assert(NS == 3 || (NS - 1) * A_BYTES + (AKM ? 36 * A_PITCH : (FM - 1) * 2048) <= 65535 &&
-                    (NS - 1) * B_BYTES + (BKN ? 36 * B_PITCH : (FN - 1) * 2048) <= 65535,
-                "immediate LDS offsets");
+  static_assert(NSA >= 2 && NSB >= 2 && NSA * A_DMA + NSB * B_DMA - DMA <= 63, "vmcnt range");
+  // offsets of a slot's reads are immediates up to 64 KiB; third slots of 32 KiB have a second base
+  static_assert((NSA == 3 || (NSA - 1) * A_BYTES + (AKM ? 36 * A_PITCH : (FM - 1) * 2048) <= 65535) &&
+                    (NSB == 3 || (NSB - 1) * B_BYTES + (BKN ? 36 * B_PITCH : (FN - 1) * 2048) <= 65535),
+                "LDS offsets");
 };
 
 // O: the output's type.  KCHECK: K (of every part and split) is no multiple of a step.  SPLITK: grid.z =
 // batch * splits; a workgroup stores its sums into p.partials.
-template <typename T, typename O, int MODE, bool AKM, bool BKN, int BM, int BN, int WM, int WN, int MINB, int NS, bool KCHECK, bool SPLITK>
+template <typename T, typename O, int MODE, bool AKM, bool BKN, int BM, int BN, int WM, int WN, int MINB, int NSA, int NSB, bool KCHECK, bool SPLITK>
 __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(const ProjParams p) {
-  using S = ProjTileShape<BM, BN, AKM, BKN, WM, WN, NS>;
+  using S = ProjTileShape<BM, BN, AKM, BKN, WM, WN, NSA, NSB>;
   using Acc = typename Prod<T>::Acc;
   constexpr int FM = S::FM, FN = S::FN;
   constexpr bool GATED = MODE == kProjGated, SUM = MODE == kProjSum, CODES = sizeof(T) == 1;
@@ -208,10 +209,10 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
   };
   // LDS read r of sub-step s of a step's slot into fragment buffer buf
   constexpr int RA = (AKM ? 2 : 1) * FM, RD = RA + (BKN ? 2 : 1) * FN;
-  auto read_one = [&](auto slotc, int s, int buf, auto rc) {
-    constexpr int r = decltype(rc)::value, slot = decltype(slotc)::value;
-    const unsigned char* sa = smem + slot * S::A_BYTES;
-    const unsigned char* sb = smem + slot * S::B_BYTES;  // fb_off includes the B region's start
+  auto read_one = [&](auto slotac, auto slotbc, int s, int buf, auto rc) {
+    constexpr int r = decltype(rc)::value;
+    const unsigned char* sa = smem + decltype(slotac)::value * S::A_BYTES;
+    const unsigned char* sb = smem + decltype(slotbc)::value * S::B_BYTES;  // fb_off includes the B region's start
     if constexpr (r < RA && AKM) {
       constexpr int i = r >> 1, half = r & 1;
       const u32x2 v = read_tr(sa + fa_off[i] + (32 * s + 4 * half) * S::A_PITCH);
@@ -230,39 +231,72 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
     }
   };
   // One sub-step of products on fragment buffer BUF; product x also issues its share of the reads of
-  // sub-step RS of ring slot RSLOT into the other buffer and of DMA pieces D0 .. D1-1 of step dkt.
+  // sub-step RS of ring slots RA and RB into the other buffer and of ND DMA pieces.
   constexpr int X = FM * FN;
-  auto substep = [&](auto bufc, auto rslotc, int rs, auto d0c, auto d1c, int dkt, auto dslotc) {
-    constexpr int buf = decltype(bufc)::value;
-    constexpr int d0 = decltype(d0c)::value, nd = decltype(d1c)::value - d0;
+  auto substep = [&](auto bufc, auto rac, auto rbc, int rs, auto ndc, auto&& piece) {
+    constexpr int buf = decltype(bufc)::value, nd = decltype(ndc)::value;
     static_for<X>([&](auto xc) {
       constexpr int x = decltype(xc)::value;
       constexpr int i = x / FN, j = x % FN;
       acc[i][j] = Prod<T>::mma(fb[buf][j], fa[buf][i], acc[i][j]);
       static_for<RD>([&](auto rc) {
-        if constexpr (decltype(rc)::value * X / RD == x) read_one(rslotc, rs, buf ^ 1, rc);
+        if constexpr (decltype(rc)::value * X / RD == x) read_one(rac, rbc, rs, buf ^ 1, rc);
       });
       static_for<nd>([&](auto dc) {
-        if constexpr (decltype(dc)::value * X / nd == x) dma_piece(dkt, dslotc, std::integral_constant<int, d0 + decltype(dc)::value>{});
+        if constexpr (decltype(dc)::value * X / nd == x) piece(dc);
       });
       __builtin_amdgcn_sched_barrier(0);  // keep the slots in this order
     });
   };
   using B0 = std::integral_constant<int, 0>;
   using B1 = std::integral_constant<int, 1>;
-  using DH = std::integral_constant<int, NS == 2 ? 0 : S::DMA / 2>;  // pieces left for the next step's first half
-  using DL = std::integral_constant<int, S::DMA - DH::value>;
   using DA = std::integral_constant<int, S::DMA>;
-  // Step kt from ring slot SLOT: all of its reads are issued by the end of the first sub-step, so that one
-  // barrier both frees the slot and certifies the next step's data.
-  auto step = [&](int kt, auto slotc) {
-    using Next = std::integral_constant<int, (decltype(slotc)::value + 1) % NS>;
-    using Prev = std::integral_constant<int, (decltype(slotc)::value + NS - 1) % NS>;
-    substep(B0{}, slotc, 1, DL{}, DA{}, kt + NS - 1, Prev{});
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NS - 2) * S::DMA) : "memory");
-    substep(B1{}, Next{}, 0, B0{}, DL{}, kt + NS, slotc);
-  };
-  if (nk > 0) {
+  // Step kt, in every ring: all reads of its slots are issued by the end of the first sub-step, so that one
+  // barrier both frees them and certifies the next step's data.
+  if constexpr (NSA != NSB) {
+    // One operand has a slot more, and a step more to arrive: its step kt + 3 is loaded behind the other's kt + 2, so
+    // that it is what may be on its way at the next barrier.
+    static_assert(NSA + NSB == 5, "rings of two and three steps");
+    constexpr bool A_MORE = NSA == 3;
+    constexpr int MORE = A_MORE ? S::A_DMA : S::B_DMA, LESS = S::DMA - MORE;
+    auto load_both = [&](int kt, auto sac, auto sbc, auto dc) {
+      constexpr int d = A_MORE ? (decltype(dc)::value + S::A_DMA) % S::DMA : decltype(dc)::value;
+      if constexpr (d < S::A_DMA)
+        dma_piece(kt + NSA, sac, std::integral_constant<int, d>{});
+      else
+        dma_piece(kt + NSB, sbc, std::integral_constant<int, d>{});
+    };
+    auto step = [&](int kt, auto sac, auto sbc) {
+      substep(B0{}, sac, sbc, 1, B0{}, [](auto) {});
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"(MORE) : "memory");
+      substep(B1{}, std::integral_constant<int, (decltype(sac)::value + 1) % NSA>{}, std::integral_constant<int, (decltype(sbc)::value + 1) % NSB>{}, 0,
+              DA{}, [&](auto dc) { load_both(kt, sac, sbc, dc); });
+    };
+    static_for<2>([&](auto sc) { static_for<S::DMA>([&](auto dc) { dma_piece(decltype(sc)::value, sc, dc); }); });
+    static_for<MORE>([&](auto dc) {
+      dma_piece(2, std::integral_constant<int, 2>{}, std::integral_constant<int, (A_MORE ? 0 : S::A_DMA) + decltype(dc)::value>{});
+    });
+    asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(S::DMA + MORE) : "memory");  // step 0 landed
+    static_for<RD>([&](auto rc) { read_one(B0{}, B0{}, 0, 0, rc); });
+    for (int kt = 0; kt < nk; kt += 6) {
+      static_for<6>([&](auto sc) {
+        constexpr int s = decltype(sc)::value;
+        if (s == 0 || kt + s < nk) step(kt + s, std::integral_constant<int, s % NSA>{}, std::integral_constant<int, s % NSB>{});
+      });
+    }
+    asm volatile("s_waitcnt vmcnt(0)" : : : "memory");  // no LDS DMA may outlive the workgroup
+  } else {
+    constexpr int NS = NSA;
+    using DH = std::integral_constant<int, NS == 2 ? 0 : S::DMA / 2>;  // pieces left for the next step's first half
+    using DL = std::integral_constant<int, S::DMA - DH::value>;
+    auto step = [&](int kt, auto slotc) {
+      using Next = std::integral_constant<int, (decltype(slotc)::value + 1) % NS>;
+      using Prev = std::integral_constant<int, (decltype(slotc)::value + NS - 1) % NS>;
+      substep(B0{}, slotc, slotc, 1, DH{},
+              [&](auto dc) { dma_piece(kt + NS - 1, Prev{}, std::integral_constant<int, DL::value + decltype(dc)::value>{}); });
+      asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" : : "n"((NS - 2) * S::DMA) : "memory");
+      substep(B1{}, Next{}, Next{}, 0, DL{}, [&](auto dc) { dma_piece(kt + NS, slotc, dc); });
+    };
     auto fill = [&](auto sc) {
       static_for<S::DMA>([&](auto dc) {
         if constexpr (NS == 2 || decltype(sc)::value < NS - 1 || decltype(dc)::value < DL::value) dma_piece(decltype(sc)::value, sc, dc);
@@ -271,7 +305,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
     fill(B0{});
     fill(B1{});
     asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" : : "n"(S::DMA) : "memory");  // step 0 landed
-    static_for<RD>([&](auto rc) { read_one(B0{}, 0, 0, rc); });
+    static_for<RD>([&](auto rc) { read_one(B0{}, B0{}, 0, 0, rc); });
     static_for<NS - 2>([&](auto sc) { fill(std::integral_constant<int, decltype(sc)::value + 2>{}); });
     for (int kt = 0; kt < nk; kt += NS) {
       static_for<NS>([&](auto sc) {
@@ -418,26 +452,31 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
     finish(std::integral_constant<int, 0>{});
 }
 
+// Rings of two steps of one operand and three of the other fill the LDS of a CU (160 KiB) with one 256 x 256 tile or two of
+// 128 x 128: the operand that more often comes from HBM, the weights (for their gradients dgate and dup), has a
+// step more to arrive.  MI355X, rings of two steps -> this: gated bf16 4096 x 4096, two of 14336, 707 -> 656 us, codes 4096 x 14336
+// x 4096 177 -> 165, dx 672 -> 650, dw 696 -> 681.  (dx with k of no whole steps would spill registers: two and two.)
 // Tiles: 256 x 256 with 8 waves, one workgroup per CU; 128 x 128 with 4 waves, two per CU, or one with
 // a ring of four steps where no CU gets a second (see the plan); and, along k, 256 x 128 with 8 waves and a ring
 // of three steps, for some hundred rows whose weights come from HBM: the time is that of loads on their way (x[256,
 // 4096], two weights of 14336 rows, bf16: 256 x 256 101 us, 128 x 128 85, 256 x 128 with a ring of two 84, of three 68).
 template <typename T, typename O, int MODE, bool AKM, bool BKN, bool KCHECK>
 hipError_t launch_projection_tile_k(const ProjParams& p, int bm, int bn, bool deep, dim3 grid, hipStream_t s) {
+  constexpr int A2 = AKM ? 3 : 2, B2 = AKM || (MODE == kProjSum && KCHECK) ? 2 : 3;
   if constexpr (!AKM && !BKN) {
     if (bn == 128 && bm == 256)
-      return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 128, 4, 2, 1, 3, KCHECK, false>), grid, dim3(512), 0, s, p);
+      return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 128, 4, 2, 1, 3, 3, KCHECK, false>), grid, dim3(512), 0, s, p);
   }
   if (bm == 256)
-    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 256, 4, 2, 1, 2, KCHECK, false>), grid, dim3(512), 0, s, p);
+    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 256, 4, 2, 1, A2, B2, KCHECK, false>), grid, dim3(512), 0, s, p);
   if (p.splits > 1) {
     if (deep)
-      return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 1, 4, KCHECK, true>), grid, dim3(256), 0, s, p);
-    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, 2, KCHECK, true>), grid, dim3(256), 0, s, p);
+      return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 1, 4, 4, KCHECK, true>), grid, dim3(256), 0, s, p);
+    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, AKM ? 3 : 2, AKM ? 2 : 3, KCHECK, true>), grid, dim3(256), 0, s, p);
   }
   if (deep)
-    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 1, 4, KCHECK, false>), grid, dim3(256), 0, s, p);
-  return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, 2, KCHECK, false>), grid, dim3(256), 0, s, p);
+    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 1, 4, 4, KCHECK, false>), grid, dim3(256), 0, s, p);
+  return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, AKM ? 3 : 2, AKM ? 2 : 3, KCHECK, false>), grid, dim3(256), 0, s, p);
 }
 
 template <typename T, typename O, int MODE, bool AKM, bool BKN>
