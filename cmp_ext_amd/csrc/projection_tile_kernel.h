@@ -452,17 +452,18 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
     finish(std::integral_constant<int, 0>{});
 }
 
-// Rings of two steps of one operand and three of the other fill the LDS of a CU (160 KiB) with one 256 x 256 tile or two of
-// 128 x 128: the operand that more often comes from HBM, the weights (for their gradients dgate and dup), has a
+// 256 x 256 tiles, k of whole steps: rings of two steps of one operand and three of the other fill the LDS of a CU (160 KiB).
+// The operand that more often comes from HBM, the weights (for their gradients dgate and dup), has a
 // step more to arrive.  MI355X, rings of two steps -> this: gated bf16 4096 x 4096, two of 14336, 707 -> 656 us, codes 4096 x 14336
-// x 4096 177 -> 165, dx 672 -> 650, dw 696 -> 681.  (dx with k of no whole steps would spill registers: two and two.)
+// x 4096 177 -> 165, dx 672 -> 650, dw 696 -> 681.  (128 x 128 tiles gain 0 to 3 % where they are chosen, for three
+// times the code; with the checks of a partial step dx would spill registers.)
 // Tiles: 256 x 256 with 8 waves, one workgroup per CU; 128 x 128 with 4 waves, two per CU, or one with
 // a ring of four steps where no CU gets a second (see the plan); and, along k, 256 x 128 with 8 waves and a ring
 // of three steps, for some hundred rows whose weights come from HBM: the time is that of loads on their way (x[256,
 // 4096], two weights of 14336 rows, bf16: 256 x 256 101 us, 128 x 128 85, 256 x 128 with a ring of two 84, of three 68).
 template <typename T, typename O, int MODE, bool AKM, bool BKN, bool KCHECK>
 hipError_t launch_projection_tile_k(const ProjParams& p, int bm, int bn, bool deep, dim3 grid, hipStream_t s) {
-  constexpr int A2 = AKM ? 3 : 2, B2 = AKM || (MODE == kProjSum && KCHECK) ? 2 : 3;
+  constexpr int A2 = AKM && !KCHECK ? 3 : 2, B2 = AKM || KCHECK ? 2 : 3;
   if constexpr (!AKM && !BKN) {
     if (bn == 128 && bm == 256)
       return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 256, 128, 4, 2, 1, 3, 3, KCHECK, false>), grid, dim3(512), 0, s, p);
@@ -472,11 +473,11 @@ hipError_t launch_projection_tile_k(const ProjParams& p, int bm, int bn, bool de
   if (p.splits > 1) {
     if (deep)
       return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 1, 4, 4, KCHECK, true>), grid, dim3(256), 0, s, p);
-    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, AKM ? 3 : 2, AKM ? 2 : 3, KCHECK, true>), grid, dim3(256), 0, s, p);
+    return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, 2, 2, KCHECK, true>), grid, dim3(256), 0, s, p);
   }
   if (deep)
     return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 1, 4, 4, KCHECK, false>), grid, dim3(256), 0, s, p);
-  return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, AKM ? 3 : 2, AKM ? 2 : 3, KCHECK, false>), grid, dim3(256), 0, s, p);
+  return launch_kernel((projection_tile_kernel<T, O, MODE, AKM, BKN, 128, 128, 2, 2, 2, 2, 2, KCHECK, false>), grid, dim3(256), 0, s, p);
 }
 
 template <typename T, typename O, int MODE, bool AKM, bool BKN>
