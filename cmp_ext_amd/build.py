@@ -27,12 +27,13 @@ LIB = os.path.join(LIBDIR, "libcmpext3_gemm.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 HIPCC = os.path.join(ROCM, "bin", "hipcc")
 
-HIP_SOURCES = [f"tile_{t}_{lay}_{k}.hip" for t in ("f16", "bf16") for lay in ("kn", "nk") for k in ("whole", "ragged")] + \
+# those that compile longest first
+HIP_SOURCES = [f"projection_tile_{k}.hip" for k in ("int8_gated", "int8_plain", "grad_f16", "grad_bf16", "gated_f16", "gated_bf16")] + \
+    [f"tile_{t}_{lay}_{k}.hip" for t in ("f16", "bf16") for lay in ("kn", "nk") for k in ("whole", "ragged")] + \
     ["skinny.hip", "tall.hip", "stream.hip", "stream_nk.hip", "f32.hip", "generic.hip", "pad.hip", "noalloc.hip", "sem.hip"] + \
     [f"attention_tile_{t}_{k}.hip" for t in ("f16", "bf16") for k in ("packed", "paged16", "paged8")] + \
     [f"attention_few_{t}_{k}.hip" for t in ("f16", "bf16") for k in ("paged16", "paged8")] + \
     ["attention_join.hip", "qk_norm_rope.hip", "kv_cache.hip"] + \
-    [f"projection_tile_{k}.hip" for k in ("gated_f16", "gated_bf16", "grad_f16", "grad_bf16", "int8_plain", "int8_gated")] + \
     ["projection_any.hip", "projection_pad.hip", "projection_rows.hip", "projection_join.hip",
                                                         "projection_small_f16.hip", "projection_small_bf16.hip", "projection_small_int8.hip", "quantize.hip", "gated_grad.hip"]
 HOST_SOURCES = ["selector.cpp", "api.cpp", "attention_api.cpp", "projection_api.cpp"]
