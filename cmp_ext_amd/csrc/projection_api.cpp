@@ -351,7 +351,9 @@ int check_gated_backward(const cmpext3_gated_backward_args* a) {
 int64_t grad_pitch(int N) { return cdiv(N, 8) * 8; }
 
 struct BackwardPlan {
-  int64_t d_at[2];
+  int64_t d_at[2], d_col_at[2];  // dgate and dup: bf16, or f16 for dx; f16 for the weights; -1: not needed
+  int64_t row_at[2], col_at[2], most_at[2];  // f16: units and inverses of rows, of columns; their largest values
+  GradUnits units;
   Operand w[2], x;  // [K, N] operands of the products: rows across k
   TilePlan dx, dw;
   int64_t partials_at, ws_bytes;
@@ -361,8 +363,23 @@ int plan_backward(const cmpext3_gated_backward_args* a, BackwardPlan* q) {
   const int st = check_gated_backward(a);
   if (st != CMPEXT3_OK) return st;
   *q = BackwardPlan{};
-  const int64_t held = (int64_t)a->M * grad_pitch(a->N) * 2;
-  for (int64_t& at : q->d_at) at = take(&q->ws_bytes, held);
+  const int64_t pitch = grad_pitch(a->N), held = (int64_t)a->M * pitch * 2;
+  const bool f16 = a->dtype == CMPEXT3_F16;
+  const void* dw[2] = {a->dw_gate, a->dw_up};
+  for (int i = 0; i < 2; ++i) {
+    q->d_at[i] = !f16 || a->dx != nullptr ? take(&q->ws_bytes, held) : -1;
+    q->d_col_at[i] = f16 && dw[i] != nullptr ? take(&q->ws_bytes, held) : -1;
+  }
+  if (f16 && a->M > 0 && a->N > 0) {
+    GradUnits& u = q->units;
+    grad_blocks(a->M, a->N, &u);
+    for (int i = 0; i < 2; ++i) {
+      q->row_at[i] = take(&q->ws_bytes, 4 * (int64_t)a->M);
+      q->col_at[i] = take(&q->ws_bytes, 4 * 2 * pitch);
+    }
+    q->most_at[0] = take(&q->ws_bytes, 4 * (int64_t)u.col_blocks * a->M);
+    q->most_at[1] = take(&q->ws_bytes, 4 * (int64_t)u.row_blocks * 2 * pitch);
+  }
   q->w[0] = Operand{a->w_gate, a->gate_row, a->N, a->K, -1, 0};
   q->w[1] = Operand{a->w_up, a->up_row, a->N, a->K, -1, 0};
   q->x = Operand{a->x, a->x_row, a->M, a->K, -1, 0};
@@ -485,29 +502,39 @@ extern "C" int cmpext3_gated_backward(const cmpext3_gated_backward_args* a, void
   if (st != CMPEXT3_OK) return st;
   const hipStream_t s = (hipStream_t)stream;
   char* ws = (char*)workspace;
+  const bool f16 = a->dtype == CMPEXT3_F16;
   const int64_t pitch = grad_pitch(a->N);
-  uint16_t* d[2] = {(uint16_t*)(ws + q.d_at[0]), (uint16_t*)(ws + q.d_at[1])};
+  auto at = [&](int64_t offset) -> char* { return offset >= 0 ? ws + offset : nullptr; };
+  void* const d[2] = {at(q.d_at[0]), at(q.d_at[1])};
+  void* const d_col[2] = {f16 ? at(q.d_col_at[0]) : d[0], f16 ? at(q.d_col_at[1]) : d[1]};
+  const bool units = f16 && a->M > 0 && a->N > 0;
+  GradUnits u = q.units;
   hipError_t e = hipSuccess;
   if (a->M > 0 && a->N > 0) {
     GatedGradParams g{};
     g.grad = a->grad_out;
     g.gate = a->gate;
     g.up = a->up;
-    g.dgate = d[0];
-    g.dup = d[1];
+    for (int i = 0; i < 2; ++i) g.d[i] = d[i], g.d_col[i] = f16 ? d_col[i] : nullptr;
+    if (units) {
+      u.row = (float*)at(q.row_at[0]), u.row_inverse = (float*)at(q.row_at[1]);
+      u.col = (float*)at(q.col_at[0]), u.col_inverse = (float*)at(q.col_at[1]);
+      u.row_most = (uint32_t*)at(q.most_at[0]), u.col_most = (uint32_t*)at(q.most_at[1]);
+      g.units = u;
+    }
     g.ld_grad = a->grad_row, g.ld_pre = a->pre_row, g.ld_d = pitch;
     g.act = a->activation;
     g.M = a->M, g.N = a->N;
     e = launch_gated_grad(a->dtype, g, s);
     if (e != hipSuccess) return (int)e;
   }
-  const bool f16 = a->dtype == CMPEXT3_F16;
   e = run_copies({&q.w[0], &q.w[1], &q.x}, 2, ws, s);
   if (e != hipSuccess) return (int)e;
   ProjParams p{};
   p.out_dtype = a->dtype;
   p.lda = pitch;
   p.a[0] = d[0], p.a[1] = d[1];
+  p.a_scale = units ? u.row_inverse : nullptr;
   p.batch = p.splits = 1;
   if (a->dx != nullptr && a->M > 0 && a->K > 0) {
     for (int i = 0; i < 2; ++i) p.b[i] = q.w[i].p, p.ldb[i] = q.w[i].ld;
@@ -525,7 +552,8 @@ extern "C" int cmpext3_gated_backward(const cmpext3_gated_backward_args* a, void
   const int64_t dw_row[2] = {a->dgate_row, a->dup_row};
   for (int i = 0; i < 2; ++i) {
     if (dw[i] == nullptr) continue;
-    p.a[p.batch] = d[i];
+    p.a[p.batch] = d_col[i];
+    if (units && p.batch == 0) p.a_scale = u.col_inverse + i * (int64_t)a->N;
     p.out[p.batch] = dw[i];
     p.ldo[p.batch] = dw_row[i];
     ++p.batch;

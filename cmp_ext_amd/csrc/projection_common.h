@@ -28,6 +28,14 @@ struct Prod<int8_t> {
   }
 };
 
+// f16 gradients: what undoes the unit of row m of entry bz's a (1 otherwise).  A power of two: the product with it is exact.
+template <typename T, int MODE>
+__device__ __forceinline__ float row_unit(const ProjParams& p, int bz, int64_t m) {
+  if constexpr (std::is_same<T, _Float16>::value && MODE != kProjGated)
+    return p.a_scale != nullptr ? p.a_scale[bz * (int64_t)p.M + m] : 1.f;
+  return 1.f;
+}
+
 // 16 bytes at any address.
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 

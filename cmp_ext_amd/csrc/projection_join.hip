@@ -15,6 +15,8 @@ __global__ void __launch_bounds__(256) projection_join_kernel(const ProjParams p
   const int64_t m = at / per_row;
   const int n0 = (int)(at - m * per_row) * 4;
   if (m >= p.M || n0 >= p.N) return;
+  // f16 gradients' units, whose inverse only they have
+  const float unit = sizeof(T) != 1 && MODE == kProjPlain && p.a_scale != nullptr ? p.a_scale[bz * (int64_t)p.M + m] : 1.f;
   f32x4 v[NP];
 #pragma unroll
   for (int q = 0; q < NP; ++q) {
@@ -26,6 +28,7 @@ __global__ void __launch_bounds__(256) projection_join_kernel(const ProjParams p
     for (int e = 0; e < 4; ++e) {
       v[q][e] = (float)sum[e];
       if (sizeof(T) == 1 && n0 + e < p.N) v[q][e] = v[q][e] * p.a_scale[m] * p.b_scale[q][n0 + e];
+      if (sizeof(T) != 1 && MODE == kProjPlain) v[q][e] *= unit;
     }
   }
   f32x4 y = v[0];

@@ -21,8 +21,8 @@ struct ProjParams {
   const void* a[2];  // kProjSum: both terms'; otherwise of each entry of the batch
   const void* b[2];  // kProjPlain: b[0]
   int64_t lda, ldb[2];
-  const float* a_scale;     // 8-bit codes: of a row of a,
-  const float* b_scale[2];  // of a row of b
+  const float* a_scale;     // 8-bit codes: of a row of a; f16 gradients: what undoes the units of a's rows, [batch][M], or nullptr
+  const float* b_scale[2];  // 8-bit codes: of a row of b
   const void* bias;         // kProjPlain: [N] of the output's type, or nullptr
   void* out[2];  // of each entry of the batch
   int64_t ldo[2];
@@ -88,14 +88,32 @@ struct QuantParams {
 };
 hipError_t launch_quantize_int8(int dtype, const QuantParams& p, hipStream_t s);
 
+// Units of f16 gradients, powers of two: of a row of dgate and dup (for dx), of a column of either (for its weight).
+struct GradUnits {
+  float *row, *row_inverse;  // [M]
+  float *col, *col_inverse;  // [2][ld_d], [2][N]
+  // the largest finite values' bits: of rows within blocks of columns, of columns within blocks of rows
+  uint32_t *row_most, *col_most;              // [col_blocks][M], [row_blocks][2][ld_d]
+  int col_blocks, row_blocks, rows_of_block;  // see grad_blocks
+};
+constexpr int kGradBlockCols = 512;
+// Blocks of rows: 128, or more where the columns are few, for 1024 workgroups; of 8 rows at least.
+inline void grad_blocks(int64_t M, int64_t N, GradUnits* u) {
+  u->col_blocks = (int)((N + kGradBlockCols - 1) / kGradBlockCols);
+  const int64_t most = u->col_blocks < 8 ? 1024 / u->col_blocks : 128;
+  u->rows_of_block = (int)(8 * ((M + 8 * most - 1) / (8 * most)));
+  u->row_blocks = (int)((M + u->rows_of_block - 1) / u->rows_of_block);
+}
+
 // dgate = grad * up * act'(gate), dup = grad * act(gate): [M, N] each, rows of ld_d elements of
 // which those past N are set to zero.
 struct GatedGradParams {
   const void* grad;
   const float* gate;
   const float* up;
-  void* dgate;
-  void* dup;
+  void* d[2];      // dgate, dup: bf16 for all products; f16 for dx, rows times their units; or nullptr
+  void* d_col[2];  // f16: for the weights, columns times their units; each or nullptr
+  GradUnits units;
   int64_t ld_grad, ld_pre, ld_d;
   int act, M, N;
 };

@@ -347,6 +347,12 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
     }
     __syncthreads();
   }
+  float unit[FM];  // of the rows: read before the stores, behind which they would wait
+#pragma unroll
+  for (int i = 0; i < FM; ++i) {
+    const int m = mw + 16 * i + r16;
+    unit[i] = m < M ? row_unit<T, MODE>(p, bz, m) : 1.f;
+  }
   // four results of row block i and column block q: columns 16q + 4G .. +3 of the wave's block
   auto scaled = [&](int i, int j, int q, int half) {
     f32x4 v;
@@ -357,7 +363,7 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
       for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * as * bs[e];
     } else {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e];
+      for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * unit[i];
     }
     return v;
   };

@@ -93,11 +93,14 @@ int cmpext3_projection_describe(const cmpext3_projection_args* args, char* buf, 
 /*
  * The backward pass of a gated projection: from grad_out [M, N], the gradient of its output,
  * and gate, up [M, N], its two products as gate_out and up_out gave them (fp32),
- *   dgate = grad_out * up * act'(gate),   dup = grad_out * act(gate)    (fp32, held in 16 bits)
+ *   dgate = grad_out * up * act'(gate),   dup = grad_out * act(gate)    (fp32, rounded to dtype)
  *   dx      [M, K] = dgate w_gate + dup w_up         (one fp32 sum over both)
  *   dw_gate [N, K] = dgate^T x,   dw_up [N, K] = dup^T x
  * dtype F16 or BF16 for all others; any of dx, dw_gate, dw_up may be NULL and is then not computed.
  * M = 0 gives weight gradients of zero.  The derivative of relu at 0 is 0.
+ * F16 holds dgate and dup times powers of two, of each row for dx and of each channel for dw_gate and dw_up, which the
+ * products take out again: neither need lie in the range of F16 (those below 2^-29 of their row's or channel's largest
+ * lose digits).  The workspace holds dgate and dup: 4 bytes a result, F16 8 where dx and both dw are asked for.
  */
 typedef struct cmpext3_gated_backward_args {
   int32_t dtype, activation;
