@@ -7,10 +7,12 @@
 #include <c10/hip/HIPStream.h>
 
 #include <climits>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 
 #include <string>
 #include <tuple>
+#include <unordered_set>
 #include <vector>
 
 #include "../../include/cmpext3_projection.h"
@@ -328,20 +330,40 @@ std::tuple<Tensor, Tensor, Tensor> gated_backward(const Tensor& grad, const Tens
 
 // Under graph capture the gradient of a leaf is added on the stream that its accumulating node was
 // made on.  A node that an eager graph on another stream keeps alive would pull that stream into the
-// capture, which ends the process from autograd's thread: refused here, before anything is recorded.
-void check_capture(std::initializer_list<const Tensor*> leaves) {
-  for (const Tensor* leaf : leaves) {
-    const Tensor& t = *leaf;
-    if (!t.is_cuda() || !t.requires_grad() || !t.is_leaf()) continue;
-    const auto stream = c10::hip::getCurrentHIPStream(t.get_device());
-    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-    if (hipStreamIsCapturing(stream.stream(), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) continue;
-    const auto node = torch::autograd::impl::try_get_grad_accumulator(t);
-    if (node == nullptr) continue;
+// capture, which ends the process from autograd's thread: refused here, before anything is recorded,
+// for every leaf that the backward pass from this call would reach: an input, or what an input is a view or a result of.
+void check_capture(std::initializer_list<const Tensor*> inputs) {
+  using torch::autograd::AccumulateGrad;
+  using torch::autograd::Node;
+  const Tensor& first = **inputs.begin();
+  if (!first.is_cuda()) return;
+  const auto stream = c10::hip::getCurrentHIPStream(first.get_device());
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  if (hipStreamIsCapturing(stream.stream(), &capture) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
+  auto check = [&](Node* node) {
     const auto made_on = node->stream();
     TORCH_CHECK(made_on.has_value() && made_on->id() == stream.id(),
-                "cmpext3.gated_linear: a graph that was made on another stream still holds an input of this captured call; "
-                "release it (or run it on the capturing stream) before the capture");
+                "cmpext3.gated_linear: a graph that was made on another stream still holds an input of this captured call, or a leaf "
+                "that one was made from; release it (or run it on the capturing stream) before the capture");
+  };
+  std::vector<Node*> left;
+  for (const Tensor* input : inputs) {
+    const Tensor& t = *input;
+    if (!t.requires_grad()) continue;
+    if (t.is_leaf()) {
+      if (const auto node = torch::autograd::impl::try_get_grad_accumulator(t)) check(node.get());
+    } else if (t.grad_fn() != nullptr) {
+      left.push_back(t.grad_fn().get());
+    }
+  }
+  std::unordered_set<Node*> seen(left.begin(), left.end());
+  while (!left.empty()) {
+    Node* node = left.back();
+    left.pop_back();
+    const auto* leaf = dynamic_cast<const AccumulateGrad*>(node);
+    if (leaf != nullptr && leaf->variable.device() == first.device()) check(node);
+    for (const auto& edge : node->next_edges())
+      if (edge.function != nullptr && seen.insert(edge.function.get()).second) left.push_back(edge.function.get());
   }
 }
 
