@@ -3,6 +3,7 @@
 // current stream of the tensors' device.
 #include "projection_ops.h"
 
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
 
@@ -396,7 +397,16 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
   }
 };
 
+// A dual tensor of forward-mode differentiation need not require a gradient: without this the result would have no
+// tangent, which reads as a derivative of zero.
+void refuse_forward_mode(std::initializer_list<const Tensor*> inputs) {
+  if (!c10::AutogradState::get_tls_state().get_fw_grad_mode()) return;
+  for (const Tensor* t : inputs)
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), "cmpext3.gated_linear: no forward-mode derivative; it has a backward pass only");
+}
+
 Tensor gated_linear(const Tensor& x, const Tensor& w_gate, const Tensor& w_up, const std::string& activation) {
+  refuse_forward_mode({&x, &w_gate, &w_up});
   if (!at::GradMode::is_enabled() || !(x.requires_grad() || w_gate.requires_grad() || w_up.requires_grad()))
     return std::get<0>(gated_forward(x, w_gate, w_up, activation, false));
   check_capture({&x, &w_gate, &w_up});
@@ -418,7 +428,7 @@ and the activation in fp32, rounded once.
 
 activation: "silu", "gelu" (by the error function), "gelu_tanh" or "relu".
 
-Differentiable once in all three tensors.  For the backward pass x, the weights and both products (in float32,
+Differentiable once in all three tensors, backwards only (forward mode is refused).  For the backward pass x, the weights and both products (in float32,
 8 bytes for each result) are kept; where no input needs a gradient nothing is.  Weights may be the two halves of one
 tensor.  Under graph capture the inputs' leaves must not be held by a graph of another stream (refused).)",
         py::arg("x"), py::arg("w_gate"), py::arg("w_up"), py::arg("activation") = "silu");
