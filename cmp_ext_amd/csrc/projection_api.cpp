@@ -41,10 +41,10 @@ int first_of(std::initializer_list<int> checks) {
 }
 
 // Sizes that every grid and every 32-bit count in the kernels has room for, padding included.
+constexpr int kMostSize = INT_MAX - 512;
 int check_sizes(int M, int N, int K) {
   if (M < 0 || N < 0 || K < 0) return CMPEXT3_ERR_INVALID_ARG;
-  const int most = INT_MAX - 512;
-  if (M > most || N > most || K > most) return CMPEXT3_ERR_TOO_LARGE;
+  if (M > kMostSize || N > kMostSize || K > kMostSize) return CMPEXT3_ERR_TOO_LARGE;
   return CMPEXT3_OK;
 }
 bool any_grid_fits(int64_t M, int64_t N) { return cdiv(M, 64) * 256 <= kMostThreads && cdiv(N, 64) <= kMostGridY; }
@@ -410,7 +410,7 @@ extern "C" int cmpext3_quantize_int8(const cmpext3_quantize_int8_args* a, void* 
   if (!is16(a->dtype) && a->dtype != CMPEXT3_F32) return CMPEXT3_ERR_UNSUPPORTED;
   if (a->rows < 0 || a->cols < 0) return CMPEXT3_ERR_INVALID_ARG;
   if (a->rows == 0) return CMPEXT3_OK;
-  if (a->rows > kMostThreads / 256) return CMPEXT3_ERR_TOO_LARGE;
+  if (a->rows > kMostThreads / 256 || a->cols > kMostSize) return CMPEXT3_ERR_TOO_LARGE;
   if (a->scale == nullptr || !aligned(a->scale, 4)) return CMPEXT3_ERR_INVALID_ARG;
   if (a->cols > 0) {
     if (a->x == nullptr || a->codes == nullptr || !aligned(a->x, elem_size(a->dtype))) return CMPEXT3_ERR_INVALID_ARG;

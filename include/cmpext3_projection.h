@@ -37,7 +37,7 @@ extern "C" {
  * Rows of x [rows, cols] (F16, BF16 or F32) as 8-bit codes with one scale for each:
  *   a = max(max |x|, 2^-100),   code = round(127 x / a) (ties to even),   scale = a / 127
  * so that code * scale stands for x (F32: 127 x is rounded to fp32 first).  A row that holds NaN or an infinity gets
- * codes of 0 and a scale of NaN: whatever is computed from it is NaN.
+ * codes of 0 and a scale of NaN: whatever is computed from it is NaN.  cols up to 2^31 - 513.
  */
 typedef struct cmpext3_quantize_int8_args {
   int32_t dtype;
