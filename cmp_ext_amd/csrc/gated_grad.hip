@@ -8,7 +8,7 @@
 // sums that follow may well be inside.  So f16 holds dgate and dup times powers of two, which the products' last step
 // takes out again: for dx, a sum over a row, each row's largest value is put between 2^14 and 2^15; for the weights, sums over
 // a column, each column's.  (One unit for all would take the digits of every token beside one of large gradients.)  The two
-// copies, and the pass that looks for the largest, are what f16 pays: a training step of 4096 x 4096, two of 14336, 2.49 ms for
+// copies, and the pass that looks for the largest, are what f16 pays: a training step of 4096 x 4096, two of 14336, 2.50 ms for
 // bf16's 2.20, of which the pass takes 126 us, the units 5 and the second copies 45; 500 x 1024, two of 2816, captured, 66 us for 55.
 //
 // Bound by HBM: bf16 [4096, 14336] 822 MB in 137 us, 6.0 TB/s; what is read once is read past the reusable lines, which

@@ -39,9 +39,9 @@ __device__ __forceinline__ float row_unit(const ProjParams& p, int bz, int64_t m
 // 16 bytes at any address.
 typedef u32x4 u32x4_any __attribute__((aligned(1)));
 
-// v without its first `bytes` bytes (0 to 16), zeros behind.  In steps of 32 bits: a 64-bit shift by an amount that the
-// compiler puts into the last register a wave has (v15 of 16) shifted some waves' data by other amounts here, now and
-// then, right after memory was mapped.
+// v without its first `bytes` bytes (0 to 16), zeros behind.  In steps of 32 bits: with 64-bit shifts by a variable amount
+// some waves' data were shifted by other amounts here, in 15 of 900 calls, right after memory was mapped; with these in none of
+// 2700.  The amount lay in the last register a wave has (v15 of 16), which may be the cause; that was not shown.
 __device__ __forceinline__ u32x4 drop_bytes(u32x4 v, int bytes) {
   const int words = bytes >> 2;
   if (words & 1) v = u32x4{v.y, v.z, v.w, 0};

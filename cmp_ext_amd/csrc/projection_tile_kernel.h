@@ -13,6 +13,7 @@
 //   * Sum (the gradient of x): K runs through dgate w_gate, then dup w_up, in one sum.
 //   * A across k (weight gradients, dgate^T x): [k][m] rows in LDS, read by the transposing
 //     reads that B as [K, N] has there.
+//   * f16 gradients: a row's sums times what undoes the unit that its operand was held in (gated_grad.hip).
 //
 // What bounds it at prompts and training batches: the board's power limit, as for the plain products.  MI355X, 256 x
 // 256 tiles: gated bf16 4096 x 4096, two of 14336: 650 us, 1.48 PFLOP/s; dx 4096 x 28672 x 4096 650, dw 2 x 14336 x
@@ -460,8 +461,8 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
 
 // 256 x 256 tiles, k of whole steps: rings of two steps of one operand and three of the other fill the LDS of a CU (160 KiB).
 // The operand that more often comes from HBM, the weights (for their gradients dgate and dup), has a
-// step more to arrive.  MI355X, rings of two steps -> this: gated bf16 4096 x 4096, two of 14336, 707 -> 656 us, codes 4096 x 14336
-// x 4096 177 -> 165, dx 672 -> 650, dw 696 -> 681.  (128 x 128 tiles gain 0 to 3 % where they are chosen, for three
+// step more to arrive.  MI355X, rings of two steps -> this: gated bf16 4096 x 4096, two of 14336, 707 -> 650 us, codes 4096 x 14336
+// x 4096 177 -> 163, dx 672 -> 650, dw 696 -> 681.  (128 x 128 tiles gain 0 to 3 % where they are chosen, for three
 // times the code; with the checks of a partial step dx would spill registers.)
 // Tiles: 256 x 256 with 8 waves, one workgroup per CU; 128 x 128 with 4 waves, two per CU, or one with
 // a ring of four steps where no CU gets a second (see the plan); and, along k, 256 x 128 with 8 waves and a ring
