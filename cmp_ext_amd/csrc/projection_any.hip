@@ -75,6 +75,7 @@ __global__ void __launch_bounds__(256) projection_any_kernel(const ProjParams p)
     const int64_t m = m0 + wm + 16 * i + r16;
     if (m >= p.M) continue;
     const float as = sizeof(T) == 1 ? p.a_scale[m] : row_unit<T, MODE>(p, blockIdx.z, m);
+    const RowScaled scaled(as);
 #pragma unroll
     for (int x = 0; x < 8; ++x) {
       const int j = x >> 2, e = x & 3;
@@ -84,7 +85,7 @@ __global__ void __launch_bounds__(256) projection_any_kernel(const ProjParams p)
 #pragma unroll
       for (int q = 0; q < NP; ++q) {
         v[q] = (float)acc[q][i][j][e];
-        if (sizeof(T) == 1) v[q] = v[q] * as * p.b_scale[q][n];
+        if (sizeof(T) == 1) v[q] = scaled(v[q], p.b_scale[q][n]);
         else v[q] *= as;
       }
       float y = v[0];

@@ -28,6 +28,18 @@ struct Prod<int8_t> {
   }
 };
 
+// A sum of codes times the scales of its row and column, the row's first, but last where it is large: a sum is below
+// 2^31, so that no step leaves fp32's range where the result lies in it.  (The factors of 1 change nothing.)
+struct RowScaled {
+  float first, last;
+  __device__ __forceinline__ explicit RowScaled(float scale) {
+    const bool large = __builtin_fabsf(scale) > 0x1p60f;
+    first = large ? 1.f : scale;
+    last = large ? scale : 1.f;
+  }
+  __device__ __forceinline__ float operator()(float sum, float column) const { return sum * first * column * last; }
+};
+
 // f16 gradients: what undoes the unit of row m of entry bz's a (1 otherwise).  A power of two: the product with it is exact.
 template <typename T, int MODE>
 __device__ __forceinline__ float row_unit(const ProjParams& p, int bz, int64_t m) {
@@ -106,7 +118,7 @@ __device__ __forceinline__ void finish_rows(const ProjParams& p, const void* red
 #pragma unroll
       for (int i = 0; i < WAVES; ++i) s += sums[((i * MB * 16) + (int)m) * PITCH + c];
       v[q] = (float)s;
-      if (sizeof(T) == 1) v[q] = v[q] * a_scale[m] * p.b_scale[q][n];
+      if (sizeof(T) == 1) v[q] = RowScaled(a_scale[m])(v[q], p.b_scale[q][n]);
     }
     float y = v[0];
     if constexpr (GATED) {

@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256) projection_join_kernel(const ProjParams p
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       v[q][e] = (float)sum[e];
-      if (sizeof(T) == 1 && n0 + e < p.N) v[q][e] = v[q][e] * p.a_scale[m] * p.b_scale[q][n0 + e];
+      if (sizeof(T) == 1 && n0 + e < p.N) v[q][e] = RowScaled(p.a_scale[m])(v[q][e], p.b_scale[q][n0 + e]);
       if (sizeof(T) != 1 && MODE == kProjPlain) v[q][e] *= unit;
     }
   }

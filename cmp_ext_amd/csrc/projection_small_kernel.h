@@ -281,6 +281,7 @@ __global__ void __launch_bounds__(256 * GROUPS) projection_small_kernel(const Pr
     const int64_t m = m0 + wm + 16 * (i0 + i) + r16;
     if (m >= p.M) continue;
     const float as = ESZ == 1 ? p.a_scale[m] : row_unit<T, MODE>(p, bz, m);
+    const RowScaled scaled(as);
     f32x4 v[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
@@ -289,7 +290,7 @@ __global__ void __launch_bounds__(256 * GROUPS) projection_small_kernel(const Pr
       for (int e = 0; e < 4; ++e) {
         v[j][e] = (float)acc[i][j][e];
         if (ESZ != 1) v[j][e] *= as;
-        if (ESZ == 1) v[j][e] = v[j][e] * as * (n + e < p.N ? p.b_scale[GATED ? j : 0][n + e] : 0.f);
+        if (ESZ == 1) v[j][e] = scaled(v[j][e], n + e < p.N ? p.b_scale[GATED ? j : 0][n + e] : 0.f);
         if (!GATED && ESZ == 1 && p.bias != nullptr && n + e < p.N) v[j][e] += load_elem(p.bias, n + e, p.out_dtype);
       }
     }

@@ -358,10 +358,10 @@ __global__ void __launch_bounds__(64 * WM * WN, MINB) projection_tile_kernel(con
   auto scaled = [&](int i, int j, int q, int half) {
     f32x4 v;
     if constexpr (CODES) {
-      const float as = sa[wm * S::WTM + 16 * i + r16];
+      const RowScaled scale(sa[wm * S::WTM + 16 * i + r16]);
       const f32x4 bs = *(const f32x4*)(sb + half * OBN + (nw - n0) + 16 * q + 4 * G);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * as * bs[e];
+      for (int e = 0; e < 4; ++e) v[e] = scale((float)acc[i][j][e], bs[e]);
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * unit[i];

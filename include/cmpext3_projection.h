@@ -56,7 +56,7 @@ int cmpext3_quantize_int8(const cmpext3_quantize_int8_args* args, void* stream);
  *   plain (w_up NULL; dtype CMPEXT3_I8):  out = p(w) + bias
  *   gated (both weights):                 out = act(p(w_gate)) * p(w_up)
  * where p(w)[m, n] is the sum over k of x[m, k] * w[n, k]: F16 or BF16 with fp32 sums, or I8
- * with exact 32-bit integer sums times x_scale[m] * w_scale[n].  x has x_dtype: that of the
+ * with exact 32-bit integer sums times x_scale[m] and w_scale[n] (either may be large where the result is not).  x has x_dtype: that of the
  * weights, or, with I8 weights, F16, BF16 or F32: it is then taken as cmpext3_quantize_int8 would
  * give it (x_scale NULL).  out [M, N] has out_dtype (F16,
  * BF16, F32; that of x where it is not I8), rounded once.  In the plain form the weight is
