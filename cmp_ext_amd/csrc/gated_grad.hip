@@ -159,8 +159,8 @@ __global__ void __launch_bounds__(256) gated_grad_most_kernel(const GatedGradPar
   *(u32x4*)(p.units.col_most + ((int64_t)rb * 2 + q) * p.ld_d + at) = of_col;
 }
 
-// The power of two that puts a value of these bits between 2^14 and 2^15 (2^64 at most: what is smaller than 2^-50 adds
-// nothing to a sum that f16 could hold), and its inverse.  Nothing but zeros: 1.
+// The power of two that puts a value of these bits between 2^14 and 2^15, and its inverse; nothing but zeros: 1.  2^64 at most:
+// what then still loses digits is below 2^-78, and 2^21 such terms times 2^16 do not reach f16's last digit.
 __device__ __forceinline__ void unit_of(uint32_t bits, float* unit, float* inverse) {
   const int up = bits == 0 ? 0 : min(14 + 127 - (int)(bits >> 23), 64);  // -113 at least
   *unit = __uint_as_float((uint32_t)(127 + up) << 23);
